@@ -15,6 +15,15 @@ LIB_PATH_F16 = os.path.join(HERE, "libapla_hip_f16.so")  # fp16 operands (same s
 APLA_BF16, APLA_F16, APLA_F32 = 0, 1, 2
 EPI_STORE, EPI_GELU, EPI_RESIDUAL, EPI_MUL, EPI_SWIGLU, EPI_SWIGLU_BWD, EPI_GELU_FWD = 0, 1, 2, 3, 4, 5, 6
 
+class AttnMod(ctypes.Structure):
+    """apla_attn_mod_t of include/apla_hip.h, field by field."""
+    _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "o", "lse", "cu_q", "cu_k", "len_k", "prefix", "doc_q", "doc_k", "slopes", "pos_q",
+                                         "pos_k", "d_o", "dq", "dk", "dv", "delta", "workspace")]
+                + [(n, c_long) for n in ("workspace_bytes", "ldq", "ldk", "ldv", "ldo", "lddo", "lddq", "lddk", "lddv")]
+                + [(n, c_int) for n in ("S", "Tq", "Tk", "max_q", "max_k", "Hq", "Hkv", "pos_dim", "causal")]
+                + [(n, c_float) for n in ("scale", "softcap")])
+
+
 # name -> (restype, argtypes); must list every symbol of include/apla_hip.h (tests/test_cabi.py checks this)
 SIGNATURES = {
     "apla_last_error": (c_char_p, []),
@@ -75,6 +84,15 @@ SIGNATURES = {
     "apla_attn_fwd_cls": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p]),
     "apla_attn_bwd_cls": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p]),
     "apla_attn_probs": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p]),
+    "apla_rotary": (c_int, [c_void_p, c_long, c_void_p, c_long, c_int, c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p]),
+    "apla_qk_norm_rotary_workspace_bytes": (c_long, []),
+    "apla_qk_norm_rotary_fwd": (c_int, [c_void_p, c_long, c_void_p, c_long, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p,
+                                        c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p]),
+    "apla_qk_norm_rotary_bwd": (c_int, [c_void_p, c_long, c_void_p, c_long, c_void_p, c_long, c_int, c_int, c_int, c_int, c_float, c_void_p,
+                                        c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_long, c_void_p]),
+    "apla_attn_mod_workspace_bytes": (c_long, [ctypes.POINTER(AttnMod), c_int]),
+    "apla_attn_mod_fwd": (c_int, [ctypes.POINTER(AttnMod), c_void_p]),
+    "apla_attn_mod_bwd": (c_int, [ctypes.POINTER(AttnMod), c_void_p]),
     "apla_attn_probs_dropout": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_float, c_ulonglong, c_uint, c_void_p]),
     "apla_dw_workspace_bytes": (c_long, [c_int, c_int, c_int]),
     "apla_proj_dw": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,

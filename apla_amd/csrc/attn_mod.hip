@@ -1,0 +1,978 @@
+// Attention (head_dim 64) whose scores are modified and masked on the way to the softmax, forward and deterministic backward:
+//   s_ij = scale q_i.k_j ;  s = cap tanh(s / cap) ;  s -= slope_h dist(i, j) ;  masked places = -inf ;  o_i = sum_j softmax(s)_ij v_j
+// Queries and keys have their own lengths per sequence (packed by offsets, or uniform with used lengths: a cache); several query
+// heads may share one key / value head.  Query i of a sequence stands at key position i + (nk - nq).
+//
+// Everything positional about the mask is ONE number per query row: lim_i = min(nk, causal ? max(i + nk - nq + 1, prefix) : nk), 0
+// for rows of no document; key j is visible iff j < lim_i and the two document ids are equal.  A workgroup first writes the list of
+// key tiles that any of its rows can see (lim and the [min, max] document ids of every 64-key tile), then runs over that list only;
+// a wave runs a tile without a mask where lim and the ids say that all of it is visible.
+//
+// The products are those of attention.hip (S^T = K Q^T with the query row on the lane, P^T from the accumulator as the next operand).
+// In a masked tile a weight of zero times a non-finite value is zero (mfma_select): what stands in masked places never matters.
+// P and dS are rounded to 16 bits as MFMA operands (half a step of values <= 256 resp. of dS, relative); scores, softmax
+// statistics, sums and accumulators are fp32.
+#include "attn_tiles.h"
+#include "common.h"
+
+namespace {
+
+constexpr float NEG_BIG = -1e30f;       // running maximum before the first visible key: finite, so that masked scores give exp2(-inf) = 0
+constexpr float LAZY = 8.f;             // the running maximum follows only when a score exceeds it by 2^8: weights stay <= 256
+constexpr int LIST = 256;               // tiles listed per pass (one per thread)
+
+struct ModArgs {
+  const bf16 *q, *k, *v;
+  long ldq, ldk, ldv;
+  bf16* o;
+  long ldo;
+  float* lse;
+  const int32_t *cu_q, *cu_k, *len_k, *prefix, *doc_q, *doc_k;
+  const float *slopes, *pos_q, *pos_k;
+  int S, Tq, Tk, max_q, max_k, Hq, G, causal;
+  float scale, c, k1, kx, A;            // c = scale log2e; cap: 2 scale log2e / cap, scale / cap, cap log2e
+  const int2 *rng_q, *rng_k;            // [S][tiles of 64]: smallest and largest document id
+  int nt_q, nt_k, nblk;                 // tiles per sequence in those; 128-row blocks per sequence
+  const bf16* d_o;
+  long lddo;
+  bf16 *dq, *dk, *dv;
+  long lddq, lddk, lddv;
+  float* delta;
+  float *part_o, *part_ml;              // few-row kernel: partial sums
+  int nsplit, chunk, nrt;
+};
+
+struct MSeq { long q0, k0; int nq, nk, off, pre; };
+// Offsets that do not fit the tensors are cut to them, so no access leaves the tensors whatever the device-side arrays hold.
+__device__ __forceinline__ MSeq mseq(const ModArgs& a, int s) {
+  MSeq m;
+  if (a.cu_q) {
+    const int b = min(max(a.cu_q[s], 0), a.Tq), e = min(max(a.cu_q[s + 1], b), a.Tq);
+    m.q0 = b; m.nq = min(e - b, a.max_q);
+  } else { m.q0 = (long)s * a.max_q; m.nq = a.max_q; }
+  if (a.cu_k) {
+    const int b = min(max(a.cu_k[s], 0), a.Tk), e = min(max(a.cu_k[s + 1], b), a.Tk);
+    m.k0 = b; m.nk = min(e - b, a.max_k);
+  } else { m.k0 = (long)s * a.max_k; m.nk = a.max_k; }
+  if (a.len_k) m.nk = min(max(a.len_k[s], 0), m.nk);
+  m.off = m.nk - m.nq;
+  m.pre = a.prefix ? a.prefix[s] : 0;
+  return m;
+}
+__device__ __forceinline__ int row_lim(const ModArgs& a, const MSeq& m, int i) {
+  return a.causal ? max(0, min(m.nk, max(i + m.off + 1, m.pre))) : m.nk;
+}
+
+__device__ __forceinline__ int wave_min_i(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+  return v;
+}
+__device__ __forceinline__ int wave_max_i(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+// ---- a product with weights that may be zero next to values that may be infinite or NaN
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+#if defined(APLA_FP16)
+constexpr unsigned EXP_LO = 0x7c00u, EXP_STEP = 0x04000400u, ONE_BITS = 0x3c00u;
+#else
+constexpr unsigned EXP_LO = 0x7f80u, EXP_STEP = 0x00800080u, ONE_BITS = 0x3f80u;
+#endif
+constexpr unsigned EXP_HI = EXP_LO << 16;
+// bits 15 / 31 of the result: an exponent of all ones among the fragment's values (magnitude + one exponent step carries into the sign's place)
+__device__ __forceinline__ unsigned nonfinite_bits(const bf16x8& f) {
+  const u32x4 w = __builtin_bit_cast(u32x4, f);
+  unsigned r = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r |= (w[i] & 0x7fff7fffu) + EXP_STEP;
+  return r & 0x80008000u;
+}
+// acc += A B with 0 * non-finite = 0.  Non-finite entries of A are taken out; the places that a weight other than zero leads to them
+// are found by a second product of the two indicator matrices and become NaN.
+__device__ __forceinline__ void mfma_select(f32x16& acc, const bf16x8& af, const bf16x8& bf) {
+  u32x4 fin = __builtin_bit_cast(u32x4, af), bad, wt = __builtin_bit_cast(u32x4, bf);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned x = fin[i], y = wt[i];
+    const bool bl = (x & EXP_LO) == EXP_LO, bh = (x & EXP_HI) == EXP_HI;
+    fin[i] = (bl ? 0u : x & 0xffffu) | (bh ? 0u : x & 0xffff0000u);
+    bad[i] = (bl ? ONE_BITS : 0u) | (bh ? ONE_BITS << 16 : 0u);
+    wt[i] = ((y & 0x7fffu) ? ONE_BITS : 0u) | ((y & 0x7fff0000u) ? ONE_BITS << 16 : 0u);
+  }
+  acc = MFMA_F32_32x32x16_H16(__builtin_bit_cast(bf16x8, fin), bf, acc);
+  f32x16 hits;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) hits[i] = 0.f;
+  hits = MFMA_F32_32x32x16_H16(__builtin_bit_cast(bf16x8, bad), __builtin_bit_cast(bf16x8, wt), hits);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = hits[i] > 0.f ? __builtin_nanf("") : acc[i];
+}
+// acc[2] += tile^T w: the transposed rows rbase .. rbase + 31 of an LDS tile times the weights that the accumulator w holds for them.
+// `odd`: the tile may hold non-finite values and w zeros for them.
+template <bool MASKED>
+__device__ __forceinline__ void tile_product(f32x16 (&acc)[2], const char* tile, int rbase, const f32x16& w, int lane, bool odd) {
+#pragma unroll
+  for (int sk = 0; sk < 2; ++sk) {
+    const bf16x8 wb = acc_to_operand(w, sk);
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt) {
+      const bf16x8 af = tr_frag(tile, rbase + 16 * sk, 32 * dt, lane);
+      if (MASKED && __builtin_expect(odd, 0)) mfma_select(acc[dt], af, wb);
+      else acc[dt] = MFMA_F32_32x32x16_H16(af, wb, acc[dt]);
+    }
+  }
+}
+
+// ---- staging: 64 rows x 64 columns by 256 threads (two 16-byte pieces each) through registers; rows past nrows read row nrows - 1
+struct Stage { bf16x8 v[2]; };
+__device__ __forceinline__ bool stage_odd(const Stage& t) { return __ballot((nonfinite_bits(t.v[0]) | nonfinite_bits(t.v[1])) != 0) != 0; }
+__device__ __forceinline__ void stage_load(Stage& t, const bf16* base, long ld, int row0, int nrows, int tid) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int e = tid + i * 256;
+    t.v[i] = *(const bf16x8*)(base + (long)min(row0 + (e >> 3), nrows - 1) * ld + (e & 7) * 8);
+  }
+}
+__device__ __forceinline__ void stage_store(const Stage& t, char* lds, int tid) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int e = tid + i * 256;
+    *(bf16x8*)(lds + tile_off(e >> 3, e & 7)) = t.v[i];
+  }
+}
+
+// position of a row: its own coordinates, or its place in the sequence (BIAS 1 without positions)
+template <int BIAS>
+__device__ __forceinline__ void row_pos(float (&p)[2], const float* pos, long row, int place) {
+  if constexpr (BIAS == 1) p[0] = pos ? pos[row] : (float)place;
+  if constexpr (BIAS == 2) { p[0] = pos[2 * row]; p[1] = pos[2 * row + 1]; }
+}
+template <int BIAS>
+__device__ __forceinline__ float dist(const float (&p)[2], float x, float y) {
+  if constexpr (BIAS == 1) return fabsf(x - p[0]);
+  const float dx = x - p[0], dy = y - p[1];
+  return __builtin_amdgcn_sqrtf(dx * dx + dy * dy);
+}
+
+// ------------------------------------------------------------------------------------------------ forward, one 64-key tile
+// LDS of a key tile: K, V (8 KB each), positions [2][64], document ids [64], each wave's verdict on the values it staged
+constexpr int KT_POS = 16384, KT_DOC = KT_POS + 512, KT_ODD = KT_DOC + 256, KT_BYTES = KT_ODD + 16;
+
+struct RowState { float m, l; };
+struct RowCtx { int lim, doc; float pos[2], slope; };       // slope in log2 units
+
+// cap tanh(s / cap) in log2 units: A (1 - 2 r), r = 1 / (1 + e^(2 s / cap)).  That is exact to 2^-23 A, which small scores feel relatively:
+// FINE takes the odd series below |s / cap| = 1/4 (its next term is 2^-27 there).  Masked tiles do so — every key of a short sequence is in
+// one —, full tiles hold 64 keys or more of a row, over which the difference averages out.
+template <bool FINE>
+__device__ __forceinline__ float cap_score(float s, const ModArgs& a, float& r) {
+  r = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * a.k1));
+  const float z = fmaf(-2.f * a.A, r, a.A);
+  if constexpr (!FINE) return z;
+  const float x = s * a.kx, y = x * x;
+  const float series = a.A * x * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+  return y < 0.0625f ? series : z;
+}
+
+// scores of 32 keys in log2 units (times c where nothing modifies them)
+template <bool CAP, int BIAS, bool MASKED>
+__device__ __forceinline__ void modify(f32x16& s, const ModArgs& a, const RowCtx& r, const char* tile, int kt, int j0, int h2, bool docs) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int jr = kt * 32 + 8 * g + 4 * h2;     // tile row of element 4 g
+    f32x4 px, py;
+    int4 dj;
+    if constexpr (BIAS > 0) px = *(const f32x4*)(tile + KT_POS + jr * 4);
+    if constexpr (BIAS > 1) py = *(const f32x4*)(tile + KT_POS + 256 + jr * 4);
+    if (MASKED && docs) dj = *(const int4*)(tile + KT_DOC + jr * 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float z = s[4 * g + e];
+      float rc;
+      if constexpr (CAP) z = cap_score<MASKED>(z, a, rc);
+      if constexpr (BIAS > 0) {
+        const float d = dist<BIAS>(r.pos, px[e], BIAS > 1 ? py[e] : 0.f);
+        z = CAP ? z - r.slope * d : fmaf(z, a.c, -r.slope * d);
+      }
+      if constexpr (MASKED) {
+        bool vis = j0 + jr + e < r.lim;
+        if (docs) vis = vis && (e == 0 ? dj.x : e == 1 ? dj.y : e == 2 ? dj.z : dj.w) == r.doc;
+        z = vis ? z : -INFINITY;
+      }
+      s[4 * g + e] = z;
+    }
+  }
+}
+
+template <bool CAP, int BIAS, bool MASKED>
+__device__ __forceinline__ void fwd_tile(f32x16 (&acc)[2], RowState& st, const bf16x8 (&qf)[4], const ModArgs& a, const RowCtx& r, const char* tile,
+                                         int j0, int lane, bool docs, bool odd) {
+  const int h2 = lane >> 5;
+  const float zm = (CAP || BIAS) ? 1.f : a.c;
+  const char *Ks = tile, *Vs = tile + 8192;
+  f32x16 s[2];
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[kt][i] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) s[kt] = MFMA_F32_32x32x16_H16(row_frag(Ks, kt * 32, ks, lane), qf[ks], s[kt]);
+  }
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt) modify<CAP, BIAS, MASKED>(s[kt], a, r, tile, kt, j0, h2, docs);
+  float mx = s[0][0];
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kt][i]);
+  mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+  if (__ballot((mx - st.m) * zm > LAZY)) {
+    const float m_new = fmaxf(st.m, mx), alpha = __builtin_amdgcn_exp2f((st.m - m_new) * zm);
+    st.m = m_new;
+    st.l *= alpha;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) { acc[0][i] *= alpha; acc[1][i] *= alpha; }
+  }
+  const float mc = st.m * zm;
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[kt][i] = __builtin_amdgcn_exp2f((CAP || BIAS) ? s[kt][i] - mc : fmaf(s[kt][i], zm, -mc));
+      st.l += s[kt][i];
+    }
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt) tile_product<MASKED>(acc, Vs, kt * 32, s[kt], lane, odd);
+}
+
+// ---- the list of key tiles that rows with (lim_max, documents dmin..dmax) can see, one pass of up to LIST tiles from t0
+struct TileRef { int t, lo, hi; };
+// n entries in list[]; all threads call it, ends with a barrier
+__device__ __forceinline__ int build_list(TileRef* list, int* cnt, int t0, int ntiles, const int2* rng, int dmin, int dmax, int tid) {
+  const int t = t0 + tid;
+  bool vis = t < ntiles;
+  int2 r = {0, 0};
+  if (vis && rng) {
+    r = rng[t];
+    vis = r.y >= max(dmin, 0) && r.x <= dmax;
+  }
+  const unsigned long long b = __ballot(vis);
+  if ((tid & 63) == 0) cnt[tid >> 6] = __popcll(b);
+  __syncthreads();
+  int base = 0, n = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) { const int c = cnt[w]; base += w < (tid >> 6) ? c : 0; n += c; }
+  if (vis) list[base + __popcll(b & ((1ull << (tid & 63)) - 1))] = {t, r.x, r.y};
+  __syncthreads();
+  return n;
+}
+
+// document range of the rows a workgroup holds, for its list (LDS exchange of the waves' own ranges)
+__device__ __forceinline__ void group_range(int& lo, int& hi, int& lim, int* buf, int wave, int lane) {
+  if (lane == 0) { buf[wave] = lo; buf[4 + wave] = hi; buf[8 + wave] = lim; }
+  __syncthreads();
+  lo = min(min(buf[0], buf[1]), min(buf[2], buf[3]));
+  hi = max(max(buf[4], buf[5]), max(buf[6], buf[7]));
+  lim = max(max(buf[8], buf[9]), max(buf[10], buf[11]));
+  __syncthreads();
+}
+
+// any of the four waves' verdicts
+__device__ __forceinline__ bool any_odd(const char* p) {
+  const int4 f = *(const int4*)p;
+  return __builtin_amdgcn_readfirstlane(f.x | f.y | f.z | f.w) != 0;
+}
+
+// per-key side data of a tile held in registers until its LDS buffer is free (threads 0..63)
+struct KeySide { float x, y; int d; };
+template <int BIAS>
+__device__ __forceinline__ void side_load(KeySide& ks, const ModArgs& a, const MSeq& m, int j0, int tid) {
+  if (tid < 64) {
+    const int j = min(j0 + tid, m.nk - 1);
+    float p[2] = {0.f, 0.f};
+    row_pos<BIAS>(p, a.pos_k, m.k0 + j, j);
+    ks.x = p[0]; ks.y = p[1];
+    ks.d = a.doc_k ? a.doc_k[m.k0 + j] : 0;
+  }
+}
+template <int BIAS>
+__device__ __forceinline__ void side_store(const KeySide& ks, char* tile, const ModArgs& a, int tid) {
+  if (tid < 64) {
+    if constexpr (BIAS > 0) *(float*)(tile + KT_POS + tid * 4) = ks.x;
+    if constexpr (BIAS > 1) *(float*)(tile + KT_POS + 256 + tid * 4) = ks.y;
+    if (a.doc_k) *(int*)(tile + KT_DOC + tid * 4) = ks.d;
+  }
+}
+
+// Workgroup -> (sequence, query head, block of 128 rows): consecutive logical ids (one XCD each run) share keys; with a causal mask the long
+// blocks of a head come first.
+struct Where { int s, h, blk; };
+__device__ __forceinline__ Where where(const ModArgs& a, int heads) {
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  Where w;
+  w.blk = id % a.nblk;
+  w.h = (id / a.nblk) % heads;
+  w.s = id / (a.nblk * heads);
+  return w;
+}
+
+// what a lane knows of its query row
+template <int BIAS>
+__device__ __forceinline__ RowCtx row_ctx(const ModArgs& a, const MSeq& m, int i, int h) {
+  RowCtx r;
+  r.doc = a.doc_q ? a.doc_q[m.q0 + i] : 0;
+  r.lim = r.doc < 0 ? 0 : row_lim(a, m, i);
+  r.pos[0] = r.pos[1] = 0.f;
+  row_pos<BIAS>(r.pos, a.pos_q, m.q0 + i, i + m.off);
+  r.slope = BIAS ? a.slopes[h] * LOG2E : 0.f;
+  return r;
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+template <bool CAP, int BIAS>
+__global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
+  __shared__ __attribute__((aligned(16))) char smem[2 * KT_BYTES];
+  __shared__ TileRef list[LIST];
+  __shared__ int buf[12];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
+  const Where w = where(a, a.Hq);
+  const MSeq m = mseq(a, w.s);
+  const int q0 = (a.causal ? a.nblk - 1 - w.blk : w.blk) * 128;
+  if (q0 >= m.nq) return;
+  const int qr = q0 + wave * 32 + (lane & 31);
+  const bool active = q0 + wave * 32 < m.nq;
+  const int qi = min(qr, m.nq - 1);
+  bf16x8 qf[4];
+  load_row_frags(qf, a.q + (m.q0 + qi) * a.ldq + w.h * 64, lane);
+  const RowCtx r = row_ctx<BIAS>(a, m, qi, w.h);
+  const bool docs = a.doc_k != nullptr;
+  const int wlo = wave_min_i(r.doc), whi = wave_max_i(r.doc), wlim0 = wave_min_i(r.lim), wlim1 = wave_max_i(r.lim);
+  int dlo = wlo, dhi = whi, lim = wlim1;
+  group_range(dlo, dhi, lim, buf, wave, lane);
+
+  f32x16 acc[2];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) { acc[0][i] = 0.f; acc[1][i] = 0.f; }
+  RowState st = {NEG_BIG, 0.f};
+  const bf16 *kb = a.k + m.k0 * a.ldk + (w.h / a.G) * 64, *vb = a.v + m.k0 * a.ldv + (w.h / a.G) * 64;
+  const int ntiles = (lim + 63) / 64;
+  for (int t0 = 0; t0 < ntiles; t0 += LIST) {
+    const int n = build_list(list, buf, t0, ntiles, docs ? a.rng_k + (long)w.s * a.nt_k : nullptr, dlo, dhi, tid);
+    Stage ks, vs;
+    KeySide sd;
+    auto fetch = [&](int e) {
+      const int j0 = __builtin_amdgcn_readfirstlane(list[e].t) * 64;
+      stage_load(ks, kb, a.ldk, j0, m.nk, tid);
+      stage_load(vs, vb, a.ldv, j0, m.nk, tid);
+      side_load<BIAS>(sd, a, m, j0, tid);
+    };
+    auto put = [&](char* tile) {
+      stage_store(ks, tile, tid);
+      stage_store(vs, tile + 8192, tid);
+      side_store<BIAS>(sd, tile, a, tid);
+      const bool odd = stage_odd(vs);
+      if (lane == 0) *(int*)(tile + KT_ODD + wave * 4) = odd;
+    };
+    if (n > 0) { fetch(0); put(smem); }
+    if (n > 1) fetch(1);
+    __syncthreads();
+    for (int e = 0; e < n; ++e) {
+      char* tile = smem + (e & 1) * KT_BYTES;
+      const TileRef tr = list[e];
+      const int j0 = __builtin_amdgcn_readfirstlane(tr.t) * 64, lo = __builtin_amdgcn_readfirstlane(tr.lo), hi = __builtin_amdgcn_readfirstlane(tr.hi);
+      if (active && j0 < wlim1 && (!docs || (hi >= max(wlo, 0) && lo <= whi))) {
+        if (j0 + 64 <= wlim0 && (!docs || (lo == hi && wlo == lo && whi == lo)))
+          fwd_tile<CAP, BIAS, false>(acc, st, qf, a, r, tile, j0, lane, false, false);
+        else
+          fwd_tile<CAP, BIAS, true>(acc, st, qf, a, r, tile, j0, lane, docs, any_odd(tile + KT_ODD));
+      }
+      if (e + 1 < n) put(smem + ((e + 1) & 1) * KT_BYTES);
+      if (e + 2 < n) fetch(e + 2);
+      __syncthreads();
+    }
+  }
+  const float l = st.l + __shfl_xor(st.l, 32, 64);
+  if (qr < m.nq) {
+    store_acc_T(acc, a.o + (m.q0 + qr) * a.ldo + w.h * 64, h2, l != 0.f ? 1.f / l : 0.f);
+    if (h2 == 0)
+      a.lse[(long)w.h * a.Tq + m.q0 + qr] = l != 0.f ? (st.m * ((CAP || BIAS) ? 1.f : a.c) + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ forward, few rows: keys split over waves and workgroups
+// The G * nq rows of the query heads that share a key head fill the 32 lanes of a tile, so K and V are read once for all of them.  Every wave
+// walks its own 64-key tiles (every fourth of the workgroup's chunk) through its own LDS, without a barrier; the four waves' (max, sum,
+// output) are joined in LDS, those of several workgroups by attn_mod_join_kernel, both in a fixed order.
+struct WStage { bf16x8 v[8]; };
+__device__ __forceinline__ void wstage_load(WStage& t, const bf16* base, long ld, int row0, int nrows, int lane) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t.v[i] = *(const bf16x8*)(base + (long)min(row0 + 8 * i + (lane >> 3), nrows - 1) * ld + (lane & 7) * 8);
+}
+__device__ __forceinline__ void wstage_store(const WStage& t, char* lds, int lane) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) *(bf16x8*)(lds + tile_off(8 * i + (lane >> 3), lane & 7)) = t.v[i];
+}
+
+template <bool CAP, int BIAS>
+__global__ __launch_bounds__(256, 1) void attn_mod_rows_kernel(ModArgs a) {
+  __shared__ __attribute__((aligned(16))) char smem[4 * KT_BYTES];
+  __shared__ float ml[4][2][32];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
+  const int Hkv = a.Hq / a.G;
+  const int sp = blockIdx.x % a.nsplit, rt = blockIdx.x / a.nsplit, hk = blockIdx.y, s = blockIdx.z;
+  const MSeq m = mseq(a, s);
+  const int rows = a.G * m.nq, rr = rt * 32 + (lane & 31);
+  if (rt * 32 >= rows) return;
+  const int rc = min(rr, rows - 1), h = hk * a.G + rc % a.G, qi = rc / a.G;
+  const RowCtx r = row_ctx<BIAS>(a, m, qi, h);
+  const bool docs = a.doc_k != nullptr;
+  const int wlo = wave_min_i(r.doc), whi = wave_max_i(r.doc), wlim0 = wave_min_i(r.lim), wlim1 = wave_max_i(r.lim);
+  f32x16 acc[2];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) { acc[0][i] = 0.f; acc[1][i] = 0.f; }
+  RowState st = {NEG_BIG, 0.f};
+  const int jb = sp * a.chunk, je = min(wlim1, jb + a.chunk);
+  char* tile = smem + wave * KT_BYTES;
+  const bf16 *kb = a.k + m.k0 * a.ldk + hk * 64, *vb = a.v + m.k0 * a.ldv + hk * 64;
+  if (jb + wave * 64 < je) {
+    bf16x8 qf[4];
+    load_row_frags(qf, a.q + (m.q0 + qi) * a.ldq + h * 64, lane);
+    WStage ks, vs;
+    KeySide sd;
+    auto fetch = [&](int j0) {
+      wstage_load(ks, kb, a.ldk, j0, m.nk, lane);
+      wstage_load(vs, vb, a.ldv, j0, m.nk, lane);
+      side_load<BIAS>(sd, a, m, j0, lane);
+    };
+    fetch(jb + wave * 64);
+    for (int j0 = jb + wave * 64; j0 < je; j0 += 256) {
+      wstage_store(ks, tile, lane);
+      wstage_store(vs, tile + 8192, lane);
+      side_store<BIAS>(sd, tile, a, lane);
+      unsigned bits = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) bits |= nonfinite_bits(vs.v[i]);
+      const bool odd = __ballot(bits != 0) != 0;
+      __builtin_amdgcn_wave_barrier();
+      asm volatile("" ::: "memory");
+      if (j0 + 256 < je) fetch(j0 + 256);
+      bool full = j0 + 64 <= wlim0, any = true;
+      if (docs) {
+        const int2 g = a.rng_k[(long)s * a.nt_k + j0 / 64];
+        any = g.y >= max(wlo, 0) && g.x <= whi;
+        full = full && g.x == g.y && wlo == g.x && whi == g.x;
+      }
+      if (any) {
+        if (full) fwd_tile<CAP, BIAS, false>(acc, st, qf, a, r, tile, j0, lane, false, false);
+        else fwd_tile<CAP, BIAS, true>(acc, st, qf, a, r, tile, j0, lane, docs, odd);
+      }
+      __builtin_amdgcn_wave_barrier();
+      asm volatile("" ::: "memory");
+    }
+  }
+  // join the four waves: [32 rows][64] fp32 per wave in its own 8 KB (rows XOR-spread over the banks by their 16-byte chunk)
+  float* mine = (float*)(smem + wave * 8192);
+  const float l = st.l + __shfl_xor(st.l, 32, 64);
+  __syncthreads();
+#pragma unroll
+  for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int row = lane & 31, ch = 8 * dt + 2 * g + h2;
+      *(f32x4*)(mine + row * 64 + ((ch ^ (row & 15)) << 2)) = f32x4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+    }
+  const float zm = (CAP || BIAS) ? 1.f : a.c;
+  if (h2 == 0) { ml[wave][0][lane] = st.m * zm; ml[wave][1][lane] = l; }
+  __syncthreads();
+  const int row = tid >> 3, ro = rt * 32 + row;
+  float M = fmaxf(fmaxf(ml[0][0][row], ml[1][0][row]), fmaxf(ml[2][0][row], ml[3][0][row])), L = 0.f, f[4];
+  f32x4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    f[u] = ml[u][1][row] != 0.f ? __builtin_amdgcn_exp2f(ml[u][0][row] - M) : 0.f;
+    L += f[u] * ml[u][1][row];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const f32x4 t = *(const f32x4*)((const float*)(smem + u * 8192) + row * 64 + (((2 * (tid & 7) + i) ^ (row & 15)) << 2));
+      x[i] += f[u] * t;
+    }
+  }
+  if (ro >= rows) return;
+  const int ho = hk * a.G + ro % a.G;
+  const long qo = m.q0 + ro / a.G;
+  if (a.nsplit == 1) {
+    const float inv = L != 0.f ? 1.f / L : 0.f;
+    bf16x8 y;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = (bf16)(x[i >> 2][i & 3] * inv);
+    *(bf16x8*)(a.o + qo * a.ldo + ho * 64 + (tid & 7) * 8) = y;
+    if ((tid & 7) == 0) a.lse[(long)ho * a.Tq + qo] = L != 0.f ? (M + __builtin_amdgcn_logf(L)) * LN2 : -INFINITY;
+  } else {
+    const long p = (((long)s * Hkv + hk) * a.nrt + rt) * a.nsplit + sp;
+    *(f32x4*)(a.part_o + (p * 32 + row) * 64 + (tid & 7) * 8) = x[0];
+    *(f32x4*)(a.part_o + (p * 32 + row) * 64 + (tid & 7) * 8 + 4) = x[1];
+    if ((tid & 7) == 0) { a.part_ml[(p * 32 + row) * 2] = M; a.part_ml[(p * 32 + row) * 2 + 1] = L; }
+  }
+}
+
+__global__ __launch_bounds__(256) void attn_mod_join_kernel(ModArgs a) {
+  const int tid = threadIdx.x, row = tid >> 3, rt = blockIdx.x, hk = blockIdx.y, s = blockIdx.z;
+  const MSeq m = mseq(a, s);
+  const int rows = a.G * m.nq, ro = rt * 32 + row;
+  if (ro >= rows) return;
+  const long p0 = (((long)s * (a.Hq / a.G) + hk) * a.nrt + rt) * a.nsplit;
+  float M = NEG_BIG, L = 0.f;
+  f32x4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  for (int sp = 0; sp < a.nsplit; ++sp) M = fmaxf(M, a.part_ml[((p0 + sp) * 32 + row) * 2]);
+  for (int sp = 0; sp < a.nsplit; ++sp) {
+    const long p = (p0 + sp) * 32 + row;
+    const float l = a.part_ml[p * 2 + 1], f = l != 0.f ? __builtin_amdgcn_exp2f(a.part_ml[p * 2] - M) : 0.f;
+    L += f * l;
+    x[0] += f * *(const f32x4*)(a.part_o + p * 64 + (tid & 7) * 8);
+    x[1] += f * *(const f32x4*)(a.part_o + p * 64 + (tid & 7) * 8 + 4);
+  }
+  const int ho = hk * a.G + ro % a.G;
+  const long qo = m.q0 + ro / a.G;
+  const float inv = L != 0.f ? 1.f / L : 0.f;
+  bf16x8 y;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = (bf16)(x[i >> 2][i & 3] * inv);
+  *(bf16x8*)(a.o + qo * a.ldo + ho * 64 + (tid & 7) * 8) = y;
+  if ((tid & 7) == 0) a.lse[(long)ho * a.Tq + qo] = L != 0.f ? (M + __builtin_amdgcn_logf(L)) * LN2 : -INFINITY;
+}
+
+// ------------------------------------------------------------------------------------------------ backward
+// P = exp2(z - L2) from the forward's lse, dS = P (dP - delta), with the cap times 1 - tanh^2 = 4 r (1 - r), r = 1 / (1 + e^(2 s / cap))
+template <bool CAP, int BIAS, bool MASKED>
+__device__ __forceinline__ void dq_tile(f32x16 (&acc)[2], const bf16x8 (&qf)[4], const bf16x8 (&df)[4], float L2, float delta, const ModArgs& a,
+                                        const RowCtx& r, const char* tile, int j0, int lane, bool docs, bool odd) {
+  const int h2 = lane >> 5;
+  const char *Ks = tile, *Vs = tile + 8192;
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt) {
+    f32x16 s, p;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) { s[i] = 0.f; p[i] = 0.f; }
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) s = MFMA_F32_32x32x16_H16(row_frag(Ks, kt * 32, ks, lane), qf[ks], s);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) p = MFMA_F32_32x32x16_H16(row_frag(Vs, kt * 32, ks, lane), df[ks], p);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int jr = kt * 32 + 8 * g + 4 * h2;
+      f32x4 px, py;
+      int4 dj;
+      if constexpr (BIAS > 0) px = *(const f32x4*)(tile + KT_POS + jr * 4);
+      if constexpr (BIAS > 1) py = *(const f32x4*)(tile + KT_POS + 256 + jr * 4);
+      if (MASKED && docs) dj = *(const int4*)(tile + KT_DOC + jr * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = 4 * g + e;
+        float z = s[i], rc = 0.f;
+        if constexpr (CAP) z = cap_score<MASKED>(z, a, rc);
+        if constexpr (BIAS > 0) {
+          const float d = dist<BIAS>(r.pos, px[e], BIAS > 1 ? py[e] : 0.f);
+          z = CAP ? z - r.slope * d : fmaf(z, a.c, -r.slope * d);
+        }
+        const float pr = __builtin_amdgcn_exp2f((CAP || BIAS) ? z - L2 : fmaf(z, a.c, -L2));
+        float ds = pr * (p[i] - delta);
+        if constexpr (CAP) ds *= 4.f * rc * (1.f - rc);
+        if constexpr (MASKED) {
+          bool vis = j0 + jr + e < r.lim;
+          if (docs) vis = vis && (e == 0 ? dj.x : e == 1 ? dj.y : e == 2 ? dj.z : dj.w) == r.doc;
+          ds = vis ? ds : 0.f;
+        }
+        s[i] = ds;
+      }
+    }
+    tile_product<MASKED>(acc, Ks, kt * 32, s, lane, odd);
+  }
+}
+
+template <bool CAP, int BIAS>
+__global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
+  __shared__ __attribute__((aligned(16))) char smem[2 * KT_BYTES];
+  __shared__ TileRef list[LIST];
+  __shared__ int buf[12];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
+  const Where w = where(a, a.Hq);
+  const MSeq m = mseq(a, w.s);
+  const int q0 = (a.causal ? a.nblk - 1 - w.blk : w.blk) * 128;
+  if (q0 >= m.nq) return;
+  const int qr = q0 + wave * 32 + (lane & 31);
+  const bool active = q0 + wave * 32 < m.nq;
+  const int qi = min(qr, m.nq - 1);
+  bf16x8 qf[4], df[4];
+  load_row_frags(qf, a.q + (m.q0 + qi) * a.ldq + w.h * 64, lane);
+  load_row_frags(df, a.d_o + (m.q0 + qi) * a.lddo + w.h * 64, lane);
+  const long stat = (long)w.h * a.Tq + m.q0 + qi;
+  float delta = 0.f;      // rowsum(dO o O): this lane's half of the row, then the other half
+  {
+    bf16x8 of[4];
+    load_row_frags(of, a.o + (m.q0 + qi) * a.ldo + w.h * 64, lane);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) delta = fmaf((float)df[ks][e], (float)of[ks][e], delta);
+    delta += __shfl_xor(delta, 32, 64);
+  }
+  const float ls = a.lse[stat];
+  const float L2 = ls == -INFINITY ? -NEG_BIG : ls * LOG2E;
+  if (qr < m.nq && h2 == 0) a.delta[stat] = delta;
+  const RowCtx r = row_ctx<BIAS>(a, m, qi, w.h);
+  const bool docs = a.doc_k != nullptr;
+  const int wlo = wave_min_i(r.doc), whi = wave_max_i(r.doc), wlim0 = wave_min_i(r.lim), wlim1 = wave_max_i(r.lim);
+  int dlo = wlo, dhi = whi, lim = wlim1;
+  group_range(dlo, dhi, lim, buf, wave, lane);
+  f32x16 acc[2];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) { acc[0][i] = 0.f; acc[1][i] = 0.f; }
+  const bf16 *kb = a.k + m.k0 * a.ldk + (w.h / a.G) * 64, *vb = a.v + m.k0 * a.ldv + (w.h / a.G) * 64;
+  const int ntiles = (lim + 63) / 64;
+  for (int t0 = 0; t0 < ntiles; t0 += LIST) {
+    const int n = build_list(list, buf, t0, ntiles, docs ? a.rng_k + (long)w.s * a.nt_k : nullptr, dlo, dhi, tid);
+    Stage ks, vs;
+    KeySide sd;
+    auto fetch = [&](int e) {
+      const int j0 = __builtin_amdgcn_readfirstlane(list[e].t) * 64;
+      stage_load(ks, kb, a.ldk, j0, m.nk, tid);
+      stage_load(vs, vb, a.ldv, j0, m.nk, tid);
+      side_load<BIAS>(sd, a, m, j0, tid);
+    };
+    auto put = [&](char* tile) {
+      stage_store(ks, tile, tid);
+      stage_store(vs, tile + 8192, tid);
+      side_store<BIAS>(sd, tile, a, tid);
+      const bool odd = stage_odd(ks);
+      if (lane == 0) *(int*)(tile + KT_ODD + wave * 4) = odd;
+    };
+    if (n > 0) { fetch(0); put(smem); }
+    if (n > 1) fetch(1);
+    __syncthreads();
+    for (int e = 0; e < n; ++e) {
+      char* tile = smem + (e & 1) * KT_BYTES;
+      const TileRef tr = list[e];
+      const int j0 = __builtin_amdgcn_readfirstlane(tr.t) * 64, lo = __builtin_amdgcn_readfirstlane(tr.lo), hi = __builtin_amdgcn_readfirstlane(tr.hi);
+      if (active && j0 < wlim1 && (!docs || (hi >= max(wlo, 0) && lo <= whi))) {
+        if (j0 + 64 <= wlim0 && (!docs || (lo == hi && wlo == lo && whi == lo)))
+          dq_tile<CAP, BIAS, false>(acc, qf, df, L2, delta, a, r, tile, j0, lane, false, false);
+        else
+          dq_tile<CAP, BIAS, true>(acc, qf, df, L2, delta, a, r, tile, j0, lane, docs, any_odd(tile + KT_ODD));
+      }
+      if (e + 1 < n) put(smem + ((e + 1) & 1) * KT_BYTES);
+      if (e + 2 < n) fetch(e + 2);
+      __syncthreads();
+    }
+  }
+  if (qr < m.nq) store_acc_T(acc, a.dq + (m.q0 + qr) * a.lddq + w.h * 64, h2, a.scale);
+}
+
+// dK, dV of 128 keys: every wave holds 32 keys (the key on the lane) and the workgroup walks the 64-row query tiles of all heads that share them.
+// LDS of a query tile: Q, dO (8 KB each), then per row: lse (log2 units), delta, position x / y, lim, document, verdicts
+constexpr int QT_L = 16384, QT_D = QT_L + 256, QT_X = QT_D + 256, QT_Y = QT_X + 256, QT_LIM = QT_Y + 256, QT_DOC = QT_LIM + 256, QT_ODD = QT_DOC + 256, QT_BYTES = QT_ODD + 16;
+struct QuerySide { float L2, delta, x, y; int lim, doc; };
+
+template <bool CAP, int BIAS, bool MASKED>
+__device__ __forceinline__ void dkdv_tile(f32x16 (&dk)[2], f32x16 (&dv)[2], const bf16x8 (&kf)[4], const bf16x8 (&vf)[4], const ModArgs& a, int j, int docj,
+                                          const float (&pj)[2], float slope, const char* tile, int lane, bool docs, bool odd) {
+  const int h2 = lane >> 5;
+  const char *Qs = tile, *Ds = tile + 8192;
+#pragma unroll
+  for (int qt = 0; qt < 2; ++qt) {
+    f32x16 s, p;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) { s[i] = 0.f; p[i] = 0.f; }
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) s = MFMA_F32_32x32x16_H16(row_frag(Qs, qt * 32, ks, lane), kf[ks], s);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) p = MFMA_F32_32x32x16_H16(row_frag(Ds, qt * 32, ks, lane), vf[ks], p);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int ir = qt * 32 + 8 * g + 4 * h2;
+      const f32x4 L2 = *(const f32x4*)(tile + QT_L + ir * 4), dl = *(const f32x4*)(tile + QT_D + ir * 4);
+      f32x4 px, py;
+      int4 lm, di;
+      if constexpr (BIAS > 0) px = *(const f32x4*)(tile + QT_X + ir * 4);
+      if constexpr (BIAS > 1) py = *(const f32x4*)(tile + QT_Y + ir * 4);
+      if constexpr (MASKED) lm = *(const int4*)(tile + QT_LIM + ir * 4);
+      if (MASKED && docs) di = *(const int4*)(tile + QT_DOC + ir * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = 4 * g + e;
+        float z = s[i], rc = 0.f;
+        if constexpr (CAP) z = cap_score<MASKED>(z, a, rc);
+        if constexpr (BIAS > 0) {
+          const float d = dist<BIAS>(pj, px[e], BIAS > 1 ? py[e] : 0.f);
+          z = CAP ? z - slope * d : fmaf(z, a.c, -slope * d);
+        }
+        float pr = __builtin_amdgcn_exp2f((CAP || BIAS) ? z - L2[e] : fmaf(z, a.c, -L2[e]));
+        float ds = pr * (p[i] - dl[e]);
+        if constexpr (CAP) ds *= 4.f * rc * (1.f - rc);
+        if constexpr (MASKED) {
+          bool vis = j < (e == 0 ? lm.x : e == 1 ? lm.y : e == 2 ? lm.z : lm.w);
+          if (docs) vis = vis && (e == 0 ? di.x : e == 1 ? di.y : e == 2 ? di.z : di.w) == docj;
+          pr = vis ? pr : 0.f;
+          ds = vis ? ds : 0.f;
+        }
+        s[i] = ds;
+        p[i] = pr;
+      }
+    }
+    tile_product<MASKED>(dv, Ds, qt * 32, p, lane, odd);
+    tile_product<MASKED>(dk, Qs, qt * 32, s, lane, odd);
+  }
+}
+
+template <bool CAP, int BIAS>
+__global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
+  __shared__ __attribute__((aligned(16))) char smem[2 * QT_BYTES];
+  __shared__ TileRef list[LIST];
+  __shared__ int buf[12];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
+  const Where w = where(a, a.Hq / a.G);
+  const MSeq m = mseq(a, w.s);
+  const int jb = w.blk * 128;
+  if (jb >= m.nk) return;
+  const int jr = jb + wave * 32 + (lane & 31), j = min(jr, m.nk - 1);
+  const bool active = jb + wave * 32 < m.nk;
+  bf16x8 kf[4], vf[4];
+  load_row_frags(kf, a.k + (m.k0 + j) * a.ldk + w.h * 64, lane);
+  load_row_frags(vf, a.v + (m.k0 + j) * a.ldv + w.h * 64, lane);
+  const bool docs = a.doc_k != nullptr;
+  const int docj = docs ? a.doc_k[m.k0 + j] : 0;
+  float pj[2] = {0.f, 0.f};
+  row_pos<BIAS>(pj, a.pos_k, m.k0 + j, j);
+  const int wlo = wave_min_i(docj), whi = wave_max_i(docj);
+  int dlo = wlo, dhi = whi, dummy = 0;
+  group_range(dlo, dhi, dummy, buf, wave, lane);
+  f32x16 dk[2], dv[2];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) { dk[0][i] = dk[1][i] = 0.f; dv[0][i] = dv[1][i] = 0.f; }
+  // query tiles that can see key jb: rows i with lim_i > jb, a suffix of the rows (all of them if the prefix reaches jb)
+  const int first = m.nq == 0 ? 0 : (!a.causal || m.pre > jb) ? 0 : max(0, jb - m.off) / 64;
+  const int ntiles = (m.nq + 63) / 64;
+  for (int t0 = first; t0 < ntiles; t0 += LIST) {
+    const int n = build_list(list, buf, t0, ntiles, docs ? a.rng_q + (long)w.s * a.nt_q : nullptr, dlo, dhi, tid);
+    const int total = n * a.G;
+    Stage qs, os;
+    QuerySide sd;
+    auto fetch = [&](int x) {      // entry x % n of head x / n
+      const int h = w.h * a.G + x / n, i0 = __builtin_amdgcn_readfirstlane(list[x % n].t) * 64;
+      stage_load(qs, a.q + m.q0 * a.ldq + h * 64, a.ldq, i0, m.nq, tid);
+      stage_load(os, a.d_o + m.q0 * a.lddo + h * 64, a.lddo, i0, m.nq, tid);
+      if (tid < 64) {
+        const int i = min(i0 + tid, m.nq - 1);
+        const long stat = (long)h * a.Tq + m.q0 + i;
+        const float ls = a.lse[stat];
+        sd.L2 = ls == -INFINITY ? -NEG_BIG : ls * LOG2E;
+        sd.delta = a.delta[stat];
+        float p[2] = {0.f, 0.f};
+        row_pos<BIAS>(p, a.pos_q, m.q0 + i, i + m.off);
+        sd.x = p[0]; sd.y = p[1];
+        sd.doc = a.doc_q ? a.doc_q[m.q0 + i] : 0;
+        sd.lim = i0 + tid < m.nq && sd.doc >= 0 ? row_lim(a, m, i) : 0;
+      }
+    };
+    auto put = [&](char* tile) {
+      stage_store(qs, tile, tid);
+      stage_store(os, tile + 8192, tid);
+      if (tid < 64) {
+        *(float*)(tile + QT_L + tid * 4) = sd.L2;
+        *(float*)(tile + QT_D + tid * 4) = sd.delta;
+        if constexpr (BIAS > 0) *(float*)(tile + QT_X + tid * 4) = sd.x;
+        if constexpr (BIAS > 1) *(float*)(tile + QT_Y + tid * 4) = sd.y;
+        *(int*)(tile + QT_LIM + tid * 4) = sd.lim;
+        *(int*)(tile + QT_DOC + tid * 4) = sd.doc;
+      }
+      const bool odd = stage_odd(qs) || stage_odd(os);
+      if (lane == 0) *(int*)(tile + QT_ODD + wave * 4) = odd;
+    };
+    if (total > 0) { fetch(0); put(smem); }
+    if (total > 1) fetch(1);
+    __syncthreads();
+    for (int x = 0; x < total; ++x) {
+      char* tile = smem + (x & 1) * QT_BYTES;
+      const TileRef tr = list[x % n];
+      const int i0 = __builtin_amdgcn_readfirstlane(tr.t) * 64, lo = __builtin_amdgcn_readfirstlane(tr.lo), hi = __builtin_amdgcn_readfirstlane(tr.hi);
+      const int jw = jb + wave * 32, last = min(i0 + 63, m.nq - 1);
+      if (active && row_lim(a, m, last) > jw && (!docs || (hi >= max(wlo, 0) && lo <= whi))) {
+        const float slope = BIAS ? a.slopes[w.h * a.G + x / n] * LOG2E : 0.f;
+        if (i0 + 64 <= m.nq && jw + 32 <= m.nk && row_lim(a, m, i0) >= jw + 32 && (!docs || (lo >= 0 && lo == hi && wlo == lo && whi == lo)))
+          dkdv_tile<CAP, BIAS, false>(dk, dv, kf, vf, a, j, docj, pj, slope, tile, lane, false, false);
+        else
+          dkdv_tile<CAP, BIAS, true>(dk, dv, kf, vf, a, j, docj, pj, slope, tile, lane, docs, any_odd(tile + QT_ODD));
+      }
+      if (x + 1 < total) put(smem + ((x + 1) & 1) * QT_BYTES);
+      if (x + 2 < total) fetch(x + 2);
+      __syncthreads();
+    }
+  }
+  if (jr < m.nk) {
+    store_acc_T(dk, a.dk + (m.k0 + jr) * a.lddk + w.h * 64, h2, a.scale);
+    store_acc_T(dv, a.dv + (m.k0 + jr) * a.lddv + w.h * 64, h2, 1.f);
+  }
+}
+
+// smallest and largest document id of every 64-row tile of every sequence: one wave per tile
+__global__ __launch_bounds__(256) void attn_mod_ranges_kernel(ModArgs a, int queries, int2* out, int nt) {
+  const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int s = (int)(id / nt), t = (int)(id % nt), lane = threadIdx.x & 63;
+  if (s >= a.S) return;
+  const MSeq m = mseq(a, s);
+  const int n = queries ? m.nq : m.nk;
+  const int32_t* doc = queries ? a.doc_q + m.q0 : a.doc_k + m.k0;
+  if (t * 64 >= n) return;
+  const int d = doc[min(t * 64 + lane, n - 1)];
+  const int lo = wave_min_i(d), hi = wave_max_i(d);
+  if (lane == 0) out[(long)s * nt + t] = {lo, hi};
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+struct Plan { bool rows; int nsplit, chunk, nrt; long rng_q, rng_k, part, bytes; };
+
+// Few rows (attn_mod_rows_kernel): where the rows of a head group fill at most one tile of 32 lanes, or where 128-row workgroups would leave
+// most of the card idle next to long keys.  Keys are split so that about two workgroups per CU run, 256 keys at least each.
+Plan plan_of(const apla_attn_mod_t& p, bool backward) {
+  Plan pl = {};
+  const int G = p.Hq / p.Hkv;
+  const long rows = (long)G * p.max_q, wgs = (long)p.S * p.Hq * ((p.max_q + 127) / 128);
+  pl.nrt = (int)((rows + 31) / 32);
+  pl.rows = !backward && (rows <= 32 || (wgs < 128 && p.max_k >= 512 && pl.nrt <= 64));
+  pl.nsplit = 1;
+  pl.chunk = (p.max_k + 255) / 256 * 256;
+  if (pl.rows) {
+    const long have = (long)p.S * p.Hkv * pl.nrt;
+    long want = (512 + have - 1) / have;
+    const long most = (p.max_k + 255) / 256;
+    want = want < 1 ? 1 : want > most ? most : want;
+    if (want < 1) want = 1;
+    pl.chunk = (int)(((p.max_k + want - 1) / want + 255) / 256 * 256);
+    if (pl.chunk < 256) pl.chunk = 256;
+    pl.nsplit = (p.max_k + pl.chunk - 1) / pl.chunk;
+    if (pl.nsplit < 1) pl.nsplit = 1;
+  }
+  long b = 0;
+  if (p.doc_k) {
+    pl.rng_k = b; b += ((long)p.S * ((p.max_k + 63) / 64) * 8 + 15) / 16 * 16;
+    if (backward) { pl.rng_q = b; b += ((long)p.S * ((p.max_q + 63) / 64) * 8 + 15) / 16 * 16; }
+  }
+  if (pl.rows && pl.nsplit > 1) { pl.part = b; b += (long)p.S * p.Hkv * pl.nrt * pl.nsplit * 32 * (64 + 2) * 4; }
+  pl.bytes = b;
+  return pl;
+}
+
+int mod_check(const char* who, const apla_attn_mod_t* p, bool backward) {
+  APLA_REQUIRE(p, "%s: no arguments", who);
+  APLA_REQUIRE(p->S > 0 && p->S <= 65535 && p->Hq > 0 && p->Hkv > 0 && p->Hkv <= 65535 && p->Hq % p->Hkv == 0, "%s: need 1..65535 sequences and Hq a multiple of Hkv (S=%d Hq=%d Hkv=%d)", who, p->S, p->Hq, p->Hkv);
+  APLA_REQUIRE(p->Tq > 0 && p->Tk > 0 && p->max_q > 0 && p->max_k > 0 && p->max_q <= p->Tq && p->max_k <= p->Tk, "%s: need 0 < max_q <= Tq and 0 < max_k <= Tk (%d/%d, %d/%d)", who, p->max_q, p->Tq, p->max_k, p->Tk);
+  APLA_REQUIRE((p->cu_q || (long)p->S * p->max_q == p->Tq) && (p->cu_k || (long)p->S * p->max_k == p->Tk), "%s: without offsets the rows must be S x max", who);
+  APLA_REQUIRE(p->max_q <= (1 << 24) && p->max_k <= (1 << 24), "%s: sequences of at most 2^24 tokens", who);
+  APLA_REQUIRE(p->scale > 0.f && p->scale < 1e30f && p->softcap >= 0.f && p->softcap < 1e6f, "%s: need scale > 0 and 0 <= softcap < 1e6", who);
+  APLA_REQUIRE(p->q && p->k && p->v && p->o && p->lse, "%s: a pointer is missing", who);
+  APLA_REQUIRE(apla_aligned16(p->q) && apla_aligned16(p->k) && apla_aligned16(p->v) && apla_aligned16(p->o), "%s: q, k, v, o must be 16-byte aligned", who);
+  APLA_REQUIRE(p->ldq >= p->Hq * 64L && p->ldo >= p->Hq * 64L && p->ldk >= p->Hkv * 64L && p->ldv >= p->Hkv * 64L, "%s: a row stride is shorter than its heads", who);
+  APLA_REQUIRE(((p->ldq | p->ldk | p->ldv | p->ldo) & 7) == 0, "%s: row strides must be multiples of 8", who);
+  APLA_REQUIRE((!p->doc_q) == (!p->doc_k), "%s: document ids are needed for queries and keys", who);
+  APLA_REQUIRE(p->pos_dim >= 0 && p->pos_dim <= 2 && (p->pos_dim == 0 ? !p->pos_q && !p->pos_k : p->pos_q && p->pos_k && p->slopes), "%s: positions need slopes, both sides and 1 or 2 coordinates", who);
+  APLA_REQUIRE(!p->prefix || p->causal, "%s: a prefix needs the causal mask", who);
+  if (backward) {
+    APLA_REQUIRE(p->d_o && p->dq && p->dk && p->dv && p->delta, "%s: a pointer is missing", who);
+    APLA_REQUIRE(apla_aligned16(p->d_o) && apla_aligned16(p->dq) && apla_aligned16(p->dk) && apla_aligned16(p->dv), "%s: d_o, dq, dk, dv must be 16-byte aligned", who);
+    APLA_REQUIRE(p->lddo >= p->Hq * 64L && p->lddq >= p->Hq * 64L && p->lddk >= p->Hkv * 64L && p->lddv >= p->Hkv * 64L && ((p->lddo | p->lddq | p->lddk | p->lddv) & 7) == 0,
+                 "%s: gradient row strides must cover their heads and be multiples of 8", who);
+  }
+  const Plan pl = plan_of(*p, backward);
+  APLA_REQUIRE(pl.bytes == 0 || (p->workspace && apla_aligned16(p->workspace) && p->workspace_bytes >= pl.bytes), "%s: needs %ld bytes of 16-byte aligned workspace (got %ld)", who, pl.bytes, p->workspace_bytes);
+  const long nb = (long)p->S * p->Hq * (((long)(p->max_q > p->max_k ? p->max_q : p->max_k) + 127) / 128);
+  APLA_REQUIRE(nb < (1L << 31), "%s: too many blocks", who);
+  return APLA_OK;
+}
+
+ModArgs mod_args(const apla_attn_mod_t& p, const Plan& pl) {
+  ModArgs a = {};
+  a.q = (const bf16*)p.q; a.k = (const bf16*)p.k; a.v = (const bf16*)p.v; a.ldq = p.ldq; a.ldk = p.ldk; a.ldv = p.ldv;
+  a.o = (bf16*)p.o; a.ldo = p.ldo; a.lse = p.lse;
+  a.cu_q = p.cu_q; a.cu_k = p.cu_k; a.len_k = p.len_k; a.prefix = p.prefix; a.doc_q = p.doc_q; a.doc_k = p.doc_k;
+  a.slopes = p.slopes; a.pos_q = p.pos_q; a.pos_k = p.pos_k;
+  a.S = p.S; a.Tq = p.Tq; a.Tk = p.Tk; a.max_q = p.max_q; a.max_k = p.max_k; a.Hq = p.Hq; a.G = p.Hq / p.Hkv; a.causal = p.causal;
+  a.scale = p.scale; a.c = p.scale * LOG2E;
+  if (p.softcap > 0.f) { a.k1 = 2.f * p.scale * LOG2E / p.softcap; a.kx = p.scale / p.softcap; a.A = p.softcap * LOG2E; }
+  a.nt_q = (p.max_q + 63) / 64; a.nt_k = (p.max_k + 63) / 64;
+  char* ws = (char*)p.workspace;
+  if (p.doc_k) { a.rng_k = (const int2*)(ws + pl.rng_k); a.rng_q = (const int2*)(ws + pl.rng_q); }
+  a.nsplit = pl.nsplit; a.chunk = pl.chunk; a.nrt = pl.nrt;
+  a.part_o = (float*)(ws + pl.part);
+  a.part_ml = a.part_o + (long)p.S * p.Hkv * pl.nrt * pl.nsplit * 32 * 64;
+  a.d_o = (const bf16*)p.d_o; a.lddo = p.lddo; a.dq = (bf16*)p.dq; a.dk = (bf16*)p.dk; a.dv = (bf16*)p.dv;
+  a.lddq = p.lddq; a.lddk = p.lddk; a.lddv = p.lddv; a.delta = p.delta;
+  return a;
+}
+
+void launch_ranges(const ModArgs& a, bool queries, hipStream_t stream) {
+  const int nt = queries ? a.nt_q : a.nt_k;
+  hipLaunchKernelGGL(attn_mod_ranges_kernel, dim3((unsigned)(((long)a.S * nt + 3) / 4)), dim3(256), 0, stream, a, queries ? 1 : 0, (int2*)(queries ? a.rng_q : a.rng_k), nt);
+}
+
+// KERNEL<cap?, 0 no bias | 1 distance on a line | 2 on a plane>
+#define APLA_MOD_LAUNCH(KERNEL, grid)                                                                             \
+  do {                                                                                                            \
+    const int bias_ = !p->slopes ? 0 : p->pos_dim == 2 ? 2 : 1;                                                   \
+    if (p->softcap > 0.f) {                                                                                       \
+      if (bias_ == 0) hipLaunchKernelGGL((KERNEL<true, 0>), grid, dim3(256), 0, stream, a);                       \
+      else if (bias_ == 1) hipLaunchKernelGGL((KERNEL<true, 1>), grid, dim3(256), 0, stream, a);                  \
+      else hipLaunchKernelGGL((KERNEL<true, 2>), grid, dim3(256), 0, stream, a);                                  \
+    } else {                                                                                                      \
+      if (bias_ == 0) hipLaunchKernelGGL((KERNEL<false, 0>), grid, dim3(256), 0, stream, a);                      \
+      else if (bias_ == 1) hipLaunchKernelGGL((KERNEL<false, 1>), grid, dim3(256), 0, stream, a);                 \
+      else hipLaunchKernelGGL((KERNEL<false, 2>), grid, dim3(256), 0, stream, a);                                 \
+    }                                                                                                             \
+  } while (0)
+
+}  // namespace
+
+extern "C" long apla_attn_mod_workspace_bytes(const apla_attn_mod_t* p, int backward) {
+  if (!p || p->S <= 0 || p->Hq <= 0 || p->Hkv <= 0 || p->Hq % p->Hkv || p->max_q <= 0 || p->max_k <= 0) return -1;
+  return plan_of(*p, backward != 0).bytes;
+}
+
+extern "C" int apla_attn_mod_fwd(const apla_attn_mod_t* p, hipStream_t stream) {
+  const int rc = mod_check("apla_attn_mod_fwd", p, false);
+  if (rc != APLA_OK) return rc;
+  const Plan pl = plan_of(*p, false);
+  ModArgs a = mod_args(*p, pl);
+  if (a.doc_k) launch_ranges(a, false, stream);
+  if (pl.rows) {
+    const dim3 grid((unsigned)(pl.nrt * pl.nsplit), (unsigned)p->Hkv, (unsigned)p->S);
+    APLA_MOD_LAUNCH(attn_mod_rows_kernel, grid);
+    if (pl.nsplit > 1) hipLaunchKernelGGL(attn_mod_join_kernel, dim3((unsigned)pl.nrt, (unsigned)p->Hkv, (unsigned)p->S), dim3(256), 0, stream, a);
+  } else {
+    a.nblk = (p->max_q + 127) / 128;
+    const dim3 grid((unsigned)((long)p->S * p->Hq * a.nblk));
+    APLA_MOD_LAUNCH(attn_mod_fwd_kernel, grid);
+  }
+  APLA_CHECK_LAUNCH("apla_attn_mod_fwd");
+  return APLA_OK;
+}
+
+extern "C" int apla_attn_mod_bwd(const apla_attn_mod_t* p, hipStream_t stream) {
+  const int rc = mod_check("apla_attn_mod_bwd", p, true);
+  if (rc != APLA_OK) return rc;
+  const Plan pl = plan_of(*p, true);
+  ModArgs a = mod_args(*p, pl);
+  if (a.doc_k) { launch_ranges(a, false, stream); launch_ranges(a, true, stream); }
+  a.nblk = (p->max_q + 127) / 128;
+  {
+    const dim3 grid((unsigned)((long)p->S * p->Hq * a.nblk));
+    APLA_MOD_LAUNCH(attn_mod_dq_kernel, grid);
+  }
+  a.nblk = (p->max_k + 127) / 128;
+  {
+    const dim3 grid((unsigned)((long)p->S * p->Hkv * a.nblk));
+    APLA_MOD_LAUNCH(attn_mod_dkdv_kernel, grid);
+  }
+  APLA_CHECK_LAUNCH("apla_attn_mod_bwd");
+  return APLA_OK;
+}

@@ -1,0 +1,329 @@
+// Rotary positions and the per-head norm of queries and keys (head_dim 64): forward and backward, memory bound.
+//
+// A head row is 64 x 16 bit = 128 bytes: eight lanes with 16 bytes each, so every load and store instruction of a wave moves eight whole
+// lines.  The eight lane groups of a wave are hb heads of 8 / hb tokens (hb the largest of 8, 4, 2, 1 that divides the head counts:
+// no lane idles, a wave's groups sit next to each other in the row), and a wave walks the heads of its tokens, so that the
+// cosines and sines are loaded once per token and lane and not once per head.
+//
+// Rotation of the pair (a, b) by theta: a' = a cos - b sin, b' = b cos + a sin.  "interleaved": the pair is (2i, 2i+1), both in one
+// lane.  "half": (i, i + rot/2), exchanged as fp32 through the wave's own 2 KB of LDS (rot may be any even number: neither a lane nor a
+// 16-byte boundary; no barrier, a wave's LDS operations run in order).  The inverse rotation is the same with -sin: the backward pass.
+// cos / sin come from a fp32 table built in 64 bits (angles of far positions lose 2^-24 * position in fp32 arithmetic).
+//
+// Norm backward, g = R^T dy, u = g w, x^ = (x - mean) rstd:  dx = rstd (u - mean(u) - x^ mean(u x^))  (RMS: without mean(u));
+// dw = sum g x^, db = sum g over tokens and heads.  The statistics are recomputed from x (it has to be read for x^ anyway).
+// All arithmetic is fp32; the only rounding is that of the stored result.
+#include "common.h"
+
+namespace {
+
+struct RotArgs {
+  const bf16* x; long ldx;       // rotated / normalised rows [T, (h1 + h2) * 64]
+  const bf16* dy; long lddy;     // backward: incoming gradient of the result
+  bf16* y; long ldy;             // result, or dx
+  int T, nb1, nb, hbl;           // head blocks of the first group (queries), of both; log2 of heads per block
+  const float* table; int P, rot, interleaved;
+  const int32_t* pos; int seq_len;
+  float sign, eps;
+  const float *qw, *kw, *qb, *kb;
+  float* partial;                // [workgroups][4][64]: dqw, dkw, dqb, dkb
+  int bpy;                       // head blocks per blockIdx.y
+};
+
+__device__ __forceinline__ float group8_sum(float v) {
+  v += __shfl_xor(v, 1, 64);
+  v += __shfl_xor(v, 2, 64);
+  v += __shfl_xor(v, 4, 64);
+  return v;
+}
+__device__ __forceinline__ void unpack8(const bf16x8& r, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (float)r[e];
+}
+
+// v: this lane's 8 elements of a head row (e0 = 8 * lane-in-group); cs / sn: cosine and signed sine of each element (1 / 0 past rot)
+__device__ __forceinline__ void rotate8(float (&v)[8], const float (&cs)[8], const float (&sn)[8], int interleaved, int r, int e0, float* xch) {
+  float pr[8];
+  if (interleaved) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) pr[e] = v[e ^ 1];
+  } else {
+    *(f32x4*)(xch + e0) = f32x4{v[0], v[1], v[2], v[3]};
+    *(f32x4*)(xch + e0 + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+    if ((r & 3) == 0) {          // four-element groups never straddle a boundary
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int e = e0 + 4 * h, p = e < r ? e + r : e < 2 * r ? e - r : e;
+        const f32x4 t = *(const f32x4*)(xch + p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pr[4 * h + i] = t[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int e = e0 + i, p = e < r ? e + r : e < 2 * r ? e - r : e;
+        pr[i] = xch[p];
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = e0 + e < 2 * r ? v[e] * cs[e] + pr[e] * sn[e] : v[e];
+}
+
+// NORM: 0 none, 1 LayerNorm, 2 RMS.
+template <int NORM, bool BWD, bool PAR>
+__global__ __launch_bounds__(256) void rotary_kernel(RotArgs a) {
+  __shared__ __attribute__((aligned(16))) float xch_all[4][8][68];
+  __shared__ float red[PAR ? 4 : 1][256];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int g = lane >> 3, e0 = (lane & 7) * 8;
+  const int hb = 1 << a.hbl, sub = g & (hb - 1), tsub = g >> a.hbl, tpw = 8 >> a.hbl;
+  float* xch = xch_all[wave][g];
+  const int r = a.rot >> 1;
+  const int b0 = blockIdx.y * a.bpy, b1 = min(a.nb, b0 + a.bpy);
+  float w[2][8], bi[2][8];
+  if constexpr (NORM != 0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      w[0][e] = a.qw ? a.qw[e0 + e] : 1.f; w[1][e] = a.kw ? a.kw[e0 + e] : 1.f;
+      bi[0][e] = a.qb ? a.qb[e0 + e] : 0.f; bi[1][e] = a.kb ? a.kb[e0 + e] : 0.f;
+    }
+  }
+  float aw[2][8], ab[2][8];
+  if constexpr (PAR) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { aw[0][e] = aw[1][e] = ab[0][e] = ab[1][e] = 0.f; }
+  }
+  for (long tb = ((long)blockIdx.x * 4 + wave) * tpw; tb < a.T; tb += (long)gridDim.x * 4 * tpw) {
+    const bool tv = tb + tsub < a.T;
+    const long t = tv ? tb + tsub : a.T - 1;
+    float cs[8], sn[8];
+    if (r > 0) {
+      long p = a.pos ? (long)a.pos[t] : a.seq_len ? t % a.seq_len : t;
+      const bool pv = p >= 0 && p < a.P;      // a position outside the table gives NaN, not a read outside it
+      const float* row = a.table + (pv ? p : 0) * a.rot;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int el = e0 + e;
+        const bool in = el < 2 * r;
+        const int idx = !in ? 0 : a.interleaved ? el >> 1 : el < r ? el : el - r;
+        const bool first = a.interleaved ? !(el & 1) : el < r;
+        const float s = row[r + idx] * a.sign;
+        cs[e] = pv ? row[idx] : __builtin_nanf("");
+        sn[e] = first ? -s : s;
+      }
+    }
+    const bf16* xr = a.x + t * a.ldx + sub * 64 + e0;
+    const bf16* dr = BWD ? a.dy + t * a.lddy + sub * 64 + e0 : nullptr;
+    bf16* yr = a.y + t * a.ldy + sub * 64 + e0;
+    bf16x8 nx, nd;
+    if (b0 < b1) {
+      nx = *(const bf16x8*)(xr + (long)b0 * hb * 64);
+      if constexpr (BWD) nd = *(const bf16x8*)(dr + (long)b0 * hb * 64);
+    }
+    for (int b = b0; b < b1; ++b) {
+      float v[8], d[8];
+      unpack8(nx, v);
+      if constexpr (BWD) unpack8(nd, d);
+      if (b + 1 < b1) {
+        nx = *(const bf16x8*)(xr + (long)(b + 1) * hb * 64);
+        if constexpr (BWD) nd = *(const bf16x8*)(dr + (long)(b + 1) * hb * 64);
+      }
+      float rs = 1.f;
+      if constexpr (NORM != 0) {
+        if constexpr (NORM == 1) {
+          float m = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) m += v[e];
+          m = group8_sum(m) * (1.f / 64.f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] -= m;
+        }
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += v[e] * v[e];
+        rs = rsqrtf(group8_sum(s) * (1.f / 64.f) + a.eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= rs;       // x^
+      }
+      const bool isk = b >= a.nb1;                    // the same for the whole wave
+      if constexpr (!BWD) {
+        if constexpr (NORM != 0) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = isk ? v[e] * w[1][e] + bi[1][e] : v[e] * w[0][e] + bi[0][e];
+        }
+        if (r > 0) rotate8(v, cs, sn, a.interleaved, r, e0, xch);
+      } else {
+        if (r > 0) rotate8(d, cs, sn, a.interleaved, r, e0, xch);
+        if constexpr (PAR) {
+          if (tv) {
+            if (isk) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) { aw[1][e] += d[e] * v[e]; ab[1][e] += d[e]; }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) { aw[0][e] += d[e] * v[e]; ab[0][e] += d[e]; }
+            }
+          }
+        }
+        float m1 = 0.f, m2 = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          d[e] *= isk ? w[1][e] : w[0][e];
+          m1 += d[e];
+          m2 += d[e] * v[e];
+        }
+        m1 = NORM == 1 ? group8_sum(m1) * (1.f / 64.f) : 0.f;
+        m2 = group8_sum(m2) * (1.f / 64.f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = rs * (d[e] - m1 - v[e] * m2);
+      }
+      if (tv) {
+        bf16x8 out;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[e] = (bf16)v[e];
+        *(bf16x8*)(yr + (long)b * hb * 64) = out;
+      }
+    }
+  }
+  if constexpr (PAR) {     // lanes of the same columns (8 groups), then the four waves, in a fixed order
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float u = aw[k][e], v = ab[k][e];
+#pragma unroll
+        for (int o = 8; o < 64; o <<= 1) { u += __shfl_xor(u, o, 64); v += __shfl_xor(v, o, 64); }
+        if (g == 0) { red[wave][k * 64 + e0 + e] = u; red[wave][128 + k * 64 + e0 + e] = v; }
+      }
+    __syncthreads();
+    const int i = threadIdx.x;
+    a.partial[((long)blockIdx.y * gridDim.x + blockIdx.x) * 256 + i] = red[0][i] + red[1][i] + red[2][i] + red[3][i];
+  }
+}
+
+// out[256] = column sums of partial[G][256]: 16 columns per workgroup, 16 row walkers each, summed in a fixed order
+__global__ __launch_bounds__(256) void rotary_param_sum_kernel(const float* __restrict__ partial, int G, float* __restrict__ out) {
+  __shared__ float red[16][17];
+  const int c = threadIdx.x & 15, w = threadIdx.x >> 4, col = blockIdx.x * 16 + c;
+  float s = 0.f;
+  for (int i = w; i < G; i += 16) s += partial[(long)i * 256 + col];
+  red[w][c] = s;
+  __syncthreads();
+  if (w == 0) {
+    for (int i = 1; i < 16; ++i) s += red[i][c];
+    out[col] = s;
+  }
+}
+
+constexpr int PARAM_WGS = 1024;     // at most this many partial sums of the norm parameters (1 MB)
+
+struct RotGrid { unsigned x, y; int hbl, bpy; };
+// Head blocks of hb heads; a wave takes all blocks of its tokens where that still leaves 4096 waves (16 per CU: the table values are
+// then loaded once per token), else the blocks are spread over blockIdx.y.
+RotGrid rot_grid(int T, int h1, int h2, bool par) {
+  RotGrid g;
+  int hbl = 3;
+  while (hbl && ((h1 | h2) & ((1 << hbl) - 1))) --hbl;
+  const long waves = ((long)T + (8 >> hbl) - 1) / (8 >> hbl);
+  const int nb = (h1 + h2) >> hbl;
+  long bpy = (long)nb * waves / 4096;
+  bpy = bpy < 1 ? 1 : bpy > nb ? nb : bpy;
+  g.hbl = hbl;
+  g.bpy = (int)bpy;
+  g.y = (unsigned)((nb + bpy - 1) / bpy);
+  long gx = (waves + 3) / 4;
+  if (par && gx * g.y > PARAM_WGS) gx = PARAM_WGS / g.y > 0 ? PARAM_WGS / g.y : 1;
+  g.x = (unsigned)gx;
+  return g;
+}
+
+int rot_check(const char* who, int T, int h1, int h2, const float* table, int P, int rot, int layout, const int32_t* pos, int seq_len) {
+  APLA_REQUIRE(T > 0 && h1 >= 0 && h2 >= 0 && h1 + h2 > 0 && h1 + h2 <= 1024, "%s: need T > 0 and 1..1024 heads (T=%d heads=%d+%d)", who, T, h1, h2);
+  APLA_REQUIRE(rot >= 0 && rot <= 64 && rot % 2 == 0 && (rot == 0 || (table && P > 0)), "%s: rot must be even, 0..64, with a table (rot=%d P=%d)", who, rot, P);
+  APLA_REQUIRE(layout == APLA_ROT_HALF || layout == APLA_ROT_INTERLEAVED, "%s: unknown layout %d", who, layout);
+  APLA_REQUIRE(seq_len >= 0 && (rot == 0 || pos || (seq_len ? seq_len : T) <= P), "%s: positions 0..%d without `pos` do not fit a table of %d rows", who,
+               (seq_len ? seq_len : T) - 1, P);
+  return APLA_OK;
+}
+int rows_check(const char* who, const char* name, const void* p, long ld, int heads) {
+  APLA_REQUIRE(p && apla_aligned16(p) && ld >= heads * 64L && ld % 8 == 0, "%s: %s must be 16-byte aligned with a row stride >= %d that is a multiple of 8 (got %ld)",
+               who, name, heads * 64, ld);
+  return APLA_OK;
+}
+
+}  // namespace
+
+extern "C" int apla_rotary(const void* x, long ldx, void* y, long ldy, int T, int heads, const float* table, int P, int rot, int layout,
+                           const int32_t* pos, int seq_len, int inverse, hipStream_t stream) {
+  int rc = rot_check("apla_rotary", T, heads, 0, table, P, rot, layout, pos, seq_len);
+  if (rc == APLA_OK) rc = rows_check("apla_rotary", "x", x, ldx, heads);
+  if (rc == APLA_OK) rc = rows_check("apla_rotary", "y", y, ldy, heads);
+  if (rc != APLA_OK) return rc;
+  const RotGrid g = rot_grid(T, heads, 0, false);
+  RotArgs a = {};
+  a.x = (const bf16*)x; a.ldx = ldx; a.y = (bf16*)y; a.ldy = ldy; a.T = T; a.hbl = g.hbl; a.nb1 = a.nb = heads >> g.hbl;
+  a.table = table; a.P = P; a.rot = rot; a.interleaved = layout == APLA_ROT_INTERLEAVED; a.pos = pos; a.seq_len = seq_len;
+  a.sign = inverse ? -1.f : 1.f; a.bpy = g.bpy;
+  hipLaunchKernelGGL((rotary_kernel<0, false, false>), dim3(g.x, g.y), dim3(256), 0, stream, a);
+  APLA_CHECK_LAUNCH("apla_rotary");
+  return APLA_OK;
+}
+
+extern "C" long apla_qk_norm_rotary_workspace_bytes(void) { return (long)PARAM_WGS * 256 * 4; }
+
+extern "C" int apla_qk_norm_rotary_fwd(const void* x, long ldx, void* y, long ldy, int T, int Hq, int Hkv, int norm, float eps, const float* qw,
+                                       const float* kw, const float* qb, const float* kb, const float* table, int P, int rot, int layout,
+                                       const int32_t* pos, int seq_len, hipStream_t stream) {
+  int rc = rot_check("apla_qk_norm_rotary_fwd", T, Hq, Hkv, table, P, rot, layout, pos, seq_len);
+  if (rc == APLA_OK) rc = rows_check("apla_qk_norm_rotary_fwd", "x", x, ldx, Hq + Hkv);
+  if (rc == APLA_OK) rc = rows_check("apla_qk_norm_rotary_fwd", "y", y, ldy, Hq + Hkv);
+  if (rc != APLA_OK) return rc;
+  APLA_REQUIRE((norm == APLA_NORM_LAYER || norm == APLA_NORM_RMS) && eps >= 0.f, "apla_qk_norm_rotary_fwd: unknown norm %d or eps < 0", norm);
+  const RotGrid g = rot_grid(T, Hq, Hkv, false);
+  RotArgs a = {};
+  a.x = (const bf16*)x; a.ldx = ldx; a.y = (bf16*)y; a.ldy = ldy; a.T = T; a.hbl = g.hbl; a.nb1 = Hq >> g.hbl; a.nb = (Hq + Hkv) >> g.hbl;
+  a.table = table; a.P = P; a.rot = rot; a.interleaved = layout == APLA_ROT_INTERLEAVED; a.pos = pos; a.seq_len = seq_len;
+  a.sign = 1.f; a.eps = eps; a.qw = qw; a.kw = kw; a.qb = qb; a.kb = kb; a.bpy = g.bpy;
+  if (norm == APLA_NORM_LAYER) hipLaunchKernelGGL((rotary_kernel<1, false, false>), dim3(g.x, g.y), dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((rotary_kernel<2, false, false>), dim3(g.x, g.y), dim3(256), 0, stream, a);
+  APLA_CHECK_LAUNCH("apla_qk_norm_rotary_fwd");
+  return APLA_OK;
+}
+
+extern "C" int apla_qk_norm_rotary_bwd(const void* dy, long lddy, const void* x, long ldx, void* dx, long lddx, int T, int Hq, int Hkv, int norm,
+                                       float eps, const float* qw, const float* kw, const float* table, int P, int rot, int layout,
+                                       const int32_t* pos, int seq_len, float* dparams, void* workspace, long workspace_bytes, hipStream_t stream) {
+  int rc = rot_check("apla_qk_norm_rotary_bwd", T, Hq, Hkv, table, P, rot, layout, pos, seq_len);
+  if (rc == APLA_OK) rc = rows_check("apla_qk_norm_rotary_bwd", "dy", dy, lddy, Hq + Hkv);
+  if (rc == APLA_OK) rc = rows_check("apla_qk_norm_rotary_bwd", "x", x, ldx, Hq + Hkv);
+  if (rc == APLA_OK) rc = rows_check("apla_qk_norm_rotary_bwd", "dx", dx, lddx, Hq + Hkv);
+  if (rc != APLA_OK) return rc;
+  APLA_REQUIRE((norm == APLA_NORM_LAYER || norm == APLA_NORM_RMS) && eps >= 0.f, "apla_qk_norm_rotary_bwd: unknown norm %d or eps < 0", norm);
+  APLA_REQUIRE(!dparams || (workspace && workspace_bytes >= apla_qk_norm_rotary_workspace_bytes()), "apla_qk_norm_rotary_bwd: parameter gradients need %ld bytes of workspace (got %ld)",
+               apla_qk_norm_rotary_workspace_bytes(), workspace_bytes);
+  const RotGrid g = rot_grid(T, Hq, Hkv, dparams != nullptr);
+  RotArgs a = {};
+  a.dy = (const bf16*)dy; a.lddy = lddy; a.x = (const bf16*)x; a.ldx = ldx; a.y = (bf16*)dx; a.ldy = lddx; a.T = T; a.hbl = g.hbl;
+  a.nb1 = Hq >> g.hbl; a.nb = (Hq + Hkv) >> g.hbl;
+  a.table = table; a.P = P; a.rot = rot; a.interleaved = layout == APLA_ROT_INTERLEAVED; a.pos = pos; a.seq_len = seq_len;
+  a.sign = -1.f; a.eps = eps; a.qw = qw; a.kw = kw; a.bpy = g.bpy; a.partial = (float*)workspace;
+  const dim3 grid(g.x, g.y);
+  if (norm == APLA_NORM_LAYER) {
+    if (dparams) hipLaunchKernelGGL((rotary_kernel<1, true, true>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((rotary_kernel<1, true, false>), grid, dim3(256), 0, stream, a);
+  } else {
+    if (dparams) hipLaunchKernelGGL((rotary_kernel<2, true, true>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((rotary_kernel<2, true, false>), grid, dim3(256), 0, stream, a);
+  }
+  APLA_CHECK_LAUNCH("apla_qk_norm_rotary_bwd");
+  if (dparams) {
+    hipLaunchKernelGGL(rotary_param_sum_kernel, dim3(16), dim3(256), 0, stream, (const float*)workspace, (int)(g.x * g.y), dparams);
+    APLA_CHECK_LAUNCH("apla_qk_norm_rotary_bwd");
+  }
+  return APLA_OK;
+}

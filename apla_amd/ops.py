@@ -651,6 +651,340 @@ def attn_probs(qkv: torch.Tensor, lse: torch.Tensor, B: int, N: int, H: int, sca
     return attn
 
 
+# ------------------------------------------------------------------------------------------------ rotary positions, norm of q and k
+ROT_LAYOUTS = {"half": 0, "interleaved": 1}
+QK_NORMS = {"layer": 1, "rms": 2}
+
+
+def _strided_rows(t: torch.Tensor, name: str, cols: int, rows: Optional[int] = None):
+    """A [rows, cols] 16-bit matrix whose rows may lie apart (column slices of a fused activation); returns its row stride."""
+    _req(t, half(), name, 2)
+    if t.shape[1] != cols or (rows is not None and t.shape[0] != rows):
+        raise ValueError(f"{name}: expected [{'T' if rows is None else rows}, {cols}], got {tuple(t.shape)}")
+    ld = cols if t.shape[0] <= 1 else t.stride(0)
+    if ld < cols or ld % 8 or t.data_ptr() % 16:
+        raise ValueError(f"{name}: rows must be 16-byte aligned, apart by a multiple of 8 elements and not overlap (row stride {t.stride(0)})")
+    return ld
+
+
+def _on_device(first: torch.Tensor, *others):
+    """Device guard + stream of `first`'s device; every other tensor (or None) must live there too."""
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on {first.device} and {t.device}")
+    return torch.cuda.device(first.device)
+
+
+def _aux(t: Optional[torch.Tensor], dtype, name: str, shape):
+    """An optional side array: contiguous, of one dtype and shape (None entries of `shape` are free)."""
+    if t is None:
+        return None
+    _req(t, dtype, name, len(shape))
+    if not t.is_contiguous() or any(w is not None and n != w for n, w in zip(t.shape, shape)):
+        raise ValueError(f"{name}: expected a contiguous {shape}, got {tuple(t.shape)}")
+    return t
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Do two row-strided matrices touch the same bytes?  Column slices of one buffer with the same row stride may interleave."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    sa, sb = a.data_ptr(), b.data_ptr()
+    ea = sa + ((a.shape[0] - 1) * a.stride(0) + a.shape[1]) * a.element_size()
+    eb = sb + ((b.shape[0] - 1) * b.stride(0) + b.shape[1]) * b.element_size()
+    if ea <= sb or eb <= sa:
+        return False
+    pitch = a.stride(0) * a.element_size()
+    if a.stride(0) == b.stride(0):
+        d = (sb - sa) % pitch
+        return d < a.shape[1] * a.element_size() or d + b.shape[1] * b.element_size() > pitch
+    return True
+
+
+def _rot_table(table, rows, pos, seq_len: int, layout: str, who: str):
+    if layout not in ROT_LAYOUTS:
+        raise ValueError(f"{who}: layout must be one of {sorted(ROT_LAYOUTS)}, got {layout!r}")
+    if table is None:
+        if pos is not None or seq_len:
+            raise ValueError(f"{who}: positions without a table")
+        return 0, 0
+    _aux(table, torch.float32, "table", (None, None))
+    P, rot = table.shape
+    if rot % 2 or not 2 <= rot <= 64 or P < 1:
+        raise ValueError(f"{who}: the table is [positions, rot] with rot even, 2..64; got {tuple(table.shape)}")
+    _aux(pos, torch.int32, "pos", (rows,))
+    if seq_len < 0 or (pos is None and (seq_len or rows) > P):
+        raise ValueError(f"{who}: {seq_len or rows} positions do not fit a table of {P}")
+    return P, rot
+
+
+def _rotary(x, table, heads: int, layout, pos, seq_len: int, out, inverse: bool, who: str):
+    ldx = _strided_rows(x, "x", heads * 64)
+    T = x.shape[0]
+    if table is None:
+        raise ValueError(f"{who}: no table")
+    P, rot = _rot_table(table, T, pos, seq_len, layout, who)
+    with _on_device(x, table, pos, out):
+        if out is None:
+            out = torch.empty(T, heads * 64, device=x.device, dtype=x.dtype)
+        ldo = _strided_rows(out, "out", heads * 64, T)
+        if T == 0:
+            return out
+        if _overlap(x, out) and (x.data_ptr() != out.data_ptr() or ldx != ldo):
+            raise ValueError(f"{who}: out may be x itself, not another view of the same memory")
+        check(lib().apla_rotary(x.data_ptr(), ldx, out.data_ptr(), ldo, T, heads, table.data_ptr(), P, rot, ROT_LAYOUTS[layout], _ptr(pos),
+                                seq_len, int(inverse), _stream()), "apla_rotary")
+    return out
+
+
+def rotary_fwd(x: torch.Tensor, table: torch.Tensor, heads: int, *, layout: str = "half", pos: Optional[torch.Tensor] = None, seq_len: int = 0,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotary positions on [T, heads*64] rows (a column slice of fused qkv rows is fine; ``out`` may be ``x``): the first ``rot`` values of
+    every head turned by the angles of table row pos[t] (int32 [T]), or t % seq_len, or t.  ``table``: fp32 [P, rot], cosines then
+    sines (apla_amd.rotary.rotary_table).  A ``pos`` outside the table gives NaN in its row (include/apla_hip.h: apla_rotary)."""
+    return _rotary(x, table, heads, layout, pos, seq_len, out, False, "rotary_fwd")
+
+
+def rotary_bwd(dy: torch.Tensor, table: torch.Tensor, heads: int, *, layout: str = "half", pos: Optional[torch.Tensor] = None, seq_len: int = 0,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The gradient of rotary_fwd with respect to x: dy turned back."""
+    return _rotary(dy, table, heads, layout, pos, seq_len, out, True, "rotary_bwd")
+
+
+def _qk_params(norm, eps, params, who):
+    if norm not in QK_NORMS:
+        raise ValueError(f"{who}: norm must be one of {sorted(QK_NORMS)}, got {norm!r}")
+    if not eps >= 0:
+        raise ValueError(f"{who}: eps must not be negative")
+    for n, p in params.items():
+        _aux(p, torch.float32, n, (64,))
+
+
+def _qk_rows(t, name, Hq, Hkv, rows=None):
+    """qkv rows [T, >= (Hq + Hkv) * 64] -> (their query / key columns, row stride)."""
+    _req(t, half(), name, 2)
+    if Hq < 1 or Hkv < 0:
+        raise ValueError(f"{name}: bad head counts {Hq}, {Hkv}")
+    n = (Hq + Hkv) * 64
+    if t.shape[1] < n:
+        raise ValueError(f"{name}: rows of {t.shape[1]} values do not hold {Hq} + {Hkv} heads of 64")
+    t = t[:, :n]
+    return t, _strided_rows(t, name, n, rows)
+
+
+def qk_norm_rotary_fwd(qkv: torch.Tensor, Hq: int, Hkv: int, *, norm: str = "layer", q_weight=None, k_weight=None, q_bias=None, k_bias=None,
+                       eps: float = 1e-6, table: Optional[torch.Tensor] = None, layout: str = "half", pos: Optional[torch.Tensor] = None,
+                       seq_len: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Norm of every query and key head ("layer" or "rms", fp32 [64] weights / biases, None = 1 / 0) and the rotation of rotary_fwd in one
+    pass.  ``qkv``: rows that begin with Hq query and Hkv key heads of 64 (what follows is not read).  Returns [T, (Hq+Hkv)*64]."""
+    x, ldx = _qk_rows(qkv, "qkv", Hq, Hkv)
+    T, n = x.shape
+    P, rot = _rot_table(table, T, pos, seq_len, layout, "qk_norm_rotary_fwd")
+    _qk_params(norm, eps, dict(q_weight=q_weight, k_weight=k_weight, q_bias=q_bias, k_bias=k_bias), "qk_norm_rotary_fwd")
+    with _on_device(x, table, pos, out, q_weight, k_weight, q_bias, k_bias):
+        if out is None:
+            out = torch.empty(T, n, device=x.device, dtype=x.dtype)
+        ldo = _strided_rows(out, "out", n, T)
+        if T == 0:
+            return out
+        if _overlap(x, out) and (x.data_ptr() != out.data_ptr() or ldx != ldo):
+            raise ValueError("qk_norm_rotary_fwd: out may be the query / key columns themselves, not another view of the same memory")
+        check(lib().apla_qk_norm_rotary_fwd(x.data_ptr(), ldx, out.data_ptr(), ldo, T, Hq, Hkv, QK_NORMS[norm], float(eps), _ptr(q_weight),
+                                            _ptr(k_weight), _ptr(q_bias), _ptr(k_bias), _ptr(table), P, rot, ROT_LAYOUTS[layout], _ptr(pos),
+                                            seq_len, _stream()), "apla_qk_norm_rotary_fwd")
+    return out
+
+
+def qk_norm_rotary_bwd(dqk: torch.Tensor, qkv: torch.Tensor, Hq: int, Hkv: int, *, norm: str = "layer", q_weight=None, k_weight=None, q_bias=None,
+                       k_bias=None, eps: float = 1e-6, table: Optional[torch.Tensor] = None, layout: str = "half",
+                       pos: Optional[torch.Tensor] = None, seq_len: int = 0, out: Optional[torch.Tensor] = None, want_params: bool = True):
+    """Gradients of qk_norm_rotary_fwd: (d of the query / key columns [T, (Hq+Hkv)*64], fp32 [4, 64] = d q_weight, d k_weight, d q_bias,
+    d k_bias, or None without ``want_params``).  ``qkv``: the forward's input; ``out`` may be columns of a fused gradient buffer."""
+    x, ldx = _qk_rows(qkv, "qkv", Hq, Hkv)
+    T, n = x.shape
+    ldd = _strided_rows(dqk, "dqk", n, T)
+    P, rot = _rot_table(table, T, pos, seq_len, layout, "qk_norm_rotary_bwd")
+    _qk_params(norm, eps, dict(q_weight=q_weight, k_weight=k_weight, q_bias=q_bias, k_bias=k_bias), "qk_norm_rotary_bwd")
+    with _on_device(x, dqk, table, pos, out, q_weight, k_weight, q_bias, k_bias):
+        if out is None:
+            out = torch.empty(T, n, device=x.device, dtype=x.dtype)
+        ldo = _strided_rows(out, "out", n, T)
+        if any(_overlap(t, out) and (t.data_ptr() != out.data_ptr() or ld != ldo) for t, ld in ((x, ldx), (dqk, ldd))):
+            raise ValueError("qk_norm_rotary_bwd: out may be dqk or the query / key columns themselves, not another view of the same memory")
+        dpar = ws = None
+        if want_params:
+            dpar = torch.empty(4, 64, device=x.device, dtype=torch.float32) if T else torch.zeros(4, 64, device=x.device)
+            ws = torch.empty(lib().apla_qk_norm_rotary_workspace_bytes() // 4, device=x.device, dtype=torch.float32)
+        if T == 0:
+            return out, dpar
+        check(lib().apla_qk_norm_rotary_bwd(dqk.data_ptr(), ldd, x.data_ptr(), ldx, out.data_ptr(), ldo, T, Hq, Hkv, QK_NORMS[norm], float(eps),
+                                            _ptr(q_weight), _ptr(k_weight), _ptr(table), P, rot, ROT_LAYOUTS[layout], _ptr(pos), seq_len,
+                                            _ptr(dpar), _ptr(ws), 0 if ws is None else ws.numel() * 4, _stream()), "apla_qk_norm_rotary_bwd")
+    return out, dpar
+
+
+# ------------------------------------------------------------------------------------------------ attention with modified scores
+class ScoreMod:
+    """What happens to the scores between scale * q k^T and the softmax (include/apla_hip.h: apla_attn_mod_fwd), in this order:
+    ``softcap``: s = softcap * tanh(s / softcap);  ``slopes`` (fp32 [Hq]): s -= slopes[h] * dist(i, j), the distance of the two places in the
+    sequence (queries aligned to the last key), or the Euclidean distance of ``pos_q`` / ``pos_k`` (fp32 [T] or [T, 1 | 2], e.g. patch
+    coordinates);  masks: ``causal`` (aligned to the last key) with ``prefix`` (int32 [S]: keys every row may see), ``doc_q`` / ``doc_k``
+    (int32 [T]: a key is seen by the rows of its own document only, negative ids by nobody)."""
+    __slots__ = ("softcap", "slopes", "pos_q", "pos_k", "doc_q", "doc_k", "causal", "prefix")
+
+    def __init__(self, softcap: float = 0.0, slopes=None, pos_q=None, pos_k=None, doc_q=None, doc_k=None, causal: bool = False, prefix=None):
+        if not 0.0 <= float(softcap) < 1e6:
+            raise ValueError(f"softcap must be 0 (none) or positive, below 1e6; got {softcap}")
+        if (pos_q is None) != (pos_k is None) or (doc_q is None) != (doc_k is None):
+            raise ValueError("positions and document ids are given for queries and keys, or for neither")
+        if pos_q is not None and slopes is None:
+            raise ValueError("positions without slopes")
+        if prefix is not None and not causal:
+            raise ValueError("a prefix needs the causal mask")
+        for n, t in (("slopes", slopes), ("pos_q", pos_q), ("pos_k", pos_k)):
+            if t is not None and t.requires_grad:
+                raise NotImplementedError(f"{n}: no gradient is computed for it")
+        self.softcap, self.slopes, self.pos_q, self.pos_k = float(softcap), slopes, pos_q, pos_k
+        self.doc_q, self.doc_k, self.causal, self.prefix = doc_q, doc_k, bool(causal), prefix
+
+
+_NO_MOD = ScoreMod()
+
+
+def _attn_mod_args(q, k, v, Hq: int, Hkv: int, scale: float, mod, batch, cu_q, cu_k, max_q, max_k, len_k, who: str):
+    """Checked geometry and masks of a modified-score attention call as an apla_attn_mod_t (outputs and workspace still empty)."""
+    m = _NO_MOD if mod is None else mod
+    if Hq < 1 or Hkv < 1 or Hq % Hkv:
+        raise ValueError(f"{who}: the {Hq} query heads must be a multiple of the {Hkv} key heads")
+    if not 0.0 < float(scale) < 1e30:
+        raise ValueError(f"{who}: scale must be positive, got {scale}")
+    a = _lib.AttnMod()
+    a.ldq, a.ldk = _strided_rows(q, "q", Hq * 64), _strided_rows(k, "k", Hkv * 64)
+    a.ldv = _strided_rows(v, "v", Hkv * 64, k.shape[0])
+    Tq, Tk = q.shape[0], k.shape[0]
+    if (cu_q is None) != (cu_k is None):
+        raise ValueError(f"{who}: offsets are given for queries and keys, or for neither")
+    if cu_q is not None:
+        if batch is not None or max_q is None or max_k is None:
+            raise ValueError(f"{who}: packed sequences take cu_q, cu_k, max_q and max_k, and no batch")
+        S = _check_cu(cu_q, Tq, who)
+        if _check_cu(cu_k, Tk, who) != S:
+            raise ValueError(f"{who}: cu_q and cu_k describe different numbers of sequences")
+        max_q, max_k = int(max_q), int(max_k)
+        if max_q < 0 or max_k < 0 or max_q > Tq or max_k > Tk:
+            raise ValueError(f"{who}: max_q / max_k lie outside 0..rows ({max_q} of {Tq}, {max_k} of {Tk})")
+    else:
+        if batch is None or max_q is not None or max_k is not None:
+            raise ValueError(f"{who}: give batch (equal sequences), or cu_q, cu_k, max_q and max_k (packed ones)")
+        S = int(batch)
+        if S < 1 or Tq % S or Tk % S:
+            raise ValueError(f"{who}: {Tq} query and {Tk} key rows are not {S} equal sequences")
+        max_q, max_k = Tq // S, Tk // S
+    if S > 65535:
+        raise ValueError(f"{who}: at most 65535 sequences, got {S}")
+    if max(max_q, max_k) > 1 << 24:
+        raise ValueError(f"{who}: sequences of at most 2^24 tokens")
+    _aux(len_k, torch.int32, "len_k", (S,)), _aux(m.prefix, torch.int32, "prefix", (S,))
+    _aux(m.slopes, torch.float32, "slopes", (Hq,))
+    _aux(m.doc_q, torch.int32, "doc_q", (Tq,)), _aux(m.doc_k, torch.int32, "doc_k", (Tk,))
+    if m.pos_q is not None:
+        a.pos_dim = 1 if m.pos_q.ndim == 1 else m.pos_q.shape[1]
+        if a.pos_dim not in (1, 2):
+            raise ValueError(f"{who}: positions have 1 or 2 coordinates")
+        for n, t, rows in (("pos_q", m.pos_q, Tq), ("pos_k", m.pos_k, Tk)):
+            _aux(t, torch.float32, n, (rows,) if t.ndim == 1 else (rows, a.pos_dim))
+        if (1 if m.pos_k.ndim == 1 else m.pos_k.shape[1]) != a.pos_dim:
+            raise ValueError(f"{who}: pos_q and pos_k have different numbers of coordinates")
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.cu_q, a.cu_k, a.len_k, a.prefix = _ptr(cu_q), _ptr(cu_k), _ptr(len_k), _ptr(m.prefix)
+    a.doc_q, a.doc_k, a.slopes, a.pos_q, a.pos_k = _ptr(m.doc_q), _ptr(m.doc_k), _ptr(m.slopes), _ptr(m.pos_q), _ptr(m.pos_k)
+    a.S, a.Tq, a.Tk, a.max_q, a.max_k, a.Hq, a.Hkv, a.causal = S, Tq, Tk, max_q, max_k, Hq, Hkv, int(m.causal)
+    a.scale, a.softcap = float(scale), m.softcap
+    return a, _on_device(q, k, v, cu_q, cu_k, len_k, m.prefix, m.doc_q, m.doc_k, m.slopes, m.pos_q, m.pos_k)
+
+
+def _mod_workspace(a, backward: bool, device):
+    """Scratch of ONE call (never shared: two captured graphs may run at once)."""
+    n = lib().apla_attn_mod_workspace_bytes(a, int(backward))
+    ws = torch.empty(max(n, 0) // 4, device=device, dtype=torch.float32) if n > 0 else None
+    a.workspace, a.workspace_bytes = _ptr(ws), max(n, 0)
+    return ws
+
+
+def attn_mod_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, Hq: int, Hkv: int, scale: float, mod: Optional[ScoreMod] = None, *,
+                 batch: Optional[int] = None, cu_q: Optional[torch.Tensor] = None, cu_k: Optional[torch.Tensor] = None, max_q: Optional[int] = None,
+                 max_k: Optional[int] = None, len_k: Optional[torch.Tensor] = None, o: Optional[torch.Tensor] = None,
+                 lse: Optional[torch.Tensor] = None):
+    """Attention with modified and masked scores (``mod``), queries and keys with lengths of their own and Hq / Hkv query heads to a key head.
+    q [Tq, Hq*64], k / v [Tk, Hkv*64]: 16-bit rows, row-strided views allowed (columns of fused qkv rows, class-token rows, a cache).
+    ``batch``: equal sequences one behind the other, of whose keys ``len_k`` (int32 [batch]) are used; or ``cu_q`` / ``cu_k`` (int32 [S+1]
+    offsets on the device) with the longest lengths ``max_q`` / ``max_k``.  Returns (o [Tq, Hq*64], lse fp32 [Hq, Tq]); a row that sees no
+    key has o = 0 and lse = -inf.  Rows behind the last packed sequence are not computed: as they were in a given ``o`` / ``lse``,
+    else 0 / -inf."""
+    a, guard = _attn_mod_args(q, k, v, Hq, Hkv, scale, mod, batch, cu_q, cu_k, max_q, max_k, len_k, "attn_mod_fwd")
+    with guard:
+        if o is None:
+            o = (torch.empty if cu_q is None else torch.zeros)(a.Tq, Hq * 64, device=q.device, dtype=half())
+        if lse is None:
+            shape = (Hq, a.Tq)
+            lse = torch.empty(shape, device=q.device) if cu_q is None else torch.full(shape, float("-inf"), device=q.device)
+        a.ldo = _strided_rows(o, "o", Hq * 64, a.Tq)
+        _aux(lse, torch.float32, "lse", (Hq, a.Tq))
+        if o.device != q.device or lse.device != q.device or any(_overlap(t, o) for t in (q, k, v)):
+            raise ValueError("attn_mod_fwd: o / lse must lie on q's device and apart from q, k, v")
+        a.o, a.lse = o.data_ptr(), lse.data_ptr()
+        if a.max_q == 0:
+            return o, lse
+        if a.max_k == 0:       # no keys at all: every computed row sees nothing
+            _zero_rows(o, cu_q, 0.0), _zero_rows(lse.t(), cu_q, float("-inf"))
+            return o, lse
+        ws = _mod_workspace(a, False, q.device)     # noqa: F841  (alive until the launch)
+        check(lib().apla_attn_mod_fwd(a, _stream()), "apla_attn_mod_fwd")
+    return o, lse
+
+
+def _zero_rows(t, cu, value):
+    if cu is None:
+        t.fill_(value)
+    else:
+        rows = torch.arange(t.shape[0], device=t.device)
+        t.masked_fill_(((rows >= cu[0]) & (rows < cu[-1]))[:, None], value)
+
+
+def attn_mod_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, do: torch.Tensor, lse: torch.Tensor, Hq: int, Hkv: int,
+                 scale: float, mod: Optional[ScoreMod] = None, *, batch: Optional[int] = None, cu_q: Optional[torch.Tensor] = None,
+                 cu_k: Optional[torch.Tensor] = None, max_q: Optional[int] = None, max_k: Optional[int] = None, len_k: Optional[torch.Tensor] = None,
+                 dq: Optional[torch.Tensor] = None, dk: Optional[torch.Tensor] = None, dv: Optional[torch.Tensor] = None):
+    """(dq, dk, dv) of attn_mod_fwd for the same arguments, its o and lse, and do [Tq, Hq*64].  Given gradient buffers may be columns of one
+    fused buffer; rows that no sequence holds (behind the last one, keys past ``len_k``) are left as they were there, else 0."""
+    a, guard = _attn_mod_args(q, k, v, Hq, Hkv, scale, mod, batch, cu_q, cu_k, max_q, max_k, len_k, "attn_mod_bwd")
+    a.ldo, a.lddo = _strided_rows(o, "o", Hq * 64, a.Tq), _strided_rows(do, "do", Hq * 64, a.Tq)
+    _aux(lse, torch.float32, "lse", (Hq, a.Tq))
+    with guard:
+        if dq is None:
+            dq = (torch.empty if cu_q is None else torch.zeros)(a.Tq, Hq * 64, device=q.device, dtype=half())
+        make = torch.empty if cu_k is None and len_k is None else torch.zeros
+        if dk is None:
+            dk = make(a.Tk, Hkv * 64, device=q.device, dtype=half())
+        if dv is None:
+            dv = make(a.Tk, Hkv * 64, device=q.device, dtype=half())
+        a.lddq, a.lddk, a.lddv = _strided_rows(dq, "dq", Hq * 64, a.Tq), _strided_rows(dk, "dk", Hkv * 64, a.Tk), _strided_rows(dv, "dv", Hkv * 64, a.Tk)
+        if any(t.device != q.device for t in (o, do, lse, dq, dk, dv)):
+            raise ValueError("attn_mod_bwd: every tensor must lie on q's device")
+        outs = (dq, dk, dv)
+        if any(_overlap(t, g) for t in (q, k, v, o, do) for g in outs) or any(_overlap(outs[i], outs[j]) for i in range(3) for j in range(i)):
+            raise ValueError("attn_mod_bwd: the gradients must lie apart from the operands and from each other")
+        if a.max_q == 0 or a.max_k == 0:
+            _zero_rows(dq, cu_q, 0.0), _zero_rows(dk, cu_k, 0.0), _zero_rows(dv, cu_k, 0.0)
+            return dq, dk, dv
+        delta = torch.empty(Hq, a.Tq, device=q.device, dtype=torch.float32)
+        a.o, a.lse, a.d_o, a.delta = o.data_ptr(), lse.data_ptr(), do.data_ptr(), delta.data_ptr()
+        a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        ws = _mod_workspace(a, True, q.device)      # noqa: F841
+        check(lib().apla_attn_mod_bwd(a, _stream()), "apla_attn_mod_bwd")
+    return dq, dk, dv
+
+
 def dw_workspace(M: int, r: int, D: int, device) -> torch.Tensor:
     if D % 64 == 0:
         D = (D + 127) // 128 * 128        # widths that are multiples of 64 only run padded (proj_dw)

@@ -295,6 +295,57 @@ int apla_attn_probs(const void* qkv, const float* lse, float* attn, int B, int N
 int apla_attn_probs_dropout(const void* qkv, const float* lse, float* attn, int B, int N, int H, float scale, float p,
                             unsigned long long seed, unsigned offset, hipStream_t stream);
 
+/* Rotary positions (head_dim 64), beside the qkv Linear and the attention entry points above.  x, y: [T, heads * 64] rows of 16-bit values
+ * with row strides ldx / ldy (the query and key columns of a fused qkv activation are such a view; y may be x itself).  The first `rot` values
+ * of every head are turned, pair i by the angle of table row `position`: table [P, rot] fp32 = cos of the rot / 2 angles, then their sin.
+ * APLA_ROT_HALF pairs (i, i + rot / 2), APLA_ROT_INTERLEAVED (2i, 2i + 1); rot even, 0..64.  Position of row t: pos[t] if given, else
+ * t % seq_len (seq_len 0: t).  A pos outside [0, P) makes the turned values of its row NaN.  inverse != 0 turns back: the backward pass. */
+enum { APLA_ROT_HALF = 0, APLA_ROT_INTERLEAVED = 1 };
+int apla_rotary(const void* x, long ldx, void* y, long ldy, int T, int heads, const float* table, int P, int rot, int layout,
+                const int32_t* pos, int seq_len, int inverse, hipStream_t stream);
+
+/* Norm of every query and key head (LayerNorm or RMS norm over its 64 values, fp32 statistics; qw / qb for the first Hq heads of a row, kw /
+ * kb for the Hkv behind them; NULL: 1 / 0), then the rotation above (rot 0: none), in one pass: the q_norm / k_norm modules of timm-style
+ * attention (the host-model contract of apla_vit.py:17-37).  x: [T, >= (Hq + Hkv) * 64] rows, y: [T, (Hq + Hkv) * 64] rows.
+ * Backward: dy, x -> dx (same columns); dparams [4][64] = d qw, d kw, d qb, d kb (fp32, overwritten; NULL: not wanted) through a
+ * workspace of apla_qk_norm_rotary_workspace_bytes().  Deterministic. */
+enum { APLA_NORM_LAYER = 1, APLA_NORM_RMS = 2 };
+long apla_qk_norm_rotary_workspace_bytes(void);
+int apla_qk_norm_rotary_fwd(const void* x, long ldx, void* y, long ldy, int T, int Hq, int Hkv, int norm, float eps, const float* qw,
+                            const float* kw, const float* qb, const float* kb, const float* table, int P, int rot, int layout,
+                            const int32_t* pos, int seq_len, hipStream_t stream);
+int apla_qk_norm_rotary_bwd(const void* dy, long lddy, const void* x, long ldx, void* dx, long lddx, int T, int Hq, int Hkv, int norm,
+                            float eps, const float* qw, const float* kw, const float* table, int P, int rot, int layout, const int32_t* pos,
+                            int seq_len, float* dparams, void* workspace, long workspace_bytes, hipStream_t stream);
+
+/* Attention with modified and masked scores (head_dim 64), next to apla_attn_fwd / apla_attn_varlen_fwd:
+ *   s_ij = scale q_i.k_j; softcap > 0: s = softcap tanh(s / softcap); slopes [Hq]: s -= slope_h dist(i, j); masked: -inf; softmax; times v.
+ * Query head h reads key head h / (Hq / Hkv).  q, o [Tq, Hq * 64], k, v [Tk, Hkv * 64] rows with their own strides; lse [Hq, Tq].
+ * Sequence s holds queries cu_q[s] .. cu_q[s+1] (NULL: s * max_q, max_q of them) and keys likewise, of which len_k[s] are used (NULL: all);
+ * query i of nq stands at key position i + nk - nq.  max_q / max_k: the longest sequences (longer ones are cut there).
+ * dist: |i + nk - nq - j|, or the Euclidean distance of pos_q / pos_k [T, pos_dim] (pos_dim 1 or 2).
+ * Visible: j < nk; causal: j <= i + nk - nq or j < prefix[s]; documents: doc_q[i] == doc_k[j] >= 0.  A row that sees nothing gives
+ * o = 0, lse = -inf and zero gradients; rows behind the last sequence and keys past len_k are not written.
+ * Values in masked places may be anything (infinities and NaN too).  Backward: lse and o from the forward, delta [Hq, Tq] scratch.
+ * workspace: apla_attn_mod_workspace_bytes(p, backward) bytes, 16-byte aligned, of this call alone.  Deterministic. */
+typedef struct {
+  const void *q, *k, *v;
+  void* o;
+  float* lse;
+  const int32_t *cu_q, *cu_k, *len_k, *prefix, *doc_q, *doc_k;
+  const float *slopes, *pos_q, *pos_k;
+  const void* d_o;
+  void *dq, *dk, *dv;
+  float* delta;
+  void* workspace;
+  long workspace_bytes, ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
+  int S, Tq, Tk, max_q, max_k, Hq, Hkv, pos_dim, causal;
+  float scale, softcap;
+} apla_attn_mod_t;
+long apla_attn_mod_workspace_bytes(const apla_attn_mod_t* p, int backward);
+int apla_attn_mod_fwd(const apla_attn_mod_t* p, hipStream_t stream);
+int apla_attn_mod_bwd(const apla_attn_mod_t* p, hipStream_t stream);
+
 /* The APLA output projection as one forward and one backward operator (appla_attn.py:62-79 and its autograd), composed of
  * the entry points of this header — no kernels of their own.
  *   apla_proj_fwd:  y[M,D] = x[M,D] @ Wnat^T + bnat, Wnat = the natural-order merged weight kept by apla_pack_proj_rows
