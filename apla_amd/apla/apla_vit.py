@@ -9,6 +9,8 @@ import os
 
 import torch
 
+from ..attn_features import AttnFeatures, real_norm
+from ..functional import qk_norm_kind
 from .appla_attn import APLA_Attention
 from .appla_attn_mem_eff import APLA_MemEffAttention
 
@@ -37,6 +39,17 @@ def indices_from_trainable(trainable, dim):
     return torch.tensor([int(t) for t in trainable] + [i for i in range(dim) if i not in chosen], dtype=torch.int64)
 
 
+def _keep_features(attn, new):
+    """What the replaced attention does between its qkv Linear and the softmax stays: the q_norm / k_norm modules of timm-style attention and
+    the features of this package's own (attn_features.py).  A q / k norm that the kernels do not compute is refused here."""
+    q_norm, k_norm = getattr(attn, "q_norm", None), getattr(attn, "k_norm", None)
+    if real_norm(q_norm) or real_norm(k_norm):
+        qk_norm_kind(q_norm, k_norm)
+        new.q_norm, new.k_norm = q_norm, k_norm
+    features = getattr(attn, "features", None)
+    new.features = features if isinstance(features, AttnFeatures) else None
+
+
 def replace_attn_with_apla(model, config, attn_module):
     inds_dict = load_inds(_cfg_get(config, "inds_path")) if _cfg_has(config, "inds_path") else None
     for i, block in enumerate(model.blocks):
@@ -60,6 +73,7 @@ def replace_attn_with_apla(model, config, attn_module):
             else:  # reference leaves torch.empty garbage here (apla_vit.py:54-56); a missing bias is a zero bias
                 new.proj_bias1.data.zero_()
                 new.proj_bias2.data.zero_()
+        _keep_features(attn, new)
         new.to(attn.qkv.weight.device)
         block.attn = new
 

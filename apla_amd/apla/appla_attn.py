@@ -15,6 +15,7 @@ always builds it; ``Block.forward`` discards it unless ``return_attention=True``
 import torch
 import torch.nn as nn
 
+from .. import attn_features as FT
 from .. import functional as AF
 from .. import ops
 
@@ -49,6 +50,7 @@ class APLA_Attention(nn.Module):
         self.attn_drop = nn.Dropout(attn_drop)
         self.proj_drop = nn.Dropout(proj_drop)
         self.return_attn_matrix = False
+        self.features = None        # attn_features.AttnFeatures / q_norm, k_norm modules of the attention this one replaced (apla_vit.py)
         self._proj_state = AF.AplaProjState()
 
     def _attend(self, x):
@@ -67,6 +69,9 @@ class APLA_Attention(nn.Module):
         """``ls_gamma`` (extension, used by VisionTransformer.run_blocks): the block's frozen LayerScale vector; when given,
         x is ls1(attention(x)) with the scale folded into the projection GEMM."""
         B, N, _ = x.shape
+        if FT.has_features(self):
+            o = AF.attention_features(self, AF.linear(x, self.qkv.weight, self.qkv.bias))
+            return AF.dropout(self._project(o, ls_gamma).to(x.dtype), self.proj_drop, self.training), None
         qkv, o, lse, (p, seed) = self._attend(x)
         # proj_drop (appla_attn.py:82) commutes with the LayerScale vector folded into the projection: both are element-wise
         y = AF.dropout(self._project(o, ls_gamma).to(x.dtype), self.proj_drop, self.training)

@@ -10,6 +10,7 @@ kernels as cumulative sequence offsets (``apla_attn_varlen_fwd/bwd``); the qkv L
 token-wise and run on the packed tensor unchanged (appla_attn_mem_eff.py:37-65).
 """
 from .appla_attn import APLA_Attention
+from .. import attn_features as FT
 from .. import functional as AF
 from ..nested import BlockDiagonalMask
 
@@ -30,8 +31,11 @@ class APLA_MemEffAttention(APLA_Attention):
         if x.ndim != 3 or x.shape[0] != 1 or x.shape[1] != attn_bias.total:
             raise ValueError(f"a packed batch must be [1, {attn_bias.total}, C]; got {tuple(x.shape)}")
         qkv = AF.linear(x, self.qkv.weight, self.qkv.bias)
-        o = AF.attention_core_varlen(qkv, attn_bias.cu_seqlens(x.device), attn_bias.max_seqlen, self.num_heads, self.scale,
-                                        runs=attn_bias.runs())
+        if FT.has_features(self):
+            o = AF.attention_features(self, qkv, attn_bias)
+        else:
+            o = AF.attention_core_varlen(qkv, attn_bias.cu_seqlens(x.device), attn_bias.max_seqlen, self.num_heads, self.scale,
+                                         runs=attn_bias.runs())
         if rows is not None:
             o = o.index_select(1, rows)
         return AF.dropout(self._project(o, ls_gamma).to(x.dtype), self.proj_drop, self.training)

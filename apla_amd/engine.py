@@ -34,6 +34,7 @@ import torch.nn as nn
 from . import ops
 from ._lib import AplaHipError
 from .apla.appla_attn import APLA_Attention
+from .attn_features import has_features
 from .dist import GradExchanger
 
 
@@ -89,6 +90,9 @@ class AplaTrainEngine:
         self.D, self.L, self.H = bb.embed_dim, bb.depth, bb.num_heads
         if self.D != 64 * self.H:
             raise NotImplementedError("HIP attention kernel needs head_dim == 64")
+        if any(has_features(blk.attn) for blk in bb.blocks):
+            raise NotImplementedError("q / k norm, rotary positions and modified scores (block_conf['attention']) train on the module path "
+                                      "(apla_amd.module_trainer)")
         # Element-wise dropout (main.py --dr / --adr; 0 in every shipped configuration): the nn.Dropout sites of the reference — pos_drop
         # (vit.py:395), attn_drop on the attention probabilities and proj_drop (appla_attn.py:58, :82), Mlp.drop after the activation and
         # after fc2 (vit.py:152-168) — run as counter-based mask passes around the step's launches (apla_dropout_fwd / _bwd,

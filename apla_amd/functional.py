@@ -530,6 +530,173 @@ def attention_module_forward(x, qkv_w, qkv_b, proj_w, proj_b, num_heads, scale, 
     return y, attn
 
 
+# ------------------------------------------------------------------------------------------------ rotary positions, q / k norm, modified scores
+def _rows_h16(x):
+    """[..., C] as 16-bit rows [T, C]; a row-strided 16-bit view stays a view."""
+    x2 = x.reshape(-1, x.shape[-1])
+    return x2 if x2.dtype == _h() else x2.to(_h())
+
+
+class _RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, table, heads, layout, pos, seq_len):
+        _require_cuda(x, "rotary")
+        ctx.args, ctx.pos, ctx.table, ctx.dtype = (heads, layout, seq_len), pos, table, x.dtype
+        return ops.rotary_fwd(_rows_h16(x), table, heads, layout=layout, pos=pos, seq_len=seq_len).reshape(x.shape)
+
+    @staticmethod
+    def backward(ctx, dy):
+        heads, layout, seq_len = ctx.args
+        dx = ops.rotary_bwd(_as2d_bf16(dy), ctx.table, heads, layout=layout, pos=ctx.pos, seq_len=seq_len)
+        return dx.reshape(dy.shape).to(ctx.dtype), None, None, None, None, None
+
+
+def rotary(x, table, heads: int, *, layout: str = "half", pos=None, seq_len: int = 0):
+    """Rotary positions on [..., heads * 64] (16-bit result); ``table`` from apla_amd.rotary, see ops.rotary_fwd for the positions."""
+    return _RotaryFn.apply(x, table, heads, layout, pos, seq_len)
+
+
+class _QkNormRotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, qw, kw, qb, kb, Hq, Hkv, norm, eps, rot):
+        _require_cuda(qkv, "qk_norm_rotary")
+        x = _rows_h16(qkv)
+        par = [b_f32(p) for p in (qw, kw, qb, kb)]
+        args = dict(zip(("q_weight", "k_weight", "q_bias", "k_bias"), par), norm=norm, eps=eps, **rot)
+        ctx.save_for_backward(x)
+        ctx.args, ctx.heads, ctx.shape, ctx.dtype, ctx.pdt = args, (Hq, Hkv), qkv.shape, qkv.dtype, [None if p is None else p.dtype for p in (qw, kw, qb, kb)]
+        return ops.qk_norm_rotary_fwd(x, Hq, Hkv, **args).reshape(qkv.shape[:-1] + ((Hq + Hkv) * 64,))
+
+    @staticmethod
+    def backward(ctx, dy):
+        (x,), (Hq, Hkv) = ctx.saved_tensors, ctx.heads
+        n = (Hq + Hkv) * 64
+        full = torch.zeros(x.shape, device=x.device, dtype=x.dtype) if x.shape[1] > n else torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        _, dpar = ops.qk_norm_rotary_bwd(_as2d_bf16(dy), x, Hq, Hkv, out=full[:, :n], want_params=any(ctx.needs_input_grad[1:5]), **ctx.args)
+        g = [None if not ctx.needs_input_grad[1 + i] else dpar[i].to(ctx.pdt[i]) for i in range(4)]
+        return full.reshape(ctx.shape).to(ctx.dtype), *g, None, None, None, None, None
+
+
+def qk_norm_rotary(qkv, Hq: int, Hkv: int, *, norm: str = "layer", q_weight=None, k_weight=None, q_bias=None, k_bias=None, eps: float = 1e-6,
+                   table=None, layout: str = "half", pos=None, seq_len: int = 0):
+    """Norm of every query / key head and rotation: [..., >= (Hq + Hkv) * 64] -> [..., (Hq + Hkv) * 64] (16 bits), with the gradients of the
+    weights and biases that ask for one."""
+    return _QkNormRotaryFn.apply(qkv, q_weight, k_weight, q_bias, k_bias, Hq, Hkv, norm, eps, dict(table=table, layout=layout, pos=pos, seq_len=seq_len))
+
+
+class _AttnModFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, Hq, Hkv, scale, mod, seq):
+        _require_cuda(q, "attention_mod")
+        q2, k2, v2 = _rows_h16(q), _rows_h16(k), _rows_h16(v)
+        o, lse = ops.attn_mod_fwd(q2, k2, v2, Hq, Hkv, scale, mod, **seq)
+        ctx.save_for_backward(q2, k2, v2, o, lse)
+        ctx.args, ctx.like = (Hq, Hkv, scale, mod, seq), [(t.shape, t.dtype) for t in (q, k, v)]
+        ctx.mark_non_differentiable(lse)
+        return o.reshape(q.shape), lse
+
+    @staticmethod
+    def backward(ctx, do, _dlse):
+        q, k, v, o, lse = ctx.saved_tensors
+        Hq, Hkv, scale, mod, seq = ctx.args
+        g = ops.attn_mod_bwd(q, k, v, o, _as2d_bf16(do), lse, Hq, Hkv, scale, mod, **seq)
+        return (*(t.reshape(s).to(dt) for t, (s, dt) in zip(g, ctx.like)), None, None, None, None, None)
+
+
+def attention_mod(q, k, v, Hq: int, Hkv: int, scale: float, mod=None, **seq):
+    """(o, lse) of attention with modified and masked scores (ops.ScoreMod) on [..., H * 64] tensors; ``seq``: batch / len_k, or cu_q, cu_k,
+    max_q, max_k, as in ops.attn_mod_fwd."""
+    return _AttnModFn.apply(q, k, v, Hq, Hkv, scale, mod, seq)
+
+
+class _AttnModQkvFn(torch.autograd.Function):
+    """q / k norm, rotation and attention on fused qkv rows as one node: the backward writes dq, dk (through the norm and the rotation) and dv
+    into one gradient buffer of the qkv Linear's output, with no copy or addition between."""
+
+    @staticmethod
+    def forward(ctx, qkv, qw, kw, qb, kb, H, scale, norm, eps, rot, mod, seq):
+        _require_cuda(qkv, "attention_mod_qkv")
+        x, n = _rows_h16(qkv), H * 64
+        args = None
+        if norm is not None:
+            args = dict(zip(("q_weight", "k_weight", "q_bias", "k_bias"), [b_f32(p) for p in (qw, kw, qb, kb)]), norm=norm, eps=eps, **rot)
+            qk = ops.qk_norm_rotary_fwd(x, H, H, **args)
+        elif rot["table"] is not None:
+            qk = ops.rotary_fwd(x[:, :2 * n], rot["table"], 2 * H, **{a: b for a, b in rot.items() if a != "table"})
+        else:
+            qk = x[:, :2 * n]
+        o, lse = ops.attn_mod_fwd(qk[:, :n], qk[:, n:], x[:, 2 * n:], H, H, scale, mod, **seq)
+        ctx.save_for_backward(x, qk, o, lse)
+        ctx.args, ctx.norm, ctx.like, ctx.pdt = (H, scale, rot, mod, seq), args, (qkv.shape, qkv.dtype), [None if p is None else p.dtype for p in (qw, kw, qb, kb)]
+        return o.reshape(qkv.shape[:-1] + (n,))
+
+    @staticmethod
+    def backward(ctx, do):
+        x, qk, o, lse = ctx.saved_tensors
+        H, scale, rot, mod, seq = ctx.args
+        n = H * 64
+        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if "cu_q" not in seq else torch.zeros(x.shape, device=x.device, dtype=x.dtype)
+        ops.attn_mod_bwd(qk[:, :n], qk[:, n:], x[:, 2 * n:], o, _as2d_bf16(do), lse, H, H, scale, mod, dq=dx[:, :n], dk=dx[:, n:2 * n], dv=dx[:, 2 * n:], **seq)
+        g = [None] * 4
+        if ctx.norm is not None:        # in place: every lane reads its row's gradient before it writes it
+            want = any(ctx.needs_input_grad[1:5])
+            _, dpar = ops.qk_norm_rotary_bwd(dx[:, :2 * n], x, H, H, out=dx[:, :2 * n], want_params=want, **ctx.norm)
+            g = [dpar[i].to(ctx.pdt[i]) if ctx.needs_input_grad[1 + i] else None for i in range(4)]
+        elif rot["table"] is not None:
+            ops.rotary_bwd(dx[:, :2 * n], rot["table"], 2 * H, out=dx[:, :2 * n], **{a: b for a, b in rot.items() if a != "table"})
+        return dx.reshape(ctx.like[0]).to(ctx.like[1]), *g, None, None, None, None, None, None, None
+
+
+def attention_mod_qkv(qkv, H: int, scale: float, *, mod=None, q_norm=None, k_norm=None, table=None, layout: str = "half", pos=None, seq_len: int = 0, **seq):
+    """Attention of fused qkv rows [..., 3 * H * 64] with the norm modules ``q_norm`` / ``k_norm`` (both or neither: nn.LayerNorm / nn.RMSNorm over 64),
+    the rotation of ``table`` (None: none) and the score modification ``mod``; ``seq`` as in attention_mod.  Returns o [..., H * 64]."""
+    if qkv.shape[-1] != 3 * H * 64:
+        raise NotImplementedError(f"the HIP attention kernel needs head_dim 64 (got {qkv.shape[-1] // (3 * H)})")
+    norm, eps, w = None, 0.0, [None] * 4
+    if q_norm is not None or k_norm is not None:
+        norm, eps = qk_norm_kind(q_norm, k_norm)
+        w = [getattr(m, a, None) for a in ("weight", "bias") for m in (q_norm, k_norm)]
+    return _AttnModQkvFn.apply(qkv, *w, H, scale, norm, eps, dict(table=table, layout=layout, pos=pos, seq_len=seq_len), mod, seq)
+
+
+def attention_features(attn, qkv, attn_bias=None):
+    """The attention of a module with features (attn_features.py, and / or q_norm / k_norm modules) on its qkv activation [B, N, 3 * dim], or a packed one
+    [1, total, 3 * dim] with its BlockDiagonalMask; returns o [.., dim].  What these kernels do not do is refused, never ignored."""
+    from .attn_features import real_norm
+    if attn.return_attn_matrix:
+        raise NotImplementedError("the attention matrix is not available from modules with q / k norm, rotary positions or modified scores")
+    if active_p(attn.attn_drop, attn.training) > 0.0:
+        raise NotImplementedError("attention-probability dropout is not supported next to q / k norm, rotary positions or modified scores")
+    q_norm, k_norm = getattr(attn, "q_norm", None), getattr(attn, "k_norm", None)
+    if real_norm(q_norm) != real_norm(k_norm):
+        raise NotImplementedError("q_norm without k_norm (or the other way round) is not supported on the HIP path")
+    if not real_norm(q_norm):
+        q_norm = k_norm = None
+    if attn.features is not None:
+        lens = attn_bias.seqlens if attn_bias is not None else [qkv.shape[1]] * qkv.shape[0]
+        kw = attn.features.plan(lens, qkv.device, attn_bias)
+    elif attn_bias is not None:
+        cu = attn_bias.cu_seqlens(qkv.device)
+        kw = dict(cu_q=cu, cu_k=cu, max_q=attn_bias.max_seqlen, max_k=attn_bias.max_seqlen)
+    else:
+        kw = dict(batch=qkv.shape[0])
+    return attention_mod_qkv(qkv, attn.num_heads, attn.scale, q_norm=q_norm, k_norm=k_norm, **kw)
+
+
+def qk_norm_kind(q_norm, k_norm):
+    """("layer" | "rms", eps) of a pair of q / k norm modules, or NotImplementedError: nn.LayerNorm or nn.RMSNorm over the 64 values of a head,
+    the same kind and eps for both."""
+    kinds = []
+    for m in (q_norm, k_norm):
+        kind = "layer" if isinstance(m, torch.nn.LayerNorm) else "rms" if isinstance(m, torch.nn.RMSNorm) else None
+        if kind is None or tuple(m.normalized_shape) != (64,):
+            raise NotImplementedError(f"q / k norm {type(m).__name__}: only LayerNorm and RMSNorm over a head of 64 values run on the HIP path")
+        kinds.append((kind, float(m.eps) if m.eps is not None else float(torch.finfo(torch.float32).eps)))
+    if kinds[0] != kinds[1]:
+        raise NotImplementedError(f"q and k norms differ: {kinds[0]} and {kinds[1]}")
+    return kinds[0]
+
+
 # ------------------------------------------------------------------------------------------------ APLA projection
 class AplaProjState:
     """Kernel-layout copies of one APLA projection: natural-order bf16 weight, its transpose, fp32 bias, int32 indices.

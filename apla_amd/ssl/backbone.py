@@ -13,6 +13,7 @@ from typing import List, Optional
 import torch
 from torch import nn
 
+from .. import attn_features as FT
 from .. import functional as AF
 from .. import ops
 from ..apla.appla_attn_mem_eff import APLA_MemEffAttention
@@ -34,8 +35,11 @@ class MemEffAttention(Attention):
         if x.ndim != 3 or x.shape[0] != 1 or x.shape[1] != attn_bias.total:
             raise ValueError(f"a packed batch must be [1, {attn_bias.total}, C]; got {tuple(x.shape)}")
         qkv = AF.linear(x, self.qkv.weight, self.qkv.bias)
-        o = AF.attention_core_varlen(qkv, attn_bias.cu_seqlens(x.device), attn_bias.max_seqlen, self.num_heads, self.scale,
-                                        runs=attn_bias.runs())
+        if FT.has_features(self):
+            o = AF.attention_features(self, qkv, attn_bias)
+        else:
+            o = AF.attention_core_varlen(qkv, attn_bias.cu_seqlens(x.device), attn_bias.max_seqlen, self.num_heads, self.scale,
+                                         runs=attn_bias.runs())
         if rows is not None:
             o = o.index_select(1, rows)
         return AF.dropout(AF.linear(o, self.proj.weight, self.proj.bias).to(x.dtype), self.proj_drop, self.training)

@@ -42,7 +42,8 @@ def build_model(backbone, backbone_args, only_teacher=False, img_size=224):
     def make():
         return DinoVisionTransformer(img_size=[img_size], patch_size=backbone_args.patch_size, embed_dim=dim, depth=depth, num_heads=heads,
                                      qkv_bias=True, norm_layer=partial(nn.LayerNorm, eps=1e-6), use_swiglu=swiglu,
-                                     block_conf=dict(has_layerscale=bool(init), layerscale_init_values=init or 1.0),
+                                     block_conf=dict(has_layerscale=bool(init), layerscale_init_values=init or 1.0,
+                                                     attention=getattr(backbone_args, "attention", None)),
                                      interpolate_offset=getattr(backbone_args, "interpolate_offset", 0.1),
                                      interpolate_antialias=getattr(backbone_args, "interpolate_antialias", False))
     teacher = make()

@@ -18,6 +18,7 @@ from functools import partial
 import torch
 import torch.nn as nn
 
+from . import attn_features as FT
 from . import functional as AF
 
 
@@ -73,7 +74,7 @@ class Attention(nn.Module):
     """Plain MHSA, vit.py:171-196: the module APLA swaps out (exposes dim/num_heads/scale/qkv/proj/attn_drop/proj_drop,
     which is the host-model contract of apla_vit.py:17-37)."""
 
-    def __init__(self, dim, num_heads=8, qkv_bias=False, qk_scale=None, attn_drop=0.0, proj_drop=0.0):
+    def __init__(self, dim, num_heads=8, qkv_bias=False, qk_scale=None, attn_drop=0.0, proj_drop=0.0, features=None):
         super().__init__()
         self.dim = dim
         self.num_heads = num_heads
@@ -83,8 +84,14 @@ class Attention(nn.Module):
         self.proj = nn.Linear(dim, dim)
         self.proj_drop = nn.Dropout(proj_drop)
         self.return_attn_matrix = False
+        self.features = FT.AttnFeatures(features, num_heads) if features else None     # attn_features.py
+        if self.features is not None and self.features.qk_norm:
+            self.q_norm, self.k_norm = FT.make_norms(self.features.qk_norm)
 
     def forward(self, x):
+        if FT.has_features(self):
+            o = AF.attention_features(self, AF.linear(x, self.qkv.weight, self.qkv.bias))
+            return AF.dropout(AF.linear(o, self.proj.weight, self.proj.bias).to(x.dtype), self.proj_drop, self.training), None
         y, attn = AF.attention_module_forward(x, self.qkv.weight, self.qkv.bias, self.proj.weight, self.proj.bias,
                                               self.num_heads, self.scale, self.return_attn_matrix,
                                               AF.active_p(self.attn_drop, self.training))   # vit.py:190-192
@@ -110,7 +117,7 @@ class Block(nn.Module):
         super().__init__()
         self.norm1 = norm_layer(dim)
         self.attn = Attention(dim, num_heads=num_heads, qkv_bias=qkv_bias, qk_scale=qk_scale, attn_drop=attn_drop,
-                              proj_drop=drop)
+                              proj_drop=drop, features=_cfg_get(conf, "attention", None) if conf else None)
         self.drop_path = DropPath(drop_path) if drop_path > 0.0 else nn.Identity()   # vit.py:257
         self.norm2 = norm_layer(dim)
         hidden = int(dim * mlp_ratio)
