@@ -32,7 +32,7 @@ struct ModArgs {
   int S, Tq, Tk, max_q, max_k, Hq, G, causal;
   float scale, c, k1, kx, A;            // c = scale log2e; cap: 2 scale log2e / cap, scale / cap, cap log2e
   const int2 *rng_q, *rng_k;            // [S][tiles of 64]: smallest and largest document id
-  int nt_q, nt_k, nblk;                 // tiles per sequence in those; 128-row blocks per sequence
+  int nt_q, nt_k, nblk, np;             // tiles per sequence in those; 128-row blocks per sequence; see where()
   const bf16* d_o;
   long lddo;
   bf16 *dq, *dk, *dv;
@@ -110,21 +110,52 @@ __device__ __forceinline__ void mfma_select(f32x16& acc, const bf16x8& af, const
 #pragma unroll
   for (int i = 0; i < 16; ++i) acc[i] = hits[i] > 0.f ? __builtin_nanf("") : acc[i];
 }
-// acc[2] += tile^T w: the transposed rows rbase .. rbase + 31 of an LDS tile times the weights that the accumulator w holds for them.
-// `odd`: the tile may hold non-finite values and w zeros for them.
-template <bool MASKED>
-__device__ __forceinline__ void tile_product(f32x16 (&acc)[2], const char* tile, int rbase, const f32x16& w, int lane, bool odd) {
+// ---- fragments by lane constants: tile_off's swizzle looks at bits 1-3 of the row only, so next to a first row that is a multiple of 16 the byte offset
+// of a fragment is that row * 128 + a constant of the lane; left to itself hipcc keeps an address per fragment (40 registers)
+struct Frag { unsigned rf[4], tr[4]; };
+__device__ __forceinline__ Frag frag_consts(int lane) {
+  Frag f;
 #pragma unroll
-  for (int sk = 0; sk < 2; ++sk) {
-    const bf16x8 wb = acc_to_operand(w, sk);
+  for (int ks = 0; ks < 4; ++ks) f.rf[ks] = (unsigned)tile_off(lane & 31, 2 * ks + (lane >> 5));
+  const int g = lane >> 4, i = lane & 15, r = 4 * (g >> 1) + (i >> 2);
+#pragma unroll
+  for (int dt = 0; dt < 2; ++dt) {
+    const int col = 32 * dt + 16 * (g & 1) + 4 * (i & 3);
+    f.tr[2 * dt] = (unsigned)(tile_off(r, col >> 3) + ((col & 4) << 1));
+    f.tr[2 * dt + 1] = (unsigned)(tile_off(r + 8, col >> 3) + ((col & 4) << 1));
+  }
+  return f;
+}
+__device__ __forceinline__ unsigned lds_of(const char* p) { return (unsigned)(size_t)(__attribute__((address_space(3))) const char*)p; }
+__device__ __forceinline__ bf16x8 row_at(unsigned tile, int row, unsigned c) {
+  return *(const __attribute__((address_space(3))) bf16x8*)(size_t)(tile + c + row * 128);
+}
+__device__ __forceinline__ bf16x8 tr_at(unsigned tile, int row, unsigned c0, unsigned c1) {
+  const bf16x4 lo = DS_READ_TR16_B64_H16((__attribute__((address_space(3))) char*)(size_t)(tile + c0 + row * 128));
+  const bf16x4 hi = DS_READ_TR16_B64_H16((__attribute__((address_space(3))) char*)(size_t)(tile + c1 + row * 128));
+  return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+}
+
+// acc[2] += tile^T w: the transposed rows rbase .. rbase + 31 of an LDS tile times the weights that the accumulator w holds for them.
+// `odd` (the same for the wave): the tile may hold non-finite values and w zeros for them.
+__device__ __forceinline__ void tile_product(f32x16 (&acc)[2], unsigned tile, int rbase, const f32x16& w, const Frag& fr, bool odd) {
+  const bf16x8 w0 = acc_to_operand(w, 0), w1 = acc_to_operand(w, 1);
+  if (__builtin_expect(odd, 0)) {
 #pragma unroll
     for (int dt = 0; dt < 2; ++dt) {
-      const bf16x8 af = tr_frag(tile, rbase + 16 * sk, 32 * dt, lane);
-      if (MASKED && __builtin_expect(odd, 0)) mfma_select(acc[dt], af, wb);
-      else acc[dt] = MFMA_F32_32x32x16_H16(af, wb, acc[dt]);
+      mfma_select(acc[dt], tr_at(tile, rbase, fr.tr[2 * dt], fr.tr[2 * dt + 1]), w0);
+      mfma_select(acc[dt], tr_at(tile, rbase + 16, fr.tr[2 * dt], fr.tr[2 * dt + 1]), w1);
+    }
+  } else {
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt) {
+      acc[dt] = MFMA_F32_32x32x16_H16(tr_at(tile, rbase, fr.tr[2 * dt], fr.tr[2 * dt + 1]), w0, acc[dt]);
+      acc[dt] = MFMA_F32_32x32x16_H16(tr_at(tile, rbase + 16, fr.tr[2 * dt], fr.tr[2 * dt + 1]), w1, acc[dt]);
     }
   }
 }
+// a condition that is the same for the whole wave, as a scalar: branches on it need no execution mask
+__device__ __forceinline__ bool uniform(bool c) { return __builtin_amdgcn_readfirstlane((int)c) != 0; }
 
 // ---- staging: 64 rows x 64 columns by 256 threads (two 16-byte pieces each) through registers; rows past nrows read row nrows - 1
 struct Stage { bf16x8 v[2]; };
@@ -164,65 +195,76 @@ constexpr int KT_POS = 16384, KT_DOC = KT_POS + 512, KT_ODD = KT_DOC + 256, KT_B
 struct RowState { float m, l; };
 struct RowCtx { int lim, doc; float pos[2], slope; };       // slope in log2 units
 
-// cap tanh(s / cap) in log2 units: A (1 - 2 r), r = 1 / (1 + e^(2 s / cap)).  That is exact to 2^-23 A, which small scores feel relatively:
-// FINE takes the odd series below |s / cap| = 1/4 (its next term is 2^-27 there).  Masked tiles do so — every key of a short sequence is in
-// one —, full tiles hold 64 keys or more of a row, over which the difference averages out.
-template <bool FINE>
+// cap tanh(s / cap) in log2 units: A (1 - 2 r), r = 1 / (1 + e^(2 s / cap)).  That is exact to 2^-23 A, which small scores feel relatively; cap_fine
+// takes the odd series below |s / cap| = 1/4 (its next term is 2^-27 there).  Masked tiles do so — every key of a short sequence is in one —,
+// full tiles hold 64 keys or more of a row, over which the difference averages out.
 __device__ __forceinline__ float cap_score(float s, const ModArgs& a, float& r) {
   r = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * a.k1));
-  const float z = fmaf(-2.f * a.A, r, a.A);
-  if constexpr (!FINE) return z;
-  const float x = s * a.kx, y = x * x;
+  return fmaf(-2.f * a.A, r, a.A);
+}
+__device__ __forceinline__ float cap_fine(float s, const ModArgs& a, float& r) {
+  const float z = cap_score(s, a, r), x = s * a.kx, y = x * x;
   const float series = a.A * x * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
   return y < 0.0625f ? series : z;
 }
+__device__ __forceinline__ int pick(const int4& v, int e) { return e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w; }
 
-// scores of 32 keys in log2 units (times c where nothing modifies them)
-template <bool CAP, int BIAS, bool MASKED>
-__device__ __forceinline__ void modify(f32x16& s, const ModArgs& a, const RowCtx& r, const char* tile, int kt, int j0, int h2, bool docs) {
+// Scores s[16] of one row (on the lane) and 32 keys, or of one key and 32 rows, in log2 units; with neither cap nor bias they stay raw and the
+// caller multiplies by c.  `side`: LDS address of the positions of the other 32 (x, then y 256 bytes behind), r: cap_score's r of every score.
+// masked (the same for the wave) only chooses the finer cap here.
+template <bool CAP, int BIAS>
+__device__ __forceinline__ void modify(f32x16& s, f32x16& r, const ModArgs& a, const float (&pos)[2], float slope, const char* side, int h2, bool masked) {
+  if constexpr (CAP) {
+    if (masked) {
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const int jr = kt * 32 + 8 * g + 4 * h2;     // tile row of element 4 g
-    f32x4 px, py;
-    int4 dj;
-    if constexpr (BIAS > 0) px = *(const f32x4*)(tile + KT_POS + jr * 4);
-    if constexpr (BIAS > 1) py = *(const f32x4*)(tile + KT_POS + 256 + jr * 4);
-    if (MASKED && docs) dj = *(const int4*)(tile + KT_DOC + jr * 4);
+      for (int i = 0; i < 16; ++i) { float t; s[i] = cap_fine(s[i], a, t); r[i] = t; }
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float z = s[4 * g + e];
-      float rc;
-      if constexpr (CAP) z = cap_score<MASKED>(z, a, rc);
-      if constexpr (BIAS > 0) {
-        const float d = dist<BIAS>(r.pos, px[e], BIAS > 1 ? py[e] : 0.f);
-        z = CAP ? z - r.slope * d : fmaf(z, a.c, -r.slope * d);
+      for (int i = 0; i < 16; ++i) { float t; s[i] = cap_score(s[i], a, t); r[i] = t; }
+    }
+  }
+  if constexpr (BIAS > 0) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 px = *(const f32x4*)(side + (8 * g + 4 * h2) * 4);
+      f32x4 py;
+      if constexpr (BIAS > 1) py = *(const f32x4*)(side + 256 + (8 * g + 4 * h2) * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float d = dist<BIAS>(pos, px[e], BIAS > 1 ? py[e] : 0.f);
+        s[4 * g + e] = CAP ? s[4 * g + e] - slope * d : fmaf(s[4 * g + e], a.c, -slope * d);
       }
-      if constexpr (MASKED) {
-        bool vis = j0 + jr + e < r.lim;
-        if (docs) vis = vis && (e == 0 ? dj.x : e == 1 ? dj.y : e == 2 ? dj.z : dj.w) == r.doc;
-        z = vis ? z : -INFINITY;
-      }
-      s[4 * g + e] = z;
     }
   }
 }
 
-template <bool CAP, int BIAS, bool MASKED>
+template <bool CAP, int BIAS>
 __device__ __forceinline__ void fwd_tile(f32x16 (&acc)[2], RowState& st, const bf16x8 (&qf)[4], const ModArgs& a, const RowCtx& r, const char* tile,
-                                         int j0, int lane, bool docs, bool odd) {
+                                         int j0, int lane, const Frag& fr, bool masked, bool docs, bool odd) {
   const int h2 = lane >> 5;
   const float zm = (CAP || BIAS) ? 1.f : a.c;
-  const char *Ks = tile, *Vs = tile + 8192;
-  f32x16 s[2];
+  const unsigned Ks = lds_of(tile), Vs = Ks + 8192;
+  f32x16 s[2], unused;
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[kt][i] = 0.f;
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) s[kt] = MFMA_F32_32x32x16_H16(row_frag(Ks, kt * 32, ks, lane), qf[ks], s[kt]);
+    for (int ks = 0; ks < 4; ++ks) s[kt] = MFMA_F32_32x32x16_H16(row_at(Ks, kt * 32, fr.rf[ks]), qf[ks], s[kt]);
   }
 #pragma unroll
-  for (int kt = 0; kt < 2; ++kt) modify<CAP, BIAS, MASKED>(s[kt], a, r, tile, kt, j0, h2, docs);
+  for (int kt = 0; kt < 2; ++kt) modify<CAP, BIAS>(s[kt], unused, a, r.pos, r.slope, tile + KT_POS + kt * 128, h2, masked);
+  if (masked) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int jr = kt * 32 + 8 * g + 4 * h2;
+        const int4 dj = docs ? *(const int4*)(tile + KT_DOC + jr * 4) : int4{0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[kt][4 * g + e] = j0 + jr + e < r.lim && (!docs || pick(dj, e) == r.doc) ? s[kt][4 * g + e] : -INFINITY;
+      }
+  }
   float mx = s[0][0];
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt)
@@ -237,15 +279,27 @@ __device__ __forceinline__ void fwd_tile(f32x16 (&acc)[2], RowState& st, const b
     for (int i = 0; i < 16; ++i) { acc[0][i] *= alpha; acc[1][i] *= alpha; }
   }
   const float mc = st.m * zm;
+  if (odd) {      // (both forms of the products behind their own branch: the usual one is one straight run of instructions)
 #pragma unroll
-  for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < 2; ++kt) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[kt][i] = __builtin_amdgcn_exp2f((CAP || BIAS) ? s[kt][i] - mc : fmaf(s[kt][i], zm, -mc));
-      st.l += s[kt][i];
+      for (int i = 0; i < 16; ++i) {
+        s[kt][i] = __builtin_amdgcn_exp2f((CAP || BIAS) ? s[kt][i] - mc : fmaf(s[kt][i], zm, -mc));
+        st.l += s[kt][i];
+      }
+      tile_product(acc, Vs, kt * 32, s[kt], fr, true);
     }
+  } else {
 #pragma unroll
-  for (int kt = 0; kt < 2; ++kt) tile_product<MASKED>(acc, Vs, kt * 32, s[kt], lane, odd);
+    for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[kt][i] = __builtin_amdgcn_exp2f((CAP || BIAS) ? s[kt][i] - mc : fmaf(s[kt][i], zm, -mc));
+        st.l += s[kt][i];
+      }
+      tile_product(acc, Vs, kt * 32, s[kt], fr, false);
+    }
+  }
 }
 
 // ---- the list of key tiles that rows with (lim_max, documents dmin..dmax) can see, one pass of up to LIST tiles from t0
@@ -307,17 +361,18 @@ __device__ __forceinline__ void side_store(const KeySide& ks, char* tile, const 
   }
 }
 
-// Workgroup -> (sequence, query head, block of 128 rows): consecutive logical ids (one XCD each run) share keys; with a causal mask the long
-// blocks of a head come first.
-struct Where { int s, h, blk; };
-__device__ __forceinline__ Where where(const ModArgs& a, int heads) {
-  const int id = xcd_remap(blockIdx.x, gridDim.x);
-  Where w;
-  w.blk = id % a.nblk;
-  w.h = (id / a.nblk) % heads;
-  w.s = id / (a.nblk * heads);
-  return w;
+// Workgroup -> (sequence, head, block of 128 rows).  Blocks go to the 8 XCDs in turn (blockIdx & 7), each with an L2 of its own: the workgroups that read
+// the same rows (one key head of one sequence: `per` of them) stay on one XCD, in `np` parts on np of them where the number of such units is
+// no multiple of 8, and the units go round the XCDs, so that long and short sequences mix.  j counts the unit's workgroups, long causal blocks first.
+struct Where { int unit, j; };
+__device__ __forceinline__ Where where(const ModArgs& a, int per) {
+  const int xcd = blockIdx.x & 7, idx = blockIdx.x >> 3, each = (per + a.np - 1) / a.np;
+  const int u = idx / each * 8 + xcd;      // (unit, part)
+  return {u / a.np, idx % each * a.np + u % a.np};
 }
+// parts per unit, and the grid's size
+static inline int unit_parts(long units) { return units % 8 == 0 ? 1 : units % 4 == 0 ? 2 : units % 2 == 0 ? 4 : 8; }
+static inline long unit_grid(long units, int np, long per) { return units * np * ((per + np - 1) / np); }
 
 // what a lane knows of its query row
 template <int BIAS>
@@ -338,16 +393,19 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
   __shared__ TileRef list[LIST];
   __shared__ int buf[12];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
-  const Where w = where(a, a.Hq);
-  const MSeq m = mseq(a, w.s);
-  const int q0 = (a.causal ? a.nblk - 1 - w.blk : w.blk) * 128;
+  const Frag fr = frag_consts(lane);
+  const Where w = where(a, a.G * a.nblk);
+  if (w.j >= a.G * a.nblk) return;
+  const int Hkv = a.Hq / a.G, hk = w.unit % Hkv, h = hk * a.G + w.j % a.G, blk = w.j / a.G;
+  const MSeq m = mseq(a, w.unit / Hkv);
+  const int q0 = (a.causal ? a.nblk - 1 - blk : blk) * 128;
   if (q0 >= m.nq) return;
   const int qr = q0 + wave * 32 + (lane & 31);
   const bool active = q0 + wave * 32 < m.nq;
   const int qi = min(qr, m.nq - 1);
   bf16x8 qf[4];
-  load_row_frags(qf, a.q + (m.q0 + qi) * a.ldq + w.h * 64, lane);
-  const RowCtx r = row_ctx<BIAS>(a, m, qi, w.h);
+  load_row_frags(qf, a.q + (m.q0 + qi) * a.ldq + h * 64, lane);
+  const RowCtx r = row_ctx<BIAS>(a, m, qi, h);
   const bool docs = a.doc_k != nullptr;
   const int wlo = wave_min_i(r.doc), whi = wave_max_i(r.doc), wlim0 = wave_min_i(r.lim), wlim1 = wave_max_i(r.lim);
   int dlo = wlo, dhi = whi, lim = wlim1;
@@ -357,10 +415,10 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) { acc[0][i] = 0.f; acc[1][i] = 0.f; }
   RowState st = {NEG_BIG, 0.f};
-  const bf16 *kb = a.k + m.k0 * a.ldk + (w.h / a.G) * 64, *vb = a.v + m.k0 * a.ldv + (w.h / a.G) * 64;
+  const bf16 *kb = a.k + m.k0 * a.ldk + (hk) * 64, *vb = a.v + m.k0 * a.ldv + (hk) * 64;
   const int ntiles = (lim + 63) / 64;
   for (int t0 = 0; t0 < ntiles; t0 += LIST) {
-    const int n = build_list(list, buf, t0, ntiles, docs ? a.rng_k + (long)w.s * a.nt_k : nullptr, dlo, dhi, tid);
+    const int n = build_list(list, buf, t0, ntiles, docs ? a.rng_k + (long)(w.unit / Hkv) * a.nt_k : nullptr, dlo, dhi, tid);
     Stage ks, vs;
     KeySide sd;
     auto fetch = [&](int e) {
@@ -383,11 +441,9 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
       char* tile = smem + (e & 1) * KT_BYTES;
       const TileRef tr = list[e];
       const int j0 = __builtin_amdgcn_readfirstlane(tr.t) * 64, lo = __builtin_amdgcn_readfirstlane(tr.lo), hi = __builtin_amdgcn_readfirstlane(tr.hi);
-      if (active && j0 < wlim1 && (!docs || (hi >= max(wlo, 0) && lo <= whi))) {
-        if (j0 + 64 <= wlim0 && (!docs || (lo == hi && wlo == lo && whi == lo)))
-          fwd_tile<CAP, BIAS, false>(acc, st, qf, a, r, tile, j0, lane, false, false);
-        else
-          fwd_tile<CAP, BIAS, true>(acc, st, qf, a, r, tile, j0, lane, docs, any_odd(tile + KT_ODD));
+      if (uniform(active && j0 < wlim1 && (!docs || (hi >= max(wlo, 0) && lo <= whi)))) {
+        const bool masked = !uniform(j0 + 64 <= wlim0 && (!docs || (lo == hi && wlo == lo && whi == lo)));
+        fwd_tile<CAP, BIAS>(acc, st, qf, a, r, tile, j0, lane, fr, masked, docs, masked && any_odd(tile + KT_ODD));
       }
       if (e + 1 < n) put(smem + ((e + 1) & 1) * KT_BYTES);
       if (e + 2 < n) fetch(e + 2);
@@ -396,9 +452,9 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
   }
   const float l = st.l + __shfl_xor(st.l, 32, 64);
   if (qr < m.nq) {
-    store_acc_T(acc, a.o + (m.q0 + qr) * a.ldo + w.h * 64, h2, l != 0.f ? 1.f / l : 0.f);
+    store_acc_T(acc, a.o + (m.q0 + qr) * a.ldo + h * 64, h2, l != 0.f ? 1.f / l : 0.f);
     if (h2 == 0)
-      a.lse[(long)w.h * a.Tq + m.q0 + qr] = l != 0.f ? (st.m * ((CAP || BIAS) ? 1.f : a.c) + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+      a.lse[(long)h * a.Tq + m.q0 + qr] = l != 0.f ? (st.m * ((CAP || BIAS) ? 1.f : a.c) + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
   }
 }
 
@@ -421,6 +477,7 @@ __global__ __launch_bounds__(256, 1) void attn_mod_rows_kernel(ModArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[4 * KT_BYTES];
   __shared__ float ml[4][2][32];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
+  const Frag fr = frag_consts(lane);
   const int Hkv = a.Hq / a.G;
   const int sp = blockIdx.x % a.nsplit, rt = blockIdx.x / a.nsplit, hk = blockIdx.y, s = blockIdx.z;
   const MSeq m = mseq(a, s);
@@ -465,10 +522,7 @@ __global__ __launch_bounds__(256, 1) void attn_mod_rows_kernel(ModArgs a) {
         any = g.y >= max(wlo, 0) && g.x <= whi;
         full = full && g.x == g.y && wlo == g.x && whi == g.x;
       }
-      if (any) {
-        if (full) fwd_tile<CAP, BIAS, false>(acc, st, qf, a, r, tile, j0, lane, false, false);
-        else fwd_tile<CAP, BIAS, true>(acc, st, qf, a, r, tile, j0, lane, docs, odd);
-      }
+      if (uniform(any)) fwd_tile<CAP, BIAS>(acc, st, qf, a, r, tile, j0, lane, fr, !uniform(full), docs, !uniform(full) && odd);
       __builtin_amdgcn_wave_barrier();
       asm volatile("" ::: "memory");
     }
@@ -546,49 +600,36 @@ __global__ __launch_bounds__(256) void attn_mod_join_kernel(ModArgs a) {
 
 // ------------------------------------------------------------------------------------------------ backward
 // P = exp2(z - L2) from the forward's lse, dS = P (dP - delta), with the cap times 1 - tanh^2 = 4 r (1 - r), r = 1 / (1 + e^(2 s / cap))
-template <bool CAP, int BIAS, bool MASKED>
+template <bool CAP, int BIAS>
 __device__ __forceinline__ void dq_tile(f32x16 (&acc)[2], const bf16x8 (&qf)[4], const bf16x8 (&df)[4], float L2, float delta, const ModArgs& a,
-                                        const RowCtx& r, const char* tile, int j0, int lane, bool docs, bool odd) {
+                                        const RowCtx& r, const char* tile, int j0, int lane, const Frag& fr, bool masked, bool docs, bool odd) {
   const int h2 = lane >> 5;
-  const char *Ks = tile, *Vs = tile + 8192;
+  const unsigned Ks = lds_of(tile), Vs = Ks + 8192;
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt) {
-    f32x16 s, p;
+    f32x16 s, p, rc;
 #pragma unroll
     for (int i = 0; i < 16; ++i) { s[i] = 0.f; p[i] = 0.f; }
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) s = MFMA_F32_32x32x16_H16(row_frag(Ks, kt * 32, ks, lane), qf[ks], s);
+    for (int ks = 0; ks < 4; ++ks) s = MFMA_F32_32x32x16_H16(row_at(Ks, kt * 32, fr.rf[ks]), qf[ks], s);
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) p = MFMA_F32_32x32x16_H16(row_frag(Vs, kt * 32, ks, lane), df[ks], p);
+    for (int ks = 0; ks < 4; ++ks) p = MFMA_F32_32x32x16_H16(row_at(Vs, kt * 32, fr.rf[ks]), df[ks], p);
+    modify<CAP, BIAS>(s, rc, a, r.pos, r.slope, tile + KT_POS + kt * 128, h2, masked);
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int jr = kt * 32 + 8 * g + 4 * h2;
-      f32x4 px, py;
-      int4 dj;
-      if constexpr (BIAS > 0) px = *(const f32x4*)(tile + KT_POS + jr * 4);
-      if constexpr (BIAS > 1) py = *(const f32x4*)(tile + KT_POS + 256 + jr * 4);
-      if (MASKED && docs) dj = *(const int4*)(tile + KT_DOC + jr * 4);
+    for (int i = 0; i < 16; ++i) {
+      s[i] = __builtin_amdgcn_exp2f((CAP || BIAS) ? s[i] - L2 : fmaf(s[i], a.c, -L2)) * (p[i] - delta);
+      if constexpr (CAP) s[i] *= 4.f * rc[i] * (1.f - rc[i]);
+    }
+    if (masked) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = 4 * g + e;
-        float z = s[i], rc = 0.f;
-        if constexpr (CAP) z = cap_score<MASKED>(z, a, rc);
-        if constexpr (BIAS > 0) {
-          const float d = dist<BIAS>(r.pos, px[e], BIAS > 1 ? py[e] : 0.f);
-          z = CAP ? z - r.slope * d : fmaf(z, a.c, -r.slope * d);
-        }
-        const float pr = __builtin_amdgcn_exp2f((CAP || BIAS) ? z - L2 : fmaf(z, a.c, -L2));
-        float ds = pr * (p[i] - delta);
-        if constexpr (CAP) ds *= 4.f * rc * (1.f - rc);
-        if constexpr (MASKED) {
-          bool vis = j0 + jr + e < r.lim;
-          if (docs) vis = vis && (e == 0 ? dj.x : e == 1 ? dj.y : e == 2 ? dj.z : dj.w) == r.doc;
-          ds = vis ? ds : 0.f;
-        }
-        s[i] = ds;
+      for (int g = 0; g < 4; ++g) {
+        const int jr = kt * 32 + 8 * g + 4 * h2;
+        const int4 dj = docs ? *(const int4*)(tile + KT_DOC + jr * 4) : int4{0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[4 * g + e] = j0 + jr + e < r.lim && (!docs || pick(dj, e) == r.doc) ? s[4 * g + e] : 0.f;
       }
     }
-    tile_product<MASKED>(acc, Ks, kt * 32, s, lane, odd);
+    tile_product(acc, Ks, kt * 32, s, fr, odd);
   }
 }
 
@@ -598,21 +639,24 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
   __shared__ TileRef list[LIST];
   __shared__ int buf[12];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
-  const Where w = where(a, a.Hq);
-  const MSeq m = mseq(a, w.s);
-  const int q0 = (a.causal ? a.nblk - 1 - w.blk : w.blk) * 128;
+  const Frag fr = frag_consts(lane);
+  const Where w = where(a, a.G * a.nblk);
+  if (w.j >= a.G * a.nblk) return;
+  const int Hkv = a.Hq / a.G, hk = w.unit % Hkv, h = hk * a.G + w.j % a.G, blk = w.j / a.G;
+  const MSeq m = mseq(a, w.unit / Hkv);
+  const int q0 = (a.causal ? a.nblk - 1 - blk : blk) * 128;
   if (q0 >= m.nq) return;
   const int qr = q0 + wave * 32 + (lane & 31);
   const bool active = q0 + wave * 32 < m.nq;
   const int qi = min(qr, m.nq - 1);
   bf16x8 qf[4], df[4];
-  load_row_frags(qf, a.q + (m.q0 + qi) * a.ldq + w.h * 64, lane);
-  load_row_frags(df, a.d_o + (m.q0 + qi) * a.lddo + w.h * 64, lane);
-  const long stat = (long)w.h * a.Tq + m.q0 + qi;
+  load_row_frags(qf, a.q + (m.q0 + qi) * a.ldq + h * 64, lane);
+  load_row_frags(df, a.d_o + (m.q0 + qi) * a.lddo + h * 64, lane);
+  const long stat = (long)h * a.Tq + m.q0 + qi;
   float delta = 0.f;      // rowsum(dO o O): this lane's half of the row, then the other half
   {
     bf16x8 of[4];
-    load_row_frags(of, a.o + (m.q0 + qi) * a.ldo + w.h * 64, lane);
+    load_row_frags(of, a.o + (m.q0 + qi) * a.ldo + h * 64, lane);
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
@@ -622,7 +666,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
   const float ls = a.lse[stat];
   const float L2 = ls == -INFINITY ? -NEG_BIG : ls * LOG2E;
   if (qr < m.nq && h2 == 0) a.delta[stat] = delta;
-  const RowCtx r = row_ctx<BIAS>(a, m, qi, w.h);
+  const RowCtx r = row_ctx<BIAS>(a, m, qi, h);
   const bool docs = a.doc_k != nullptr;
   const int wlo = wave_min_i(r.doc), whi = wave_max_i(r.doc), wlim0 = wave_min_i(r.lim), wlim1 = wave_max_i(r.lim);
   int dlo = wlo, dhi = whi, lim = wlim1;
@@ -630,10 +674,10 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
   f32x16 acc[2];
 #pragma unroll
   for (int i = 0; i < 16; ++i) { acc[0][i] = 0.f; acc[1][i] = 0.f; }
-  const bf16 *kb = a.k + m.k0 * a.ldk + (w.h / a.G) * 64, *vb = a.v + m.k0 * a.ldv + (w.h / a.G) * 64;
+  const bf16 *kb = a.k + m.k0 * a.ldk + (hk) * 64, *vb = a.v + m.k0 * a.ldv + (hk) * 64;
   const int ntiles = (lim + 63) / 64;
   for (int t0 = 0; t0 < ntiles; t0 += LIST) {
-    const int n = build_list(list, buf, t0, ntiles, docs ? a.rng_k + (long)w.s * a.nt_k : nullptr, dlo, dhi, tid);
+    const int n = build_list(list, buf, t0, ntiles, docs ? a.rng_k + (long)(w.unit / Hkv) * a.nt_k : nullptr, dlo, dhi, tid);
     Stage ks, vs;
     KeySide sd;
     auto fetch = [&](int e) {
@@ -656,18 +700,16 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
       char* tile = smem + (e & 1) * KT_BYTES;
       const TileRef tr = list[e];
       const int j0 = __builtin_amdgcn_readfirstlane(tr.t) * 64, lo = __builtin_amdgcn_readfirstlane(tr.lo), hi = __builtin_amdgcn_readfirstlane(tr.hi);
-      if (active && j0 < wlim1 && (!docs || (hi >= max(wlo, 0) && lo <= whi))) {
-        if (j0 + 64 <= wlim0 && (!docs || (lo == hi && wlo == lo && whi == lo)))
-          dq_tile<CAP, BIAS, false>(acc, qf, df, L2, delta, a, r, tile, j0, lane, false, false);
-        else
-          dq_tile<CAP, BIAS, true>(acc, qf, df, L2, delta, a, r, tile, j0, lane, docs, any_odd(tile + KT_ODD));
+      if (uniform(active && j0 < wlim1 && (!docs || (hi >= max(wlo, 0) && lo <= whi)))) {
+        const bool masked = !uniform(j0 + 64 <= wlim0 && (!docs || (lo == hi && wlo == lo && whi == lo)));
+        dq_tile<CAP, BIAS>(acc, qf, df, L2, delta, a, r, tile, j0, lane, fr, masked, docs, masked && any_odd(tile + KT_ODD));
       }
       if (e + 1 < n) put(smem + ((e + 1) & 1) * KT_BYTES);
       if (e + 2 < n) fetch(e + 2);
       __syncthreads();
     }
   }
-  if (qr < m.nq) store_acc_T(acc, a.dq + (m.q0 + qr) * a.lddq + w.h * 64, h2, a.scale);
+  if (qr < m.nq) store_acc_T(acc, a.dq + (m.q0 + qr) * a.lddq + h * 64, h2, a.scale);
 }
 
 // dK, dV of 128 keys: every wave holds 32 keys (the key on the lane) and the workgroup walks the 64-row query tiles of all heads that share them.
@@ -675,54 +717,49 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
 constexpr int QT_L = 16384, QT_D = QT_L + 256, QT_X = QT_D + 256, QT_Y = QT_X + 256, QT_LIM = QT_Y + 256, QT_DOC = QT_LIM + 256, QT_ODD = QT_DOC + 256, QT_BYTES = QT_ODD + 16;
 struct QuerySide { float L2, delta, x, y; int lim, doc; };
 
-template <bool CAP, int BIAS, bool MASKED>
+template <bool CAP, int BIAS>
 __device__ __forceinline__ void dkdv_tile(f32x16 (&dk)[2], f32x16 (&dv)[2], const bf16x8 (&kf)[4], const bf16x8 (&vf)[4], const ModArgs& a, int j, int docj,
-                                          const float (&pj)[2], float slope, const char* tile, int lane, bool docs, bool odd) {
+                                          const float (&pj)[2], float slope, const char* tile, int lane, const Frag& fr, bool masked, bool docs, bool odd) {
   const int h2 = lane >> 5;
-  const char *Qs = tile, *Ds = tile + 8192;
+  const unsigned Qs = lds_of(tile), Ds = Qs + 8192;
 #pragma unroll
   for (int qt = 0; qt < 2; ++qt) {
-    f32x16 s, p;
+    f32x16 s, p, rc;
 #pragma unroll
     for (int i = 0; i < 16; ++i) { s[i] = 0.f; p[i] = 0.f; }
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) s = MFMA_F32_32x32x16_H16(row_frag(Qs, qt * 32, ks, lane), kf[ks], s);
+    for (int ks = 0; ks < 4; ++ks) s = MFMA_F32_32x32x16_H16(row_at(Qs, qt * 32, fr.rf[ks]), kf[ks], s);
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) p = MFMA_F32_32x32x16_H16(row_frag(Ds, qt * 32, ks, lane), vf[ks], p);
+    for (int ks = 0; ks < 4; ++ks) p = MFMA_F32_32x32x16_H16(row_at(Ds, qt * 32, fr.rf[ks]), vf[ks], p);
+    modify<CAP, BIAS>(s, rc, a, pj, slope, tile + QT_X + qt * 128, h2, masked);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int ir = qt * 32 + 8 * g + 4 * h2;
       const f32x4 L2 = *(const f32x4*)(tile + QT_L + ir * 4), dl = *(const f32x4*)(tile + QT_D + ir * 4);
-      f32x4 px, py;
-      int4 lm, di;
-      if constexpr (BIAS > 0) px = *(const f32x4*)(tile + QT_X + ir * 4);
-      if constexpr (BIAS > 1) py = *(const f32x4*)(tile + QT_Y + ir * 4);
-      if constexpr (MASKED) lm = *(const int4*)(tile + QT_LIM + ir * 4);
-      if (MASKED && docs) di = *(const int4*)(tile + QT_DOC + ir * 4);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = 4 * g + e;
-        float z = s[i], rc = 0.f;
-        if constexpr (CAP) z = cap_score<MASKED>(z, a, rc);
-        if constexpr (BIAS > 0) {
-          const float d = dist<BIAS>(pj, px[e], BIAS > 1 ? py[e] : 0.f);
-          z = CAP ? z - slope * d : fmaf(z, a.c, -slope * d);
-        }
-        float pr = __builtin_amdgcn_exp2f((CAP || BIAS) ? z - L2[e] : fmaf(z, a.c, -L2[e]));
-        float ds = pr * (p[i] - dl[e]);
-        if constexpr (CAP) ds *= 4.f * rc * (1.f - rc);
-        if constexpr (MASKED) {
-          bool vis = j < (e == 0 ? lm.x : e == 1 ? lm.y : e == 2 ? lm.z : lm.w);
-          if (docs) vis = vis && (e == 0 ? di.x : e == 1 ? di.y : e == 2 ? di.z : di.w) == docj;
-          pr = vis ? pr : 0.f;
-          ds = vis ? ds : 0.f;
-        }
-        s[i] = ds;
+        const float pr = __builtin_amdgcn_exp2f((CAP || BIAS) ? s[i] - L2[e] : fmaf(s[i], a.c, -L2[e]));
+        s[i] = pr * (p[i] - dl[e]);
+        if constexpr (CAP) s[i] *= 4.f * rc[i] * (1.f - rc[i]);
         p[i] = pr;
       }
     }
-    tile_product<MASKED>(dv, Ds, qt * 32, p, lane, odd);
-    tile_product<MASKED>(dk, Qs, qt * 32, s, lane, odd);
+    if (masked) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int ir = qt * 32 + 8 * g + 4 * h2;
+        const int4 lm = *(const int4*)(tile + QT_LIM + ir * 4), di = docs ? *(const int4*)(tile + QT_DOC + ir * 4) : int4{0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool vis = j < pick(lm, e) && (!docs || pick(di, e) == docj);
+          p[4 * g + e] = vis ? p[4 * g + e] : 0.f;
+          s[4 * g + e] = vis ? s[4 * g + e] : 0.f;
+        }
+      }
+    }
+    tile_product(dv, Ds, qt * 32, p, fr, odd);
+    tile_product(dk, Qs, qt * 32, s, fr, odd);
   }
 }
 
@@ -732,15 +769,18 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
   __shared__ TileRef list[LIST];
   __shared__ int buf[12];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
-  const Where w = where(a, a.Hq / a.G);
-  const MSeq m = mseq(a, w.s);
-  const int jb = w.blk * 128;
+  const Frag fr = frag_consts(lane);
+  const Where w = where(a, a.nblk);
+  if (w.j >= a.nblk) return;
+  const int Hkv = a.Hq / a.G, hk = w.unit % Hkv;
+  const MSeq m = mseq(a, w.unit / Hkv);
+  const int jb = w.j * 128;
   if (jb >= m.nk) return;
   const int jr = jb + wave * 32 + (lane & 31), j = min(jr, m.nk - 1);
   const bool active = jb + wave * 32 < m.nk;
   bf16x8 kf[4], vf[4];
-  load_row_frags(kf, a.k + (m.k0 + j) * a.ldk + w.h * 64, lane);
-  load_row_frags(vf, a.v + (m.k0 + j) * a.ldv + w.h * 64, lane);
+  load_row_frags(kf, a.k + (m.k0 + j) * a.ldk + hk * 64, lane);
+  load_row_frags(vf, a.v + (m.k0 + j) * a.ldv + hk * 64, lane);
   const bool docs = a.doc_k != nullptr;
   const int docj = docs ? a.doc_k[m.k0 + j] : 0;
   float pj[2] = {0.f, 0.f};
@@ -755,12 +795,12 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
   const int first = m.nq == 0 ? 0 : (!a.causal || m.pre > jb) ? 0 : max(0, jb - m.off) / 64;
   const int ntiles = (m.nq + 63) / 64;
   for (int t0 = first; t0 < ntiles; t0 += LIST) {
-    const int n = build_list(list, buf, t0, ntiles, docs ? a.rng_q + (long)w.s * a.nt_q : nullptr, dlo, dhi, tid);
+    const int n = build_list(list, buf, t0, ntiles, docs ? a.rng_q + (long)(w.unit / Hkv) * a.nt_q : nullptr, dlo, dhi, tid);
     const int total = n * a.G;
     Stage qs, os;
     QuerySide sd;
     auto fetch = [&](int x) {      // entry x % n of head x / n
-      const int h = w.h * a.G + x / n, i0 = __builtin_amdgcn_readfirstlane(list[x % n].t) * 64;
+      const int h = hk * a.G + x / n, i0 = __builtin_amdgcn_readfirstlane(list[x % n].t) * 64;
       stage_load(qs, a.q + m.q0 * a.ldq + h * 64, a.ldq, i0, m.nq, tid);
       stage_load(os, a.d_o + m.q0 * a.lddo + h * 64, a.lddo, i0, m.nq, tid);
       if (tid < 64) {
@@ -798,12 +838,10 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
       const TileRef tr = list[x % n];
       const int i0 = __builtin_amdgcn_readfirstlane(tr.t) * 64, lo = __builtin_amdgcn_readfirstlane(tr.lo), hi = __builtin_amdgcn_readfirstlane(tr.hi);
       const int jw = jb + wave * 32, last = min(i0 + 63, m.nq - 1);
-      if (active && row_lim(a, m, last) > jw && (!docs || (hi >= max(wlo, 0) && lo <= whi))) {
-        const float slope = BIAS ? a.slopes[w.h * a.G + x / n] * LOG2E : 0.f;
-        if (i0 + 64 <= m.nq && jw + 32 <= m.nk && row_lim(a, m, i0) >= jw + 32 && (!docs || (lo >= 0 && lo == hi && wlo == lo && whi == lo)))
-          dkdv_tile<CAP, BIAS, false>(dk, dv, kf, vf, a, j, docj, pj, slope, tile, lane, false, false);
-        else
-          dkdv_tile<CAP, BIAS, true>(dk, dv, kf, vf, a, j, docj, pj, slope, tile, lane, docs, any_odd(tile + QT_ODD));
+      if (uniform(active && row_lim(a, m, last) > jw && (!docs || (hi >= max(wlo, 0) && lo <= whi)))) {
+        const float slope = BIAS ? a.slopes[hk * a.G + x / n] * LOG2E : 0.f;
+        const bool masked = !uniform(i0 + 64 <= m.nq && jw + 32 <= m.nk && row_lim(a, m, i0) >= jw + 32 && (!docs || (lo >= 0 && lo == hi && wlo == lo && whi == lo)));
+        dkdv_tile<CAP, BIAS>(dk, dv, kf, vf, a, j, docj, pj, slope, tile, lane, fr, masked, docs, masked && any_odd(tile + QT_ODD));
       }
       if (x + 1 < total) put(smem + ((x + 1) & 1) * QT_BYTES);
       if (x + 2 < total) fetch(x + 2);
@@ -811,8 +849,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
     }
   }
   if (jr < m.nk) {
-    store_acc_T(dk, a.dk + (m.k0 + jr) * a.lddk + w.h * 64, h2, a.scale);
-    store_acc_T(dv, a.dv + (m.k0 + jr) * a.lddv + w.h * 64, h2, 1.f);
+    store_acc_T(dk, a.dk + (m.k0 + jr) * a.lddk + hk * 64, h2, a.scale);
+    store_acc_T(dv, a.dv + (m.k0 + jr) * a.lddv + hk * 64, h2, 1.f);
   }
 }
 
@@ -886,7 +924,7 @@ int mod_check(const char* who, const apla_attn_mod_t* p, bool backward) {
   }
   const Plan pl = plan_of(*p, backward);
   APLA_REQUIRE(pl.bytes == 0 || (p->workspace && apla_aligned16(p->workspace) && p->workspace_bytes >= pl.bytes), "%s: needs %ld bytes of 16-byte aligned workspace (got %ld)", who, pl.bytes, p->workspace_bytes);
-  const long nb = (long)p->S * p->Hq * (((long)(p->max_q > p->max_k ? p->max_q : p->max_k) + 127) / 128);
+  const long nb = (long)p->S * p->Hkv * 8 * ((long)(p->Hq / p->Hkv) * (((long)(p->max_q > p->max_k ? p->max_q : p->max_k) + 127) / 128) + 1);
   APLA_REQUIRE(nb < (1L << 31), "%s: too many blocks", who);
   return APLA_OK;
 }
@@ -903,6 +941,7 @@ ModArgs mod_args(const apla_attn_mod_t& p, const Plan& pl) {
   a.nt_q = (p.max_q + 63) / 64; a.nt_k = (p.max_k + 63) / 64;
   char* ws = (char*)p.workspace;
   if (p.doc_k) { a.rng_k = (const int2*)(ws + pl.rng_k); a.rng_q = (const int2*)(ws + pl.rng_q); }
+  a.np = unit_parts((long)p.S * p.Hkv);
   a.nsplit = pl.nsplit; a.chunk = pl.chunk; a.nrt = pl.nrt;
   a.part_o = (float*)(ws + pl.part);
   a.part_ml = a.part_o + (long)p.S * p.Hkv * pl.nrt * pl.nsplit * 32 * 64;
@@ -943,6 +982,7 @@ extern "C" int apla_attn_mod_fwd(const apla_attn_mod_t* p, hipStream_t stream) {
   if (rc != APLA_OK) return rc;
   const Plan pl = plan_of(*p, false);
   ModArgs a = mod_args(*p, pl);
+  const long units = (long)p->S * p->Hkv;
   if (a.doc_k) launch_ranges(a, false, stream);
   if (pl.rows) {
     const dim3 grid((unsigned)(pl.nrt * pl.nsplit), (unsigned)p->Hkv, (unsigned)p->S);
@@ -950,7 +990,7 @@ extern "C" int apla_attn_mod_fwd(const apla_attn_mod_t* p, hipStream_t stream) {
     if (pl.nsplit > 1) hipLaunchKernelGGL(attn_mod_join_kernel, dim3((unsigned)pl.nrt, (unsigned)p->Hkv, (unsigned)p->S), dim3(256), 0, stream, a);
   } else {
     a.nblk = (p->max_q + 127) / 128;
-    const dim3 grid((unsigned)((long)p->S * p->Hq * a.nblk));
+    const dim3 grid((unsigned)unit_grid(units, a.np, (long)a.G * a.nblk));
     APLA_MOD_LAUNCH(attn_mod_fwd_kernel, grid);
   }
   APLA_CHECK_LAUNCH("apla_attn_mod_fwd");
@@ -962,15 +1002,16 @@ extern "C" int apla_attn_mod_bwd(const apla_attn_mod_t* p, hipStream_t stream) {
   if (rc != APLA_OK) return rc;
   const Plan pl = plan_of(*p, true);
   ModArgs a = mod_args(*p, pl);
+  const long units = (long)p->S * p->Hkv;
   if (a.doc_k) { launch_ranges(a, false, stream); launch_ranges(a, true, stream); }
   a.nblk = (p->max_q + 127) / 128;
   {
-    const dim3 grid((unsigned)((long)p->S * p->Hq * a.nblk));
+    const dim3 grid((unsigned)unit_grid(units, a.np, (long)a.G * a.nblk));
     APLA_MOD_LAUNCH(attn_mod_dq_kernel, grid);
   }
   a.nblk = (p->max_k + 127) / 128;
   {
-    const dim3 grid((unsigned)((long)p->S * p->Hkv * a.nblk));
+    const dim3 grid((unsigned)unit_grid(units, a.np, a.nblk));
     APLA_MOD_LAUNCH(attn_mod_dkdv_kernel, grid);
   }
   APLA_CHECK_LAUNCH("apla_attn_mod_bwd");
