@@ -9,7 +9,7 @@
 // a wave runs a tile without a mask where lim and the ids say that all of it is visible.
 //
 // The products are those of attention.hip (S^T = K Q^T with the query row on the lane, P^T from the accumulator as the next operand).
-// In a masked tile a weight of zero times a non-finite value is zero (mfma_select): what stands in masked places never matters.
+// In a masked tile a weight of zero times a non-finite value is zero (poison_bits): what stands in masked places never matters.
 // P and dS are rounded to 16 bits as MFMA operands (half a step of values <= 256 resp. of dS, relative); scores, softmax
 // statistics, sums and accumulators are fp32.
 #include "attn_tiles.h"
@@ -90,26 +90,6 @@ __device__ __forceinline__ unsigned nonfinite_bits(const bf16x8& f) {
   for (int i = 0; i < 4; ++i) r |= (w[i] & 0x7fff7fffu) + EXP_STEP;
   return r & 0x80008000u;
 }
-// acc += A B with 0 * non-finite = 0.  Non-finite entries of A are taken out; the places that a weight other than zero leads to them
-// are found by a second product of the two indicator matrices and become NaN.
-__device__ __forceinline__ void mfma_select(f32x16& acc, const bf16x8& af, const bf16x8& bf) {
-  u32x4 fin = __builtin_bit_cast(u32x4, af), bad, wt = __builtin_bit_cast(u32x4, bf);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const unsigned x = fin[i], y = wt[i];
-    const bool bl = (x & EXP_LO) == EXP_LO, bh = (x & EXP_HI) == EXP_HI;
-    fin[i] = (bl ? 0u : x & 0xffffu) | (bh ? 0u : x & 0xffff0000u);
-    bad[i] = (bl ? ONE_BITS : 0u) | (bh ? ONE_BITS << 16 : 0u);
-    wt[i] = ((y & 0x7fffu) ? ONE_BITS : 0u) | ((y & 0x7fff0000u) ? ONE_BITS << 16 : 0u);
-  }
-  acc = MFMA_F32_32x32x16_H16(__builtin_bit_cast(bf16x8, fin), bf, acc);
-  f32x16 hits;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) hits[i] = 0.f;
-  hits = MFMA_F32_32x32x16_H16(__builtin_bit_cast(bf16x8, bad), __builtin_bit_cast(bf16x8, wt), hits);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) acc[i] = hits[i] > 0.f ? __builtin_nanf("") : acc[i];
-}
 // ---- fragments by lane constants: tile_off's swizzle looks at bits 1-3 of the row only, so next to a first row that is a multiple of 16 the byte offset
 // of a fragment is that row * 128 + a constant of the lane; left to itself hipcc keeps an address per fragment (40 registers)
 struct Frag { unsigned rf[4], tr[4]; };
@@ -136,43 +116,87 @@ __device__ __forceinline__ bf16x8 tr_at(unsigned tile, int row, unsigned c0, uns
   return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
-// acc[2] += tile^T w: the transposed rows rbase .. rbase + 31 of an LDS tile times the weights that the accumulator w holds for them.
-// `odd` (the same for the wave): the tile may hold non-finite values and w zeros for them.
-__device__ __forceinline__ void tile_product(f32x16 (&acc)[2], unsigned tile, int rbase, const f32x16& w, const Frag& fr, bool odd) {
-  const bf16x8 w0 = acc_to_operand(w, 0), w1 = acc_to_operand(w, 1);
-  if (__builtin_expect(odd, 0)) {
+// The 32 transposed fragments' product acc[2] += tile^T w: rows rbase .. rbase + 31 of an LDS tile times the weights that the accumulator w holds for them.
+struct TrFrags { bf16x8 f[4]; };      // [dt][sk]
+__device__ __forceinline__ void tr_load(TrFrags& t, unsigned tile, int rbase, const Frag& fr) {
 #pragma unroll
-    for (int dt = 0; dt < 2; ++dt) {
-      mfma_select(acc[dt], tr_at(tile, rbase, fr.tr[2 * dt], fr.tr[2 * dt + 1]), w0);
-      mfma_select(acc[dt], tr_at(tile, rbase + 16, fr.tr[2 * dt], fr.tr[2 * dt + 1]), w1);
-    }
-  } else {
+  for (int sk = 0; sk < 2; ++sk)
 #pragma unroll
-    for (int dt = 0; dt < 2; ++dt) {
-      acc[dt] = MFMA_F32_32x32x16_H16(tr_at(tile, rbase, fr.tr[2 * dt], fr.tr[2 * dt + 1]), w0, acc[dt]);
-      acc[dt] = MFMA_F32_32x32x16_H16(tr_at(tile, rbase + 16, fr.tr[2 * dt], fr.tr[2 * dt + 1]), w1, acc[dt]);
-    }
+    for (int dt = 0; dt < 2; ++dt) t.f[2 * dt + sk] = tr_at(tile, rbase + 16 * sk, fr.tr[2 * dt], fr.tr[2 * dt + 1]);
+}
+__device__ __forceinline__ void tr_product(f32x16 (&acc)[2], const TrFrags& t, const f32x16& w) {
+#pragma unroll
+  for (int sk = 0; sk < 2; ++sk) {
+    const bf16x8 wb = acc_to_operand(w, sk);
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt) acc[dt] = MFMA_F32_32x32x16_H16(t.f[2 * dt + sk], wb, acc[dt]);
   }
 }
+
+// Zero times a non-finite value is zero: where a tile that holds such values meets a mask, the product runs over a copy of the tile with those values
+// taken out (clean_tile), and the results that a weight other than zero would lead one to are remembered as bits (poison_bits: the product of
+// the two indicator matrices; bit 16 dt + i for accumulator element [dt][i]) and become NaN at the end (apply_poison).
+__device__ __forceinline__ bf16x8 finite_part(const bf16x8& f) {
+  u32x4 w = __builtin_bit_cast(u32x4, f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = ((w[i] & EXP_LO) == EXP_LO ? 0u : w[i] & 0xffffu) | ((w[i] & EXP_HI) == EXP_HI ? 0u : w[i] & 0xffff0000u);
+  return __builtin_bit_cast(bf16x8, w);
+}
+__device__ __forceinline__ unsigned poison_bits(unsigned raw, int rbase, const f32x16& w, const Frag& fr) {
+  unsigned m = 0;
+#pragma unroll
+  for (int dt = 0; dt < 2; ++dt) {
+    f32x16 hits;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) hits[i] = 0.f;
+#pragma unroll
+    for (int sk = 0; sk < 2; ++sk) {
+      u32x4 x = __builtin_bit_cast(u32x4, tr_at(raw, rbase + 16 * sk, fr.tr[2 * dt], fr.tr[2 * dt + 1])), y = __builtin_bit_cast(u32x4, acc_to_operand(w, sk));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = ((x[i] & EXP_LO) == EXP_LO ? ONE_BITS : 0u) | ((x[i] & EXP_HI) == EXP_HI ? ONE_BITS << 16 : 0u);
+        y[i] = ((y[i] & 0x7fffu) ? ONE_BITS : 0u) | ((y[i] & 0x7fff0000u) ? ONE_BITS << 16 : 0u);
+      }
+      hits = MFMA_F32_32x32x16_H16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), hits);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m |= hits[i] > 0.f ? 1u << (16 * dt + i) : 0u;
+  }
+  return m;
+}
+__device__ __forceinline__ void apply_poison(f32x16 (&acc)[2], unsigned m) {
+  if (__ballot(m != 0) == 0) return;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) acc[i >> 4][i & 15] = (m >> i) & 1 ? __builtin_nanf("") : acc[i >> 4][i & 15];
+}
+
 // a condition that is the same for the whole wave, as a scalar: branches on it need no execution mask
 __device__ __forceinline__ bool uniform(bool c) { return __builtin_amdgcn_readfirstlane((int)c) != 0; }
 
 // ---- staging: 64 rows x 64 columns by 256 threads (two 16-byte pieces each) through registers; rows past nrows read row nrows - 1
 struct Stage { bf16x8 v[2]; };
 __device__ __forceinline__ bool stage_odd(const Stage& t) { return __ballot((nonfinite_bits(t.v[0]) | nonfinite_bits(t.v[1])) != 0) != 0; }
-__device__ __forceinline__ void stage_load(Stage& t, const bf16* base, long ld, int row0, int nrows, int tid) {
+// byte offset of a thread's first piece from the tile's first row (its second lies 32 rows further)
+__device__ __forceinline__ unsigned stage_off(long ld, int tid) { return (unsigned)((tid >> 3) * (int)ld * 2 + (tid & 7) * 16); }
+__device__ __forceinline__ void stage_load(Stage& t, const bf16* base, long ld, unsigned off, int row0, int nrows, int tid) {
+  const char* p = (const char*)(base + (long)row0 * ld);
+  if (row0 + 64 <= nrows) {       // whole tile: scalar addresses next to the lane's constant
+    t.v[0] = *(const bf16x8*)(p + off);
+    t.v[1] = *(const bf16x8*)(p + ld * 64 + off);
+  } else {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int e = tid + i * 256;
-    t.v[i] = *(const bf16x8*)(base + (long)min(row0 + (e >> 3), nrows - 1) * ld + (e & 7) * 8);
+    for (int i = 0; i < 2; ++i) t.v[i] = *(const bf16x8*)(p + (long)min((tid >> 3) + 32 * i, nrows - 1 - row0) * ld * 2 + (tid & 7) * 16);
   }
 }
 __device__ __forceinline__ void stage_store(const Stage& t, char* lds, int tid) {
+  const int o = tile_off(tid >> 3, tid & 7);
+  *(bf16x8*)(lds + o) = t.v[0];
+  *(bf16x8*)(lds + o + 32 * 128) = t.v[1];
+}
+// copy of an 8 KB LDS tile without its non-finite values, by the whole workgroup (a barrier before it is used)
+__device__ __forceinline__ void clean_tile(const char* raw, char* clean, int tid) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int e = tid + i * 256;
-    *(bf16x8*)(lds + tile_off(e >> 3, e & 7)) = t.v[i];
-  }
+  for (int i = 0; i < 2; ++i) *(bf16x8*)(clean + (tid + i * 256) * 16) = finite_part(*(const bf16x8*)(raw + (tid + i * 256) * 16));
 }
 
 // position of a row: its own coordinates, or its place in the sequence (BIAS 1 without positions)
@@ -238,20 +262,40 @@ __device__ __forceinline__ void modify(f32x16& s, f32x16& r, const ModArgs& a, c
   }
 }
 
+// both halves of a wave hold the same rows: their larger value, in both
+__device__ __forceinline__ float half_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+  return fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
+}
+
+// masked: some of the 64 keys are hidden from some of the wave's rows.  odd: V holds non-finite values; `clean` is then its copy without them.
 template <bool CAP, int BIAS>
-__device__ __forceinline__ void fwd_tile(f32x16 (&acc)[2], RowState& st, const bf16x8 (&qf)[4], const ModArgs& a, const RowCtx& r, const char* tile,
-                                         int j0, int lane, const Frag& fr, bool masked, bool docs, bool odd) {
+__device__ __forceinline__ void fwd_tile(f32x16 (&acc)[2], RowState& st, unsigned& poison, const bf16x8 (&qf)[4], const ModArgs& a, const RowCtx& r,
+                                         const char* tile, const char* clean, int j0, int lane, const Frag& fr, bool masked, bool docs, bool odd) {
   const int h2 = lane >> 5;
   const float zm = (CAP || BIAS) ? 1.f : a.c;
-  const unsigned Ks = lds_of(tile), Vs = Ks + 8192;
+  const unsigned Ks = lds_of(tile), Vs = odd ? lds_of(clean) : Ks + 8192;
   f32x16 s[2], unused;
+  {
+    bf16x8 kf[2][4];
 #pragma unroll
-  for (int kt = 0; kt < 2; ++kt) {
+    for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[kt][i] = 0.f;
+      for (int kt = 0; kt < 2; ++kt) kf[kt][ks] = row_at(Ks, kt * 32, fr.rf[ks]);
+    __builtin_amdgcn_sched_barrier(0);     // all eight reads under way before the first product waits for one
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) s[kt] = MFMA_F32_32x32x16_H16(row_at(Ks, kt * 32, fr.rf[ks]), qf[ks], s[kt]);
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[kt][i] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) s[kt] = MFMA_F32_32x32x16_H16(kf[kt][ks], qf[ks], s[kt]);
   }
+  TrFrags vf[2];                           // V's fragments arrive under the softmax
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt) tr_load(vf[kt], Vs, kt * 32, fr);
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt) modify<CAP, BIAS>(s[kt], unused, a, r.pos, r.slope, tile + KT_POS + kt * 128, h2, masked);
   if (masked) {
@@ -270,7 +314,7 @@ __device__ __forceinline__ void fwd_tile(f32x16 (&acc)[2], RowState& st, const b
   for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kt][i]);
-  mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+  mx = half_max(mx);
   if (__ballot((mx - st.m) * zm > LAZY)) {
     const float m_new = fmaxf(st.m, mx), alpha = __builtin_amdgcn_exp2f((st.m - m_new) * zm);
     st.m = m_new;
@@ -279,33 +323,23 @@ __device__ __forceinline__ void fwd_tile(f32x16 (&acc)[2], RowState& st, const b
     for (int i = 0; i < 16; ++i) { acc[0][i] *= alpha; acc[1][i] *= alpha; }
   }
   const float mc = st.m * zm;
-  if (odd) {      // (both forms of the products behind their own branch: the usual one is one straight run of instructions)
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
+  for (int kt = 0; kt < 2; ++kt) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[kt][i] = __builtin_amdgcn_exp2f((CAP || BIAS) ? s[kt][i] - mc : fmaf(s[kt][i], zm, -mc));
-        st.l += s[kt][i];
-      }
-      tile_product(acc, Vs, kt * 32, s[kt], fr, true);
+    for (int i = 0; i < 16; ++i) {
+      s[kt][i] = __builtin_amdgcn_exp2f((CAP || BIAS) ? s[kt][i] - mc : fmaf(s[kt][i], zm, -mc));
+      st.l += s[kt][i];
     }
-  } else {
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[kt][i] = __builtin_amdgcn_exp2f((CAP || BIAS) ? s[kt][i] - mc : fmaf(s[kt][i], zm, -mc));
-        st.l += s[kt][i];
-      }
-      tile_product(acc, Vs, kt * 32, s[kt], fr, false);
-    }
+    if (__builtin_expect(odd, 0)) poison |= poison_bits(Ks + 8192, kt * 32, s[kt], fr);
+    tr_product(acc, vf[kt], s[kt]);
   }
 }
 
 // ---- the list of key tiles that rows with (lim_max, documents dmin..dmax) can see, one pass of up to LIST tiles from t0
-struct TileRef { int t, lo, hi; };
-// n entries in list[]; all threads call it, ends with a barrier
-__device__ __forceinline__ int build_list(TileRef* list, int* cnt, int t0, int ntiles, const int2* rng, int dmin, int dmax, int tid) {
+struct TileRef { int t, lo, hi, whole; };      // whole: all of it is visible to all rows of the workgroup
+// n entries in list[] and three more that repeat the last; all threads call it, ends with a barrier.  Tiles w0 .. w1 - 1 lie
+// within the limits of all rows.
+__device__ __forceinline__ int build_list(TileRef* list, int* cnt, int t0, int ntiles, int w0, int w1, const int2* rng, int dmin, int dmax, int tid) {
   const int t = t0 + tid;
   bool vis = t < ntiles;
   int2 r = {0, 0};
@@ -319,19 +353,30 @@ __device__ __forceinline__ int build_list(TileRef* list, int* cnt, int t0, int n
   int base = 0, n = 0;
 #pragma unroll
   for (int w = 0; w < 4; ++w) { const int c = cnt[w]; base += w < (tid >> 6) ? c : 0; n += c; }
-  if (vis) list[base + __popcll(b & ((1ull << (tid & 63)) - 1))] = {t, r.x, r.y};
+  if (vis) {
+    const int at = base + __popcll(b & ((1ull << (tid & 63)) - 1));
+    const TileRef e = {t, r.x, r.y, t >= w0 && t < w1 && (!rng || (r.x >= 0 && r.x == r.y && dmin == r.x && dmax == r.x))};
+    list[at] = e;
+    if (at == n - 1) list[n] = list[n + 1] = list[n + 2] = e;
+  }
   __syncthreads();
   return n;
 }
 
-// document range of the rows a workgroup holds, for its list (LDS exchange of the waves' own ranges)
-__device__ __forceinline__ void group_range(int& lo, int& hi, int& lim, int* buf, int wave, int lane) {
-  if (lane == 0) { buf[wave] = lo; buf[4 + wave] = hi; buf[8 + wave] = lim; }
+// document range and limits (smallest, largest) of the rows a workgroup holds, for its list (LDS exchange of the waves' own)
+__device__ __forceinline__ void group_range(int& lo, int& hi, int& lim0, int& lim, int* buf, int wave, int lane) {
+  if (lane == 0) { buf[wave] = lo; buf[4 + wave] = hi; buf[8 + wave] = lim; buf[12 + wave] = lim0; }
   __syncthreads();
   lo = min(min(buf[0], buf[1]), min(buf[2], buf[3]));
   hi = max(max(buf[4], buf[5]), max(buf[6], buf[7]));
   lim = max(max(buf[8], buf[9]), max(buf[10], buf[11]));
+  lim0 = min(min(buf[12], buf[13]), min(buf[14], buf[15]));
   __syncthreads();
+}
+
+// a list entry as scalars
+__device__ __forceinline__ TileRef scalar_ref(const TileRef& r) {
+  return {__builtin_amdgcn_readfirstlane(r.t), __builtin_amdgcn_readfirstlane(r.lo), __builtin_amdgcn_readfirstlane(r.hi), __builtin_amdgcn_readfirstlane(r.whole)};
 }
 
 // any of the four waves' verdicts
@@ -389,9 +434,9 @@ __device__ __forceinline__ RowCtx row_ctx(const ModArgs& a, const MSeq& m, int i
 // ------------------------------------------------------------------------------------------------ forward
 template <bool CAP, int BIAS>
 __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
-  __shared__ __attribute__((aligned(16))) char smem[2 * KT_BYTES];
-  __shared__ TileRef list[LIST];
-  __shared__ int buf[12];
+  __shared__ __attribute__((aligned(16))) char smem[2 * KT_BYTES], clean[8192];
+  __shared__ TileRef list[LIST + 3];
+  __shared__ int buf[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
   const Frag fr = frag_consts(lane);
   const Where w = where(a, a.G * a.nblk);
@@ -408,48 +453,68 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
   const RowCtx r = row_ctx<BIAS>(a, m, qi, h);
   const bool docs = a.doc_k != nullptr;
   const int wlo = wave_min_i(r.doc), whi = wave_max_i(r.doc), wlim0 = wave_min_i(r.lim), wlim1 = wave_max_i(r.lim);
-  int dlo = wlo, dhi = whi, lim = wlim1;
-  group_range(dlo, dhi, lim, buf, wave, lane);
+  int dlo = wlo, dhi = whi, lim0 = wlim0, lim = wlim1;
+  group_range(dlo, dhi, lim0, lim, buf, wave, lane);
 
   f32x16 acc[2];
 #pragma unroll
   for (int i = 0; i < 16; ++i) { acc[0][i] = 0.f; acc[1][i] = 0.f; }
   RowState st = {NEG_BIG, 0.f};
+  unsigned poison = 0;
   const bf16 *kb = a.k + m.k0 * a.ldk + (hk) * 64, *vb = a.v + m.k0 * a.ldv + (hk) * 64;
+  const unsigned offk = stage_off(a.ldk, tid), offv = stage_off(a.ldv, tid);
   const int ntiles = (lim + 63) / 64;
   for (int t0 = 0; t0 < ntiles; t0 += LIST) {
-    const int n = build_list(list, buf, t0, ntiles, docs ? a.rng_k + (long)(w.unit / Hkv) * a.nt_k : nullptr, dlo, dhi, tid);
+    const int n = build_list(list, buf, t0, ntiles, 0, lim0 / 64, docs ? a.rng_k + (long)(w.unit / Hkv) * a.nt_k : nullptr, dlo, dhi, tid);
     Stage ks, vs;
     KeySide sd;
-    auto fetch = [&](int e) {
-      const int j0 = __builtin_amdgcn_readfirstlane(list[e].t) * 64;
-      stage_load(ks, kb, a.ldk, j0, m.nk, tid);
-      stage_load(vs, vb, a.ldv, j0, m.nk, tid);
-      side_load<BIAS>(sd, a, m, j0, tid);
+    auto fetch = [&](int t) {
+      stage_load(ks, kb, a.ldk, offk, t * 64, m.nk, tid);
+      stage_load(vs, vb, a.ldv, offv, t * 64, m.nk, tid);
+      side_load<BIAS>(sd, a, m, t * 64, tid);
     };
-    auto put = [&](char* tile) {
+    auto put = [&](char* tile, bool whole) {
       stage_store(ks, tile, tid);
       stage_store(vs, tile + 8192, tid);
       side_store<BIAS>(sd, tile, a, tid);
-      const bool odd = stage_odd(vs);
-      if (lane == 0) *(int*)(tile + KT_ODD + wave * 4) = odd;
-    };
-    if (n > 0) { fetch(0); put(smem); }
-    if (n > 1) fetch(1);
-    __syncthreads();
-    for (int e = 0; e < n; ++e) {
-      char* tile = smem + (e & 1) * KT_BYTES;
-      const TileRef tr = list[e];
-      const int j0 = __builtin_amdgcn_readfirstlane(tr.t) * 64, lo = __builtin_amdgcn_readfirstlane(tr.lo), hi = __builtin_amdgcn_readfirstlane(tr.hi);
-      if (uniform(active && j0 < wlim1 && (!docs || (hi >= max(wlo, 0) && lo <= whi)))) {
-        const bool masked = !uniform(j0 + 64 <= wlim0 && (!docs || (lo == hi && wlo == lo && whi == lo)));
-        fwd_tile<CAP, BIAS>(acc, st, qf, a, r, tile, j0, lane, fr, masked, docs, masked && any_odd(tile + KT_ODD));
+      if (!whole) {
+        const bool odd = stage_odd(vs);
+        if (lane == 0) *(int*)(tile + KT_ODD + wave * 4) = odd;
       }
-      if (e + 1 < n) put(smem + ((e + 1) & 1) * KT_BYTES);
-      if (e + 2 < n) fetch(e + 2);
+    };
+    TileRef cur, next;
+    int t2 = 0;
+    if (n > 0) {
+      cur = scalar_ref(list[0]); next = scalar_ref(list[1]);
+      t2 = __builtin_amdgcn_readfirstlane(list[2].t);
+      fetch(cur.t);
+      put(smem, cur.whole);
+      fetch(next.t);
+    }
+    __syncthreads();
+    for (int e = 0; e < n; ++e) {      // tile e is in LDS, e + 1 in registers; e + 2 is requested when those are free
+      char* tile = smem + (e & 1) * KT_BYTES;
+      const TileRef ahead = list[e + 2 < n ? e + 2 : n - 1];
+      const int t3 = list[e + 3 < n ? e + 3 : n - 1].t;
+      const int j0 = cur.t * 64;
+      const bool odd = !cur.whole && any_odd(tile + KT_ODD);
+      if (__builtin_expect(odd, 0)) {
+        clean_tile(tile + 8192, clean, tid);
+        __syncthreads();
+      }
+      if (uniform(active && j0 < wlim1 && (!docs || (cur.hi >= max(wlo, 0) && cur.lo <= whi)))) {
+        const bool masked = !cur.whole && !uniform(j0 + 64 <= wlim0 && (!docs || (cur.lo == cur.hi && wlo == cur.lo && whi == cur.lo)));
+        fwd_tile<CAP, BIAS>(acc, st, poison, qf, a, r, tile, clean, j0, lane, fr, masked, docs, masked && odd);
+      }
+      if (e + 1 < n) put(smem + ((e + 1) & 1) * KT_BYTES, next.whole);
+      if (e + 2 < n) fetch(t2);
+      cur = next;
+      next = scalar_ref(ahead);
+      t2 = __builtin_amdgcn_readfirstlane(t3);
       __syncthreads();
     }
   }
+  apply_poison(acc, poison);
   const float l = st.l + __shfl_xor(st.l, 32, 64);
   if (qr < m.nq) {
     store_acc_T(acc, a.o + (m.q0 + qr) * a.ldo + h * 64, h2, l != 0.f ? 1.f / l : 0.f);
@@ -474,7 +539,7 @@ __device__ __forceinline__ void wstage_store(const WStage& t, char* lds, int lan
 
 template <bool CAP, int BIAS>
 __global__ __launch_bounds__(256, 1) void attn_mod_rows_kernel(ModArgs a) {
-  __shared__ __attribute__((aligned(16))) char smem[4 * KT_BYTES];
+  __shared__ __attribute__((aligned(16))) char smem[4 * (KT_BYTES + 8192)];
   __shared__ float ml[4][2][32];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
   const Frag fr = frag_consts(lane);
@@ -491,8 +556,9 @@ __global__ __launch_bounds__(256, 1) void attn_mod_rows_kernel(ModArgs a) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) { acc[0][i] = 0.f; acc[1][i] = 0.f; }
   RowState st = {NEG_BIG, 0.f};
+  unsigned poison = 0;
   const int jb = sp * a.chunk, je = min(wlim1, jb + a.chunk);
-  char* tile = smem + wave * KT_BYTES;
+  char* tile = smem + wave * (KT_BYTES + 8192);
   const bf16 *kb = a.k + m.k0 * a.ldk + hk * 64, *vb = a.v + m.k0 * a.ldv + hk * 64;
   if (jb + wave * 64 < je) {
     bf16x8 qf[4];
@@ -522,11 +588,19 @@ __global__ __launch_bounds__(256, 1) void attn_mod_rows_kernel(ModArgs a) {
         any = g.y >= max(wlo, 0) && g.x <= whi;
         full = full && g.x == g.y && wlo == g.x && whi == g.x;
       }
-      if (uniform(any)) fwd_tile<CAP, BIAS>(acc, st, qf, a, r, tile, j0, lane, fr, !uniform(full), docs, !uniform(full) && odd);
+      const bool masked = !uniform(full);
+      if (masked && odd) {      // this wave's own copy of V
+#pragma unroll
+        for (int i = 0; i < 8; ++i) *(bf16x8*)(tile + KT_BYTES + (i * 64 + lane) * 16) = finite_part(*(const bf16x8*)(tile + 8192 + (i * 64 + lane) * 16));
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("" ::: "memory");
+      }
+      if (uniform(any)) fwd_tile<CAP, BIAS>(acc, st, poison, qf, a, r, tile, tile + KT_BYTES, j0, lane, fr, masked, docs, masked && odd);
       __builtin_amdgcn_wave_barrier();
       asm volatile("" ::: "memory");
     }
   }
+  apply_poison(acc, poison);
   // join the four waves: [32 rows][64] fp32 per wave in its own 8 KB (rows XOR-spread over the banks by their 16-byte chunk)
   float* mine = (float*)(smem + wave * 8192);
   const float l = st.l + __shfl_xor(st.l, 32, 64);
@@ -601,19 +675,24 @@ __global__ __launch_bounds__(256) void attn_mod_join_kernel(ModArgs a) {
 // ------------------------------------------------------------------------------------------------ backward
 // P = exp2(z - L2) from the forward's lse, dS = P (dP - delta), with the cap times 1 - tanh^2 = 4 r (1 - r), r = 1 / (1 + e^(2 s / cap))
 template <bool CAP, int BIAS>
-__device__ __forceinline__ void dq_tile(f32x16 (&acc)[2], const bf16x8 (&qf)[4], const bf16x8 (&df)[4], float L2, float delta, const ModArgs& a,
-                                        const RowCtx& r, const char* tile, int j0, int lane, const Frag& fr, bool masked, bool docs, bool odd) {
+__device__ __forceinline__ void dq_tile(f32x16 (&acc)[2], unsigned& poison, const bf16x8 (&qf)[4], const bf16x8 (&df)[4], float L2, float delta, const ModArgs& a,
+                                        const RowCtx& r, const char* tile, const char* clean, int j0, int lane, const Frag& fr, bool masked, bool docs, bool odd) {
   const int h2 = lane >> 5;
-  const unsigned Ks = lds_of(tile), Vs = Ks + 8192;
+  const unsigned Ks = lds_of(tile), Vs = Ks + 8192, Kt = odd ? lds_of(clean) : Ks;
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt) {
     f32x16 s, p, rc;
+    bf16x8 kf[4], vf[4];
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) { kf[ks] = row_at(Ks, kt * 32, fr.rf[ks]); vf[ks] = row_at(Vs, kt * 32, fr.rf[ks]); }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < 16; ++i) { s[i] = 0.f; p[i] = 0.f; }
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) s = MFMA_F32_32x32x16_H16(row_at(Ks, kt * 32, fr.rf[ks]), qf[ks], s);
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) p = MFMA_F32_32x32x16_H16(row_at(Vs, kt * 32, fr.rf[ks]), df[ks], p);
+    for (int ks = 0; ks < 4; ++ks) { s = MFMA_F32_32x32x16_H16(kf[ks], qf[ks], s); p = MFMA_F32_32x32x16_H16(vf[ks], df[ks], p); }
+    TrFrags tk;
+    tr_load(tk, Kt, kt * 32, fr);
+    __builtin_amdgcn_sched_barrier(0);
     modify<CAP, BIAS>(s, rc, a, r.pos, r.slope, tile + KT_POS + kt * 128, h2, masked);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -628,16 +707,17 @@ __device__ __forceinline__ void dq_tile(f32x16 (&acc)[2], const bf16x8 (&qf)[4],
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[4 * g + e] = j0 + jr + e < r.lim && (!docs || pick(dj, e) == r.doc) ? s[4 * g + e] : 0.f;
       }
+      if (__builtin_expect(odd, 0)) poison |= poison_bits(Ks, kt * 32, s, fr);
     }
-    tile_product(acc, Ks, kt * 32, s, fr, odd);
+    tr_product(acc, tk, s);
   }
 }
 
 template <bool CAP, int BIAS>
 __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
-  __shared__ __attribute__((aligned(16))) char smem[2 * KT_BYTES];
-  __shared__ TileRef list[LIST];
-  __shared__ int buf[12];
+  __shared__ __attribute__((aligned(16))) char smem[2 * KT_BYTES], clean[8192];
+  __shared__ TileRef list[LIST + 3];
+  __shared__ int buf[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
   const Frag fr = frag_consts(lane);
   const Where w = where(a, a.G * a.nblk);
@@ -669,46 +749,66 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
   const RowCtx r = row_ctx<BIAS>(a, m, qi, h);
   const bool docs = a.doc_k != nullptr;
   const int wlo = wave_min_i(r.doc), whi = wave_max_i(r.doc), wlim0 = wave_min_i(r.lim), wlim1 = wave_max_i(r.lim);
-  int dlo = wlo, dhi = whi, lim = wlim1;
-  group_range(dlo, dhi, lim, buf, wave, lane);
+  int dlo = wlo, dhi = whi, lim0 = wlim0, lim = wlim1;
+  group_range(dlo, dhi, lim0, lim, buf, wave, lane);
   f32x16 acc[2];
 #pragma unroll
   for (int i = 0; i < 16; ++i) { acc[0][i] = 0.f; acc[1][i] = 0.f; }
+  unsigned poison = 0;
   const bf16 *kb = a.k + m.k0 * a.ldk + (hk) * 64, *vb = a.v + m.k0 * a.ldv + (hk) * 64;
+  const unsigned offk = stage_off(a.ldk, tid), offv = stage_off(a.ldv, tid);
   const int ntiles = (lim + 63) / 64;
   for (int t0 = 0; t0 < ntiles; t0 += LIST) {
-    const int n = build_list(list, buf, t0, ntiles, docs ? a.rng_k + (long)(w.unit / Hkv) * a.nt_k : nullptr, dlo, dhi, tid);
+    const int n = build_list(list, buf, t0, ntiles, 0, lim0 / 64, docs ? a.rng_k + (long)(w.unit / Hkv) * a.nt_k : nullptr, dlo, dhi, tid);
     Stage ks, vs;
     KeySide sd;
-    auto fetch = [&](int e) {
-      const int j0 = __builtin_amdgcn_readfirstlane(list[e].t) * 64;
-      stage_load(ks, kb, a.ldk, j0, m.nk, tid);
-      stage_load(vs, vb, a.ldv, j0, m.nk, tid);
-      side_load<BIAS>(sd, a, m, j0, tid);
+    auto fetch = [&](int t) {
+      stage_load(ks, kb, a.ldk, offk, t * 64, m.nk, tid);
+      stage_load(vs, vb, a.ldv, offv, t * 64, m.nk, tid);
+      side_load<BIAS>(sd, a, m, t * 64, tid);
     };
-    auto put = [&](char* tile) {
+    auto put = [&](char* tile, bool whole) {
       stage_store(ks, tile, tid);
       stage_store(vs, tile + 8192, tid);
       side_store<BIAS>(sd, tile, a, tid);
-      const bool odd = stage_odd(ks);
-      if (lane == 0) *(int*)(tile + KT_ODD + wave * 4) = odd;
-    };
-    if (n > 0) { fetch(0); put(smem); }
-    if (n > 1) fetch(1);
-    __syncthreads();
-    for (int e = 0; e < n; ++e) {
-      char* tile = smem + (e & 1) * KT_BYTES;
-      const TileRef tr = list[e];
-      const int j0 = __builtin_amdgcn_readfirstlane(tr.t) * 64, lo = __builtin_amdgcn_readfirstlane(tr.lo), hi = __builtin_amdgcn_readfirstlane(tr.hi);
-      if (uniform(active && j0 < wlim1 && (!docs || (hi >= max(wlo, 0) && lo <= whi)))) {
-        const bool masked = !uniform(j0 + 64 <= wlim0 && (!docs || (lo == hi && wlo == lo && whi == lo)));
-        dq_tile<CAP, BIAS>(acc, qf, df, L2, delta, a, r, tile, j0, lane, fr, masked, docs, masked && any_odd(tile + KT_ODD));
+      if (!whole) {
+        const bool odd = stage_odd(ks);
+        if (lane == 0) *(int*)(tile + KT_ODD + wave * 4) = odd;
       }
-      if (e + 1 < n) put(smem + ((e + 1) & 1) * KT_BYTES);
-      if (e + 2 < n) fetch(e + 2);
+    };
+    TileRef cur, next;
+    int t2 = 0;
+    if (n > 0) {
+      cur = scalar_ref(list[0]); next = scalar_ref(list[1]);
+      t2 = __builtin_amdgcn_readfirstlane(list[2].t);
+      fetch(cur.t);
+      put(smem, cur.whole);
+      fetch(next.t);
+    }
+    __syncthreads();
+    for (int e = 0; e < n; ++e) {      // tile e is in LDS, e + 1 in registers; e + 2 is requested when those are free
+      char* tile = smem + (e & 1) * KT_BYTES;
+      const TileRef ahead = list[e + 2 < n ? e + 2 : n - 1];
+      const int t3 = list[e + 3 < n ? e + 3 : n - 1].t;
+      const int j0 = cur.t * 64;
+      const bool odd = !cur.whole && any_odd(tile + KT_ODD);
+      if (__builtin_expect(odd, 0)) {
+        clean_tile(tile + 0, clean, tid);
+        __syncthreads();
+      }
+      if (uniform(active && j0 < wlim1 && (!docs || (cur.hi >= max(wlo, 0) && cur.lo <= whi)))) {
+        const bool masked = !cur.whole && !uniform(j0 + 64 <= wlim0 && (!docs || (cur.lo == cur.hi && wlo == cur.lo && whi == cur.lo)));
+        dq_tile<CAP, BIAS>(acc, poison, qf, df, L2, delta, a, r, tile, clean, j0, lane, fr, masked, docs, masked && odd);
+      }
+      if (e + 1 < n) put(smem + ((e + 1) & 1) * KT_BYTES, next.whole);
+      if (e + 2 < n) fetch(t2);
+      cur = next;
+      next = scalar_ref(ahead);
+      t2 = __builtin_amdgcn_readfirstlane(t3);
       __syncthreads();
     }
   }
+  apply_poison(acc, poison);
   if (qr < m.nq) store_acc_T(acc, a.dq + (m.q0 + qr) * a.lddq + h * 64, h2, a.scale);
 }
 
@@ -718,19 +818,26 @@ constexpr int QT_L = 16384, QT_D = QT_L + 256, QT_X = QT_D + 256, QT_Y = QT_X + 
 struct QuerySide { float L2, delta, x, y; int lim, doc; };
 
 template <bool CAP, int BIAS>
-__device__ __forceinline__ void dkdv_tile(f32x16 (&dk)[2], f32x16 (&dv)[2], const bf16x8 (&kf)[4], const bf16x8 (&vf)[4], const ModArgs& a, int j, int docj,
-                                          const float (&pj)[2], float slope, const char* tile, int lane, const Frag& fr, bool masked, bool docs, bool odd) {
+__device__ __forceinline__ void dkdv_tile(f32x16 (&dk)[2], f32x16 (&dv)[2], unsigned& pk, unsigned& pv, const bf16x8 (&kf)[4], const bf16x8 (&vf)[4], const ModArgs& a, int j, int docj,
+                                          const float (&pj)[2], float slope, const char* tile, const char* clean, int lane, const Frag& fr, bool masked, bool docs, bool odd) {
   const int h2 = lane >> 5;
-  const unsigned Qs = lds_of(tile), Ds = Qs + 8192;
+  const unsigned Qs = lds_of(tile), Ds = Qs + 8192, Qt = odd ? lds_of(clean) : Qs;
 #pragma unroll
   for (int qt = 0; qt < 2; ++qt) {
     f32x16 s, p, rc;
+    {
+      bf16x8 qf[4], df[4];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) { s[i] = 0.f; p[i] = 0.f; }
+      for (int ks = 0; ks < 4; ++ks) { qf[ks] = row_at(Qs, qt * 32, fr.rf[ks]); df[ks] = row_at(Ds, qt * 32, fr.rf[ks]); }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) s = MFMA_F32_32x32x16_H16(row_at(Qs, qt * 32, fr.rf[ks]), kf[ks], s);
+      for (int i = 0; i < 16; ++i) { s[i] = 0.f; p[i] = 0.f; }
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) p = MFMA_F32_32x32x16_H16(row_at(Ds, qt * 32, fr.rf[ks]), vf[ks], p);
+      for (int ks = 0; ks < 4; ++ks) { s = MFMA_F32_32x32x16_H16(qf[ks], kf[ks], s); p = MFMA_F32_32x32x16_H16(df[ks], vf[ks], p); }
+    }
+    TrFrags td;
+    tr_load(td, Qt + 8192, qt * 32, fr);
+    __builtin_amdgcn_sched_barrier(0);
     modify<CAP, BIAS>(s, rc, a, pj, slope, tile + QT_X + qt * 128, h2, masked);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -757,17 +864,23 @@ __device__ __forceinline__ void dkdv_tile(f32x16 (&dk)[2], f32x16 (&dv)[2], cons
           s[4 * g + e] = vis ? s[4 * g + e] : 0.f;
         }
       }
+      if (__builtin_expect(odd, 0)) {
+        pv |= poison_bits(Ds, qt * 32, p, fr);
+        pk |= poison_bits(Qs, qt * 32, s, fr);
+      }
     }
-    tile_product(dv, Ds, qt * 32, p, fr, odd);
-    tile_product(dk, Qs, qt * 32, s, fr, odd);
+    TrFrags tq;
+    tr_load(tq, Qt, qt * 32, fr);
+    tr_product(dv, td, p);
+    tr_product(dk, tq, s);
   }
 }
 
 template <bool CAP, int BIAS>
 __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
-  __shared__ __attribute__((aligned(16))) char smem[2 * QT_BYTES];
-  __shared__ TileRef list[LIST];
-  __shared__ int buf[12];
+  __shared__ __attribute__((aligned(16))) char smem[2 * QT_BYTES], clean[16384];
+  __shared__ TileRef list[LIST + 3];
+  __shared__ int buf[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
   const Frag fr = frag_consts(lane);
   const Where w = where(a, a.nblk);
@@ -786,23 +899,28 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
   float pj[2] = {0.f, 0.f};
   row_pos<BIAS>(pj, a.pos_k, m.k0 + j, j);
   const int wlo = wave_min_i(docj), whi = wave_max_i(docj);
-  int dlo = wlo, dhi = whi, dummy = 0;
-  group_range(dlo, dhi, dummy, buf, wave, lane);
+  int dlo = wlo, dhi = whi, none0 = 0, none1 = 0;
+  group_range(dlo, dhi, none0, none1, buf, wave, lane);
+  unsigned pk = 0, pv = 0;
+  const unsigned offq = stage_off(a.ldq, tid), offd = stage_off(a.lddo, tid);
   f32x16 dk[2], dv[2];
 #pragma unroll
   for (int i = 0; i < 16; ++i) { dk[0][i] = dk[1][i] = 0.f; dv[0][i] = dv[1][i] = 0.f; }
   // query tiles that can see key jb: rows i with lim_i > jb, a suffix of the rows (all of them if the prefix reaches jb)
   const int first = m.nq == 0 ? 0 : (!a.causal || m.pre > jb) ? 0 : max(0, jb - m.off) / 64;
   const int ntiles = (m.nq + 63) / 64;
+  // whole tiles: every row of theirs sees all 128 keys, all of them rows and keys of the sequence
+  const int jlast = jb + 127;
+  const int w0 = jlast >= m.nk ? ntiles : (!a.causal || m.pre > jlast) ? 0 : (max(0, jlast - m.off) + 63) / 64, w1 = m.nq / 64;
   for (int t0 = first; t0 < ntiles; t0 += LIST) {
-    const int n = build_list(list, buf, t0, ntiles, docs ? a.rng_q + (long)(w.unit / Hkv) * a.nt_q : nullptr, dlo, dhi, tid);
+    const int n = build_list(list, buf, t0, ntiles, w0, w1, docs ? a.rng_q + (long)(w.unit / Hkv) * a.nt_q : nullptr, dlo, dhi, tid);
     const int total = n * a.G;
     Stage qs, os;
     QuerySide sd;
-    auto fetch = [&](int x) {      // entry x % n of head x / n
-      const int h = hk * a.G + x / n, i0 = __builtin_amdgcn_readfirstlane(list[x % n].t) * 64;
-      stage_load(qs, a.q + m.q0 * a.ldq + h * 64, a.ldq, i0, m.nq, tid);
-      stage_load(os, a.d_o + m.q0 * a.lddo + h * 64, a.lddo, i0, m.nq, tid);
+    auto fetch = [&](int t, int g) {      // a query tile of head g of the group
+      const int h = hk * a.G + g, i0 = t * 64;
+      stage_load(qs, a.q + m.q0 * a.ldq + h * 64, a.ldq, offq, i0, m.nq, tid);
+      stage_load(os, a.d_o + m.q0 * a.lddo + h * 64, a.lddo, offd, i0, m.nq, tid);
       if (tid < 64) {
         const int i = min(i0 + tid, m.nq - 1);
         const long stat = (long)h * a.Tq + m.q0 + i;
@@ -816,7 +934,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
         sd.lim = i0 + tid < m.nq && sd.doc >= 0 ? row_lim(a, m, i) : 0;
       }
     };
-    auto put = [&](char* tile) {
+    auto put = [&](char* tile, bool whole) {
       stage_store(qs, tile, tid);
       stage_store(os, tile + 8192, tid);
       if (tid < 64) {
@@ -827,27 +945,56 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
         *(int*)(tile + QT_LIM + tid * 4) = sd.lim;
         *(int*)(tile + QT_DOC + tid * 4) = sd.doc;
       }
-      const bool odd = stage_odd(qs) || stage_odd(os);
-      if (lane == 0) *(int*)(tile + QT_ODD + wave * 4) = odd;
+      if (!whole) {
+        const bool odd = stage_odd(qs) || stage_odd(os);
+        if (lane == 0) *(int*)(tile + QT_ODD + wave * 4) = odd;
+      }
     };
-    if (total > 0) { fetch(0); put(smem); }
-    if (total > 1) fetch(1);
+    // entry e of head g is in LDS, the next in registers; the one behind that, e2 of head g2, is requested when those are free
+    TileRef cur, next;
+    int e = 0, g = 0, e2 = 0, g2 = 0, t2 = 0;
+    auto step = [&](int& e_, int& g_) { if (++e_ == n) { e_ = 0; ++g_; } };
+    if (n > 0) {
+      cur = scalar_ref(list[0]);
+      step(e2, g2);
+      next = scalar_ref(list[e2]);
+      fetch(cur.t, 0);
+      put(smem, cur.whole);
+      if (total > 1) fetch(next.t, g2);
+      step(e2, g2);
+      t2 = __builtin_amdgcn_readfirstlane(list[e2].t);
+    }
     __syncthreads();
     for (int x = 0; x < total; ++x) {
       char* tile = smem + (x & 1) * QT_BYTES;
-      const TileRef tr = list[x % n];
-      const int i0 = __builtin_amdgcn_readfirstlane(tr.t) * 64, lo = __builtin_amdgcn_readfirstlane(tr.lo), hi = __builtin_amdgcn_readfirstlane(tr.hi);
-      const int jw = jb + wave * 32, last = min(i0 + 63, m.nq - 1);
-      if (uniform(active && row_lim(a, m, last) > jw && (!docs || (hi >= max(wlo, 0) && lo <= whi)))) {
-        const float slope = BIAS ? a.slopes[hk * a.G + x / n] * LOG2E : 0.f;
-        const bool masked = !uniform(i0 + 64 <= m.nq && jw + 32 <= m.nk && row_lim(a, m, i0) >= jw + 32 && (!docs || (lo >= 0 && lo == hi && wlo == lo && whi == lo)));
-        dkdv_tile<CAP, BIAS>(dk, dv, kf, vf, a, j, docj, pj, slope, tile, lane, fr, masked, docs, masked && any_odd(tile + QT_ODD));
+      const TileRef ahead = list[e2];
+      const int gn = g2;
+      step(e2, g2);
+      const int t3 = list[e2].t;
+      const int i0 = cur.t * 64, jw = jb + wave * 32, last = min(i0 + 63, m.nq - 1);
+      const bool odd = !cur.whole && any_odd(tile + QT_ODD);
+      if (__builtin_expect(odd, 0)) {
+        clean_tile(tile, clean, tid);
+        clean_tile(tile + 8192, clean + 8192, tid);
+        __syncthreads();
       }
-      if (x + 1 < total) put(smem + ((x + 1) & 1) * QT_BYTES);
-      if (x + 2 < total) fetch(x + 2);
+      if (uniform(active && row_lim(a, m, last) > jw && (!docs || (cur.hi >= max(wlo, 0) && cur.lo <= whi)))) {
+        const float slope = BIAS ? a.slopes[hk * a.G + g] * LOG2E : 0.f;
+        const bool masked = !cur.whole && !uniform(i0 + 64 <= m.nq && jw + 32 <= m.nk && row_lim(a, m, i0) >= jw + 32 &&
+                                                   (!docs || (cur.lo >= 0 && cur.lo == cur.hi && wlo == cur.lo && whi == cur.lo)));
+        dkdv_tile<CAP, BIAS>(dk, dv, pk, pv, kf, vf, a, j, docj, pj, slope, tile, clean, lane, fr, masked, docs, masked && odd);
+      }
+      if (x + 1 < total) put(smem + ((x + 1) & 1) * QT_BYTES, next.whole);
+      if (x + 2 < total) fetch(t2, gn);
+      step(e, g);
+      cur = next;
+      next = scalar_ref(ahead);
+      t2 = __builtin_amdgcn_readfirstlane(t3);
       __syncthreads();
     }
   }
+  apply_poison(dk, pk);
+  apply_poison(dv, pv);
   if (jr < m.nk) {
     store_acc_T(dk, a.dk + (m.k0 + jr) * a.lddk + hk * 64, h2, a.scale);
     store_acc_T(dv, a.dv + (m.k0 + jr) * a.lddv + hk * 64, h2, 1.f);
@@ -912,15 +1059,15 @@ int mod_check(const char* who, const apla_attn_mod_t* p, bool backward) {
   APLA_REQUIRE(p->q && p->k && p->v && p->o && p->lse, "%s: a pointer is missing", who);
   APLA_REQUIRE(apla_aligned16(p->q) && apla_aligned16(p->k) && apla_aligned16(p->v) && apla_aligned16(p->o), "%s: q, k, v, o must be 16-byte aligned", who);
   APLA_REQUIRE(p->ldq >= p->Hq * 64L && p->ldo >= p->Hq * 64L && p->ldk >= p->Hkv * 64L && p->ldv >= p->Hkv * 64L, "%s: a row stride is shorter than its heads", who);
-  APLA_REQUIRE(((p->ldq | p->ldk | p->ldv | p->ldo) & 7) == 0, "%s: row strides must be multiples of 8", who);
+  APLA_REQUIRE(((p->ldq | p->ldk | p->ldv | p->ldo) & 7) == 0 && p->ldq < (1L << 23) && p->ldk < (1L << 23) && p->ldv < (1L << 23), "%s: row strides must be multiples of 8, below 2^23", who);
   APLA_REQUIRE((!p->doc_q) == (!p->doc_k), "%s: document ids are needed for queries and keys", who);
   APLA_REQUIRE(p->pos_dim >= 0 && p->pos_dim <= 2 && (p->pos_dim == 0 ? !p->pos_q && !p->pos_k : p->pos_q && p->pos_k && p->slopes), "%s: positions need slopes, both sides and 1 or 2 coordinates", who);
   APLA_REQUIRE(!p->prefix || p->causal, "%s: a prefix needs the causal mask", who);
   if (backward) {
     APLA_REQUIRE(p->d_o && p->dq && p->dk && p->dv && p->delta, "%s: a pointer is missing", who);
     APLA_REQUIRE(apla_aligned16(p->d_o) && apla_aligned16(p->dq) && apla_aligned16(p->dk) && apla_aligned16(p->dv), "%s: d_o, dq, dk, dv must be 16-byte aligned", who);
-    APLA_REQUIRE(p->lddo >= p->Hq * 64L && p->lddq >= p->Hq * 64L && p->lddk >= p->Hkv * 64L && p->lddv >= p->Hkv * 64L && ((p->lddo | p->lddq | p->lddk | p->lddv) & 7) == 0,
-                 "%s: gradient row strides must cover their heads and be multiples of 8", who);
+    APLA_REQUIRE(p->lddo >= p->Hq * 64L && p->lddq >= p->Hq * 64L && p->lddk >= p->Hkv * 64L && p->lddv >= p->Hkv * 64L && ((p->lddo | p->lddq | p->lddk | p->lddv) & 7) == 0 && p->lddo < (1L << 23),
+                 "%s: gradient row strides must cover their heads and be multiples of 8, below 2^23", who);
   }
   const Plan pl = plan_of(*p, backward);
   APLA_REQUIRE(pl.bytes == 0 || (p->workspace && apla_aligned16(p->workspace) && p->workspace_bytes >= pl.bytes), "%s: needs %ld bytes of 16-byte aligned workspace (got %ld)", who, pl.bytes, p->workspace_bytes);
