@@ -50,6 +50,11 @@ def _stream():
     return torch.cuda.current_stream().cuda_stream
 
 
+def _raw_stream(device):
+    """The current stream of a device as the integer the entry points take (no Stream object: a third of the cost per call)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
@@ -656,48 +661,60 @@ ROT_LAYOUTS = {"half": 0, "interleaved": 1}
 QK_NORMS = {"layer": 1, "rms": 2}
 
 
-def _strided_rows(t: torch.Tensor, name: str, cols: int, rows: Optional[int] = None):
+def _strided_rows(t: torch.Tensor, name: str, cols: int, rows: Optional[int] = None) -> int:
     """A [rows, cols] 16-bit matrix whose rows may lie apart (column slices of a fused activation); returns its row stride."""
-    _req(t, half(), name, 2)
-    if t.shape[1] != cols or (rows is not None and t.shape[0] != rows):
-        raise ValueError(f"{name}: expected [{'T' if rows is None else rows}, {cols}], got {tuple(t.shape)}")
-    ld = cols if t.shape[0] <= 1 else t.stride(0)
-    if ld < cols or ld % 8 or t.data_ptr() % 16:
-        raise ValueError(f"{name}: rows must be 16-byte aligned, apart by a multiple of 8 elements and not overlap (row stride {t.stride(0)})")
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != _HALF or t.dim() != 2:
+        _req(t, half(), name, 2)
+    shape = t.shape
+    if shape[1] != cols or (rows is not None and shape[0] != rows):
+        raise ValueError(f"{name}: expected [{'T' if rows is None else rows}, {cols}], got {tuple(shape)}")
+    ld, inner = t.stride()
+    if shape[0] <= 1:
+        ld = cols
+    if inner != 1 or ld < cols or ld & 7 or t.data_ptr() & 15:
+        raise ValueError(f"{name}: rows must be contiguous, 16-byte aligned, apart by a multiple of 8 elements and not overlap (strides {tuple(t.stride())})")
     return ld
 
 
+class _Here:
+    """No device guard needed: the tensors live on the current device."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
 def _on_device(first: torch.Tensor, *others):
-    """Device guard + stream of `first`'s device; every other tensor (or None) must live there too."""
+    """Guard that makes `first`'s device the current one; every other tensor (or None) must live there too."""
+    dev = first.device
     for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"tensors on {first.device} and {t.device}")
-    return torch.cuda.device(first.device)
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}")
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _aux(t: Optional[torch.Tensor], dtype, name: str, shape):
-    """An optional side array: contiguous, of one dtype and shape (None entries of `shape` are free)."""
-    if t is None:
-        return None
+    """An optional side array: contiguous, of one dtype and shape."""
+    if t is None or (t.dtype is dtype and t.is_cuda and t.shape == shape and t.is_contiguous()):
+        return t
     _req(t, dtype, name, len(shape))
-    if not t.is_contiguous() or any(w is not None and n != w for n, w in zip(t.shape, shape)):
-        raise ValueError(f"{name}: expected a contiguous {shape}, got {tuple(t.shape)}")
-    return t
+    raise ValueError(f"{name}: expected a contiguous {shape}, got {tuple(t.shape)}")
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Do two row-strided matrices touch the same bytes?  Column slices of one buffer with the same row stride may interleave."""
-    if a.numel() == 0 or b.numel() == 0:
-        return False
     sa, sb = a.data_ptr(), b.data_ptr()
-    ea = sa + ((a.shape[0] - 1) * a.stride(0) + a.shape[1]) * a.element_size()
-    eb = sb + ((b.shape[0] - 1) * b.stride(0) + b.shape[1]) * b.element_size()
-    if ea <= sb or eb <= sa:
+    (ra, ca), (rb, cb), la, lb, w = a.shape, b.shape, a.stride(0), b.stride(0), a.element_size()
+    if ra * ca == 0 or rb * cb == 0 or sa + ((ra - 1) * la + ca) * w <= sb or sb + ((rb - 1) * lb + cb) * w <= sa:
         return False
-    pitch = a.stride(0) * a.element_size()
-    if a.stride(0) == b.stride(0):
-        d = (sb - sa) % pitch
-        return d < a.shape[1] * a.element_size() or d + b.shape[1] * b.element_size() > pitch
+    if la == lb:
+        d = (sb - sa) % (la * w)
+        return d < ca * w or d + cb * w > la * w
     return True
 
 
@@ -708,7 +725,9 @@ def _rot_table(table, rows, pos, seq_len: int, layout: str, who: str):
         if pos is not None or seq_len:
             raise ValueError(f"{who}: positions without a table")
         return 0, 0
-    _aux(table, torch.float32, "table", (None, None))
+    if table.dtype is not torch.float32 or not table.is_cuda or table.dim() != 2 or not table.is_contiguous():
+        _req(table, torch.float32, "table", 2)
+        raise ValueError(f"{who}: the table must be contiguous")
     P, rot = table.shape
     if rot % 2 or not 2 <= rot <= 64 or P < 1:
         raise ValueError(f"{who}: the table is [positions, rot] with rot even, 2..64; got {tuple(table.shape)}")
@@ -726,14 +745,15 @@ def _rotary(x, table, heads: int, layout, pos, seq_len: int, out, inverse: bool,
     P, rot = _rot_table(table, T, pos, seq_len, layout, who)
     with _on_device(x, table, pos, out):
         if out is None:
-            out = torch.empty(T, heads * 64, device=x.device, dtype=x.dtype)
-        ldo = _strided_rows(out, "out", heads * 64, T)
+            out, ldo = x.new_empty(T, heads * 64), heads * 64
+        else:
+            ldo = _strided_rows(out, "out", heads * 64, T)
+            if _overlap(x, out) and (x.data_ptr() != out.data_ptr() or ldx != ldo):
+                raise ValueError(f"{who}: out may be x itself, not another view of the same memory")
         if T == 0:
             return out
-        if _overlap(x, out) and (x.data_ptr() != out.data_ptr() or ldx != ldo):
-            raise ValueError(f"{who}: out may be x itself, not another view of the same memory")
         check(lib().apla_rotary(x.data_ptr(), ldx, out.data_ptr(), ldo, T, heads, table.data_ptr(), P, rot, ROT_LAYOUTS[layout], _ptr(pos),
-                                seq_len, int(inverse), _stream()), "apla_rotary")
+                                seq_len, int(inverse), _raw_stream(x.device)), "apla_rotary")
     return out
 
 
@@ -751,24 +771,26 @@ def rotary_bwd(dy: torch.Tensor, table: torch.Tensor, heads: int, *, layout: str
     return _rotary(dy, table, heads, layout, pos, seq_len, out, True, "rotary_bwd")
 
 
-def _qk_params(norm, eps, params, who):
+def _qk_params(norm, eps, qw, kw, qb, kb, who):
     if norm not in QK_NORMS:
         raise ValueError(f"{who}: norm must be one of {sorted(QK_NORMS)}, got {norm!r}")
     if not eps >= 0:
         raise ValueError(f"{who}: eps must not be negative")
-    for n, p in params.items():
-        _aux(p, torch.float32, n, (64,))
+    f32, shape = torch.float32, (64,)
+    _aux(qw, f32, "q_weight", shape), _aux(kw, f32, "k_weight", shape), _aux(qb, f32, "q_bias", shape), _aux(kb, f32, "k_bias", shape)
 
 
 def _qk_rows(t, name, Hq, Hkv, rows=None):
     """qkv rows [T, >= (Hq + Hkv) * 64] -> (their query / key columns, row stride)."""
-    _req(t, half(), name, 2)
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
+        _req(t, half(), name, 2)
     if Hq < 1 or Hkv < 0:
         raise ValueError(f"{name}: bad head counts {Hq}, {Hkv}")
     n = (Hq + Hkv) * 64
     if t.shape[1] < n:
         raise ValueError(f"{name}: rows of {t.shape[1]} values do not hold {Hq} + {Hkv} heads of 64")
-    t = t[:, :n]
+    if t.shape[1] != n:
+        t = t[:, :n]
     return t, _strided_rows(t, name, n, rows)
 
 
@@ -780,18 +802,19 @@ def qk_norm_rotary_fwd(qkv: torch.Tensor, Hq: int, Hkv: int, *, norm: str = "lay
     x, ldx = _qk_rows(qkv, "qkv", Hq, Hkv)
     T, n = x.shape
     P, rot = _rot_table(table, T, pos, seq_len, layout, "qk_norm_rotary_fwd")
-    _qk_params(norm, eps, dict(q_weight=q_weight, k_weight=k_weight, q_bias=q_bias, k_bias=k_bias), "qk_norm_rotary_fwd")
+    _qk_params(norm, eps, q_weight, k_weight, q_bias, k_bias, "qk_norm_rotary_fwd")
     with _on_device(x, table, pos, out, q_weight, k_weight, q_bias, k_bias):
         if out is None:
-            out = torch.empty(T, n, device=x.device, dtype=x.dtype)
-        ldo = _strided_rows(out, "out", n, T)
+            out, ldo = x.new_empty(T, n), n
+        else:
+            ldo = _strided_rows(out, "out", n, T)
+            if _overlap(x, out) and (x.data_ptr() != out.data_ptr() or ldx != ldo):
+                raise ValueError("qk_norm_rotary_fwd: out may be the query / key columns themselves, not another view of the same memory")
         if T == 0:
             return out
-        if _overlap(x, out) and (x.data_ptr() != out.data_ptr() or ldx != ldo):
-            raise ValueError("qk_norm_rotary_fwd: out may be the query / key columns themselves, not another view of the same memory")
         check(lib().apla_qk_norm_rotary_fwd(x.data_ptr(), ldx, out.data_ptr(), ldo, T, Hq, Hkv, QK_NORMS[norm], float(eps), _ptr(q_weight),
                                             _ptr(k_weight), _ptr(q_bias), _ptr(k_bias), _ptr(table), P, rot, ROT_LAYOUTS[layout], _ptr(pos),
-                                            seq_len, _stream()), "apla_qk_norm_rotary_fwd")
+                                            seq_len, _raw_stream(x.device)), "apla_qk_norm_rotary_fwd")
     return out
 
 
@@ -804,13 +827,14 @@ def qk_norm_rotary_bwd(dqk: torch.Tensor, qkv: torch.Tensor, Hq: int, Hkv: int, 
     T, n = x.shape
     ldd = _strided_rows(dqk, "dqk", n, T)
     P, rot = _rot_table(table, T, pos, seq_len, layout, "qk_norm_rotary_bwd")
-    _qk_params(norm, eps, dict(q_weight=q_weight, k_weight=k_weight, q_bias=q_bias, k_bias=k_bias), "qk_norm_rotary_bwd")
+    _qk_params(norm, eps, q_weight, k_weight, q_bias, k_bias, "qk_norm_rotary_bwd")
     with _on_device(x, dqk, table, pos, out, q_weight, k_weight, q_bias, k_bias):
         if out is None:
-            out = torch.empty(T, n, device=x.device, dtype=x.dtype)
-        ldo = _strided_rows(out, "out", n, T)
-        if any(_overlap(t, out) and (t.data_ptr() != out.data_ptr() or ld != ldo) for t, ld in ((x, ldx), (dqk, ldd))):
-            raise ValueError("qk_norm_rotary_bwd: out may be dqk or the query / key columns themselves, not another view of the same memory")
+            out, ldo = x.new_empty(T, n), n
+        else:
+            ldo = _strided_rows(out, "out", n, T)
+            if any(_overlap(t, out) and (t.data_ptr() != out.data_ptr() or ld != ldo) for t, ld in ((x, ldx), (dqk, ldd))):
+                raise ValueError("qk_norm_rotary_bwd: out may be dqk or the query / key columns themselves, not another view of the same memory")
         dpar = ws = None
         if want_params:
             dpar = torch.empty(4, 64, device=x.device, dtype=torch.float32) if T else torch.zeros(4, 64, device=x.device)
@@ -819,7 +843,7 @@ def qk_norm_rotary_bwd(dqk: torch.Tensor, qkv: torch.Tensor, Hq: int, Hkv: int, 
             return out, dpar
         check(lib().apla_qk_norm_rotary_bwd(dqk.data_ptr(), ldd, x.data_ptr(), ldx, out.data_ptr(), ldo, T, Hq, Hkv, QK_NORMS[norm], float(eps),
                                             _ptr(q_weight), _ptr(k_weight), _ptr(table), P, rot, ROT_LAYOUTS[layout], _ptr(pos), seq_len,
-                                            _ptr(dpar), _ptr(ws), 0 if ws is None else ws.numel() * 4, _stream()), "apla_qk_norm_rotary_bwd")
+                                            _ptr(dpar), _ptr(ws), 0 if ws is None else ws.numel() * 4, _raw_stream(x.device)), "apla_qk_norm_rotary_bwd")
     return out, dpar
 
 
@@ -884,9 +908,14 @@ def _attn_mod_args(q, k, v, Hq: int, Hkv: int, scale: float, mod, batch, cu_q, c
         raise ValueError(f"{who}: at most 65535 sequences, got {S}")
     if max(max_q, max_k) > 1 << 24:
         raise ValueError(f"{who}: sequences of at most 2^24 tokens")
-    _aux(len_k, torch.int32, "len_k", (S,)), _aux(m.prefix, torch.int32, "prefix", (S,))
-    _aux(m.slopes, torch.float32, "slopes", (Hq,))
-    _aux(m.doc_q, torch.int32, "doc_q", (Tq,)), _aux(m.doc_k, torch.int32, "doc_k", (Tk,))
+    if len_k is not None:
+        a.len_k = _aux(len_k, torch.int32, "len_k", (S,)).data_ptr()
+    if m.prefix is not None:
+        a.prefix = _aux(m.prefix, torch.int32, "prefix", (S,)).data_ptr()
+    if m.slopes is not None:
+        a.slopes = _aux(m.slopes, torch.float32, "slopes", (Hq,)).data_ptr()
+    if m.doc_q is not None:
+        a.doc_q, a.doc_k = _aux(m.doc_q, torch.int32, "doc_q", (Tq,)).data_ptr(), _aux(m.doc_k, torch.int32, "doc_k", (Tk,)).data_ptr()
     if m.pos_q is not None:
         a.pos_dim = 1 if m.pos_q.ndim == 1 else m.pos_q.shape[1]
         if a.pos_dim not in (1, 2):
@@ -895,9 +924,10 @@ def _attn_mod_args(q, k, v, Hq: int, Hkv: int, scale: float, mod, batch, cu_q, c
             _aux(t, torch.float32, n, (rows,) if t.ndim == 1 else (rows, a.pos_dim))
         if (1 if m.pos_k.ndim == 1 else m.pos_k.shape[1]) != a.pos_dim:
             raise ValueError(f"{who}: pos_q and pos_k have different numbers of coordinates")
+        a.pos_q, a.pos_k = m.pos_q.data_ptr(), m.pos_k.data_ptr()
     a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.cu_q, a.cu_k, a.len_k, a.prefix = _ptr(cu_q), _ptr(cu_k), _ptr(len_k), _ptr(m.prefix)
-    a.doc_q, a.doc_k, a.slopes, a.pos_q, a.pos_k = _ptr(m.doc_q), _ptr(m.doc_k), _ptr(m.slopes), _ptr(m.pos_q), _ptr(m.pos_k)
+    if cu_q is not None:
+        a.cu_q, a.cu_k = cu_q.data_ptr(), cu_k.data_ptr()
     a.S, a.Tq, a.Tk, a.max_q, a.max_k, a.Hq, a.Hkv, a.causal = S, Tq, Tk, max_q, max_k, Hq, Hkv, int(m.causal)
     a.scale, a.softcap = float(scale), m.softcap
     return a, _on_device(q, k, v, cu_q, cu_k, len_k, m.prefix, m.doc_q, m.doc_k, m.slopes, m.pos_q, m.pos_k)
@@ -906,8 +936,10 @@ def _attn_mod_args(q, k, v, Hq: int, Hkv: int, scale: float, mod, batch, cu_q, c
 def _mod_workspace(a, backward: bool, device):
     """Scratch of ONE call (never shared: two captured graphs may run at once)."""
     n = lib().apla_attn_mod_workspace_bytes(a, int(backward))
-    ws = torch.empty(max(n, 0) // 4, device=device, dtype=torch.float32) if n > 0 else None
-    a.workspace, a.workspace_bytes = _ptr(ws), max(n, 0)
+    if n <= 0:
+        return None
+    ws = torch.empty(n // 4, device=device, dtype=torch.float32)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), n
     return ws
 
 
@@ -923,15 +955,20 @@ def attn_mod_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, Hq: int, Hkv
     else 0 / -inf."""
     a, guard = _attn_mod_args(q, k, v, Hq, Hkv, scale, mod, batch, cu_q, cu_k, max_q, max_k, len_k, "attn_mod_fwd")
     with guard:
+        Tq = a.Tq
         if o is None:
-            o = (torch.empty if cu_q is None else torch.zeros)(a.Tq, Hq * 64, device=q.device, dtype=half())
+            o = q.new_empty(Tq, Hq * 64) if cu_q is None else q.new_zeros(Tq, Hq * 64)
+            a.ldo = Hq * 64
+        else:
+            a.ldo = _strided_rows(o, "o", Hq * 64, Tq)
+            if o.device != q.device or any(_overlap(t, o) for t in (q, k, v)):
+                raise ValueError("attn_mod_fwd: o must lie on q's device and apart from q, k, v")
         if lse is None:
-            shape = (Hq, a.Tq)
-            lse = torch.empty(shape, device=q.device) if cu_q is None else torch.full(shape, float("-inf"), device=q.device)
-        a.ldo = _strided_rows(o, "o", Hq * 64, a.Tq)
-        _aux(lse, torch.float32, "lse", (Hq, a.Tq))
-        if o.device != q.device or lse.device != q.device or any(_overlap(t, o) for t in (q, k, v)):
-            raise ValueError("attn_mod_fwd: o / lse must lie on q's device and apart from q, k, v")
+            lse = torch.empty((Hq, Tq), device=q.device, dtype=torch.float32) if cu_q is None else torch.full((Hq, Tq), float("-inf"), device=q.device, dtype=torch.float32)
+        else:
+            _aux(lse, torch.float32, "lse", (Hq, Tq))
+            if lse.device != q.device:
+                raise ValueError("attn_mod_fwd: lse must lie on q's device")
         a.o, a.lse = o.data_ptr(), lse.data_ptr()
         if a.max_q == 0:
             return o, lse
@@ -939,7 +976,7 @@ def attn_mod_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, Hq: int, Hkv
             _zero_rows(o, cu_q, 0.0), _zero_rows(lse.t(), cu_q, float("-inf"))
             return o, lse
         ws = _mod_workspace(a, False, q.device)     # noqa: F841  (alive until the launch)
-        check(lib().apla_attn_mod_fwd(a, _stream()), "apla_attn_mod_fwd")
+        check(lib().apla_attn_mod_fwd(a, _raw_stream(q.device)), "apla_attn_mod_fwd")
     return o, lse
 
 
@@ -961,27 +998,35 @@ def attn_mod_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Ten
     a.ldo, a.lddo = _strided_rows(o, "o", Hq * 64, a.Tq), _strided_rows(do, "do", Hq * 64, a.Tq)
     _aux(lse, torch.float32, "lse", (Hq, a.Tq))
     with guard:
-        if dq is None:
-            dq = (torch.empty if cu_q is None else torch.zeros)(a.Tq, Hq * 64, device=q.device, dtype=half())
-        make = torch.empty if cu_k is None and len_k is None else torch.zeros
-        if dk is None:
-            dk = make(a.Tk, Hkv * 64, device=q.device, dtype=half())
-        if dv is None:
-            dv = make(a.Tk, Hkv * 64, device=q.device, dtype=half())
-        a.lddq, a.lddk, a.lddv = _strided_rows(dq, "dq", Hq * 64, a.Tq), _strided_rows(dk, "dk", Hkv * 64, a.Tk), _strided_rows(dv, "dv", Hkv * 64, a.Tk)
-        if any(t.device != q.device for t in (o, do, lse, dq, dk, dv)):
+        Tq, Tk, dev = a.Tq, a.Tk, q.device
+        given = [g for g in (dq, dk, dv) if g is not None]
+        if any(t.device != dev for t in (o, do, lse, *given)):
             raise ValueError("attn_mod_bwd: every tensor must lie on q's device")
-        outs = (dq, dk, dv)
-        if any(_overlap(t, g) for t in (q, k, v, o, do) for g in outs) or any(_overlap(outs[i], outs[j]) for i in range(3) for j in range(i)):
+        if any(_overlap(t, g) for g in given for t in (q, k, v, o, do)) or any(_overlap(given[i], given[j]) for i in range(len(given)) for j in range(i)):
             raise ValueError("attn_mod_bwd: the gradients must lie apart from the operands and from each other")
+        nq, nk = Hq * 64, Hkv * 64
+        make = q.new_empty if cu_k is None and len_k is None else q.new_zeros
+        a.lddq, a.lddk, a.lddv = nq, nk, nk
+        if dq is None:
+            dq = q.new_empty(Tq, nq) if cu_q is None else q.new_zeros(Tq, nq)
+        else:
+            a.lddq = _strided_rows(dq, "dq", nq, Tq)
+        if dk is None:
+            dk = make(Tk, nk)
+        else:
+            a.lddk = _strided_rows(dk, "dk", nk, Tk)
+        if dv is None:
+            dv = make(Tk, nk)
+        else:
+            a.lddv = _strided_rows(dv, "dv", nk, Tk)
         if a.max_q == 0 or a.max_k == 0:
             _zero_rows(dq, cu_q, 0.0), _zero_rows(dk, cu_k, 0.0), _zero_rows(dv, cu_k, 0.0)
             return dq, dk, dv
-        delta = torch.empty(Hq, a.Tq, device=q.device, dtype=torch.float32)
+        delta = torch.empty_like(lse)
         a.o, a.lse, a.d_o, a.delta = o.data_ptr(), lse.data_ptr(), do.data_ptr(), delta.data_ptr()
         a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         ws = _mod_workspace(a, True, q.device)      # noqa: F841
-        check(lib().apla_attn_mod_bwd(a, _stream()), "apla_attn_mod_bwd")
+        check(lib().apla_attn_mod_bwd(a, _raw_stream(q.device)), "apla_attn_mod_bwd")
     return dq, dk, dv
 
 
