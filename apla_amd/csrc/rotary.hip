@@ -1,9 +1,10 @@
 // Rotary positions and the per-head norm of queries and keys (head_dim 64): forward and backward, memory bound.
 //
 // A head row is 64 x 16 bit = 128 bytes: eight lanes with 16 bytes each, so every load and store instruction of a wave moves eight whole
-// lines.  The eight lane groups of a wave are hb heads of 8 / hb tokens (hb the largest of 8, 4, 2, 1 that divides the head counts:
-// no lane idles, a wave's groups sit next to each other in the row), and a wave walks the heads of its tokens, so that the
-// cosines and sines are loaded once per token and lane and not once per head.
+// lines.  A wave holds either query or key heads (one set of norm parameters, one set of their sums): hb heads of 8 / hb tokens at a
+// time (hb the largest of 8, 4, 2, 1 that divides the head count: no lane idles, neighbouring groups are neighbours in memory).  It walks the
+// heads of its tokens, so that cosines and sines are loaded once per token and lane and not once per head, DEPTH head blocks requested
+// ahead of their use.
 //
 // Rotation of the pair (a, b) by theta: a' = a cos - b sin, b' = b cos + a sin.  "interleaved": the pair is (2i, 2i+1), both in one
 // lane.  "half": (i, i + rot/2), exchanged as fp32 through the wave's own 2 KB of LDS (rot may be any even number: neither a lane nor a
@@ -17,17 +18,18 @@
 
 namespace {
 
+constexpr int DEPTH = 4;
+
 struct RotArgs {
-  const bf16* x; long ldx;       // rotated / normalised rows [T, (h1 + h2) * 64]
+  const bf16* x; long ldx;       // rotated / normalised rows [T, (heads[0] + heads[1]) * 64]
   const bf16* dy; long lddy;     // backward: incoming gradient of the result
   bf16* y; long ldy;             // result, or dx
-  int T, nb1, nb, hbl;           // head blocks of the first group (queries), of both; log2 of heads per block
-  const float* table; int P, rot, interleaved;
+  int T, hbl[2], nb[2], splits;  // of queries and keys: log2 of heads per block, blocks; workgroups that share a token's blocks
+  const float* table; int P, rot, interleaved, vec;
   const int32_t* pos; int seq_len;
   float sign, eps;
-  const float *qw, *kw, *qb, *kb;
-  float* partial;                // [workgroups][4][64]: dqw, dkw, dqb, dkb
-  int bpy;                       // head blocks per blockIdx.y
+  const float *w[2], *b[2];
+  float* partial;                // [2][workgroups][128]: sums for the weight, then the bias
 };
 
 __device__ __forceinline__ float group8_sum(float v) {
@@ -74,29 +76,28 @@ __device__ __forceinline__ void rotate8(float (&v)[8], const float (&cs)[8], con
   for (int e = 0; e < 8; ++e) v[e] = e0 + e < 2 * r ? v[e] * cs[e] + pr[e] * sn[e] : v[e];
 }
 
-// NORM: 0 none, 1 LayerNorm, 2 RMS.
+// NORM: 0 none, 1 LayerNorm, 2 RMS.  blockIdx.y: queries or keys, and which of their blocks.
 template <int NORM, bool BWD, bool PAR>
 __global__ __launch_bounds__(256) void rotary_kernel(RotArgs a) {
   __shared__ __attribute__((aligned(16))) float xch_all[4][8][68];
-  __shared__ float red[PAR ? 4 : 1][256];
+  __shared__ float red[PAR ? 4 : 1][128];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int grp = blockIdx.y / a.splits, sp = blockIdx.y % a.splits;
+  const int hbl = a.hbl[grp], nb = a.nb[grp];
   const int g = lane >> 3, e0 = (lane & 7) * 8;
-  const int hb = 1 << a.hbl, sub = g & (hb - 1), tsub = g >> a.hbl, tpw = 8 >> a.hbl;
+  const int hb = 1 << hbl, sub = g & (hb - 1), tsub = g >> hbl, tpw = 8 >> hbl;
+  const int col = (grp ? a.nb[0] << (a.hbl[0] + 6) : 0) + sub * 64 + e0, step = hb * 64;
   float* xch = xch_all[wave][g];
   const int r = a.rot >> 1;
-  const int b0 = blockIdx.y * a.bpy, b1 = min(a.nb, b0 + a.bpy);
-  float w[2][8], bi[2][8];
+  const int each = (nb + a.splits - 1) / a.splits, b0 = sp * each, b1 = min(nb, b0 + each);
+  float w[8], bi[8], aw[8], ab[8];
   if constexpr (NORM != 0) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      w[0][e] = a.qw ? a.qw[e0 + e] : 1.f; w[1][e] = a.kw ? a.kw[e0 + e] : 1.f;
-      bi[0][e] = a.qb ? a.qb[e0 + e] : 0.f; bi[1][e] = a.kb ? a.kb[e0 + e] : 0.f;
+      w[e] = a.w[grp] ? a.w[grp][e0 + e] : 1.f;
+      bi[e] = !BWD && a.b[grp] ? a.b[grp][e0 + e] : 0.f;
+      aw[e] = ab[e] = 0.f;
     }
-  }
-  float aw[2][8], ab[2][8];
-  if constexpr (PAR) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) { aw[0][e] = aw[1][e] = ab[0][e] = ab[1][e] = 0.f; }
   }
   for (long tb = ((long)blockIdx.x * 4 + wave) * tpw; tb < a.T; tb += (long)gridDim.x * 4 * tpw) {
     const bool tv = tb + tsub < a.T;
@@ -106,140 +107,163 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotArgs a) {
       long p = a.pos ? (long)a.pos[t] : a.seq_len ? t % a.seq_len : t;
       const bool pv = p >= 0 && p < a.P;      // a position outside the table gives NaN, not a read outside it
       const float* row = a.table + (pv ? p : 0) * a.rot;
+if (a.vec) {      // the lane's eight angles are four (interleaved) or eight (half) neighbours in the table
+        const bool in = e0 < 2 * r;
+        const float* c = row + (!in ? 0 : a.interleaved ? e0 >> 1 : e0 < r ? e0 : e0 - r);
+        const f32x4 c0 = *(const f32x4*)c, s0 = *(const f32x4*)(c + r);
+        if (a.interleaved) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int el = e0 + e;
-        const bool in = el < 2 * r;
-        const int idx = !in ? 0 : a.interleaved ? el >> 1 : el < r ? el : el - r;
-        const bool first = a.interleaved ? !(el & 1) : el < r;
-        const float s = row[r + idx] * a.sign;
-        cs[e] = pv ? row[idx] : __builtin_nanf("");
-        sn[e] = first ? -s : s;
-      }
-    }
-    const bf16* xr = a.x + t * a.ldx + sub * 64 + e0;
-    const bf16* dr = BWD ? a.dy + t * a.lddy + sub * 64 + e0 : nullptr;
-    bf16* yr = a.y + t * a.ldy + sub * 64 + e0;
-    bf16x8 nx, nd;
-    if (b0 < b1) {
-      nx = *(const bf16x8*)(xr + (long)b0 * hb * 64);
-      if constexpr (BWD) nd = *(const bf16x8*)(dr + (long)b0 * hb * 64);
-    }
-    for (int b = b0; b < b1; ++b) {
-      float v[8], d[8];
-      unpack8(nx, v);
-      if constexpr (BWD) unpack8(nd, d);
-      if (b + 1 < b1) {
-        nx = *(const bf16x8*)(xr + (long)(b + 1) * hb * 64);
-        if constexpr (BWD) nd = *(const bf16x8*)(dr + (long)(b + 1) * hb * 64);
-      }
-      float rs = 1.f;
-      if constexpr (NORM != 0) {
-        if constexpr (NORM == 1) {
-          float m = 0.f;
+          for (int e = 0; e < 8; ++e) { cs[e] = c0[e >> 1]; sn[e] = (e & 1) ? s0[e >> 1] : -s0[e >> 1]; }
+        } else {
+          const f32x4 c1 = *(const f32x4*)(c + 4), s1 = *(const f32x4*)(c + r + 4);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) m += v[e];
-          m = group8_sum(m) * (1.f / 64.f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] -= m;
+          for (int e = 0; e < 4; ++e) { cs[e] = c0[e]; cs[4 + e] = c1[e]; sn[e] = e0 < r ? -s0[e] : s0[e]; sn[4 + e] = e0 < r ? -s1[e] : s1[e]; }
         }
-        float s = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s += v[e] * v[e];
-        rs = rsqrtf(group8_sum(s) * (1.f / 64.f) + a.eps);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= rs;       // x^
-      }
-      const bool isk = b >= a.nb1;                    // the same for the whole wave
-      if constexpr (!BWD) {
-        if constexpr (NORM != 0) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = isk ? v[e] * w[1][e] + bi[1][e] : v[e] * w[0][e] + bi[0][e];
-        }
-        if (r > 0) rotate8(v, cs, sn, a.interleaved, r, e0, xch);
       } else {
-        if (r > 0) rotate8(d, cs, sn, a.interleaved, r, e0, xch);
-        if constexpr (PAR) {
-          if (tv) {
-            if (isk) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) { aw[1][e] += d[e] * v[e]; ab[1][e] += d[e]; }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) { aw[0][e] += d[e] * v[e]; ab[0][e] += d[e]; }
-            }
-          }
-        }
-        float m1 = 0.f, m2 = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          d[e] *= isk ? w[1][e] : w[0][e];
-          m1 += d[e];
-          m2 += d[e] * v[e];
+          const int el = e0 + e, idx = el >= 2 * r ? 0 : a.interleaved ? el >> 1 : el < r ? el : el - r;
+          cs[e] = row[idx];
+          sn[e] = (a.interleaved ? !(el & 1) : el < r) ? -row[r + idx] : row[r + idx];
         }
-        m1 = NORM == 1 ? group8_sum(m1) * (1.f / 64.f) : 0.f;
-        m2 = group8_sum(m2) * (1.f / 64.f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = rs * (d[e] - m1 - v[e] * m2);
       }
-      if (tv) {
-        bf16x8 out;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) out[e] = (bf16)v[e];
-        *(bf16x8*)(yr + (long)b * hb * 64) = out;
+      for (int e = 0; e < 8; ++e) { cs[e] = pv ? cs[e] : __builtin_nanf(""); sn[e] *= a.sign; }
+    }
+    const bf16* xr = a.x + t * a.ldx + col;
+    const bf16* dr = BWD ? a.dy + t * a.lddy + col : nullptr;
+    bf16* yr = a.y + t * a.ldy + col;
+    for (int bb = b0; bb < b1; bb += DEPTH) {
+      bf16x8 nx[DEPTH], nd[DEPTH];
+#pragma unroll
+      for (int i = 0; i < DEPTH; ++i)
+        if (bb + i < b1) {
+          if constexpr (!BWD || NORM != 0) nx[i] = *(const bf16x8*)(xr + (bb + i) * step);
+          if constexpr (BWD) nd[i] = *(const bf16x8*)(dr + (bb + i) * step);
+        }
+#pragma unroll
+      for (int i = 0; i < DEPTH; ++i) {
+        if (bb + i >= b1) break;
+        float v[8], d[8];
+        unpack8(nx[i], v);
+        if constexpr (BWD) unpack8(nd[i], d);
+        float rs = 1.f;
+        if constexpr (NORM != 0) {
+          if constexpr (NORM == 1) {
+            float m = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m += v[e];
+            m = group8_sum(m) * (1.f / 64.f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] -= m;
+          }
+          float s = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s += v[e] * v[e];
+          rs = rsqrtf(group8_sum(s) * (1.f / 64.f) + a.eps);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] *= rs;       // x^
+        }
+        if constexpr (!BWD) {
+          if constexpr (NORM != 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = v[e] * w[e] + bi[e];
+          }
+          if (r > 0) rotate8(v, cs, sn, a.interleaved, r, e0, xch);
+        } else {
+          if (r > 0) rotate8(d, cs, sn, a.interleaved, r, e0, xch);
+          if constexpr (PAR) {
+            if (tv) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) { aw[e] += d[e] * v[e]; ab[e] += d[e]; }
+            }
+          }
+          float m1 = 0.f, m2 = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            d[e] *= w[e];
+            m1 += d[e];
+            m2 += d[e] * v[e];
+          }
+          m1 = NORM == 1 ? group8_sum(m1) * (1.f / 64.f) : 0.f;
+          m2 = group8_sum(m2) * (1.f / 64.f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = rs * (d[e] - m1 - v[e] * m2);
+        }
+        if (tv) {
+          bf16x8 out;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) out[e] = (bf16)v[e];
+          *(bf16x8*)(yr + (bb + i) * step) = out;
+        }
       }
     }
   }
   if constexpr (PAR) {     // lanes of the same columns (8 groups), then the four waves, in a fixed order
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int e = 0; e < 8; ++e) {
+      float u = aw[e], v = ab[e];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float u = aw[k][e], v = ab[k][e];
-#pragma unroll
-        for (int o = 8; o < 64; o <<= 1) { u += __shfl_xor(u, o, 64); v += __shfl_xor(v, o, 64); }
-        if (g == 0) { red[wave][k * 64 + e0 + e] = u; red[wave][128 + k * 64 + e0 + e] = v; }
-      }
+      for (int o = 8; o < 64; o <<= 1) { u += __shfl_xor(u, o, 64); v += __shfl_xor(v, o, 64); }
+      if (g == 0) { red[wave][e0 + e] = u; red[wave][64 + e0 + e] = v; }
+    }
     __syncthreads();
     const int i = threadIdx.x;
-    a.partial[((long)blockIdx.y * gridDim.x + blockIdx.x) * 256 + i] = red[0][i] + red[1][i] + red[2][i] + red[3][i];
+    if (i < 128) a.partial[((long)blockIdx.y * gridDim.x + blockIdx.x) * 128 + i] = red[0][i] + red[1][i] + red[2][i] + red[3][i];
   }
 }
 
-// out[256] = column sums of partial[G][256]: 16 columns per workgroup, 16 row walkers each, summed in a fixed order
-__global__ __launch_bounds__(256) void rotary_param_sum_kernel(const float* __restrict__ partial, int G, float* __restrict__ out) {
+// out [4][64] (query weight, key weight, query bias, key bias) = column sums of partial [2][G][128]: 16 columns per workgroup, 16 row walkers each,
+// eight rows requested at a time, summed in a fixed order
+__global__ __launch_bounds__(256) void rotary_param_sum_kernel(const float* __restrict__ partial, int G, int groups, float* __restrict__ out) {
   __shared__ float red[16][17];
-  const int c = threadIdx.x & 15, w = threadIdx.x >> 4, col = blockIdx.x * 16 + c;
+  const int c = threadIdx.x & 15, w = threadIdx.x >> 4, grp = blockIdx.x >> 3, col = (blockIdx.x & 7) * 16 + c;
+  const float* p = partial + (long)grp * G * 128 + col;
   float s = 0.f;
-  for (int i = w; i < G; i += 16) s += partial[(long)i * 256 + col];
+  for (int i = w; grp < groups && i < G; i += 128) {
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = i + 16 * k < G ? p[(long)(i + 16 * k) * 128] : 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += v[k];
+  }
   red[w][c] = s;
   __syncthreads();
   if (w == 0) {
     for (int i = 1; i < 16; ++i) s += red[i][c];
-    out[col] = s;
+    out[(col >> 6) * 128 + grp * 64 + (col & 63)] = s;
   }
 }
 
-constexpr int PARAM_WGS = 1024;     // at most this many partial sums of the norm parameters (1 MB)
+// Workgroups of a launch: as many as are resident at once (four per CU, three of the backward with parameter sums, by their registers), each walking
+// the tokens; measured at 25 216 tokens of 24 heads, forward: 31 us against 43 with a workgroup per 8 tokens, backward: 46 us against 57 with 1024.
+constexpr int ROT_WGS = 1024, PARAM_WGS = 768;
 
-struct RotGrid { unsigned x, y; int hbl, bpy; };
-// Head blocks of hb heads; a wave takes all blocks of its tokens where that still leaves 4096 waves (16 per CU: the table values are
-// then loaded once per token), else the blocks are spread over blockIdx.y.
-RotGrid rot_grid(int T, int h1, int h2, bool par) {
-  RotGrid g;
-  int hbl = 3;
-  while (hbl && ((h1 | h2) & ((1 << hbl) - 1))) --hbl;
-  const long waves = ((long)T + (8 >> hbl) - 1) / (8 >> hbl);
-  const int nb = (h1 + h2) >> hbl;
-  long bpy = (long)nb * waves / 4096;
-  bpy = bpy < 1 ? 1 : bpy > nb ? nb : bpy;
-  g.hbl = hbl;
-  g.bpy = (int)bpy;
-  g.y = (unsigned)((nb + bpy - 1) / bpy);
+// A wave takes all head blocks of its tokens where that still leaves 4096 waves (16 per CU), else the blocks are spread over blockIdx.y.
+dim3 rot_plan(RotArgs& a, int T, int h1, int h2, bool par) {
+  const int h[2] = {h1, h2};
+  long waves = 0, most = 1;
+  for (int g = 0; g < 2; ++g) {
+    int hbl = 3;
+    while (hbl && (h[g] & ((1 << hbl) - 1))) --hbl;
+    a.hbl[g] = hbl;
+    a.nb[g] = h[g] >> hbl;
+    if (h[g]) {
+      const long w = ((long)T + (8 >> hbl) - 1) / (8 >> hbl);
+      waves = w > waves ? w : waves;
+    }
+    most = a.nb[g] > most ? a.nb[g] : most;
+  }
+  const int r = a.rot >> 1;
+  a.vec = r > 0 && r % (a.interleaved ? 4 : 8) == 0 && apla_aligned16(a.table);
+  const int groups = h2 ? 2 : 1;
+  long sp = (4096 + waves * groups - 1) / (waves * groups);
+  a.splits = (int)(sp < most ? sp : most);
+  a.T = T;
   long gx = (waves + 3) / 4;
-  if (par && gx * g.y > PARAM_WGS) gx = PARAM_WGS / g.y > 0 ? PARAM_WGS / g.y : 1;
-  g.x = (unsigned)gx;
-  return g;
+  const long cap = (par ? PARAM_WGS : ROT_WGS) / groups;
+  if (gx * a.splits > cap) gx = cap / a.splits > 0 ? cap / a.splits : 1;
+  return dim3((unsigned)gx, (unsigned)(groups * a.splits));
 }
 
 int rot_check(const char* who, int T, int h1, int h2, const float* table, int P, int rot, int layout, const int32_t* pos, int seq_len) {
@@ -264,17 +288,17 @@ extern "C" int apla_rotary(const void* x, long ldx, void* y, long ldy, int T, in
   if (rc == APLA_OK) rc = rows_check("apla_rotary", "x", x, ldx, heads);
   if (rc == APLA_OK) rc = rows_check("apla_rotary", "y", y, ldy, heads);
   if (rc != APLA_OK) return rc;
-  const RotGrid g = rot_grid(T, heads, 0, false);
   RotArgs a = {};
-  a.x = (const bf16*)x; a.ldx = ldx; a.y = (bf16*)y; a.ldy = ldy; a.T = T; a.hbl = g.hbl; a.nb1 = a.nb = heads >> g.hbl;
   a.table = table; a.P = P; a.rot = rot; a.interleaved = layout == APLA_ROT_INTERLEAVED; a.pos = pos; a.seq_len = seq_len;
-  a.sign = inverse ? -1.f : 1.f; a.bpy = g.bpy;
-  hipLaunchKernelGGL((rotary_kernel<0, false, false>), dim3(g.x, g.y), dim3(256), 0, stream, a);
+  const dim3 grid = rot_plan(a, T, heads, 0, false);
+  a.x = (const bf16*)x; a.ldx = ldx; a.y = (bf16*)y; a.ldy = ldy;
+  a.sign = inverse ? -1.f : 1.f;
+  hipLaunchKernelGGL((rotary_kernel<0, false, false>), grid, dim3(256), 0, stream, a);
   APLA_CHECK_LAUNCH("apla_rotary");
   return APLA_OK;
 }
 
-extern "C" long apla_qk_norm_rotary_workspace_bytes(void) { return (long)PARAM_WGS * 256 * 4; }
+extern "C" long apla_qk_norm_rotary_workspace_bytes(void) { return (long)PARAM_WGS * 128 * 4; }
 
 extern "C" int apla_qk_norm_rotary_fwd(const void* x, long ldx, void* y, long ldy, int T, int Hq, int Hkv, int norm, float eps, const float* qw,
                                        const float* kw, const float* qb, const float* kb, const float* table, int P, int rot, int layout,
@@ -284,13 +308,13 @@ extern "C" int apla_qk_norm_rotary_fwd(const void* x, long ldx, void* y, long ld
   if (rc == APLA_OK) rc = rows_check("apla_qk_norm_rotary_fwd", "y", y, ldy, Hq + Hkv);
   if (rc != APLA_OK) return rc;
   APLA_REQUIRE((norm == APLA_NORM_LAYER || norm == APLA_NORM_RMS) && eps >= 0.f, "apla_qk_norm_rotary_fwd: unknown norm %d or eps < 0", norm);
-  const RotGrid g = rot_grid(T, Hq, Hkv, false);
   RotArgs a = {};
-  a.x = (const bf16*)x; a.ldx = ldx; a.y = (bf16*)y; a.ldy = ldy; a.T = T; a.hbl = g.hbl; a.nb1 = Hq >> g.hbl; a.nb = (Hq + Hkv) >> g.hbl;
   a.table = table; a.P = P; a.rot = rot; a.interleaved = layout == APLA_ROT_INTERLEAVED; a.pos = pos; a.seq_len = seq_len;
-  a.sign = 1.f; a.eps = eps; a.qw = qw; a.kw = kw; a.qb = qb; a.kb = kb; a.bpy = g.bpy;
-  if (norm == APLA_NORM_LAYER) hipLaunchKernelGGL((rotary_kernel<1, false, false>), dim3(g.x, g.y), dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((rotary_kernel<2, false, false>), dim3(g.x, g.y), dim3(256), 0, stream, a);
+  const dim3 grid = rot_plan(a, T, Hq, Hkv, false);
+  a.x = (const bf16*)x; a.ldx = ldx; a.y = (bf16*)y; a.ldy = ldy;
+  a.sign = 1.f; a.eps = eps; a.w[0] = qw; a.w[1] = kw; a.b[0] = qb; a.b[1] = kb;
+  if (norm == APLA_NORM_LAYER) hipLaunchKernelGGL((rotary_kernel<1, false, false>), grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((rotary_kernel<2, false, false>), grid, dim3(256), 0, stream, a);
   APLA_CHECK_LAUNCH("apla_qk_norm_rotary_fwd");
   return APLA_OK;
 }
@@ -306,13 +330,11 @@ extern "C" int apla_qk_norm_rotary_bwd(const void* dy, long lddy, const void* x,
   APLA_REQUIRE((norm == APLA_NORM_LAYER || norm == APLA_NORM_RMS) && eps >= 0.f, "apla_qk_norm_rotary_bwd: unknown norm %d or eps < 0", norm);
   APLA_REQUIRE(!dparams || (workspace && workspace_bytes >= apla_qk_norm_rotary_workspace_bytes()), "apla_qk_norm_rotary_bwd: parameter gradients need %ld bytes of workspace (got %ld)",
                apla_qk_norm_rotary_workspace_bytes(), workspace_bytes);
-  const RotGrid g = rot_grid(T, Hq, Hkv, dparams != nullptr);
   RotArgs a = {};
-  a.dy = (const bf16*)dy; a.lddy = lddy; a.x = (const bf16*)x; a.ldx = ldx; a.y = (bf16*)dx; a.ldy = lddx; a.T = T; a.hbl = g.hbl;
-  a.nb1 = Hq >> g.hbl; a.nb = (Hq + Hkv) >> g.hbl;
   a.table = table; a.P = P; a.rot = rot; a.interleaved = layout == APLA_ROT_INTERLEAVED; a.pos = pos; a.seq_len = seq_len;
-  a.sign = -1.f; a.eps = eps; a.qw = qw; a.kw = kw; a.bpy = g.bpy; a.partial = (float*)workspace;
-  const dim3 grid(g.x, g.y);
+  const dim3 grid = rot_plan(a, T, Hq, Hkv, dparams != nullptr);
+  a.dy = (const bf16*)dy; a.lddy = lddy; a.x = (const bf16*)x; a.ldx = ldx; a.y = (bf16*)dx; a.ldy = lddx;
+  a.sign = -1.f; a.eps = eps; a.w[0] = qw; a.w[1] = kw; a.partial = (float*)workspace;
   if (norm == APLA_NORM_LAYER) {
     if (dparams) hipLaunchKernelGGL((rotary_kernel<1, true, true>), grid, dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((rotary_kernel<1, true, false>), grid, dim3(256), 0, stream, a);
@@ -322,7 +344,7 @@ extern "C" int apla_qk_norm_rotary_bwd(const void* dy, long lddy, const void* x,
   }
   APLA_CHECK_LAUNCH("apla_qk_norm_rotary_bwd");
   if (dparams) {
-    hipLaunchKernelGGL(rotary_param_sum_kernel, dim3(16), dim3(256), 0, stream, (const float*)workspace, (int)(g.x * g.y), dparams);
+    hipLaunchKernelGGL(rotary_param_sum_kernel, dim3(16), dim3(256), 0, stream, (const float*)workspace, (int)(grid.x * a.splits), Hkv ? 2 : 1, dparams);
     APLA_CHECK_LAUNCH("apla_qk_norm_rotary_bwd");
   }
   return APLA_OK;
