@@ -66,20 +66,20 @@ __device__ __forceinline__ int row_lim(const ModArgs& a, const MSeq& m, int i) {
 __device__ __forceinline__ int wave_min_i(int v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
-  return v;
+  return __builtin_amdgcn_readfirstlane(v);
 }
 __device__ __forceinline__ int wave_max_i(int v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
-  return v;
+  return __builtin_amdgcn_readfirstlane(v);
 }
 
 // ---- a product with weights that may be zero next to values that may be infinite or NaN
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 #if defined(APLA_FP16)
-constexpr unsigned EXP_LO = 0x7c00u, EXP_STEP = 0x04000400u, ONE_BITS = 0x3c00u;
+constexpr unsigned EXP_LO = 0x7c00u, EXP_STEP = 0x04000400u;
 #else
-constexpr unsigned EXP_LO = 0x7f80u, EXP_STEP = 0x00800080u, ONE_BITS = 0x3f80u;
+constexpr unsigned EXP_LO = 0x7f80u, EXP_STEP = 0x00800080u;
 #endif
 constexpr unsigned EXP_HI = EXP_LO << 16;
 // bits 15 / 31 of the result: an exponent of all ones among the fragment's values (magnitude + one exponent step carries into the sign's place)
@@ -90,39 +90,31 @@ __device__ __forceinline__ unsigned nonfinite_bits(const bf16x8& f) {
   for (int i = 0; i < 4; ++i) r |= (w[i] & 0x7fff7fffu) + EXP_STEP;
   return r & 0x80008000u;
 }
-// ---- fragments by lane constants: tile_off's swizzle looks at bits 1-3 of the row only, so next to a first row that is a multiple of 16 the byte offset
-// of a fragment is that row * 128 + a constant of the lane; left to itself hipcc keeps an address per fragment (40 registers)
-struct Frag { unsigned rf[4], tr[4]; };
+// ---- fragments by lane constants.  tile_off XORs the 16-byte chunk with bits 1-3 of the row, so next to a first row that is a multiple of 16 every
+// fragment's address is that row * 128 plus one constant of the lane, up to an XOR of bits 5 and 6: k-step ks of a row fragment ^ (ks << 5), column
+// half dt of a transposed one ^ (dt << 6), its rows + 8 ^ 32 (tiles start at multiples of 128 bytes).  Left to itself hipcc keeps 40 addresses.
+struct Frag { unsigned rf, tr; };
 __device__ __forceinline__ Frag frag_consts(int lane) {
-  Frag f;
-#pragma unroll
-  for (int ks = 0; ks < 4; ++ks) f.rf[ks] = (unsigned)tile_off(lane & 31, 2 * ks + (lane >> 5));
-  const int g = lane >> 4, i = lane & 15, r = 4 * (g >> 1) + (i >> 2);
-#pragma unroll
-  for (int dt = 0; dt < 2; ++dt) {
-    const int col = 32 * dt + 16 * (g & 1) + 4 * (i & 3);
-    f.tr[2 * dt] = (unsigned)(tile_off(r, col >> 3) + ((col & 4) << 1));
-    f.tr[2 * dt + 1] = (unsigned)(tile_off(r + 8, col >> 3) + ((col & 4) << 1));
-  }
-  return f;
+  const int g = lane >> 4, i = lane & 15, r = 4 * (g >> 1) + (i >> 2), col = 16 * (g & 1) + 4 * (i & 3);
+  return {(unsigned)tile_off(lane & 31, lane >> 5), (unsigned)(tile_off(r, col >> 3) + ((col & 4) << 1))};
 }
 __device__ __forceinline__ unsigned lds_of(const char* p) { return (unsigned)(size_t)(__attribute__((address_space(3))) const char*)p; }
-__device__ __forceinline__ bf16x8 row_at(unsigned tile, int row, unsigned c) {
-  return *(const __attribute__((address_space(3))) bf16x8*)(size_t)(tile + c + row * 128);
+__device__ __forceinline__ bf16x8 row_at(unsigned base, int row, int ks) {      // base = tile + rf
+  return *(const __attribute__((address_space(3))) bf16x8*)(size_t)((base ^ (unsigned)(ks << 5)) + row * 128);
 }
-__device__ __forceinline__ bf16x8 tr_at(unsigned tile, int row, unsigned c0, unsigned c1) {
-  const bf16x4 lo = DS_READ_TR16_B64_H16((__attribute__((address_space(3))) char*)(size_t)(tile + c0 + row * 128));
-  const bf16x4 hi = DS_READ_TR16_B64_H16((__attribute__((address_space(3))) char*)(size_t)(tile + c1 + row * 128));
+__device__ __forceinline__ bf16x8 tr_at(unsigned base, int row, int dt) {      // base = tile + tr
+  const bf16x4 lo = DS_READ_TR16_B64_H16((__attribute__((address_space(3))) char*)(size_t)((base ^ (unsigned)(dt << 6)) + row * 128));
+  const bf16x4 hi = DS_READ_TR16_B64_H16((__attribute__((address_space(3))) char*)(size_t)((base ^ (unsigned)(dt << 6) ^ 32u) + (row + 8) * 128));
   return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
 // The 32 transposed fragments' product acc[2] += tile^T w: rows rbase .. rbase + 31 of an LDS tile times the weights that the accumulator w holds for them.
 struct TrFrags { bf16x8 f[4]; };      // [dt][sk]
-__device__ __forceinline__ void tr_load(TrFrags& t, unsigned tile, int rbase, const Frag& fr) {
+__device__ __forceinline__ void tr_load(TrFrags& t, unsigned base, int rbase) {       // base = tile + tr
 #pragma unroll
   for (int sk = 0; sk < 2; ++sk)
 #pragma unroll
-    for (int dt = 0; dt < 2; ++dt) t.f[2 * dt + sk] = tr_at(tile, rbase + 16 * sk, fr.tr[2 * dt], fr.tr[2 * dt + 1]);
+    for (int dt = 0; dt < 2; ++dt) t.f[2 * dt + sk] = tr_at(base, rbase + 16 * sk, dt);
 }
 __device__ __forceinline__ void tr_product(f32x16 (&acc)[2], const TrFrags& t, const f32x16& w) {
 #pragma unroll
@@ -134,33 +126,32 @@ __device__ __forceinline__ void tr_product(f32x16 (&acc)[2], const TrFrags& t, c
 }
 
 // Zero times a non-finite value is zero: where a tile that holds such values meets a mask, the product runs over a copy of the tile with those values
-// taken out (clean_tile), and the results that a weight other than zero would lead one to are remembered as bits (poison_bits: the product of
-// the two indicator matrices; bit 16 dt + i for accumulator element [dt][i]) and become NaN at the end (apply_poison).
+// taken out (clean_tile), and the results that a weight other than zero would lead one to are remembered as bits (poison_bits; bit 16 dt + i
+// for accumulator element [dt][i]) and become NaN at the end (apply_poison).
 __device__ __forceinline__ bf16x8 finite_part(const bf16x8& f) {
   u32x4 w = __builtin_bit_cast(u32x4, f);
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = ((w[i] & EXP_LO) == EXP_LO ? 0u : w[i] & 0xffffu) | ((w[i] & EXP_HI) == EXP_HI ? 0u : w[i] & 0xffff0000u);
   return __builtin_bit_cast(bf16x8, w);
 }
-__device__ __forceinline__ unsigned poison_bits(unsigned raw, int rbase, const f32x16& w, const Frag& fr) {
-  unsigned m = 0;
+// (nearly no registers, however slow: the path must not set the kernel's register count.)  w: weights of rows rbase .. rbase + 31 of the tile `raw`.
+__device__ __forceinline__ unsigned poison_bits(const char* raw, int rbase, const f32x16& w, int lane) {
+  unsigned own = 0, m = 0;             // bit i: this lane's weight i is not zero; the other 16 rows' weights are in the other half of the wave
 #pragma unroll
-  for (int dt = 0; dt < 2; ++dt) {
-    f32x16 hits;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) hits[i] = 0.f;
-#pragma unroll
-    for (int sk = 0; sk < 2; ++sk) {
-      u32x4 x = __builtin_bit_cast(u32x4, tr_at(raw, rbase + 16 * sk, fr.tr[2 * dt], fr.tr[2 * dt + 1])), y = __builtin_bit_cast(u32x4, acc_to_operand(w, sk));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = ((x[i] & EXP_LO) == EXP_LO ? ONE_BITS : 0u) | ((x[i] & EXP_HI) == EXP_HI ? ONE_BITS << 16 : 0u);
-        y[i] = ((y[i] & 0x7fffu) ? ONE_BITS : 0u) | ((y[i] & 0x7fff0000u) ? ONE_BITS << 16 : 0u);
-      }
-      hits = MFMA_F32_32x32x16_H16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), hits);
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) m |= hits[i] > 0.f ? 1u << (16 * dt + i) : 0u;
+  for (int i = 0; i < 16; ++i) own |= w[i] != 0.f ? 1u << i : 0u;
+  const auto sw = __builtin_amdgcn_permlane32_swap(own, own, false, false);
+  const unsigned nz[2] = {(unsigned)sw[0], (unsigned)sw[1]};
+  const int h = lane >> 5;
+#pragma unroll 1
+  for (int r = 0; r < 32; ++r) {       // row r = acc_row(i, half)
+    const unsigned short x = *(const unsigned short*)(raw + tile_off(rbase + r, lane >> 3) + (lane & 7) * 2);
+    const unsigned long long bad = __ballot((x & EXP_LO) == EXP_LO);       // bit d
+    if (bad == 0) continue;
+    const unsigned lo = ((unsigned)bad >> (4 * h)) & 0x0f0f0f0fu, hi = ((unsigned)(bad >> 32) >> (4 * h)) & 0x0f0f0f0fu;
+    const unsigned mine = (lo & 0xf) | (lo >> 4 & 0xf0) | (lo >> 8 & 0xf00) | (lo >> 12 & 0xf000) |
+                          ((hi & 0xf) | (hi >> 4 & 0xf0) | (hi >> 8 & 0xf00) | (hi >> 12 & 0xf000)) << 16;
+    const unsigned z = (r >> 2) & 1 ? nz[1] : nz[0];
+    m |= (z >> ((r & 3) + 4 * (r >> 3))) & 1 ? mine : 0u;
   }
   return m;
 }
@@ -214,7 +205,7 @@ __device__ __forceinline__ float dist(const float (&p)[2], float x, float y) {
 
 // ------------------------------------------------------------------------------------------------ forward, one 64-key tile
 // LDS of a key tile: K, V (8 KB each), positions [2][64], document ids [64], each wave's verdict on the values it staged
-constexpr int KT_POS = 16384, KT_DOC = KT_POS + 512, KT_ODD = KT_DOC + 256, KT_BYTES = KT_ODD + 16;
+constexpr int KT_POS = 16384, KT_DOC = KT_POS + 512, KT_ODD = KT_DOC + 256, KT_BYTES = KT_ODD + 128;
 
 struct RowState { float m, l; };
 struct RowCtx { int lim, doc; float pos[2], slope; };       // slope in log2 units
@@ -232,6 +223,49 @@ __device__ __forceinline__ float cap_fine(float s, const ModArgs& a, float& r) {
   return y < 0.0625f ? series : z;
 }
 __device__ __forceinline__ int pick(const int4& v, int e) { return e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w; }
+// x[16] of one row and 32 keys, first key jr0, hidden ones replaced: by the row's limit, then by the documents (ids of the 32 at LDS `ids`).  One read at a
+// time: this path must not set the kernel's register count.
+__device__ __forceinline__ void hide_keys(f32x16& x, float hidden, int lim, int doc, int jr0, const char* ids, int h2, bool docs) {
+  const int left = lim - jr0 - 4 * h2;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = (i & 3) + 8 * (i >> 2) < left ? x[i] : hidden;
+  if (docs) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int4 d = *(const int4*)(ids + (8 * g + 4 * h2) * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * g + e] = pick(d, e) == doc ? x[4 * g + e] : hidden;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+// x and y [16] of one key j and 32 rows (their limits and ids in LDS): hidden ones become 0
+__device__ __forceinline__ void hide_rows(f32x16& x, f32x16& y, int j, int doc, const char* lims, const char* ids, int h2, bool docs) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int4 l = *(const int4*)(lims + (8 * g + 4 * h2) * 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool vis = j < pick(l, e);
+      x[4 * g + e] = vis ? x[4 * g + e] : 0.f;
+      y[4 * g + e] = vis ? y[4 * g + e] : 0.f;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  if (docs) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int4 d = *(const int4*)(ids + (8 * g + 4 * h2) * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool vis = pick(d, e) == doc;
+        x[4 * g + e] = vis ? x[4 * g + e] : 0.f;
+        y[4 * g + e] = vis ? y[4 * g + e] : 0.f;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
 
 // Scores s[16] of one row (on the lane) and 32 keys, or of one key and 32 rows, in log2 units; with neither cap nor bias they stay raw and the
 // caller multiplies by c.  `side`: LDS address of the positions of the other 32 (x, then y 256 bytes behind), r: cap_score's r of every score.
@@ -269,70 +303,83 @@ __device__ __forceinline__ float half_max(float v) {
 }
 
 // masked: some of the 64 keys are hidden from some of the wave's rows.  odd: V holds non-finite values; `clean` is then its copy without them.
+// One wave's 32 rows against 64 keys in two halves: while the matrix unit multiplies Q with the second half's keys the wave exponentiates the first half,
+// and the first half's product with V runs under the second half's exponentials.
+// masked: some of the 64 keys are hidden from some of the wave's rows.  odd: V holds non-finite values; `clean` is then its copy without them.
 template <bool CAP, int BIAS>
 __device__ __forceinline__ void fwd_tile(f32x16 (&acc)[2], RowState& st, unsigned& poison, const bf16x8 (&qf)[4], const ModArgs& a, const RowCtx& r,
                                          const char* tile, const char* clean, int j0, int lane, const Frag& fr, bool masked, bool docs, bool odd) {
   const int h2 = lane >> 5;
   const float zm = (CAP || BIAS) ? 1.f : a.c;
-  const unsigned Ks = lds_of(tile), Vs = odd ? lds_of(clean) : Ks + 8192;
+  const unsigned Ks = lds_of(tile) + fr.rf, Vs = (odd ? lds_of(clean) : lds_of(tile) + 8192) + fr.tr;
   f32x16 s[2], unused;
-  {
-    bf16x8 kf[2][4];
+  auto scores = [&](int kt) {
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
+    for (int i = 0; i < 16; ++i) s[kt][i] = 0.f;
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) kf[kt][ks] = row_at(Ks, kt * 32, fr.rf[ks]);
-    __builtin_amdgcn_sched_barrier(0);     // all eight reads under way before the first product waits for one
+    for (int ks = 0; ks < 4; ++ks) s[kt] = MFMA_F32_32x32x16_H16(row_at(Ks, kt * 32, ks), qf[ks], s[kt]);
+  };
+  auto finish = [&](int kt) {       // cap, bias, mask, running maximum
+    modify<CAP, BIAS>(s[kt], unused, a, r.pos, r.slope, tile + KT_POS + kt * 128, h2, masked);
+    if (masked) hide_keys(s[kt], -INFINITY, r.lim, r.doc, j0 + kt * 32, tile + KT_DOC + kt * 128, h2, docs);
+    float mx = s[kt][0];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[kt][i]);
+    mx = half_max(mx);
+    if (__ballot((mx - st.m) * zm > LAZY)) {
+      const float m_new = fmaxf(st.m, mx), alpha = __builtin_amdgcn_exp2f((st.m - m_new) * zm);
+      st.m = m_new;
+      st.l *= alpha;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[kt][i] = 0.f;
+      for (int i = 0; i < 16; ++i) { acc[0][i] *= alpha; acc[1][i] *= alpha; }
+      if (kt == 1) {         // the first half's weights are not in acc yet
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) s[kt] = MFMA_F32_32x32x16_H16(kf[kt][ks], qf[ks], s[kt]);
-  }
-  TrFrags vf[2];                           // V's fragments arrive under the softmax
-#pragma unroll
-  for (int kt = 0; kt < 2; ++kt) tr_load(vf[kt], Vs, kt * 32, fr);
-  __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-  for (int kt = 0; kt < 2; ++kt) modify<CAP, BIAS>(s[kt], unused, a, r.pos, r.slope, tile + KT_POS + kt * 128, h2, masked);
-  if (masked) {
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int jr = kt * 32 + 8 * g + 4 * h2;
-        const int4 dj = docs ? *(const int4*)(tile + KT_DOC + jr * 4) : int4{0, 0, 0, 0};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[kt][4 * g + e] = j0 + jr + e < r.lim && (!docs || pick(dj, e) == r.doc) ? s[kt][4 * g + e] : -INFINITY;
+        for (int i = 0; i < 16; ++i) s[0][i] *= alpha;
       }
-  }
-  float mx = s[0][0];
+    }
+  };
+  float mc;
+  auto weights = [&](int kt, int g) {      // four of the sixteen
 #pragma unroll
-  for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kt][i]);
-  mx = half_max(mx);
-  if (__ballot((mx - st.m) * zm > LAZY)) {
-    const float m_new = fmaxf(st.m, mx), alpha = __builtin_amdgcn_exp2f((st.m - m_new) * zm);
-    st.m = m_new;
-    st.l *= alpha;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) { acc[0][i] *= alpha; acc[1][i] *= alpha; }
-  }
-  const float mc = st.m * zm;
-#pragma unroll
-  for (int kt = 0; kt < 2; ++kt) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 4 * g; i < 4 * g + 4; ++i) {
       s[kt][i] = __builtin_amdgcn_exp2f((CAP || BIAS) ? s[kt][i] - mc : fmaf(s[kt][i], zm, -mc));
       st.l += s[kt][i];
     }
-    if (__builtin_expect(odd, 0)) poison |= poison_bits(Ks + 8192, kt * 32, s[kt], fr);
-    tr_product(acc, vf[kt], s[kt]);
+  };
+  scores(0);
+  finish(0);
+  mc = st.m * zm;
+  {
+    bf16x8 kf[4];
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) kf[ks] = row_at(Ks, 32, ks);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[1][i] = 0.f;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      weights(0, g);
+      s[1] = MFMA_F32_32x32x16_H16(kf[g], qf[g], s[1]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
+  asm volatile("" : "+v"(s[0]));           // (hipcc would move the exponentials behind the branches that follow)
+  TrFrags vf;
+  tr_load(vf, Vs, 0);
+  finish(1);
+  if (__builtin_expect(odd, 0)) poison |= poison_bits(tile + 8192, 0, s[0], lane);
+  mc = st.m * zm;
+  {
+    const bf16x8 w0 = acc_to_operand(s[0], 0), w1 = acc_to_operand(s[0], 1);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      acc[g & 1] = MFMA_F32_32x32x16_H16(vf.f[2 * (g & 1) + (g >> 1)], g < 2 ? w0 : w1, acc[g & 1]);
+      weights(1, g);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  tr_load(vf, Vs, 32);
+  if (__builtin_expect(odd, 0)) poison |= poison_bits(tile + 8192, 32, s[1], lane);
+  tr_product(acc, vf, s[1]);
 }
 
 // ---- the list of key tiles that rows with (lim_max, documents dmin..dmax) can see, one pass of up to LIST tiles from t0
@@ -367,10 +414,10 @@ __device__ __forceinline__ int build_list(TileRef* list, int* cnt, int t0, int n
 __device__ __forceinline__ void group_range(int& lo, int& hi, int& lim0, int& lim, int* buf, int wave, int lane) {
   if (lane == 0) { buf[wave] = lo; buf[4 + wave] = hi; buf[8 + wave] = lim; buf[12 + wave] = lim0; }
   __syncthreads();
-  lo = min(min(buf[0], buf[1]), min(buf[2], buf[3]));
-  hi = max(max(buf[4], buf[5]), max(buf[6], buf[7]));
-  lim = max(max(buf[8], buf[9]), max(buf[10], buf[11]));
-  lim0 = min(min(buf[12], buf[13]), min(buf[14], buf[15]));
+  lo = __builtin_amdgcn_readfirstlane(min(min(buf[0], buf[1]), min(buf[2], buf[3])));
+  hi = __builtin_amdgcn_readfirstlane(max(max(buf[4], buf[5]), max(buf[6], buf[7])));
+  lim = __builtin_amdgcn_readfirstlane(max(max(buf[8], buf[9]), max(buf[10], buf[11])));
+  lim0 = __builtin_amdgcn_readfirstlane(min(min(buf[12], buf[13]), min(buf[14], buf[15])));
   __syncthreads();
 }
 
@@ -434,7 +481,7 @@ __device__ __forceinline__ RowCtx row_ctx(const ModArgs& a, const MSeq& m, int i
 // ------------------------------------------------------------------------------------------------ forward
 template <bool CAP, int BIAS>
 __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
-  __shared__ __attribute__((aligned(16))) char smem[2 * KT_BYTES], clean[8192];
+  __shared__ __attribute__((aligned(128))) char smem[2 * KT_BYTES], clean[8192];
   __shared__ TileRef list[LIST + 3];
   __shared__ int buf[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
@@ -539,7 +586,7 @@ __device__ __forceinline__ void wstage_store(const WStage& t, char* lds, int lan
 
 template <bool CAP, int BIAS>
 __global__ __launch_bounds__(256, 1) void attn_mod_rows_kernel(ModArgs a) {
-  __shared__ __attribute__((aligned(16))) char smem[4 * (KT_BYTES + 8192)];
+  __shared__ __attribute__((aligned(128))) char smem[4 * (KT_BYTES + 8192)];
   __shared__ float ml[4][2][32];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
   const Frag fr = frag_consts(lane);
@@ -684,14 +731,14 @@ __device__ __forceinline__ void dq_tile(f32x16 (&acc)[2], unsigned& poison, cons
     f32x16 s, p, rc;
     bf16x8 kf[4], vf[4];
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) { kf[ks] = row_at(Ks, kt * 32, fr.rf[ks]); vf[ks] = row_at(Vs, kt * 32, fr.rf[ks]); }
+    for (int ks = 0; ks < 4; ++ks) { kf[ks] = row_at(Ks + fr.rf, kt * 32, ks); vf[ks] = row_at(Vs + fr.rf, kt * 32, ks); }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < 16; ++i) { s[i] = 0.f; p[i] = 0.f; }
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) { s = MFMA_F32_32x32x16_H16(kf[ks], qf[ks], s); p = MFMA_F32_32x32x16_H16(vf[ks], df[ks], p); }
     TrFrags tk;
-    tr_load(tk, Kt, kt * 32, fr);
+    tr_load(tk, Kt + fr.tr, kt * 32);
     __builtin_amdgcn_sched_barrier(0);
     modify<CAP, BIAS>(s, rc, a, r.pos, r.slope, tile + KT_POS + kt * 128, h2, masked);
 #pragma unroll
@@ -700,14 +747,8 @@ __device__ __forceinline__ void dq_tile(f32x16 (&acc)[2], unsigned& poison, cons
       if constexpr (CAP) s[i] *= 4.f * rc[i] * (1.f - rc[i]);
     }
     if (masked) {
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int jr = kt * 32 + 8 * g + 4 * h2;
-        const int4 dj = docs ? *(const int4*)(tile + KT_DOC + jr * 4) : int4{0, 0, 0, 0};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[4 * g + e] = j0 + jr + e < r.lim && (!docs || pick(dj, e) == r.doc) ? s[4 * g + e] : 0.f;
-      }
-      if (__builtin_expect(odd, 0)) poison |= poison_bits(Ks, kt * 32, s, fr);
+      hide_keys(s, 0.f, r.lim, r.doc, j0 + kt * 32, tile + KT_DOC + kt * 128, h2, docs);
+      if (__builtin_expect(odd, 0)) poison |= poison_bits(tile, kt * 32, s, lane);
     }
     tr_product(acc, tk, s);
   }
@@ -715,7 +756,7 @@ __device__ __forceinline__ void dq_tile(f32x16 (&acc)[2], unsigned& poison, cons
 
 template <bool CAP, int BIAS>
 __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
-  __shared__ __attribute__((aligned(16))) char smem[2 * KT_BYTES], clean[8192];
+  __shared__ __attribute__((aligned(128))) char smem[2 * KT_BYTES], clean[8192];
   __shared__ TileRef list[LIST + 3];
   __shared__ int buf[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
@@ -814,7 +855,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
 
 // dK, dV of 128 keys: every wave holds 32 keys (the key on the lane) and the workgroup walks the 64-row query tiles of all heads that share them.
 // LDS of a query tile: Q, dO (8 KB each), then per row: lse (log2 units), delta, position x / y, lim, document, verdicts
-constexpr int QT_L = 16384, QT_D = QT_L + 256, QT_X = QT_D + 256, QT_Y = QT_X + 256, QT_LIM = QT_Y + 256, QT_DOC = QT_LIM + 256, QT_ODD = QT_DOC + 256, QT_BYTES = QT_ODD + 16;
+constexpr int QT_L = 16384, QT_D = QT_L + 256, QT_X = QT_D + 256, QT_Y = QT_X + 256, QT_LIM = QT_Y + 256, QT_DOC = QT_LIM + 256, QT_ODD = QT_DOC + 256, QT_BYTES = QT_ODD + 128;
 struct QuerySide { float L2, delta, x, y; int lim, doc; };
 
 template <bool CAP, int BIAS>
@@ -828,7 +869,7 @@ __device__ __forceinline__ void dkdv_tile(f32x16 (&dk)[2], f32x16 (&dv)[2], unsi
     {
       bf16x8 qf[4], df[4];
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) { qf[ks] = row_at(Qs, qt * 32, fr.rf[ks]); df[ks] = row_at(Ds, qt * 32, fr.rf[ks]); }
+      for (int ks = 0; ks < 4; ++ks) { qf[ks] = row_at(Qs + fr.rf, qt * 32, ks); df[ks] = row_at(Ds + fr.rf, qt * 32, ks); }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < 16; ++i) { s[i] = 0.f; p[i] = 0.f; }
@@ -836,7 +877,7 @@ __device__ __forceinline__ void dkdv_tile(f32x16 (&dk)[2], f32x16 (&dv)[2], unsi
       for (int ks = 0; ks < 4; ++ks) { s = MFMA_F32_32x32x16_H16(qf[ks], kf[ks], s); p = MFMA_F32_32x32x16_H16(df[ks], vf[ks], p); }
     }
     TrFrags td;
-    tr_load(td, Qt + 8192, qt * 32, fr);
+    tr_load(td, Qt + 8192 + fr.tr, qt * 32);
     __builtin_amdgcn_sched_barrier(0);
     modify<CAP, BIAS>(s, rc, a, pj, slope, tile + QT_X + qt * 128, h2, masked);
 #pragma unroll
@@ -853,24 +894,14 @@ __device__ __forceinline__ void dkdv_tile(f32x16 (&dk)[2], f32x16 (&dv)[2], unsi
       }
     }
     if (masked) {
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int ir = qt * 32 + 8 * g + 4 * h2;
-        const int4 lm = *(const int4*)(tile + QT_LIM + ir * 4), di = docs ? *(const int4*)(tile + QT_DOC + ir * 4) : int4{0, 0, 0, 0};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool vis = j < pick(lm, e) && (!docs || pick(di, e) == docj);
-          p[4 * g + e] = vis ? p[4 * g + e] : 0.f;
-          s[4 * g + e] = vis ? s[4 * g + e] : 0.f;
-        }
-      }
+      hide_rows(p, s, j, docj, tile + QT_LIM + qt * 128, tile + QT_DOC + qt * 128, h2, docs);
       if (__builtin_expect(odd, 0)) {
-        pv |= poison_bits(Ds, qt * 32, p, fr);
-        pk |= poison_bits(Qs, qt * 32, s, fr);
+        pv |= poison_bits(tile + 8192, qt * 32, p, lane);
+        pk |= poison_bits(tile, qt * 32, s, lane);
       }
     }
     TrFrags tq;
-    tr_load(tq, Qt, qt * 32, fr);
+    tr_load(tq, Qt + fr.tr, qt * 32);
     tr_product(dv, td, p);
     tr_product(dk, tq, s);
   }
@@ -878,7 +909,7 @@ __device__ __forceinline__ void dkdv_tile(f32x16 (&dk)[2], f32x16 (&dv)[2], unsi
 
 template <bool CAP, int BIAS>
 __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
-  __shared__ __attribute__((aligned(16))) char smem[2 * QT_BYTES], clean[16384];
+  __shared__ __attribute__((aligned(128))) char smem[2 * QT_BYTES], clean[16384];
   __shared__ TileRef list[LIST + 3];
   __shared__ int buf[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
