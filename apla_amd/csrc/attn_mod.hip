@@ -313,12 +313,6 @@ __device__ __forceinline__ void fwd_tile(f32x16 (&acc)[2], RowState& st, unsigne
   const float zm = (CAP || BIAS) ? 1.f : a.c;
   const unsigned Ks = lds_of(tile) + fr.rf, Vs = (odd ? lds_of(clean) : lds_of(tile) + 8192) + fr.tr;
   f32x16 s[2], unused;
-  auto scores = [&](int kt) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[kt][i] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) s[kt] = MFMA_F32_32x32x16_H16(row_at(Ks, kt * 32, ks), qf[ks], s[kt]);
-  };
   auto finish = [&](int kt) {       // cap, bias, mask, running maximum
     modify<CAP, BIAS>(s[kt], unused, a, r.pos, r.slope, tile + KT_POS + kt * 128, h2, masked);
     if (masked) hide_keys(s[kt], -INFINITY, r.lim, r.doc, j0 + kt * 32, tile + KT_DOC + kt * 128, h2, docs);
@@ -346,7 +340,16 @@ __device__ __forceinline__ void fwd_tile(f32x16 (&acc)[2], RowState& st, unsigne
       st.l += s[kt][i];
     }
   };
-  scores(0);
+  {
+    bf16x8 kf[4];
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) kf[ks] = row_at(Ks, 0, ks);
+    __builtin_amdgcn_sched_barrier(0);     // the four reads are under way before the first product waits for one
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[0][i] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) s[0] = MFMA_F32_32x32x16_H16(kf[ks], qf[ks], s[0]);
+  }
   finish(0);
   mc = st.m * zm;
   {
@@ -518,12 +521,12 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
     auto fetch = [&](int t) {
       stage_load(ks, kb, a.ldk, offk, t * 64, m.nk, tid);
       stage_load(vs, vb, a.ldv, offv, t * 64, m.nk, tid);
-      side_load<BIAS>(sd, a, m, t * 64, tid);
+      if (BIAS || docs) side_load<BIAS>(sd, a, m, t * 64, tid);
     };
     auto put = [&](char* tile, bool whole) {
       stage_store(ks, tile, tid);
       stage_store(vs, tile + 8192, tid);
-      side_store<BIAS>(sd, tile, a, tid);
+      if (BIAS || docs) side_store<BIAS>(sd, tile, a, tid);
       if (!whole) {
         const bool odd = stage_odd(vs);
         if (lane == 0) *(int*)(tile + KT_ODD + wave * 4) = odd;
@@ -549,8 +552,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
         clean_tile(tile + 8192, clean, tid);
         __syncthreads();
       }
-      if (uniform(active && j0 < wlim1 && (!docs || (cur.hi >= max(wlo, 0) && cur.lo <= whi)))) {
-        const bool masked = !cur.whole && !uniform(j0 + 64 <= wlim0 && (!docs || (cur.lo == cur.hi && wlo == cur.lo && whi == cur.lo)));
+      if (active && j0 < wlim1 && (!docs || (cur.hi >= max(wlo, 0) && cur.lo <= whi))) {
+        const bool masked = !cur.whole && !(j0 + 64 <= wlim0 && (!docs || (cur.lo == cur.hi && wlo == cur.lo && whi == cur.lo)));
         fwd_tile<CAP, BIAS>(acc, st, poison, qf, a, r, tile, clean, j0, lane, fr, masked, docs, masked && odd);
       }
       if (e + 1 < n) put(smem + ((e + 1) & 1) * KT_BYTES, next.whole);
@@ -806,12 +809,12 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
     auto fetch = [&](int t) {
       stage_load(ks, kb, a.ldk, offk, t * 64, m.nk, tid);
       stage_load(vs, vb, a.ldv, offv, t * 64, m.nk, tid);
-      side_load<BIAS>(sd, a, m, t * 64, tid);
+      if (BIAS || docs) side_load<BIAS>(sd, a, m, t * 64, tid);
     };
     auto put = [&](char* tile, bool whole) {
       stage_store(ks, tile, tid);
       stage_store(vs, tile + 8192, tid);
-      side_store<BIAS>(sd, tile, a, tid);
+      if (BIAS || docs) side_store<BIAS>(sd, tile, a, tid);
       if (!whole) {
         const bool odd = stage_odd(ks);
         if (lane == 0) *(int*)(tile + KT_ODD + wave * 4) = odd;
@@ -837,8 +840,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
         clean_tile(tile + 0, clean, tid);
         __syncthreads();
       }
-      if (uniform(active && j0 < wlim1 && (!docs || (cur.hi >= max(wlo, 0) && cur.lo <= whi)))) {
-        const bool masked = !cur.whole && !uniform(j0 + 64 <= wlim0 && (!docs || (cur.lo == cur.hi && wlo == cur.lo && whi == cur.lo)));
+      if (active && j0 < wlim1 && (!docs || (cur.hi >= max(wlo, 0) && cur.lo <= whi))) {
+        const bool masked = !cur.whole && !(j0 + 64 <= wlim0 && (!docs || (cur.lo == cur.hi && wlo == cur.lo && whi == cur.lo)));
         dq_tile<CAP, BIAS>(acc, poison, qf, df, L2, delta, a, r, tile, clean, j0, lane, fr, masked, docs, masked && odd);
       }
       if (e + 1 < n) put(smem + ((e + 1) & 1) * KT_BYTES, next.whole);
@@ -1009,9 +1012,9 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
         clean_tile(tile + 8192, clean + 8192, tid);
         __syncthreads();
       }
-      if (uniform(active && row_lim(a, m, last) > jw && (!docs || (cur.hi >= max(wlo, 0) && cur.lo <= whi)))) {
+      if (active && row_lim(a, m, last) > jw && (!docs || (cur.hi >= max(wlo, 0) && cur.lo <= whi))) {
         const float slope = BIAS ? a.slopes[hk * a.G + g] * LOG2E : 0.f;
-        const bool masked = !cur.whole && !uniform(i0 + 64 <= m.nq && jw + 32 <= m.nk && row_lim(a, m, i0) >= jw + 32 &&
+        const bool masked = !cur.whole && !(i0 + 64 <= m.nq && jw + 32 <= m.nk && row_lim(a, m, i0) >= jw + 32 &&
                                                    (!docs || (cur.lo >= 0 && cur.lo == cur.hi && wlo == cur.lo && whi == cur.lo)));
         dkdv_tile<CAP, BIAS>(dk, dv, pk, pv, kf, vf, a, j, docj, pj, slope, tile, clean, lane, fr, masked, docs, masked && odd);
       }
