@@ -39,6 +39,8 @@ struct ModArgs {
   long lddq, lddk, lddv;
   float* delta;
   float *part_o, *part_ml;              // few-row kernel: partial sums
+  float *part_q, *part_k;               // backward: partial dQ [sq][Tq][Hq * 64]; dK, then dV [sk][Tk][Hkv * 64]
+  int sq, sk;                           // workgroups that share a block's tiles
   int nsplit, chunk, nrt;
 };
 
@@ -469,6 +471,14 @@ __device__ __forceinline__ Where where(const ModArgs& a, int per) {
 static inline int unit_parts(long units) { return units % 8 == 0 ? 1 : units % 4 == 0 ? 2 : units % 2 == 0 ? 4 : 8; }
 static inline long unit_grid(long units, int np, long per) { return units * np * ((per + np - 1) / np); }
 
+// a transposed accumulator pair (store_acc_T's layout) as fp32 partial sums of one split
+__device__ __forceinline__ void store_part(const f32x16 (&acc)[2], float* rowptr, int h) {
+#pragma unroll
+  for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) *(f32x4*)(rowptr + 32 * dt + 8 * g + 4 * h) = f32x4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+}
+
 // what a lane knows of its query row
 template <int BIAS>
 __device__ __forceinline__ RowCtx row_ctx(const ModArgs& a, const MSeq& m, int i, int h) {
@@ -574,152 +584,241 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ forward, few rows: keys split over waves and workgroups
-// The G * nq rows of the query heads that share a key head fill the 32 lanes of a tile, so K and V are read once for all of them.  Every wave
-// walks its own 64-key tiles (every fourth of the workgroup's chunk) through its own LDS, without a barrier; the four waves' (max, sum,
-// output) are joined in LDS, those of several workgroups by attn_mod_join_kernel, both in a fixed order.
-struct WStage { bf16x8 v[8]; };
-__device__ __forceinline__ void wstage_load(WStage& t, const bf16* base, long ld, int row0, int nrows, int lane) {
+// The G * nq rows of the query heads that share a key head fill tiles of 16 columns (v_mfma_f32_16x16x32: a single token of 1 .. 16 heads is one
+// tile).  Every wave walks its own
+// 64-key tiles (every fourth of the workgroup's chunk) without a barrier: K straight into operand registers, V through the wave's own LDS for the
+// transposed read, both a tile ahead.  The four waves' (maximum, sum, output) are joined in LDS, those of several workgroups by
+// attn_mod_join_kernel, both in a fixed order.
+constexpr int RT_POS = 8192, RT_DOC = RT_POS + 512, RT_BYTES = RT_DOC + 256;      // LDS of a wave: V, positions [2][64], document ids
+constexpr int ROWS = 16;
+
+// Scores [4][4] of row (lane & 15) and keys 16 kb + 4 (lane >> 4) + i, as modify() for the wide tiles
+template <bool CAP, int BIAS>
+__device__ __forceinline__ void modify_few(f32x4 (&s)[4], const ModArgs& a, const RowCtx& r, const char* side, int g, bool masked) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) t.v[i] = *(const bf16x8*)(base + (long)min(row0 + 8 * i + (lane >> 3), nrows - 1) * ld + (lane & 7) * 8);
+  for (int kb = 0; kb < 4; ++kb) {
+    f32x4 px, py;
+    if constexpr (BIAS > 0) px = *(const f32x4*)(side + (16 * kb + 4 * g) * 4);
+    if constexpr (BIAS > 1) py = *(const f32x4*)(side + 256 + (16 * kb + 4 * g) * 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float z = s[kb][e], rc;
+      if constexpr (CAP) z = masked ? cap_fine(z, a, rc) : cap_score(z, a, rc);
+      if constexpr (BIAS > 0) {
+        const float d = dist<BIAS>(r.pos, px[e], BIAS > 1 ? py[e] : 0.f);
+        z = CAP ? z - r.slope * d : fmaf(z, a.c, -r.slope * d);
+      }
+      s[kb][e] = z;
+    }
+  }
 }
-__device__ __forceinline__ void wstage_store(const WStage& t, char* lds, int lane) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) *(bf16x8*)(lds + tile_off(8 * i + (lane >> 3), lane & 7)) = t.v[i];
+// the four lane groups of a wave hold the same 16 rows: largest value / sum of the four, in all of them
+__device__ __forceinline__ float quad_max(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+  return half_max(fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1])));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
 }
 
 template <bool CAP, int BIAS>
-__global__ __launch_bounds__(256, 1) void attn_mod_rows_kernel(ModArgs a) {
-  __shared__ __attribute__((aligned(128))) char smem[4 * (KT_BYTES + 8192)];
-  __shared__ float ml[4][2][32];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
-  const Frag fr = frag_consts(lane);
+__global__ __launch_bounds__(256, 2) void attn_mod_rows_kernel(ModArgs a) {
+  __shared__ __attribute__((aligned(128))) char smem[4 * RT_BYTES];
+  __shared__ float ml[4][2][ROWS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c16 = lane & 15;
   const int Hkv = a.Hq / a.G;
-  const int sp = blockIdx.x % a.nsplit, rt = blockIdx.x / a.nsplit, hk = blockIdx.y, s = blockIdx.z;
+  // sequences and heads fastest: the XCDs (blockIdx & 7) then share every chunk number, of which the last hold keys in the longest sequences only
+  const int pairs = a.S * Hkv, pair = blockIdx.x % pairs, part = blockIdx.x / pairs;
+  const int hk = pair % Hkv, s = pair / Hkv, rt = part % a.nrt, sp = part / a.nrt;
   const MSeq m = mseq(a, s);
-  const int rows = a.G * m.nq, rr = rt * 32 + (lane & 31);
-  if (rt * 32 >= rows) return;
-  const int rc = min(rr, rows - 1), h = hk * a.G + rc % a.G, qi = rc / a.G;
-  const RowCtx r = row_ctx<BIAS>(a, m, qi, h);
+  const int rows = a.G * m.nq, rr = rt * ROWS + c16;
+  if (rt * ROWS >= rows) return;
+  const int jb = sp * a.chunk, jw = jb + wave * 64;
+  if (sp > 0 && jb >= m.nk) return;      // (the join reads no chunk past the keys)
   const bool docs = a.doc_k != nullptr;
-  const int wlo = wave_min_i(r.doc), whi = wave_max_i(r.doc), wlim0 = wave_min_i(r.lim), wlim1 = wave_max_i(r.lim);
-  f32x16 acc[2];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) { acc[0][i] = 0.f; acc[1][i] = 0.f; }
-  RowState st = {NEG_BIG, 0.f};
-  unsigned poison = 0;
-  const int jb = sp * a.chunk, je = min(wlim1, jb + a.chunk);
-  char* tile = smem + wave * (KT_BYTES + 8192);
+  char* tile = smem + wave * RT_BYTES;
   const bf16 *kb = a.k + m.k0 * a.ldk + hk * 64, *vb = a.v + m.k0 * a.ldv + hk * 64;
-  if (jb + wave * 64 < je) {
-    bf16x8 qf[4];
-    load_row_frags(qf, a.q + (m.q0 + qi) * a.ldq + h * 64, lane);
-    WStage ks, vs;
-    KeySide sd;
-    auto fetch = [&](int j0) {
-      wstage_load(ks, kb, a.ldk, j0, m.nk, lane);
-      wstage_load(vs, vb, a.ldv, j0, m.nk, lane);
-      side_load<BIAS>(sd, a, m, j0, lane);
-    };
-    fetch(jb + wave * 64);
-    for (int j0 = jb + wave * 64; j0 < je; j0 += 256) {
-      wstage_store(ks, tile, lane);
-      wstage_store(vs, tile + 8192, lane);
-      side_store<BIAS>(sd, tile, a, lane);
+  bf16x8 kf[4][2], vs[8];
+  KeySide sd;
+  auto fetch = [&](int j0) {       // keys past the last read it again
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) kf[b][ks] = *(const bf16x8*)(kb + (long)min(j0 + 16 * b + c16, m.nk - 1) * a.ldk + 32 * ks + 8 * g);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) vs[i] = *(const bf16x8*)(vb + (long)min(j0 + 8 * i + (lane >> 3), m.nk - 1) * a.ldv + (lane & 7) * 8);
+    side_load<BIAS>(sd, a, m, j0, lane);
+  };
+  if (jw < m.nk) fetch(jw);        // before anything is known of the rows: the first tile's way from memory is half of a short call
+  const int rc = min(rr, rows - 1), h = hk * a.G + rc % a.G, qi = rc / a.G;
+  bf16x8 qf[2];
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) qf[ks] = *(const bf16x8*)(a.q + (m.q0 + qi) * a.ldq + h * 64 + 32 * ks + 8 * g);
+  const RowCtx r = row_ctx<BIAS>(a, m, qi, h);
+  const int wlo = wave_min_i(r.doc), whi = wave_max_i(r.doc), wlim0 = wave_min_i(r.lim), wlim1 = wave_max_i(r.lim);
+  f32x4 acc[4];
+#pragma unroll
+  for (int d = 0; d < 4; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  RowState st = {NEG_BIG, 0.f};
+  unsigned poison = 0;             // bit 4 db + i
+  const float zm = (CAP || BIAS) ? 1.f : a.c;
+  const int je = min(wlim1, jb + a.chunk);
+  const int vo = 4 * g + (c16 >> 2), vcol = 4 * (c16 & 3);
+  const unsigned tr = lds_of(tile) + (unsigned)(tile_off(vo, vcol >> 3) + ((vcol & 4) << 1));
+  for (int j0 = jw; j0 < je; j0 += 256) {
+    bool odd = false, any = true, full = j0 + 64 <= wlim0;
+    if (docs) {
+      const int2 x = a.rng_k[(long)s * a.nt_k + j0 / 64];
+      any = uniform(x.y >= max(wlo, 0) && x.x <= whi);
+      full = full && uniform(x.x == x.y && wlo == x.x && whi == x.x);
+    }
+    f32x4 sc[4];
+    if (any) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        sc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) sc[b] = MFMA_F32_16x16x32_H16(kf[b][ks], qf[ks], sc[b]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) *(bf16x8*)(tile + tile_off(8 * i + (lane >> 3), lane & 7)) = vs[i];
+    if constexpr (BIAS > 0) *(float*)(tile + RT_POS + lane * 4) = sd.x;
+    if constexpr (BIAS > 1) *(float*)(tile + RT_POS + 256 + lane * 4) = sd.y;
+    if (docs) *(int*)(tile + RT_DOC + lane * 4) = sd.d;
+    if (!full) {
       unsigned bits = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) bits |= nonfinite_bits(vs.v[i]);
-      const bool odd = __ballot(bits != 0) != 0;
-      __builtin_amdgcn_wave_barrier();
-      asm volatile("" ::: "memory");
-      if (j0 + 256 < je) fetch(j0 + 256);
-      bool full = j0 + 64 <= wlim0, any = true;
-      if (docs) {
-        const int2 g = a.rng_k[(long)s * a.nt_k + j0 / 64];
-        any = g.y >= max(wlo, 0) && g.x <= whi;
-        full = full && g.x == g.y && wlo == g.x && whi == g.x;
-      }
-      const bool masked = !uniform(full);
-      if (masked && odd) {      // this wave's own copy of V
+      for (int i = 0; i < 8; ++i) bits |= nonfinite_bits(vs[i]);
+      odd = __ballot(bits != 0) != 0;
+    }
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+    if (j0 + 256 < je) fetch(j0 + 256);
+    if (any) {
+      modify_few<CAP, BIAS>(sc, a, r, tile + RT_POS, g, !full);
+      if (!full) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) *(bf16x8*)(tile + KT_BYTES + (i * 64 + lane) * 16) = finite_part(*(const bf16x8*)(tile + 8192 + (i * 64 + lane) * 16));
+        for (int b = 0; b < 4; ++b) {
+          const int4 d = docs ? *(const int4*)(tile + RT_DOC + (16 * b + 4 * g) * 4) : int4{0, 0, 0, 0};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[b][e] = j0 + 16 * b + 4 * g + e < r.lim && (!docs || pick(d, e) == r.doc) ? sc[b][e] : -INFINITY;
+        }
+      }
+      float mx = sc[0][0];
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[b][e]);
+      mx = quad_max(mx);
+      if (__ballot((mx - st.m) * zm > LAZY)) {
+        const float m_new = fmaxf(st.m, mx), alpha = __builtin_amdgcn_exp2f((st.m - m_new) * zm);
+        st.m = m_new;
+        st.l *= alpha;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) acc[d] *= alpha;
+      }
+      const float mc = st.m * zm;
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sc[b][e] = __builtin_amdgcn_exp2f((CAP || BIAS) ? sc[b][e] - mc : fmaf(sc[b][e], zm, -mc));
+          st.l += sc[b][e];
+        }
+      if (__builtin_expect(odd, 0)) {      // as poison_bits, then the wave's own tile is cleaned in place
+        unsigned own = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) own |= sc[i >> 2][i & 3] != 0.f ? 1u << i : 0u;
+#pragma unroll 1
+        for (int k = 0; k < 64; ++k) {
+          const unsigned short x = *(const unsigned short*)(tile + tile_off(k, lane >> 3) + (lane & 7) * 2);
+          const unsigned long long bad = __ballot((x & EXP_LO) == EXP_LO);
+          const unsigned nz = (unsigned)__shfl((int)own, c16 + 16 * ((k >> 2) & 3), 64);
+          unsigned mine = 0;
+#pragma unroll
+          for (int d = 0; d < 4; ++d) mine |= ((unsigned)(bad >> (16 * d + 4 * g)) & 0xfu) << (4 * d);
+          poison |= (nz >> (4 * (k >> 4) + (k & 3))) & 1 ? mine : 0u;
+        }
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("" ::: "memory");
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) *(bf16x8*)(tile + (i * 64 + lane) * 16) = finite_part(*(const bf16x8*)(tile + (i * 64 + lane) * 16));
         __builtin_amdgcn_wave_barrier();
         asm volatile("" ::: "memory");
       }
-      if (uniform(any)) fwd_tile<CAP, BIAS>(acc, st, poison, qf, a, r, tile, tile + KT_BYTES, j0, lane, fr, masked, docs, masked && odd);
-      __builtin_amdgcn_wave_barrier();
-      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {        // 32 keys: operand element j is key 32 t + 16 (j >> 2) + 4 g + (j & 3), on both sides
+        bf16x8 p;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = (bf16)sc[2 * t + (j >> 2)][j & 3];
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const bf16x4 lo = DS_READ_TR16_B64_H16((__attribute__((address_space(3))) char*)(size_t)((tr ^ (unsigned)(d << 5)) + 32 * t * 128));
+          const bf16x4 hi = DS_READ_TR16_B64_H16((__attribute__((address_space(3))) char*)(size_t)((tr ^ (unsigned)(d << 5)) + (32 * t + 16) * 128));
+          acc[d] = MFMA_F32_16x16x32_H16((bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}), p, acc[d]);
+        }
+      }
     }
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
   }
-  apply_poison(acc, poison);
-  // join the four waves: [32 rows][64] fp32 per wave in its own 8 KB (rows XOR-spread over the banks by their 16-byte chunk)
-  float* mine = (float*)(smem + wave * 8192);
-  const float l = st.l + __shfl_xor(st.l, 32, 64);
-  __syncthreads();
 #pragma unroll
-  for (int dt = 0; dt < 2; ++dt)
+  for (int i = 0; i < 16; ++i) acc[i >> 2][i & 3] = (poison >> i) & 1 ? __builtin_nanf("") : acc[i >> 2][i & 3];
+  // join the four waves: [16 rows][64] fp32 each in 4 KB of its own LDS, 16-byte chunks spread over the banks by their row
+  const float l = quad_sum(st.l);
+  float* mine = (float*)tile;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int row = lane & 31, ch = 8 * dt + 2 * g + h2;
-      *(f32x4*)(mine + row * 64 + ((ch ^ (row & 15)) << 2)) = f32x4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
-    }
-  const float zm = (CAP || BIAS) ? 1.f : a.c;
-  if (h2 == 0) { ml[wave][0][lane] = st.m * zm; ml[wave][1][lane] = l; }
+  for (int d = 0; d < 4; ++d) *(f32x4*)(mine + c16 * 64 + (((4 * d + g) ^ c16) << 2)) = acc[d];
+  if (g == 0) { ml[wave][0][c16] = st.m * zm; ml[wave][1][c16] = l; }
   __syncthreads();
-  const int row = tid >> 3, ro = rt * 32 + row;
-  float M = fmaxf(fmaxf(ml[0][0][row], ml[1][0][row]), fmaxf(ml[2][0][row], ml[3][0][row])), L = 0.f, f[4];
-  f32x4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  const int row = tid >> 4, ch = tid & 15, ro = rt * ROWS + row;
+  const float M = fmaxf(fmaxf(ml[0][0][row], ml[1][0][row]), fmaxf(ml[2][0][row], ml[3][0][row]));
+  float L = 0.f;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
-    f[u] = ml[u][1][row] != 0.f ? __builtin_amdgcn_exp2f(ml[u][0][row] - M) : 0.f;
-    L += f[u] * ml[u][1][row];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const f32x4 t = *(const f32x4*)((const float*)(smem + u * 8192) + row * 64 + (((2 * (tid & 7) + i) ^ (row & 15)) << 2));
-      x[i] += f[u] * t;
-    }
+    const float f = ml[u][1][row] != 0.f ? __builtin_amdgcn_exp2f(ml[u][0][row] - M) : 0.f;
+    L += f * ml[u][1][row];
+    const f32x4 t = *(const f32x4*)((const float*)(smem + u * RT_BYTES) + row * 64 + ((ch ^ row) << 2));
+    if (f != 0.f) x += f * t;
   }
   if (ro >= rows) return;
   const int ho = hk * a.G + ro % a.G;
   const long qo = m.q0 + ro / a.G;
   if (a.nsplit == 1) {
     const float inv = L != 0.f ? 1.f / L : 0.f;
-    bf16x8 y;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = (bf16)(x[i >> 2][i & 3] * inv);
-    *(bf16x8*)(a.o + qo * a.ldo + ho * 64 + (tid & 7) * 8) = y;
-    if ((tid & 7) == 0) a.lse[(long)ho * a.Tq + qo] = L != 0.f ? (M + __builtin_amdgcn_logf(L)) * LN2 : -INFINITY;
+    *(bf16x4*)(a.o + qo * a.ldo + ho * 64 + ch * 4) = pack4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+    if (ch == 0) a.lse[(long)ho * a.Tq + qo] = L != 0.f ? (M + __builtin_amdgcn_logf(L)) * LN2 : -INFINITY;
   } else {
-    const long p = (((long)s * Hkv + hk) * a.nrt + rt) * a.nsplit + sp;
-    *(f32x4*)(a.part_o + (p * 32 + row) * 64 + (tid & 7) * 8) = x[0];
-    *(f32x4*)(a.part_o + (p * 32 + row) * 64 + (tid & 7) * 8 + 4) = x[1];
-    if ((tid & 7) == 0) { a.part_ml[(p * 32 + row) * 2] = M; a.part_ml[(p * 32 + row) * 2 + 1] = L; }
+    const long p = ((((long)s * Hkv + hk) * a.nrt + rt) * a.nsplit + sp) * ROWS + row;
+    *(f32x4*)(a.part_o + p * 64 + ch * 4) = x;
+    if (ch == 0) { a.part_ml[p * 2] = M; a.part_ml[p * 2 + 1] = L; }
   }
 }
 
 __global__ __launch_bounds__(256) void attn_mod_join_kernel(ModArgs a) {
-  const int tid = threadIdx.x, row = tid >> 3, rt = blockIdx.x, hk = blockIdx.y, s = blockIdx.z;
+  const int tid = threadIdx.x, row = tid >> 4, ch = tid & 15, rt = blockIdx.x, hk = blockIdx.y, s = blockIdx.z;
   const MSeq m = mseq(a, s);
-  const int rows = a.G * m.nq, ro = rt * 32 + row;
+  const int rows = a.G * m.nq, ro = rt * ROWS + row;
   if (ro >= rows) return;
   const long p0 = (((long)s * (a.Hq / a.G) + hk) * a.nrt + rt) * a.nsplit;
   float M = NEG_BIG, L = 0.f;
-  f32x4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-  for (int sp = 0; sp < a.nsplit; ++sp) M = fmaxf(M, a.part_ml[((p0 + sp) * 32 + row) * 2]);
-  for (int sp = 0; sp < a.nsplit; ++sp) {
-    const long p = (p0 + sp) * 32 + row;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  const int n = min(a.nsplit, (m.nk + a.chunk - 1) / a.chunk);      // chunks past the sequence's keys hold nothing
+  for (int sp = 0; sp < n; ++sp) M = fmaxf(M, a.part_ml[((p0 + sp) * ROWS + row) * 2]);
+  for (int sp = 0; sp < n; ++sp) {
+    const long p = (p0 + sp) * ROWS + row;
     const float l = a.part_ml[p * 2 + 1], f = l != 0.f ? __builtin_amdgcn_exp2f(a.part_ml[p * 2] - M) : 0.f;
     L += f * l;
-    x[0] += f * *(const f32x4*)(a.part_o + p * 64 + (tid & 7) * 8);
-    x[1] += f * *(const f32x4*)(a.part_o + p * 64 + (tid & 7) * 8 + 4);
+    if (f != 0.f) x += f * *(const f32x4*)(a.part_o + p * 64 + ch * 4);
   }
   const int ho = hk * a.G + ro % a.G;
   const long qo = m.q0 + ro / a.G;
   const float inv = L != 0.f ? 1.f / L : 0.f;
-  bf16x8 y;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = (bf16)(x[i >> 2][i & 3] * inv);
-  *(bf16x8*)(a.o + qo * a.ldo + ho * 64 + (tid & 7) * 8) = y;
-  if ((tid & 7) == 0) a.lse[(long)ho * a.Tq + qo] = L != 0.f ? (M + __builtin_amdgcn_logf(L)) * LN2 : -INFINITY;
+  *(bf16x4*)(a.o + qo * a.ldo + ho * 64 + ch * 4) = pack4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+  if (ch == 0) a.lse[(long)ho * a.Tq + qo] = L != 0.f ? (M + __builtin_amdgcn_logf(L)) * LN2 : -INFINITY;
 }
 
 // ------------------------------------------------------------------------------------------------ backward
@@ -764,9 +863,9 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
   __shared__ int buf[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
   const Frag fr = frag_consts(lane);
-  const Where w = where(a, a.G * a.nblk);
-  if (w.j >= a.G * a.nblk) return;
-  const int Hkv = a.Hq / a.G, hk = w.unit % Hkv, h = hk * a.G + w.j % a.G, blk = w.j / a.G;
+  const Where w = where(a, a.G * a.nblk * a.sq);
+  if (w.j >= a.G * a.nblk * a.sq) return;
+  const int Hkv = a.Hq / a.G, hk = w.unit % Hkv, h = hk * a.G + w.j % a.G, sp = w.j / a.G % a.sq, blk = w.j / (a.G * a.sq);
   const MSeq m = mseq(a, w.unit / Hkv);
   const int q0 = (a.causal ? a.nblk - 1 - blk : blk) * 128;
   if (q0 >= m.nq) return;
@@ -789,7 +888,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
   }
   const float ls = a.lse[stat];
   const float L2 = ls == -INFINITY ? -NEG_BIG : ls * LOG2E;
-  if (qr < m.nq && h2 == 0) a.delta[stat] = delta;
+  if (sp == 0 && qr < m.nq && h2 == 0) a.delta[stat] = delta;
   const RowCtx r = row_ctx<BIAS>(a, m, qi, h);
   const bool docs = a.doc_k != nullptr;
   const int wlo = wave_min_i(r.doc), whi = wave_max_i(r.doc), wlim0 = wave_min_i(r.lim), wlim1 = wave_max_i(r.lim);
@@ -820,18 +919,19 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
         if (lane == 0) *(int*)(tile + KT_ODD + wave * 4) = odd;
       }
     };
+    const int each = (n + a.sq - 1) / a.sq, e0 = min(n, sp * each), e1 = min(n, e0 + each);      // this split's part of the list
     TileRef cur, next;
     int t2 = 0;
-    if (n > 0) {
-      cur = scalar_ref(list[0]); next = scalar_ref(list[1]);
-      t2 = __builtin_amdgcn_readfirstlane(list[2].t);
+    if (e0 < e1) {
+      cur = scalar_ref(list[e0]); next = scalar_ref(list[e0 + 1]);
+      t2 = __builtin_amdgcn_readfirstlane(list[e0 + 2].t);
       fetch(cur.t);
       put(smem, cur.whole);
       fetch(next.t);
     }
     __syncthreads();
-    for (int e = 0; e < n; ++e) {      // tile e is in LDS, e + 1 in registers; e + 2 is requested when those are free
-      char* tile = smem + (e & 1) * KT_BYTES;
+    for (int e = e0; e < e1; ++e) {      // tile e is in LDS, e + 1 in registers; e + 2 is requested when those are free
+      char* tile = smem + ((e - e0) & 1) * KT_BYTES;
       const TileRef ahead = list[e + 2 < n ? e + 2 : n - 1];
       const int t3 = list[e + 3 < n ? e + 3 : n - 1].t;
       const int j0 = cur.t * 64;
@@ -844,8 +944,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
         const bool masked = !cur.whole && !(j0 + 64 <= wlim0 && (!docs || (cur.lo == cur.hi && wlo == cur.lo && whi == cur.lo)));
         dq_tile<CAP, BIAS>(acc, poison, qf, df, L2, delta, a, r, tile, clean, j0, lane, fr, masked, docs, masked && odd);
       }
-      if (e + 1 < n) put(smem + ((e + 1) & 1) * KT_BYTES, next.whole);
-      if (e + 2 < n) fetch(t2);
+      if (e + 1 < e1) put(smem + ((e + 1 - e0) & 1) * KT_BYTES, next.whole);
+      if (e + 2 < e1) fetch(t2);
       cur = next;
       next = scalar_ref(ahead);
       t2 = __builtin_amdgcn_readfirstlane(t3);
@@ -853,7 +953,10 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
     }
   }
   apply_poison(acc, poison);
-  if (qr < m.nq) store_acc_T(acc, a.dq + (m.q0 + qr) * a.lddq + h * 64, h2, a.scale);
+  if (qr < m.nq) {
+    if (a.sq == 1) store_acc_T(acc, a.dq + (m.q0 + qr) * a.lddq + h * 64, h2, a.scale);
+    else store_part(acc, a.part_q + (((long)sp * a.Tq + m.q0 + qr) * a.Hq + h) * 64, h2);
+  }
 }
 
 // dK, dV of 128 keys: every wave holds 32 keys (the key on the lane) and the workgroup walks the 64-row query tiles of all heads that share them.
@@ -917,11 +1020,11 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
   __shared__ int buf[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
   const Frag fr = frag_consts(lane);
-  const Where w = where(a, a.nblk);
-  if (w.j >= a.nblk) return;
-  const int Hkv = a.Hq / a.G, hk = w.unit % Hkv;
+  const Where w = where(a, a.nblk * a.sk);
+  if (w.j >= a.nblk * a.sk) return;
+  const int Hkv = a.Hq / a.G, hk = w.unit % Hkv, sp = w.j % a.sk;
   const MSeq m = mseq(a, w.unit / Hkv);
-  const int jb = w.j * 128;
+  const int jb = w.j / a.sk * 128;
   if (jb >= m.nk) return;
   const int jr = jb + wave * 32 + (lane & 31), j = min(jr, m.nk - 1);
   const bool active = jb + wave * 32 < m.nk;
@@ -948,7 +1051,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
   const int w0 = jlast >= m.nk ? ntiles : (!a.causal || m.pre > jlast) ? 0 : (max(0, jlast - m.off) + 63) / 64, w1 = m.nq / 64;
   for (int t0 = first; t0 < ntiles; t0 += LIST) {
     const int n = build_list(list, buf, t0, ntiles, w0, w1, docs ? a.rng_q + (long)(w.unit / Hkv) * a.nt_q : nullptr, dlo, dhi, tid);
-    const int total = n * a.G;
+    const int each = (n * a.G + a.sk - 1) / a.sk, x0 = min(n * a.G, sp * each), total = min(n * a.G, x0 + each) - x0;      // this split's part
     Stage qs, os;
     QuerySide sd;
     auto fetch = [&](int t, int g) {      // a query tile of head g of the group
@@ -986,13 +1089,13 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
     };
     // entry e of head g is in LDS, the next in registers; the one behind that, e2 of head g2, is requested when those are free
     TileRef cur, next;
-    int e = 0, g = 0, e2 = 0, g2 = 0, t2 = 0;
+    int e = n ? x0 % n : 0, g = n ? x0 / n : 0, e2 = e, g2 = g, t2 = 0;
     auto step = [&](int& e_, int& g_) { if (++e_ == n) { e_ = 0; ++g_; } };
-    if (n > 0) {
-      cur = scalar_ref(list[0]);
+    if (total > 0) {
+      cur = scalar_ref(list[e2]);
       step(e2, g2);
       next = scalar_ref(list[e2]);
-      fetch(cur.t, 0);
+      fetch(cur.t, g);
       put(smem, cur.whole);
       if (total > 1) fetch(next.t, g2);
       step(e2, g2);
@@ -1030,9 +1133,33 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
   apply_poison(dk, pk);
   apply_poison(dv, pv);
   if (jr < m.nk) {
-    store_acc_T(dk, a.dk + (m.k0 + jr) * a.lddk + hk * 64, h2, a.scale);
-    store_acc_T(dv, a.dv + (m.k0 + jr) * a.lddv + hk * 64, h2, 1.f);
+    if (a.sk == 1) {
+      store_acc_T(dk, a.dk + (m.k0 + jr) * a.lddk + hk * 64, h2, a.scale);
+      store_acc_T(dv, a.dv + (m.k0 + jr) * a.lddv + hk * 64, h2, 1.f);
+    } else {
+      float* p = a.part_k + (((long)sp * a.Tk + m.k0 + jr) * Hkv + hk) * 64;
+      store_part(dk, p, h2);
+      store_part(dv, p + (long)a.sk * a.Tk * Hkv * 64, h2);
+    }
   }
+}
+
+// out rows = mul * the sum of n fp32 partial sums, in their order; rows that no sequence holds are left.  blockIdx: (32-row group of a sequence, head, sequence)
+__global__ __launch_bounds__(256) void attn_mod_sum_kernel(ModArgs a, const float* part, int n, int queries, bf16* out, long ldo, float mul) {
+  const int row = blockIdx.x * 32 + (threadIdx.x >> 3), h = blockIdx.y, heads = gridDim.y, c = (threadIdx.x & 7) * 8;
+  const MSeq m = mseq(a, blockIdx.z);
+  if (row >= (queries ? m.nq : m.nk)) return;
+  const long r = (queries ? m.q0 : m.k0) + row, T = queries ? a.Tq : a.Tk;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+  for (int i = 0; i < n; ++i) {
+    const float* p = part + ((i * T + r) * heads + h) * 64 + c;
+    x += *(const f32x4*)p;
+    y += *(const f32x4*)(p + 4);
+  }
+  bf16x8 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) { v[e] = (bf16)(x[e] * mul); v[4 + e] = (bf16)(y[e] * mul); }
+  *(bf16x8*)(out + r * ldo + h * 64 + c) = v;
 }
 
 // smallest and largest document id of every 64-row tile of every sequence: one wave per tile
@@ -1050,21 +1177,30 @@ __global__ __launch_bounds__(256) void attn_mod_ranges_kernel(ModArgs a, int que
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-struct Plan { bool rows; int nsplit, chunk, nrt; long rng_q, rng_k, part, bytes; };
+struct Plan { bool rows; int nsplit, chunk, nrt, sq, sk; long rng_q, rng_k, part, part_q, part_k, bytes; };
 
-// Few rows (attn_mod_rows_kernel): where the rows of a head group fill at most one tile of 32 lanes, or where 128-row workgroups would leave
-// most of the card idle next to long keys.  Keys are split so that about two workgroups per CU run, 256 keys at least each.
+// Backward: workgroups that share the tiles of one 128-row block, where the blocks alone would leave the card idle (fewer than 512 of them: two per CU),
+// each with at least four 64-row tiles; their fp32 partial sums are added by attn_mod_sum_kernel.
+int split_of(long blocks, long tiles) {
+  const long want = (768 + blocks - 1) / blocks, most = tiles / 4;
+  const long n = blocks >= 512 ? 1 : want < most ? want : most;
+  return (int)(n < 1 ? 1 : n > 8 ? 8 : n);
+}
+
+// Few rows (attn_mod_rows_kernel): up to two tiles of 16 rows of a head group, or at most 64 blocks of 128 rows in all (a quarter of the CUs; measured with
+// 39 blocks of 1654 keys 26 us against 45, 64 of 4096 keys 42 against 75, but 144 of 257 keys 22 against 12).  Keys are split so that about
+// 1024 workgroups run, 256 keys at least each (32 ragged caches of up to 8192 keys: 48 us with chunks of 2048, 80 with 4096, 52 with 1024).
 Plan plan_of(const apla_attn_mod_t& p, bool backward) {
   Plan pl = {};
   const int G = p.Hq / p.Hkv;
   const long rows = (long)G * p.max_q, wgs = (long)p.S * p.Hq * ((p.max_q + 127) / 128);
-  pl.nrt = (int)((rows + 31) / 32);
-  pl.rows = !backward && (rows <= 32 || (wgs < 128 && p.max_k >= 512 && pl.nrt <= 64));
+  pl.nrt = (int)((rows + ROWS - 1) / ROWS);
+  pl.rows = !backward && (rows <= 2 * ROWS || wgs <= 64);
   pl.nsplit = 1;
   pl.chunk = (p.max_k + 255) / 256 * 256;
   if (pl.rows) {
     const long have = (long)p.S * p.Hkv * pl.nrt;
-    long want = (512 + have - 1) / have;
+    long want = (1024 + have - 1) / have;
     const long most = (p.max_k + 255) / 256;
     want = want < 1 ? 1 : want > most ? most : want;
     if (want < 1) want = 1;
@@ -1078,14 +1214,21 @@ Plan plan_of(const apla_attn_mod_t& p, bool backward) {
     pl.rng_k = b; b += ((long)p.S * ((p.max_k + 63) / 64) * 8 + 15) / 16 * 16;
     if (backward) { pl.rng_q = b; b += ((long)p.S * ((p.max_q + 63) / 64) * 8 + 15) / 16 * 16; }
   }
-  if (pl.rows && pl.nsplit > 1) { pl.part = b; b += (long)p.S * p.Hkv * pl.nrt * pl.nsplit * 32 * (64 + 2) * 4; }
+  if (pl.rows && pl.nsplit > 1) { pl.part = b; b += (long)p.S * p.Hkv * pl.nrt * pl.nsplit * ROWS * (64 + 2) * 4; }
+  pl.sq = pl.sk = 1;
+  if (backward) {
+    pl.sq = split_of((long)p.S * p.Hq * ((p.max_q + 127) / 128), (p.max_k + 63) / 64);
+    pl.sk = split_of((long)p.S * p.Hkv * ((p.max_k + 127) / 128), (long)G * ((p.max_q + 63) / 64));
+    if (pl.sq > 1) { pl.part_q = b; b += (long)pl.sq * p.Tq * p.Hq * 256; }
+    if (pl.sk > 1) { pl.part_k = b; b += 2L * pl.sk * p.Tk * p.Hkv * 256; }
+  }
   pl.bytes = b;
   return pl;
 }
 
 int mod_check(const char* who, const apla_attn_mod_t* p, bool backward) {
   APLA_REQUIRE(p, "%s: no arguments", who);
-  APLA_REQUIRE(p->S > 0 && p->S <= 65535 && p->Hq > 0 && p->Hkv > 0 && p->Hkv <= 65535 && p->Hq % p->Hkv == 0, "%s: need 1..65535 sequences and Hq a multiple of Hkv (S=%d Hq=%d Hkv=%d)", who, p->S, p->Hq, p->Hkv);
+  APLA_REQUIRE(p->S > 0 && p->S <= 65535 && p->Hq > 0 && p->Hq <= 65535 && p->Hkv > 0 && p->Hq % p->Hkv == 0, "%s: need 1..65535 sequences and Hq a multiple of Hkv (S=%d Hq=%d Hkv=%d)", who, p->S, p->Hq, p->Hkv);
   APLA_REQUIRE(p->Tq > 0 && p->Tk > 0 && p->max_q > 0 && p->max_k > 0 && p->max_q <= p->Tq && p->max_k <= p->Tk, "%s: need 0 < max_q <= Tq and 0 < max_k <= Tk (%d/%d, %d/%d)", who, p->max_q, p->Tq, p->max_k, p->Tk);
   APLA_REQUIRE((p->cu_q || (long)p->S * p->max_q == p->Tq) && (p->cu_k || (long)p->S * p->max_k == p->Tk), "%s: without offsets the rows must be S x max", who);
   APLA_REQUIRE(p->max_q <= (1 << 24) && p->max_k <= (1 << 24), "%s: sequences of at most 2^24 tokens", who);
@@ -1105,8 +1248,8 @@ int mod_check(const char* who, const apla_attn_mod_t* p, bool backward) {
   }
   const Plan pl = plan_of(*p, backward);
   APLA_REQUIRE(pl.bytes == 0 || (p->workspace && apla_aligned16(p->workspace) && p->workspace_bytes >= pl.bytes), "%s: needs %ld bytes of 16-byte aligned workspace (got %ld)", who, pl.bytes, p->workspace_bytes);
-  const long nb = (long)p->S * p->Hkv * 8 * ((long)(p->Hq / p->Hkv) * (((long)(p->max_q > p->max_k ? p->max_q : p->max_k) + 127) / 128) + 1);
-  APLA_REQUIRE(nb < (1L << 31), "%s: too many blocks", who);
+  const long nb = (long)p->S * p->Hkv * 8 * 8 * ((long)(p->Hq / p->Hkv) * (((long)(p->max_q > p->max_k ? p->max_q : p->max_k) + 127) / 128) + 1);
+  APLA_REQUIRE(nb < (1L << 31) && (long)p->S * p->Hkv * pl.nrt * pl.nsplit < (1L << 31), "%s: too many blocks", who);
   return APLA_OK;
 }
 
@@ -1125,7 +1268,8 @@ ModArgs mod_args(const apla_attn_mod_t& p, const Plan& pl) {
   a.np = unit_parts((long)p.S * p.Hkv);
   a.nsplit = pl.nsplit; a.chunk = pl.chunk; a.nrt = pl.nrt;
   a.part_o = (float*)(ws + pl.part);
-  a.part_ml = a.part_o + (long)p.S * p.Hkv * pl.nrt * pl.nsplit * 32 * 64;
+  a.part_ml = a.part_o + (long)p.S * p.Hkv * pl.nrt * pl.nsplit * ROWS * 64;
+  a.sq = pl.sq; a.sk = pl.sk; a.part_q = (float*)(ws + pl.part_q); a.part_k = (float*)(ws + pl.part_k);
   a.d_o = (const bf16*)p.d_o; a.lddo = p.lddo; a.dq = (bf16*)p.dq; a.dk = (bf16*)p.dk; a.dv = (bf16*)p.dv;
   a.lddq = p.lddq; a.lddk = p.lddk; a.lddv = p.lddv; a.delta = p.delta;
   return a;
@@ -1166,7 +1310,7 @@ extern "C" int apla_attn_mod_fwd(const apla_attn_mod_t* p, hipStream_t stream) {
   const long units = (long)p->S * p->Hkv;
   if (a.doc_k) launch_ranges(a, false, stream);
   if (pl.rows) {
-    const dim3 grid((unsigned)(pl.nrt * pl.nsplit), (unsigned)p->Hkv, (unsigned)p->S);
+    const dim3 grid((unsigned)(units * pl.nrt * pl.nsplit));
     APLA_MOD_LAUNCH(attn_mod_rows_kernel, grid);
     if (pl.nsplit > 1) hipLaunchKernelGGL(attn_mod_join_kernel, dim3((unsigned)pl.nrt, (unsigned)p->Hkv, (unsigned)p->S), dim3(256), 0, stream, a);
   } else {
@@ -1187,13 +1331,20 @@ extern "C" int apla_attn_mod_bwd(const apla_attn_mod_t* p, hipStream_t stream) {
   if (a.doc_k) { launch_ranges(a, false, stream); launch_ranges(a, true, stream); }
   a.nblk = (p->max_q + 127) / 128;
   {
-    const dim3 grid((unsigned)unit_grid(units, a.np, (long)a.G * a.nblk));
+    const dim3 grid((unsigned)unit_grid(units, a.np, (long)a.G * a.nblk * a.sq));
     APLA_MOD_LAUNCH(attn_mod_dq_kernel, grid);
+    if (a.sq > 1)
+      hipLaunchKernelGGL(attn_mod_sum_kernel, dim3((unsigned)((p->max_q + 31) / 32), (unsigned)p->Hq, (unsigned)p->S), dim3(256), 0, stream, a, (const float*)a.part_q, a.sq, 1, a.dq, a.lddq, a.scale);
   }
   a.nblk = (p->max_k + 127) / 128;
   {
-    const dim3 grid((unsigned)unit_grid(units, a.np, a.nblk));
+    const dim3 grid((unsigned)unit_grid(units, a.np, (long)a.nblk * a.sk));
     APLA_MOD_LAUNCH(attn_mod_dkdv_kernel, grid);
+    if (a.sk > 1) {
+      const dim3 sum((unsigned)((p->max_k + 31) / 32), (unsigned)p->Hkv, (unsigned)p->S);
+      hipLaunchKernelGGL(attn_mod_sum_kernel, sum, dim3(256), 0, stream, a, (const float*)a.part_k, a.sk, 0, a.dk, a.lddk, a.scale);
+      hipLaunchKernelGGL(attn_mod_sum_kernel, sum, dim3(256), 0, stream, a, (const float*)(a.part_k + (long)a.sk * a.Tk * p->Hkv * 64), a.sk, 0, a.dv, a.lddv, 1.f);
+    }
   }
   APLA_CHECK_LAUNCH("apla_attn_mod_bwd");
   return APLA_OK;
