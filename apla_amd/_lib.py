@@ -20,7 +20,7 @@ class AttnMod(ctypes.Structure):
     _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "o", "lse", "cu_q", "cu_k", "len_k", "prefix", "doc_q", "doc_k", "slopes", "pos_q",
                                          "pos_k", "d_o", "dq", "dk", "dv", "delta", "workspace")]
                 + [(n, c_long) for n in ("workspace_bytes", "ldq", "ldk", "ldv", "ldo", "lddo", "lddq", "lddk", "lddv")]
-                + [(n, c_int) for n in ("S", "Tq", "Tk", "max_q", "max_k", "Hq", "Hkv", "pos_dim", "causal")]
+                + [(n, c_int) for n in ("S", "Tq", "Tk", "max_q", "max_k", "Hq", "Hkv", "pos_dim", "causal", "fill")]
                 + [(n, c_float) for n in ("scale", "softcap")])
 
 

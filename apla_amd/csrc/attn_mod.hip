@@ -1162,6 +1162,28 @@ __global__ __launch_bounds__(256) void attn_mod_sum_kernel(ModArgs a, const floa
   *(bf16x8*)(out + r * ldo + h * 64 + c) = v;
 }
 
+// The rows that no sequence holds (before the first, behind the last, past a sequence's used or cut length) of the outputs named in `fill`: 0, -inf in lse.
+// blockIdx.x: the rows behind sequence blockIdx.x - 1 (0: before the first), blockIdx.y: a share of them.
+__global__ __launch_bounds__(256) void attn_mod_fill_kernel(ModArgs a, int fill) {
+  const int s = (int)blockIdx.x - 1, Hkv = a.Hq / a.G;
+  const MSeq m = mseq(a, s < 0 ? 0 : s), n = mseq(a, s + 1 < a.S ? s + 1 : a.S - 1);
+  const long q0 = s < 0 ? 0 : m.q0 + m.nq, q1 = s + 1 < a.S ? n.q0 : a.Tq, k0 = s < 0 ? 0 : m.k0 + m.nk, k1 = s + 1 < a.S ? n.k0 : a.Tk;
+  const long step = (long)gridDim.y * 32, lane8 = (threadIdx.x & 7) * 8;
+  const bf16x8 zero = {};
+  for (long r = q0 + blockIdx.y * 32 + (threadIdx.x >> 3); r < q1; r += step)
+    for (int h = 0; h < a.Hq; ++h) {
+      if (fill & APLA_FILL_O) *(bf16x8*)(a.o + r * a.ldo + h * 64 + lane8) = zero;
+      if (fill & APLA_FILL_DQ) *(bf16x8*)(a.dq + r * a.lddq + h * 64 + lane8) = zero;
+      if ((fill & APLA_FILL_LSE) && lane8 == 0) a.lse[(long)h * a.Tq + r] = -INFINITY;
+    }
+  if (fill & (APLA_FILL_DK | APLA_FILL_DV))
+    for (long r = k0 + blockIdx.y * 32 + (threadIdx.x >> 3); r < k1; r += step)
+      for (int h = 0; h < Hkv; ++h) {
+        if (fill & APLA_FILL_DK) *(bf16x8*)(a.dk + r * a.lddk + h * 64 + lane8) = zero;
+        if (fill & APLA_FILL_DV) *(bf16x8*)(a.dv + r * a.lddv + h * 64 + lane8) = zero;
+      }
+}
+
 // smallest and largest document id of every 64-row tile of every sequence: one wave per tile
 __global__ __launch_bounds__(256) void attn_mod_ranges_kernel(ModArgs a, int queries, int2* out, int nt) {
   const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -1275,6 +1297,11 @@ ModArgs mod_args(const apla_attn_mod_t& p, const Plan& pl) {
   return a;
 }
 
+void launch_fill(const ModArgs& a, int fill, hipStream_t stream) {
+  const long rows = (long)a.Tq + a.Tk, each = rows / (a.S * 256L) + 1;
+  hipLaunchKernelGGL(attn_mod_fill_kernel, dim3((unsigned)a.S + 1, (unsigned)(each < 64 ? each : 64)), dim3(256), 0, stream, a, fill);
+}
+
 void launch_ranges(const ModArgs& a, bool queries, hipStream_t stream) {
   const int nt = queries ? a.nt_q : a.nt_k;
   hipLaunchKernelGGL(attn_mod_ranges_kernel, dim3((unsigned)(((long)a.S * nt + 3) / 4)), dim3(256), 0, stream, a, queries ? 1 : 0, (int2*)(queries ? a.rng_q : a.rng_k), nt);
@@ -1308,6 +1335,7 @@ extern "C" int apla_attn_mod_fwd(const apla_attn_mod_t* p, hipStream_t stream) {
   const Plan pl = plan_of(*p, false);
   ModArgs a = mod_args(*p, pl);
   const long units = (long)p->S * p->Hkv;
+  if ((p->fill & (APLA_FILL_O | APLA_FILL_LSE)) && a.cu_q) launch_fill(a, p->fill & (APLA_FILL_O | APLA_FILL_LSE), stream);
   if (a.doc_k) launch_ranges(a, false, stream);
   if (pl.rows) {
     const dim3 grid((unsigned)(units * pl.nrt * pl.nsplit));
@@ -1328,7 +1356,13 @@ extern "C" int apla_attn_mod_bwd(const apla_attn_mod_t* p, hipStream_t stream) {
   const Plan pl = plan_of(*p, true);
   ModArgs a = mod_args(*p, pl);
   const long units = (long)p->S * p->Hkv;
-  if (a.doc_k) { launch_ranges(a, false, stream); launch_ranges(a, true, stream); }
+  const int fill = p->fill & ((a.cu_q ? APLA_FILL_DQ : 0) | (a.cu_k || a.len_k ? APLA_FILL_DK | APLA_FILL_DV : 0));
+  if (fill) launch_fill(a, fill, stream);
+  if (a.doc_k) {
+    launch_ranges(a, false, stream);
+    if (p->doc_q == p->doc_k && p->cu_q == p->cu_k && p->max_q == p->max_k && !p->len_k) a.rng_q = a.rng_k;      // self-attention: the same tiles
+    else launch_ranges(a, true, stream);
+  }
   a.nblk = (p->max_q + 127) / 128;
   {
     const dim3 grid((unsigned)unit_grid(units, a.np, (long)a.G * a.nblk * a.sq));

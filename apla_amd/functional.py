@@ -635,8 +635,8 @@ class _AttnModQkvFn(torch.autograd.Function):
         x, qk, o, lse = ctx.saved_tensors
         H, scale, rot, mod, seq = ctx.args
         n = H * 64
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if "cu_q" not in seq else torch.zeros(x.shape, device=x.device, dtype=x.dtype)
-        ops.attn_mod_bwd(qk[:, :n], qk[:, n:], x[:, 2 * n:], o, _as2d_bf16(do), lse, H, H, scale, mod, dq=dx[:, :n], dk=dx[:, n:2 * n], dv=dx[:, 2 * n:], **seq)
+        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        ops.attn_mod_bwd(qk[:, :n], qk[:, n:], x[:, 2 * n:], o, _as2d_bf16(do), lse, H, H, scale, mod, dq=dx[:, :n], dk=dx[:, n:2 * n], dv=dx[:, 2 * n:], zero_rest=True, **seq)
         g = [None] * 4
         if ctx.norm is not None:        # in place: every lane reads its row's gradient before it writes it
             want = any(ctx.needs_input_grad[1:5])

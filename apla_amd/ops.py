@@ -957,31 +957,31 @@ def attn_mod_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, Hq: int, Hkv
     with guard:
         Tq = a.Tq
         if o is None:
-            o = q.new_empty(Tq, Hq * 64) if cu_q is None else q.new_zeros(Tq, Hq * 64)
-            a.ldo = Hq * 64
+            o = q.new_empty(Tq, Hq * 64)
+            a.ldo, a.fill = Hq * 64, 1
         else:
             a.ldo = _strided_rows(o, "o", Hq * 64, Tq)
             if o.device != q.device or any(_overlap(t, o) for t in (q, k, v)):
                 raise ValueError("attn_mod_fwd: o must lie on q's device and apart from q, k, v")
         if lse is None:
-            lse = torch.empty((Hq, Tq), device=q.device, dtype=torch.float32) if cu_q is None else torch.full((Hq, Tq), float("-inf"), device=q.device, dtype=torch.float32)
+            lse = torch.empty((Hq, Tq), device=q.device, dtype=torch.float32)
+            a.fill |= 2
         else:
             _aux(lse, torch.float32, "lse", (Hq, Tq))
             if lse.device != q.device:
                 raise ValueError("attn_mod_fwd: lse must lie on q's device")
         a.o, a.lse = o.data_ptr(), lse.data_ptr()
-        if a.max_q == 0:
-            return o, lse
-        if a.max_k == 0:       # no keys at all: every computed row sees nothing
-            _zero_rows(o, cu_q, 0.0), _zero_rows(lse.t(), cu_q, float("-inf"))
+        if a.max_q == 0 or a.max_k == 0:       # no rows, or no keys at all: every row sees nothing
+            _zero_rows(o, cu_q, 0.0, a.fill & 1), _zero_rows(lse.t(), cu_q, float("-inf"), a.fill & 2)
             return o, lse
         ws = _mod_workspace(a, False, q.device)     # noqa: F841  (alive until the launch)
         check(lib().apla_attn_mod_fwd(a, _raw_stream(q.device)), "apla_attn_mod_fwd")
     return o, lse
 
 
-def _zero_rows(t, cu, value):
-    if cu is None:
+def _zero_rows(t, cu, value, whole):
+    """The rows of the sequences (all rows where the buffer is ours) set to one value."""
+    if cu is None or whole:
         t.fill_(value)
     else:
         rows = torch.arange(t.shape[0], device=t.device)
@@ -991,9 +991,10 @@ def _zero_rows(t, cu, value):
 def attn_mod_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, do: torch.Tensor, lse: torch.Tensor, Hq: int, Hkv: int,
                  scale: float, mod: Optional[ScoreMod] = None, *, batch: Optional[int] = None, cu_q: Optional[torch.Tensor] = None,
                  cu_k: Optional[torch.Tensor] = None, max_q: Optional[int] = None, max_k: Optional[int] = None, len_k: Optional[torch.Tensor] = None,
-                 dq: Optional[torch.Tensor] = None, dk: Optional[torch.Tensor] = None, dv: Optional[torch.Tensor] = None):
+                 dq: Optional[torch.Tensor] = None, dk: Optional[torch.Tensor] = None, dv: Optional[torch.Tensor] = None, zero_rest: bool = False):
     """(dq, dk, dv) of attn_mod_fwd for the same arguments, its o and lse, and do [Tq, Hq*64].  Given gradient buffers may be columns of one
-    fused buffer; rows that no sequence holds (behind the last one, keys past ``len_k``) are left as they were there, else 0."""
+    fused buffer; rows that no sequence holds (behind the last one, keys past ``len_k``) are left as they were there (``zero_rest``: set to 0),
+    else 0."""
     a, guard = _attn_mod_args(q, k, v, Hq, Hkv, scale, mod, batch, cu_q, cu_k, max_q, max_k, len_k, "attn_mod_bwd")
     a.ldo, a.lddo = _strided_rows(o, "o", Hq * 64, a.Tq), _strided_rows(do, "do", Hq * 64, a.Tq)
     _aux(lse, torch.float32, "lse", (Hq, a.Tq))
@@ -1005,22 +1006,21 @@ def attn_mod_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Ten
         if any(_overlap(t, g) for g in given for t in (q, k, v, o, do)) or any(_overlap(given[i], given[j]) for i in range(len(given)) for j in range(i)):
             raise ValueError("attn_mod_bwd: the gradients must lie apart from the operands and from each other")
         nq, nk = Hq * 64, Hkv * 64
-        make = q.new_empty if cu_k is None and len_k is None else q.new_zeros
-        a.lddq, a.lddk, a.lddv = nq, nk, nk
+        a.lddq, a.lddk, a.lddv, a.fill = nq, nk, nk, 28 if zero_rest else 0
         if dq is None:
-            dq = q.new_empty(Tq, nq) if cu_q is None else q.new_zeros(Tq, nq)
+            dq, a.fill = q.new_empty(Tq, nq), a.fill | 4
         else:
             a.lddq = _strided_rows(dq, "dq", nq, Tq)
         if dk is None:
-            dk = make(Tk, nk)
+            dk, a.fill = q.new_empty(Tk, nk), a.fill | 8
         else:
             a.lddk = _strided_rows(dk, "dk", nk, Tk)
         if dv is None:
-            dv = make(Tk, nk)
+            dv, a.fill = q.new_empty(Tk, nk), a.fill | 16
         else:
             a.lddv = _strided_rows(dv, "dv", nk, Tk)
         if a.max_q == 0 or a.max_k == 0:
-            _zero_rows(dq, cu_q, 0.0), _zero_rows(dk, cu_k, 0.0), _zero_rows(dv, cu_k, 0.0)
+            _zero_rows(dq, cu_q, 0.0, a.fill & 4), _zero_rows(dk, cu_k, 0.0, a.fill & 8), _zero_rows(dv, cu_k, 0.0, a.fill & 16)
             return dq, dk, dv
         delta = torch.empty_like(lse)
         a.o, a.lse, a.d_o, a.delta = o.data_ptr(), lse.data_ptr(), do.data_ptr(), delta.data_ptr()

@@ -325,9 +325,11 @@ int apla_qk_norm_rotary_bwd(const void* dy, long lddy, const void* x, long ldx, 
  * query i of nq stands at key position i + nk - nq.  max_q / max_k: the longest sequences (longer ones are cut there).
  * dist: |i + nk - nq - j|, or the Euclidean distance of pos_q / pos_k [T, pos_dim] (pos_dim 1 or 2).
  * Visible: j < nk; causal: j <= i + nk - nq or j < prefix[s]; documents: doc_q[i] == doc_k[j] >= 0.  A row that sees nothing gives
- * o = 0, lse = -inf and zero gradients; rows behind the last sequence and keys past len_k are not written.
+ * o = 0, lse = -inf and zero gradients; rows that no sequence holds (behind the last one, keys past len_k) are not written, except in the
+ * outputs named in `fill` (APLA_FILL_*), where they become 0 (lse: -inf).
  * Values in masked places may be anything (infinities and NaN too).  Backward: lse and o from the forward, delta [Hq, Tq] scratch.
  * workspace: apla_attn_mod_workspace_bytes(p, backward) bytes, 16-byte aligned, of this call alone.  Deterministic. */
+enum { APLA_FILL_O = 1, APLA_FILL_LSE = 2, APLA_FILL_DQ = 4, APLA_FILL_DK = 8, APLA_FILL_DV = 16 };
 typedef struct {
   const void *q, *k, *v;
   void* o;
@@ -339,7 +341,7 @@ typedef struct {
   float* delta;
   void* workspace;
   long workspace_bytes, ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
-  int S, Tq, Tk, max_q, max_k, Hq, Hkv, pos_dim, causal;
+  int S, Tq, Tk, max_q, max_k, Hq, Hkv, pos_dim, causal, fill;
   float scale, softcap;
 } apla_attn_mod_t;
 long apla_attn_mod_workspace_bytes(const apla_attn_mod_t* p, int backward);

@@ -220,6 +220,8 @@ def test_strided_operands_and_outputs_and_rows_behind_the_last_sequence():
     ref = ops.attn_mod_bwd(*dense, o1, do[:n].contiguous(), l1, H, H, SCALE, None, **kw)
     assert bool((fused[n:] == 7).all()) and all(torch.equal(p[:n], r) for p, r in zip(parts, ref))
     assert all(bool((g[n:] == 0).all()) for g in ops.attn_mod_bwd(*cut, o0, do, l0, H, H, SCALE, None, **kw))
+    ops.attn_mod_bwd(*cut, o, do, lse, H, H, SCALE, None, dq=parts[0], dk=parts[1], dv=parts[2], zero_rest=True, **kw)
+    assert bool((fused[n:] == 0).all()) and all(torch.equal(p[:n], r) for p, r in zip(parts, ref))
     two = qkv[:80].view(2, 40, -1)
     ocls, _ = ops.attn_mod_fwd(two[:, 0, :H * 64], cut[1][:80], cut[2][:80], H, H, SCALE, None, batch=2)
     full, _ = ops.attn_mod_fwd(cut[0][:80], cut[1][:80], cut[2][:80], H, H, SCALE, None, batch=2)
@@ -299,6 +301,30 @@ def test_offsets_that_do_not_fit_are_cut_to_the_tensors():
     full, _ = ops.attn_mod_fwd(q, k, v, 1, 1, SCALE, batch=2, len_k=torch.tensor([99, -3], dtype=torch.int32, device="cuda"))
     part, _ = ops.attn_mod_fwd(q[:32], k[:32], v[:32], 1, 1, SCALE, batch=1)
     assert torch.equal(full[:32], part) and bool((full[32:] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("lens,Hq,Hkv,kw", [([900], 2, 1, dict(causal=True, bias=1)), ([700, 30, 520], 4, 1, dict(docs="sorted", cap=9.0)), ([1500], 1, 1, dict(docs="mixed", poison=True))], ids=str)
+def test_few_blocks_are_split_over_their_tiles(lens, Hq, Hkv, kw, dtype):
+    """Long sequences of few heads: the backward shares a block's tiles among workgroups and adds their partial sums, the forward runs in 16-row tiles."""
+    run_case(DT[dtype], lens, lens, Hq, Hkv, **kw)
+
+
+def test_many_blocks_of_long_sequences():
+    """Enough blocks that nothing is split: the 128-row forward and single-pass backward on lengths around tile and block borders."""
+    lens = [257, 256, 255, 193, 192, 129, 128, 127, 65, 64, 63, 1] * 3
+    q, k, v, do = (rnd((sum(lens), 6 * 64), torch.bfloat16, s, 1.0 + (s == 0)).cuda() for s in range(4))
+    cu = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device="cuda")
+    mod = ops.ScoreMod(softcap=20.0, causal=True)
+    kw = dict(cu_q=cu, cu_k=cu, max_q=257, max_k=257)
+    o, lse = ops.attn_mod_fwd(q, k, v, 6, 6, SCALE, mod, **kw)
+    g = ops.attn_mod_bwd(q, k, v, o, do, lse, 6, 6, SCALE, mod, **kw)
+    for s in (0, 1, 4, 11, 13, 29):        # the same sequences alone (other kernels run them): equal up to the rounding of weights and results
+        a, b = int(cu[s]), int(cu[s + 1])
+        one, l1 = ops.attn_mod_fwd(q[a:b], k[a:b], v[a:b], 6, 6, SCALE, mod, batch=1)
+        assert bool(((o[a:b] - one).abs().float() <= 2.0 ** -7 * (one.abs().float() + 3)).all()) and bool(((lse[:, a:b] - l1).abs() <= 1e-4).all())
+        for x, y in zip(g, ops.attn_mod_bwd(q[a:b], k[a:b], v[a:b], one, do[a:b], l1, 6, 6, SCALE, mod, batch=1)):
+            assert float((x[a:b].float() - y.float()).norm()) <= 4 * 2.0 ** -8 * float(y.float().norm()) + 1e-6
 
 
 def test_side_stream_and_two_captured_graphs():
