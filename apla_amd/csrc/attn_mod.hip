@@ -389,13 +389,13 @@ __device__ __forceinline__ void fwd_tile(f32x16 (&acc)[2], RowState& st, unsigne
 
 // ---- the list of key tiles that rows with (lim_max, documents dmin..dmax) can see, one pass of up to LIST tiles from t0
 struct TileRef { int t, lo, hi, whole; };      // whole: all of it is visible to all rows of the workgroup
-// n entries in list[] and three more that repeat the last; all threads call it, ends with a barrier.  Tiles w0 .. w1 - 1 lie
+// n entries in list[]; all threads call it, ends with a barrier.  Tiles w0 .. w1 - 1 lie
 // within the limits of all rows.
 __device__ __forceinline__ int build_list(TileRef* list, int* cnt, int t0, int ntiles, int w0, int w1, const int2* rng, int dmin, int dmax, int tid) {
   const int t = t0 + tid;
   bool vis = t < ntiles;
   int2 r = {0, 0};
-  if (vis && rng) {
+  if (vis) {
     r = rng[t];
     vis = r.y >= max(dmin, 0) && r.x <= dmax;
   }
@@ -407,9 +407,7 @@ __device__ __forceinline__ int build_list(TileRef* list, int* cnt, int t0, int n
   for (int w = 0; w < 4; ++w) { const int c = cnt[w]; base += w < (tid >> 6) ? c : 0; n += c; }
   if (vis) {
     const int at = base + __popcll(b & ((1ull << (tid & 63)) - 1));
-    const TileRef e = {t, r.x, r.y, t >= w0 && t < w1 && (!rng || (r.x >= 0 && r.x == r.y && dmin == r.x && dmax == r.x))};
-    list[at] = e;
-    if (at == n - 1) list[n] = list[n + 1] = list[n + 2] = e;
+    list[at] = {t, r.x, r.y, t >= w0 && t < w1 && r.x >= 0 && r.x == r.y && dmin == r.x && dmax == r.x};
   }
   __syncthreads();
   return n;
@@ -492,10 +490,10 @@ __device__ __forceinline__ RowCtx row_ctx(const ModArgs& a, const MSeq& m, int i
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-template <bool CAP, int BIAS>
+template <bool CAP, int BIAS, bool DOCS>
 __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
   __shared__ __attribute__((aligned(128))) char smem[2 * KT_BYTES], clean[8192];
-  __shared__ TileRef list[LIST + 3];
+  __shared__ TileRef list[DOCS ? LIST : 1];
   __shared__ int buf[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
   const Frag fr = frag_consts(lane);
@@ -511,10 +509,18 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
   bf16x8 qf[4];
   load_row_frags(qf, a.q + (m.q0 + qi) * a.ldq + h * 64, lane);
   const RowCtx r = row_ctx<BIAS>(a, m, qi, h);
-  const bool docs = a.doc_k != nullptr;
-  const int wlo = wave_min_i(r.doc), whi = wave_max_i(r.doc), wlim0 = wave_min_i(r.lim), wlim1 = wave_max_i(r.lim);
-  int dlo = wlo, dhi = whi, lim0 = wlim0, lim = wlim1;
-  group_range(dlo, dhi, lim0, lim, buf, wave, lane);
+  constexpr bool docs = DOCS;
+  // limits (smallest, largest) and documents of the wave's and of the workgroup's rows; without documents the limits grow with the row
+  int wlo = 0, whi = 0, dlo = 0, dhi = 0, wlim0, wlim1, lim0, lim;
+  if constexpr (DOCS) {
+    wlo = wave_min_i(r.doc); whi = wave_max_i(r.doc); wlim0 = wave_min_i(r.lim); wlim1 = wave_max_i(r.lim);
+    dlo = wlo; dhi = whi; lim0 = wlim0; lim = wlim1;
+    group_range(dlo, dhi, lim0, lim, buf, wave, lane);
+  } else {
+    const int wq = min(q0 + wave * 32, m.nq - 1);
+    wlim0 = row_lim(a, m, wq); wlim1 = row_lim(a, m, min(wq + 31, m.nq - 1));
+    lim0 = row_lim(a, m, q0); lim = row_lim(a, m, min(q0 + 127, m.nq - 1));
+  }
 
   f32x16 acc[2];
 #pragma unroll
@@ -524,8 +530,16 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
   const bf16 *kb = a.k + m.k0 * a.ldk + (hk) * 64, *vb = a.v + m.k0 * a.ldv + (hk) * 64;
   const unsigned offk = stage_off(a.ldk, tid), offv = stage_off(a.ldv, tid);
   const int ntiles = (lim + 63) / 64;
-  for (int t0 = 0; t0 < ntiles; t0 += LIST) {
-    const int n = build_list(list, buf, t0, ntiles, 0, lim0 / 64, docs ? a.rng_k + (long)(w.unit / Hkv) * a.nt_k : nullptr, dlo, dhi, tid);
+  for (int t0 = 0; t0 < ntiles; t0 = DOCS ? t0 + LIST : ntiles) {
+    int n = ntiles;
+    if constexpr (DOCS) n = build_list(list, buf, t0, ntiles, 0, lim0 / 64, a.rng_k + (long)(w.unit / Hkv) * a.nt_k, dlo, dhi, tid);
+    // entry e of the tiles to visit (past the last: the last): from the list, or simply tile e
+    auto entry = [&](int e) -> TileRef {
+      e = min(e, n - 1);
+      if constexpr (DOCS) return list[e];
+      else return TileRef{e, 0, 0, e < lim0 / 64};
+    };
+    auto known = [&](const TileRef& x) -> TileRef { return DOCS ? scalar_ref(x) : x; };
     Stage ks, vs;
     KeySide sd;
     auto fetch = [&](int t) {
@@ -545,8 +559,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
     TileRef cur, next;
     int t2 = 0;
     if (n > 0) {
-      cur = scalar_ref(list[0]); next = scalar_ref(list[1]);
-      t2 = __builtin_amdgcn_readfirstlane(list[2].t);
+      cur = known(entry(0)); next = known(entry(1));
+      t2 = known(entry(2)).t;
       fetch(cur.t);
       put(smem, cur.whole);
       fetch(next.t);
@@ -554,8 +568,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
     __syncthreads();
     for (int e = 0; e < n; ++e) {      // tile e is in LDS, e + 1 in registers; e + 2 is requested when those are free
       char* tile = smem + (e & 1) * KT_BYTES;
-      const TileRef ahead = list[e + 2 < n ? e + 2 : n - 1];
-      const int t3 = list[e + 3 < n ? e + 3 : n - 1].t;
+      const TileRef ahead = entry(e + 2);
+      const int t3 = entry(e + 3).t;
       const int j0 = cur.t * 64;
       const bool odd = !cur.whole && any_odd(tile + KT_ODD);
       if (__builtin_expect(odd, 0)) {
@@ -569,8 +583,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
       if (e + 1 < n) put(smem + ((e + 1) & 1) * KT_BYTES, next.whole);
       if (e + 2 < n) fetch(t2);
       cur = next;
-      next = scalar_ref(ahead);
-      t2 = __builtin_amdgcn_readfirstlane(t3);
+      next = known(ahead);
+      t2 = DOCS ? __builtin_amdgcn_readfirstlane(t3) : t3;
       __syncthreads();
     }
   }
@@ -856,10 +870,10 @@ __device__ __forceinline__ void dq_tile(f32x16 (&acc)[2], unsigned& poison, cons
   }
 }
 
-template <bool CAP, int BIAS>
+template <bool CAP, int BIAS, bool DOCS>
 __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
   __shared__ __attribute__((aligned(128))) char smem[2 * KT_BYTES], clean[8192];
-  __shared__ TileRef list[LIST + 3];
+  __shared__ TileRef list[DOCS ? LIST : 1];
   __shared__ int buf[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
   const Frag fr = frag_consts(lane);
@@ -890,10 +904,18 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
   const float L2 = ls == -INFINITY ? -NEG_BIG : ls * LOG2E;
   if (sp == 0 && qr < m.nq && h2 == 0) a.delta[stat] = delta;
   const RowCtx r = row_ctx<BIAS>(a, m, qi, h);
-  const bool docs = a.doc_k != nullptr;
-  const int wlo = wave_min_i(r.doc), whi = wave_max_i(r.doc), wlim0 = wave_min_i(r.lim), wlim1 = wave_max_i(r.lim);
-  int dlo = wlo, dhi = whi, lim0 = wlim0, lim = wlim1;
-  group_range(dlo, dhi, lim0, lim, buf, wave, lane);
+  constexpr bool docs = DOCS;
+  // limits (smallest, largest) and documents of the wave's and of the workgroup's rows; without documents the limits grow with the row
+  int wlo = 0, whi = 0, dlo = 0, dhi = 0, wlim0, wlim1, lim0, lim;
+  if constexpr (DOCS) {
+    wlo = wave_min_i(r.doc); whi = wave_max_i(r.doc); wlim0 = wave_min_i(r.lim); wlim1 = wave_max_i(r.lim);
+    dlo = wlo; dhi = whi; lim0 = wlim0; lim = wlim1;
+    group_range(dlo, dhi, lim0, lim, buf, wave, lane);
+  } else {
+    const int wq = min(q0 + wave * 32, m.nq - 1);
+    wlim0 = row_lim(a, m, wq); wlim1 = row_lim(a, m, min(wq + 31, m.nq - 1));
+    lim0 = row_lim(a, m, q0); lim = row_lim(a, m, min(q0 + 127, m.nq - 1));
+  }
   f32x16 acc[2];
 #pragma unroll
   for (int i = 0; i < 16; ++i) { acc[0][i] = 0.f; acc[1][i] = 0.f; }
@@ -901,8 +923,16 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
   const bf16 *kb = a.k + m.k0 * a.ldk + (hk) * 64, *vb = a.v + m.k0 * a.ldv + (hk) * 64;
   const unsigned offk = stage_off(a.ldk, tid), offv = stage_off(a.ldv, tid);
   const int ntiles = (lim + 63) / 64;
-  for (int t0 = 0; t0 < ntiles; t0 += LIST) {
-    const int n = build_list(list, buf, t0, ntiles, 0, lim0 / 64, docs ? a.rng_k + (long)(w.unit / Hkv) * a.nt_k : nullptr, dlo, dhi, tid);
+  for (int t0 = 0; t0 < ntiles; t0 = DOCS ? t0 + LIST : ntiles) {
+    int n = ntiles;
+    if constexpr (DOCS) n = build_list(list, buf, t0, ntiles, 0, lim0 / 64, a.rng_k + (long)(w.unit / Hkv) * a.nt_k, dlo, dhi, tid);
+    // entry e of the tiles to visit (past the last: the last): from the list, or simply tile e
+    auto entry = [&](int e) -> TileRef {
+      e = min(e, n - 1);
+      if constexpr (DOCS) return list[e];
+      else return TileRef{e, 0, 0, e < lim0 / 64};
+    };
+    auto known = [&](const TileRef& x) -> TileRef { return DOCS ? scalar_ref(x) : x; };
     Stage ks, vs;
     KeySide sd;
     auto fetch = [&](int t) {
@@ -923,8 +953,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
     TileRef cur, next;
     int t2 = 0;
     if (e0 < e1) {
-      cur = scalar_ref(list[e0]); next = scalar_ref(list[e0 + 1]);
-      t2 = __builtin_amdgcn_readfirstlane(list[e0 + 2].t);
+      cur = known(entry(e0)); next = known(entry(e0 + 1));
+      t2 = known(entry(e0 + 2)).t;
       fetch(cur.t);
       put(smem, cur.whole);
       fetch(next.t);
@@ -932,8 +962,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
     __syncthreads();
     for (int e = e0; e < e1; ++e) {      // tile e is in LDS, e + 1 in registers; e + 2 is requested when those are free
       char* tile = smem + ((e - e0) & 1) * KT_BYTES;
-      const TileRef ahead = list[e + 2 < n ? e + 2 : n - 1];
-      const int t3 = list[e + 3 < n ? e + 3 : n - 1].t;
+      const TileRef ahead = entry(e + 2);
+      const int t3 = entry(e + 3).t;
       const int j0 = cur.t * 64;
       const bool odd = !cur.whole && any_odd(tile + KT_ODD);
       if (__builtin_expect(odd, 0)) {
@@ -947,8 +977,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
       if (e + 1 < e1) put(smem + ((e + 1 - e0) & 1) * KT_BYTES, next.whole);
       if (e + 2 < e1) fetch(t2);
       cur = next;
-      next = scalar_ref(ahead);
-      t2 = __builtin_amdgcn_readfirstlane(t3);
+      next = known(ahead);
+      t2 = DOCS ? __builtin_amdgcn_readfirstlane(t3) : t3;
       __syncthreads();
     }
   }
@@ -1013,10 +1043,10 @@ __device__ __forceinline__ void dkdv_tile(f32x16 (&dk)[2], f32x16 (&dv)[2], unsi
   }
 }
 
-template <bool CAP, int BIAS>
+template <bool CAP, int BIAS, bool DOCS>
 __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
   __shared__ __attribute__((aligned(128))) char smem[2 * QT_BYTES], clean[16384];
-  __shared__ TileRef list[LIST + 3];
+  __shared__ TileRef list[DOCS ? LIST : 1];
   __shared__ int buf[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
   const Frag fr = frag_consts(lane);
@@ -1031,13 +1061,17 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
   bf16x8 kf[4], vf[4];
   load_row_frags(kf, a.k + (m.k0 + j) * a.ldk + hk * 64, lane);
   load_row_frags(vf, a.v + (m.k0 + j) * a.ldv + hk * 64, lane);
-  const bool docs = a.doc_k != nullptr;
+  constexpr bool docs = DOCS;
   const int docj = docs ? a.doc_k[m.k0 + j] : 0;
   float pj[2] = {0.f, 0.f};
   row_pos<BIAS>(pj, a.pos_k, m.k0 + j, j);
-  const int wlo = wave_min_i(docj), whi = wave_max_i(docj);
-  int dlo = wlo, dhi = whi, none0 = 0, none1 = 0;
-  group_range(dlo, dhi, none0, none1, buf, wave, lane);
+  int wlo = 0, whi = 0, dlo = 0, dhi = 0;
+  if constexpr (DOCS) {
+    int none0 = 0, none1 = 0;
+    wlo = wave_min_i(docj); whi = wave_max_i(docj);
+    dlo = wlo; dhi = whi;
+    group_range(dlo, dhi, none0, none1, buf, wave, lane);
+  }
   unsigned pk = 0, pv = 0;
   const unsigned offq = stage_off(a.ldq, tid), offd = stage_off(a.lddo, tid);
   f32x16 dk[2], dv[2];
@@ -1049,8 +1083,14 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
   // whole tiles: every row of theirs sees all 128 keys, all of them rows and keys of the sequence
   const int jlast = jb + 127;
   const int w0 = jlast >= m.nk ? ntiles : (!a.causal || m.pre > jlast) ? 0 : (max(0, jlast - m.off) + 63) / 64, w1 = m.nq / 64;
-  for (int t0 = first; t0 < ntiles; t0 += LIST) {
-    const int n = build_list(list, buf, t0, ntiles, w0, w1, docs ? a.rng_q + (long)(w.unit / Hkv) * a.nt_q : nullptr, dlo, dhi, tid);
+  for (int t0 = first; t0 < ntiles; t0 = DOCS ? t0 + LIST : ntiles) {
+    int n = ntiles - first;
+    if constexpr (DOCS) n = build_list(list, buf, t0, ntiles, w0, w1, a.rng_q + (long)(w.unit / Hkv) * a.nt_q, dlo, dhi, tid);
+    auto entry = [&](int e) -> TileRef {       // e < n
+      if constexpr (DOCS) return list[e];
+      else return TileRef{first + e, 0, 0, first + e >= w0 && first + e < w1};
+    };
+    auto known = [&](const TileRef& x) -> TileRef { return DOCS ? scalar_ref(x) : x; };
     const int each = (n * a.G + a.sk - 1) / a.sk, x0 = min(n * a.G, sp * each), total = min(n * a.G, x0 + each) - x0;      // this split's part
     Stage qs, os;
     QuerySide sd;
@@ -1092,22 +1132,22 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
     int e = n ? x0 % n : 0, g = n ? x0 / n : 0, e2 = e, g2 = g, t2 = 0;
     auto step = [&](int& e_, int& g_) { if (++e_ == n) { e_ = 0; ++g_; } };
     if (total > 0) {
-      cur = scalar_ref(list[e2]);
+      cur = known(entry(e2));
       step(e2, g2);
-      next = scalar_ref(list[e2]);
+      next = known(entry(e2));
       fetch(cur.t, g);
       put(smem, cur.whole);
       if (total > 1) fetch(next.t, g2);
       step(e2, g2);
-      t2 = __builtin_amdgcn_readfirstlane(list[e2].t);
+      t2 = known(entry(e2)).t;
     }
     __syncthreads();
     for (int x = 0; x < total; ++x) {
       char* tile = smem + (x & 1) * QT_BYTES;
-      const TileRef ahead = list[e2];
+      const TileRef ahead = entry(e2);
       const int gn = g2;
       step(e2, g2);
-      const int t3 = list[e2].t;
+      const int t3 = entry(e2).t;
       const int i0 = cur.t * 64, jw = jb + wave * 32, last = min(i0 + 63, m.nq - 1);
       const bool odd = !cur.whole && any_odd(tile + QT_ODD);
       if (__builtin_expect(odd, 0)) {
@@ -1125,8 +1165,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
       if (x + 2 < total) fetch(t2, gn);
       step(e, g);
       cur = next;
-      next = scalar_ref(ahead);
-      t2 = __builtin_amdgcn_readfirstlane(t3);
+      next = known(ahead);
+      t2 = DOCS ? __builtin_amdgcn_readfirstlane(t3) : t3;
       __syncthreads();
     }
   }
@@ -1307,19 +1347,24 @@ void launch_ranges(const ModArgs& a, bool queries, hipStream_t stream) {
   hipLaunchKernelGGL(attn_mod_ranges_kernel, dim3((unsigned)(((long)a.S * nt + 3) / 4)), dim3(256), 0, stream, a, queries ? 1 : 0, (int2*)(queries ? a.rng_q : a.rng_k), nt);
 }
 
-// KERNEL<cap?, 0 no bias | 1 distance on a line | 2 on a plane>
-#define APLA_MOD_LAUNCH(KERNEL, grid)                                                                             \
+// KERNEL<cap?, 0 no bias | 1 distance on a line | 2 on a plane, more...>
+#define APLA_MOD_LAUNCH(KERNEL, grid, ...)                                                                        \
   do {                                                                                                            \
     const int bias_ = !p->slopes ? 0 : p->pos_dim == 2 ? 2 : 1;                                                   \
     if (p->softcap > 0.f) {                                                                                       \
-      if (bias_ == 0) hipLaunchKernelGGL((KERNEL<true, 0>), grid, dim3(256), 0, stream, a);                       \
-      else if (bias_ == 1) hipLaunchKernelGGL((KERNEL<true, 1>), grid, dim3(256), 0, stream, a);                  \
-      else hipLaunchKernelGGL((KERNEL<true, 2>), grid, dim3(256), 0, stream, a);                                  \
+      if (bias_ == 0) hipLaunchKernelGGL((KERNEL<true, 0 __VA_ARGS__>), grid, dim3(256), 0, stream, a);           \
+      else if (bias_ == 1) hipLaunchKernelGGL((KERNEL<true, 1 __VA_ARGS__>), grid, dim3(256), 0, stream, a);      \
+      else hipLaunchKernelGGL((KERNEL<true, 2 __VA_ARGS__>), grid, dim3(256), 0, stream, a);                      \
     } else {                                                                                                      \
-      if (bias_ == 0) hipLaunchKernelGGL((KERNEL<false, 0>), grid, dim3(256), 0, stream, a);                      \
-      else if (bias_ == 1) hipLaunchKernelGGL((KERNEL<false, 1>), grid, dim3(256), 0, stream, a);                 \
-      else hipLaunchKernelGGL((KERNEL<false, 2>), grid, dim3(256), 0, stream, a);                                 \
+      if (bias_ == 0) hipLaunchKernelGGL((KERNEL<false, 0 __VA_ARGS__>), grid, dim3(256), 0, stream, a);          \
+      else if (bias_ == 1) hipLaunchKernelGGL((KERNEL<false, 1 __VA_ARGS__>), grid, dim3(256), 0, stream, a);     \
+      else hipLaunchKernelGGL((KERNEL<false, 2 __VA_ARGS__>), grid, dim3(256), 0, stream, a);                     \
     }                                                                                                             \
+  } while (0)
+#define APLA_MOD_LAUNCH_DOCS(KERNEL, grid)                                                                        \
+  do {                                                                                                            \
+    if (a.doc_k) APLA_MOD_LAUNCH(KERNEL, grid, , true);                                                           \
+    else APLA_MOD_LAUNCH(KERNEL, grid, , false);                                                                  \
   } while (0)
 
 }  // namespace
@@ -1339,12 +1384,12 @@ extern "C" int apla_attn_mod_fwd(const apla_attn_mod_t* p, hipStream_t stream) {
   if (a.doc_k) launch_ranges(a, false, stream);
   if (pl.rows) {
     const dim3 grid((unsigned)(units * pl.nrt * pl.nsplit));
-    APLA_MOD_LAUNCH(attn_mod_rows_kernel, grid);
+    APLA_MOD_LAUNCH(attn_mod_rows_kernel, grid, );
     if (pl.nsplit > 1) hipLaunchKernelGGL(attn_mod_join_kernel, dim3((unsigned)pl.nrt, (unsigned)p->Hkv, (unsigned)p->S), dim3(256), 0, stream, a);
   } else {
     a.nblk = (p->max_q + 127) / 128;
     const dim3 grid((unsigned)unit_grid(units, a.np, (long)a.G * a.nblk));
-    APLA_MOD_LAUNCH(attn_mod_fwd_kernel, grid);
+    APLA_MOD_LAUNCH_DOCS(attn_mod_fwd_kernel, grid);
   }
   APLA_CHECK_LAUNCH("apla_attn_mod_fwd");
   return APLA_OK;
@@ -1366,14 +1411,14 @@ extern "C" int apla_attn_mod_bwd(const apla_attn_mod_t* p, hipStream_t stream) {
   a.nblk = (p->max_q + 127) / 128;
   {
     const dim3 grid((unsigned)unit_grid(units, a.np, (long)a.G * a.nblk * a.sq));
-    APLA_MOD_LAUNCH(attn_mod_dq_kernel, grid);
+    APLA_MOD_LAUNCH_DOCS(attn_mod_dq_kernel, grid);
     if (a.sq > 1)
       hipLaunchKernelGGL(attn_mod_sum_kernel, dim3((unsigned)((p->max_q + 31) / 32), (unsigned)p->Hq, (unsigned)p->S), dim3(256), 0, stream, a, (const float*)a.part_q, a.sq, 1, a.dq, a.lddq, a.scale);
   }
   a.nblk = (p->max_k + 127) / 128;
   {
     const dim3 grid((unsigned)unit_grid(units, a.np, (long)a.nblk * a.sk));
-    APLA_MOD_LAUNCH(attn_mod_dkdv_kernel, grid);
+    APLA_MOD_LAUNCH_DOCS(attn_mod_dkdv_kernel, grid);
     if (a.sk > 1) {
       const dim3 sum((unsigned)((p->max_k + 31) / 32), (unsigned)p->Hkv, (unsigned)p->S);
       hipLaunchKernelGGL(attn_mod_sum_kernel, sum, dim3(256), 0, stream, a, (const float*)a.part_k, a.sk, 0, a.dk, a.lddk, a.scale);
