@@ -139,8 +139,10 @@ __device__ __forceinline__ bf16x8 finite_part(const bf16x8& f) {
 // (nearly no registers, however slow: the path must not set the kernel's register count.)  w: weights of rows rbase .. rbase + 31 of the tile `raw`.
 __device__ __forceinline__ unsigned poison_bits(const char* raw, int rbase, const f32x16& w, int lane) {
   unsigned own = 0, m = 0;             // bit i: this lane's weight i is not zero; the other 16 rows' weights are in the other half of the wave
+  unsigned one = 1;
+  asm volatile("" : "+s"(one));        // (hipcc would keep the sixteen bits in registers over the whole tile loop)
 #pragma unroll
-  for (int i = 0; i < 16; ++i) own |= w[i] != 0.f ? 1u << i : 0u;
+  for (int i = 0; i < 16; ++i) own |= w[i] != 0.f ? one << i : 0u;
   const auto sw = __builtin_amdgcn_permlane32_swap(own, own, false, false);
   const unsigned nz[2] = {(unsigned)sw[0], (unsigned)sw[1]};
   const int h = lane >> 5;
@@ -185,6 +187,34 @@ __device__ __forceinline__ void stage_store(const Stage& t, char* lds, int tid) 
   const int o = tile_off(tid >> 3, tid & 7);
   *(bf16x8*)(lds + o) = t.v[0];
   *(bf16x8*)(lds + o + 32 * 128) = t.v[1];
+}
+// The same tile straight into LDS (16 bytes a lane, no registers between): LDS takes a wave's lanes side by side, so the tile's swizzle is in the addresses read.
+// Done when the wave's vector loads are (tile_ready).
+__device__ __forceinline__ unsigned dma_off(long ld, int tid) { return (unsigned)((tid >> 3) * (int)ld * 2 + (tile_off(tid >> 3, tid & 7) & 127)); }
+__device__ __forceinline__ void dma16(unsigned lds, const char* base, unsigned off) {      // (the builtin makes hipcc wait for it before any read of LDS)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "m0", "memory");
+}
+__device__ __forceinline__ void dma4(unsigned lds, const void* base, unsigned off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "m0", "memory");
+}
+__device__ __forceinline__ void dma_tile(char* tile, const bf16* base, long ld, unsigned off, int row0, int nrows, int tid, int wave) {
+  const char* p = (const char*)(base + (long)row0 * ld);
+  const unsigned d = lds_of(tile) + wave * 1024;
+  if (row0 + 64 <= nrows) {
+    dma16(d, p, off);
+    dma16(d + 4096, p + ld * 64, off);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) dma16(d + i * 4096, p, (unsigned)min((tid >> 3) + 32 * i, nrows - 1 - row0) * (unsigned)ld * 2 + (tile_off(tid >> 3, tid & 7) & 127));
+  }
+}
+__device__ __forceinline__ void tile_ready() { __builtin_amdgcn_s_waitcnt(0x0f70); __syncthreads(); }      // vmcnt(0)
+// non-finite values in an 8 KB LDS tile (every wave looks at all of it)
+__device__ __forceinline__ bool tile_odd(const char* tile, int lane) {
+  unsigned b = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) b |= nonfinite_bits(*(const bf16x8*)(tile + (i * 64 + lane) * 16));
+  return __ballot(b != 0) != 0;
 }
 // copy of an 8 KB LDS tile without its non-finite values, by the whole workgroup (a barrier before it is used)
 __device__ __forceinline__ void clean_tile(const char* raw, char* clean, int tid) {
@@ -435,7 +465,7 @@ __device__ __forceinline__ bool any_odd(const char* p) {
   return __builtin_amdgcn_readfirstlane(f.x | f.y | f.z | f.w) != 0;
 }
 
-// per-key side data of a tile held in registers until its LDS buffer is free (threads 0..63)
+// per-key side data of a tile: positions and document (threads 0..63)
 struct KeySide { float x, y; int d; };
 template <int BIAS>
 __device__ __forceinline__ void side_load(KeySide& ks, const ModArgs& a, const MSeq& m, int j0, int tid) {
@@ -447,12 +477,21 @@ __device__ __forceinline__ void side_load(KeySide& ks, const ModArgs& a, const M
     ks.d = a.doc_k ? a.doc_k[m.k0 + j] : 0;
   }
 }
-template <int BIAS>
-__device__ __forceinline__ void side_store(const KeySide& ks, char* tile, const ModArgs& a, int tid) {
-  if (tid < 64) {
-    if constexpr (BIAS > 0) *(float*)(tile + KT_POS + tid * 4) = ks.x;
-    if constexpr (BIAS > 1) *(float*)(tile + KT_POS + 256 + tid * 4) = ks.y;
-    if (a.doc_k) *(int*)(tile + KT_DOC + tid * 4) = ks.d;
+// the same into a tile's LDS, one wave each for x, y and the documents
+template <int BIAS, bool DOCS>
+__device__ __forceinline__ void dma_side(char* tile, const ModArgs& a, const MSeq& m, int j0, int lane, int wave) {
+  const unsigned j = min(j0 + lane, m.nk - 1), d = lds_of(tile) + KT_POS;
+  if constexpr (BIAS == 1) {
+    if (wave == 0) {
+      if (a.pos_k) dma4(d, a.pos_k + m.k0, j * 4);
+      else *(float*)(tile + KT_POS + lane * 4) = (float)j;
+    }
+  }
+  if constexpr (BIAS == 2) {
+    if (wave < 2) dma4(d + wave * 256, a.pos_k + 2 * m.k0 + wave, j * 8);
+  }
+  if constexpr (DOCS) {
+    if (wave == 2) dma4(d + KT_DOC - KT_POS, a.doc_k + m.k0, j * 4);
   }
 }
 
@@ -491,7 +530,7 @@ __device__ __forceinline__ RowCtx row_ctx(const ModArgs& a, const MSeq& m, int i
 
 // ------------------------------------------------------------------------------------------------ forward
 template <bool CAP, int BIAS, bool DOCS>
-__global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
+__global__ __launch_bounds__(256, CAP ? 2 : 3) void attn_mod_fwd_kernel(ModArgs a) {
   __shared__ __attribute__((aligned(128))) char smem[2 * KT_BYTES], clean[8192];
   __shared__ TileRef list[DOCS ? LIST : 1];
   __shared__ int buf[16];
@@ -528,10 +567,10 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
   RowState st = {NEG_BIG, 0.f};
   unsigned poison = 0;
   const bf16 *kb = a.k + m.k0 * a.ldk + (hk) * 64, *vb = a.v + m.k0 * a.ldv + (hk) * 64;
-  const unsigned offk = stage_off(a.ldk, tid), offv = stage_off(a.ldv, tid);
+  const unsigned offk = dma_off(a.ldk, tid), offv = dma_off(a.ldv, tid);
   const int ntiles = (lim + 63) / 64;
   for (int t0 = 0; t0 < ntiles; t0 = DOCS ? t0 + LIST : ntiles) {
-    int n = ntiles;
+    int n = __builtin_amdgcn_readfirstlane(ntiles);
     if constexpr (DOCS) n = build_list(list, buf, t0, ntiles, 0, lim0 / 64, a.rng_k + (long)(w.unit / Hkv) * a.nt_k, dlo, dhi, tid);
     // entry e of the tiles to visit (past the last: the last): from the list, or simply tile e
     auto entry = [&](int e) -> TileRef {
@@ -540,38 +579,23 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
       else return TileRef{e, 0, 0, e < lim0 / 64};
     };
     auto known = [&](const TileRef& x) -> TileRef { return DOCS ? scalar_ref(x) : x; };
-    Stage ks, vs;
-    KeySide sd;
-    auto fetch = [&](int t) {
-      stage_load(ks, kb, a.ldk, offk, t * 64, m.nk, tid);
-      stage_load(vs, vb, a.ldv, offv, t * 64, m.nk, tid);
-      if (BIAS || docs) side_load<BIAS>(sd, a, m, t * 64, tid);
-    };
-    auto put = [&](char* tile, bool whole) {
-      stage_store(ks, tile, tid);
-      stage_store(vs, tile + 8192, tid);
-      if (BIAS || docs) side_store<BIAS>(sd, tile, a, tid);
-      if (!whole) {
-        const bool odd = stage_odd(vs);
-        if (lane == 0) *(int*)(tile + KT_ODD + wave * 4) = odd;
-      }
+    auto fetch = [&](char* tile, int t) {
+      dma_tile(tile, kb, a.ldk, offk, t * 64, m.nk, tid, wave);
+      dma_tile(tile + 8192, vb, a.ldv, offv, t * 64, m.nk, tid, wave);
+      dma_side<BIAS, DOCS>(tile, a, m, t * 64, lane, wave);
     };
     TileRef cur, next;
-    int t2 = 0;
     if (n > 0) {
-      cur = known(entry(0)); next = known(entry(1));
-      t2 = known(entry(2)).t;
-      fetch(cur.t);
-      put(smem, cur.whole);
-      fetch(next.t);
+      cur = known(entry(0)); next = known(entry(0 + 1));
+      fetch(smem, cur.t);
     }
-    __syncthreads();
-    for (int e = 0; e < n; ++e) {      // tile e is in LDS, e + 1 in registers; e + 2 is requested when those are free
-      char* tile = smem + (e & 1) * KT_BYTES;
+    tile_ready();
+    for (int e = 0; e < n; ++e) {      // tile e is in LDS, e + 1 on its way to the other half
+      char *tile = smem + (e & 1) * KT_BYTES, *other = smem + ((e + 1) & 1) * KT_BYTES;
       const TileRef ahead = entry(e + 2);
-      const int t3 = entry(e + 3).t;
+      if (e + 1 < n) fetch(other, next.t);
       const int j0 = cur.t * 64;
-      const bool odd = !cur.whole && any_odd(tile + KT_ODD);
+      const bool odd = !cur.whole && tile_odd(tile + 8192, lane);
       if (__builtin_expect(odd, 0)) {
         clean_tile(tile + 8192, clean, tid);
         __syncthreads();
@@ -580,12 +604,9 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(ModArgs a) {
         const bool masked = !cur.whole && !(j0 + 64 <= wlim0 && (!docs || (cur.lo == cur.hi && wlo == cur.lo && whi == cur.lo)));
         fwd_tile<CAP, BIAS>(acc, st, poison, qf, a, r, tile, clean, j0, lane, fr, masked, docs, masked && odd);
       }
-      if (e + 1 < n) put(smem + ((e + 1) & 1) * KT_BYTES, next.whole);
-      if (e + 2 < n) fetch(t2);
       cur = next;
       next = known(ahead);
-      t2 = DOCS ? __builtin_amdgcn_readfirstlane(t3) : t3;
-      __syncthreads();
+      tile_ready();
     }
   }
   apply_poison(acc, poison);
@@ -871,7 +892,7 @@ __device__ __forceinline__ void dq_tile(f32x16 (&acc)[2], unsigned& poison, cons
 }
 
 template <bool CAP, int BIAS, bool DOCS>
-__global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
+__global__ __launch_bounds__(256, CAP ? 2 : 3) void attn_mod_dq_kernel(ModArgs a) {
   __shared__ __attribute__((aligned(128))) char smem[2 * KT_BYTES], clean[8192];
   __shared__ TileRef list[DOCS ? LIST : 1];
   __shared__ int buf[16];
@@ -921,10 +942,10 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
   for (int i = 0; i < 16; ++i) { acc[0][i] = 0.f; acc[1][i] = 0.f; }
   unsigned poison = 0;
   const bf16 *kb = a.k + m.k0 * a.ldk + (hk) * 64, *vb = a.v + m.k0 * a.ldv + (hk) * 64;
-  const unsigned offk = stage_off(a.ldk, tid), offv = stage_off(a.ldv, tid);
+  const unsigned offk = dma_off(a.ldk, tid), offv = dma_off(a.ldv, tid);
   const int ntiles = (lim + 63) / 64;
   for (int t0 = 0; t0 < ntiles; t0 = DOCS ? t0 + LIST : ntiles) {
-    int n = ntiles;
+    int n = __builtin_amdgcn_readfirstlane(ntiles);
     if constexpr (DOCS) n = build_list(list, buf, t0, ntiles, 0, lim0 / 64, a.rng_k + (long)(w.unit / Hkv) * a.nt_k, dlo, dhi, tid);
     // entry e of the tiles to visit (past the last: the last): from the list, or simply tile e
     auto entry = [&](int e) -> TileRef {
@@ -933,39 +954,24 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
       else return TileRef{e, 0, 0, e < lim0 / 64};
     };
     auto known = [&](const TileRef& x) -> TileRef { return DOCS ? scalar_ref(x) : x; };
-    Stage ks, vs;
-    KeySide sd;
-    auto fetch = [&](int t) {
-      stage_load(ks, kb, a.ldk, offk, t * 64, m.nk, tid);
-      stage_load(vs, vb, a.ldv, offv, t * 64, m.nk, tid);
-      if (BIAS || docs) side_load<BIAS>(sd, a, m, t * 64, tid);
-    };
-    auto put = [&](char* tile, bool whole) {
-      stage_store(ks, tile, tid);
-      stage_store(vs, tile + 8192, tid);
-      if (BIAS || docs) side_store<BIAS>(sd, tile, a, tid);
-      if (!whole) {
-        const bool odd = stage_odd(ks);
-        if (lane == 0) *(int*)(tile + KT_ODD + wave * 4) = odd;
-      }
+    auto fetch = [&](char* tile, int t) {
+      dma_tile(tile, kb, a.ldk, offk, t * 64, m.nk, tid, wave);
+      dma_tile(tile + 8192, vb, a.ldv, offv, t * 64, m.nk, tid, wave);
+      dma_side<BIAS, DOCS>(tile, a, m, t * 64, lane, wave);
     };
     const int each = (n + a.sq - 1) / a.sq, e0 = min(n, sp * each), e1 = min(n, e0 + each);      // this split's part of the list
     TileRef cur, next;
-    int t2 = 0;
     if (e0 < e1) {
       cur = known(entry(e0)); next = known(entry(e0 + 1));
-      t2 = known(entry(e0 + 2)).t;
-      fetch(cur.t);
-      put(smem, cur.whole);
-      fetch(next.t);
+      fetch(smem, cur.t);
     }
-    __syncthreads();
-    for (int e = e0; e < e1; ++e) {      // tile e is in LDS, e + 1 in registers; e + 2 is requested when those are free
-      char* tile = smem + ((e - e0) & 1) * KT_BYTES;
+    tile_ready();
+    for (int e = e0; e < e1; ++e) {      // tile e is in LDS, e + 1 on its way to the other half
+      char *tile = smem + ((e - e0) & 1) * KT_BYTES, *other = smem + ((e + 1 - e0) & 1) * KT_BYTES;
       const TileRef ahead = entry(e + 2);
-      const int t3 = entry(e + 3).t;
+      if (e + 1 < e1) fetch(other, next.t);
       const int j0 = cur.t * 64;
-      const bool odd = !cur.whole && any_odd(tile + KT_ODD);
+      const bool odd = !cur.whole && tile_odd(tile + 0, lane);
       if (__builtin_expect(odd, 0)) {
         clean_tile(tile + 0, clean, tid);
         __syncthreads();
@@ -974,12 +980,9 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(ModArgs a) {
         const bool masked = !cur.whole && !(j0 + 64 <= wlim0 && (!docs || (cur.lo == cur.hi && wlo == cur.lo && whi == cur.lo)));
         dq_tile<CAP, BIAS>(acc, poison, qf, df, L2, delta, a, r, tile, clean, j0, lane, fr, masked, docs, masked && odd);
       }
-      if (e + 1 < e1) put(smem + ((e + 1 - e0) & 1) * KT_BYTES, next.whole);
-      if (e + 2 < e1) fetch(t2);
       cur = next;
       next = known(ahead);
-      t2 = DOCS ? __builtin_amdgcn_readfirstlane(t3) : t3;
-      __syncthreads();
+      tile_ready();
     }
   }
   apply_poison(acc, poison);
