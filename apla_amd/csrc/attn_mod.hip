@@ -245,9 +245,9 @@ struct RowCtx { int lim, doc; float pos[2], slope; };       // slope in log2 uni
 // cap tanh(s / cap) in log2 units: A (1 - 2 r), r = 1 / (1 + e^(2 s / cap)).  That is exact to 2^-23 A, which small scores feel relatively; cap_fine
 // takes the odd series below |s / cap| = 1/4 (its next term is 2^-27 there).  Masked tiles do so — every key of a short sequence is in one —,
 // full tiles hold 64 keys or more of a row, over which the difference averages out.
-__device__ __forceinline__ float cap_score(float s, const ModArgs& a, float& r) {
+__device__ __forceinline__ float cap_score(float s, const ModArgs& a, float& r, float sub = 0.f) {      // less `sub`
   r = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * a.k1));
-  return fmaf(-2.f * a.A, r, a.A);
+  return fmaf(-2.f * a.A, r, a.A - sub);
 }
 __device__ __forceinline__ float cap_fine(float s, const ModArgs& a, float& r) {
   const float z = cap_score(s, a, r), x = s * a.kx, y = x * x;
@@ -299,18 +299,25 @@ __device__ __forceinline__ void hide_rows(f32x16& x, f32x16& y, int j, int doc, 
   }
 }
 
-// Scores s[16] of one row (on the lane) and 32 keys, or of one key and 32 rows, in log2 units; with neither cap nor bias they stay raw and the
-// caller multiplies by c.  `side`: LDS address of the positions of the other 32 (x, then y 256 bytes behind), r: cap_score's r of every score.
-// masked (the same for the wave) only chooses the finer cap here.
-template <bool CAP, int BIAS>
-__device__ __forceinline__ void modify(f32x16& s, f32x16& r, const ModArgs& a, const float (&pos)[2], float slope, const char* side, int h2, bool masked) {
+// Scores s[16] of one row (on the lane) and 32 keys, or of one key and 32 rows, in log2 units and less sub(i); with neither cap nor bias they stay raw
+// and the caller multiplies by c.  `side`: LDS address of the positions of the other 32 (x, then y 256 bytes behind), r: cap_score's r of every
+// score.  masked (the same for the wave) only chooses the finer cap here.
+struct Nothing { __device__ __forceinline__ float operator()(int) const { return 0.f; } };
+template <bool CAP, int BIAS, class Sub = Nothing>
+__device__ __forceinline__ void modify(f32x16& s, f32x16& r, const ModArgs& a, const float (&pos)[2], float slope, const char* side, int h2, bool masked, Sub sub = {}) {
+  constexpr bool SUB = !__is_same(Sub, Nothing);
   if constexpr (CAP) {
     if (masked) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) { float t; s[i] = cap_fine(s[i], a, t); r[i] = t; }
+      for (int i = 0; i < 16; ++i) {
+        float t;
+        s[i] = cap_fine(s[i], a, t) - sub(i);
+        r[i] = t;
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);      // (this path must not set the kernel's register count)
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) { float t; s[i] = cap_score(s[i], a, t); r[i] = t; }
+      for (int i = 0; i < 16; ++i) { float t; s[i] = cap_score(s[i], a, t, sub(i)); r[i] = t; }
     }
   }
   if constexpr (BIAS > 0) {
@@ -322,7 +329,8 @@ __device__ __forceinline__ void modify(f32x16& s, f32x16& r, const ModArgs& a, c
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float d = dist<BIAS>(pos, px[e], BIAS > 1 ? py[e] : 0.f);
-        s[4 * g + e] = CAP ? s[4 * g + e] - slope * d : fmaf(s[4 * g + e], a.c, -slope * d);
+        const int i = 4 * g + e;
+        s[i] = CAP ? fmaf(-slope, d, s[i]) : fmaf(s[i], a.c, SUB ? fmaf(-slope, d, -sub(i)) : -slope * d);
       }
     }
   }
@@ -530,7 +538,7 @@ __device__ __forceinline__ RowCtx row_ctx(const ModArgs& a, const MSeq& m, int i
 
 // ------------------------------------------------------------------------------------------------ forward
 template <bool CAP, int BIAS, bool DOCS>
-__global__ __launch_bounds__(256, CAP ? 2 : 3) void attn_mod_fwd_kernel(ModArgs a) {
+__global__ __launch_bounds__(256, CAP && DOCS ? 2 : 3) void attn_mod_fwd_kernel(ModArgs a) {
   __shared__ __attribute__((aligned(128))) char smem[2 * KT_BYTES], clean[8192];
   __shared__ TileRef list[DOCS ? LIST : 1];
   __shared__ int buf[16];
@@ -857,7 +865,13 @@ __global__ __launch_bounds__(256) void attn_mod_join_kernel(ModArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward
-// P = exp2(z - L2) from the forward's lse, dS = P (dP - delta), with the cap times 1 - tanh^2 = 4 r (1 - r), r = 1 / (1 + e^(2 s / cap))
+// P = exp2(z - L2) from the forward's lse, dS = P (dP - delta), with the cap times 1 - tanh^2 = 4 (r - r^2), r = 1 / (1 + e^(2 s / cap)).
+// With the cap `delta` is 4 delta, so that the factor 4 costs nothing.
+template <bool CAP>
+__device__ __forceinline__ float dscore(float p, float dp, float delta, float r) {
+  if constexpr (CAP) return p * fmaf(4.f, dp, -delta) * fmaf(-r, r, r);
+  else return p * (dp - delta);
+}
 template <bool CAP, int BIAS>
 __device__ __forceinline__ void dq_tile(f32x16 (&acc)[2], unsigned& poison, const bf16x8 (&qf)[4], const bf16x8 (&df)[4], float L2, float delta, const ModArgs& a,
                                         const RowCtx& r, const char* tile, const char* clean, int j0, int lane, const Frag& fr, bool masked, bool docs, bool odd) {
@@ -877,12 +891,9 @@ __device__ __forceinline__ void dq_tile(f32x16 (&acc)[2], unsigned& poison, cons
     TrFrags tk;
     tr_load(tk, Kt + fr.tr, kt * 32);
     __builtin_amdgcn_sched_barrier(0);
-    modify<CAP, BIAS>(s, rc, a, r.pos, r.slope, tile + KT_POS + kt * 128, h2, masked);
+    modify<CAP, BIAS>(s, rc, a, r.pos, r.slope, tile + KT_POS + kt * 128, h2, masked, [&](int) { return L2; });
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[i] = __builtin_amdgcn_exp2f((CAP || BIAS) ? s[i] - L2 : fmaf(s[i], a.c, -L2)) * (p[i] - delta);
-      if constexpr (CAP) s[i] *= 4.f * rc[i] * (1.f - rc[i]);
-    }
+    for (int i = 0; i < 16; ++i) s[i] = dscore<CAP>(__builtin_amdgcn_exp2f((CAP || BIAS) ? s[i] : fmaf(s[i], a.c, -L2)), p[i], delta, rc[i]);
     if (masked) {
       hide_keys(s, 0.f, r.lim, r.doc, j0 + kt * 32, tile + KT_DOC + kt * 128, h2, docs);
       if (__builtin_expect(odd, 0)) poison |= poison_bits(tile, kt * 32, s, lane);
@@ -923,6 +934,7 @@ __global__ __launch_bounds__(256, CAP ? 2 : 3) void attn_mod_dq_kernel(ModArgs a
   }
   const float ls = a.lse[stat];
   const float L2 = ls == -INFINITY ? -NEG_BIG : ls * LOG2E;
+  if constexpr (CAP) delta *= 4.f;         // (as dscore takes it; the dK/dV kernel reads it so)
   if (sp == 0 && qr < m.nq && h2 == 0) a.delta[stat] = delta;
   const RowCtx r = row_ctx<BIAS>(a, m, qi, h);
   constexpr bool docs = DOCS;
@@ -1027,8 +1039,7 @@ __device__ __forceinline__ void dkdv_tile(f32x16 (&dk)[2], f32x16 (&dv)[2], unsi
       for (int e = 0; e < 4; ++e) {
         const int i = 4 * g + e;
         const float pr = __builtin_amdgcn_exp2f((CAP || BIAS) ? s[i] - L2[e] : fmaf(s[i], a.c, -L2[e]));
-        s[i] = pr * (p[i] - dl[e]);
-        if constexpr (CAP) s[i] *= 4.f * rc[i] * (1.f - rc[i]);
+        s[i] = dscore<CAP>(pr, p[i], dl[e], rc[i]);
         p[i] = pr;
       }
     }
