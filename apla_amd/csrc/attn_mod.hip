@@ -4,14 +4,17 @@
 // heads may share one key / value head.  Query i of a sequence stands at key position i + (nk - nq).
 //
 // Everything positional about the mask is ONE number per query row: lim_i = min(nk, causal ? max(i + nk - nq + 1, prefix) : nk), 0
-// for rows of no document; key j is visible iff j < lim_i and the two document ids are equal.  A workgroup first writes the list of
-// key tiles that any of its rows can see (lim and the [min, max] document ids of every 64-key tile), then runs over that list only;
-// a wave runs a tile without a mask where lim and the ids say that all of it is visible.
+// for rows of no document; key j is visible iff j < lim_i and the two document ids are equal.  So a workgroup visits the key tiles below its
+// largest lim; with documents it first lists those of them whose [min, max] of ids meets its rows'.  A wave runs a tile without a mask
+// where lim and the ids say that all of it is visible.
 //
 // The products are those of attention.hip (S^T = K Q^T with the query row on the lane, P^T from the accumulator as the next operand).
 // In a masked tile a weight of zero times a non-finite value is zero (poison_bits): what stands in masked places never matters.
 // P and dS are rounded to 16 bits as MFMA operands (half a step of values <= 256 resp. of dS, relative); scores, softmax
 // statistics, sums and accumulators are fp32.
+//
+// What bounds the tile kernels is the vector unit: a score costs a multiply-add, an exponential, an addition and half a maximum in the forward (the cap
+// a further exponential and a reciprocal).  Counters of the forward over 16384 causal rows: vector unit 79 % busy, matrix unit 45 %, no LDS conflicts; capped fp16 forward 84 / 23 %, its dQ 71 / 27 %, dK/dV 61 / 26 %.
 #include "attn_tiles.h"
 #include "common.h"
 
@@ -236,8 +239,8 @@ __device__ __forceinline__ float dist(const float (&p)[2], float x, float y) {
 }
 
 // ------------------------------------------------------------------------------------------------ forward, one 64-key tile
-// LDS of a key tile: K, V (8 KB each), positions [2][64], document ids [64], each wave's verdict on the values it staged
-constexpr int KT_POS = 16384, KT_DOC = KT_POS + 512, KT_ODD = KT_DOC + 256, KT_BYTES = KT_ODD + 128;
+// LDS of a key tile: K, V (8 KB each), positions [2][64], document ids [64]
+constexpr int KT_POS = 16384, KT_DOC = KT_POS + 512, KT_BYTES = KT_DOC + 256;
 
 struct RowState { float m, l; };
 struct RowCtx { int lim, doc; float pos[2], slope; };       // slope in log2 units
@@ -342,7 +345,6 @@ __device__ __forceinline__ float half_max(float v) {
   return fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
 }
 
-// masked: some of the 64 keys are hidden from some of the wave's rows.  odd: V holds non-finite values; `clean` is then its copy without them.
 // One wave's 32 rows against 64 keys in two halves: while the matrix unit multiplies Q with the second half's keys the wave exponentiates the first half,
 // and the first half's product with V runs under the second half's exponentials.
 // masked: some of the 64 keys are hidden from some of the wave's rows.  odd: V holds non-finite values; `clean` is then its copy without them.
@@ -427,8 +429,7 @@ __device__ __forceinline__ void fwd_tile(f32x16 (&acc)[2], RowState& st, unsigne
 
 // ---- the list of key tiles that rows with (lim_max, documents dmin..dmax) can see, one pass of up to LIST tiles from t0
 struct TileRef { int t, lo, hi, whole; };      // whole: all of it is visible to all rows of the workgroup
-// n entries in list[]; all threads call it, ends with a barrier.  Tiles w0 .. w1 - 1 lie
-// within the limits of all rows.
+// n entries in list[]; all threads call it, ends with a barrier.  Tiles w0 .. w1 - 1 lie within the limits of all rows.
 __device__ __forceinline__ int build_list(TileRef* list, int* cnt, int t0, int ntiles, int w0, int w1, const int2* rng, int dmin, int dmax, int tid) {
   const int t = t0 + tid;
   bool vis = t < ntiles;
@@ -467,7 +468,7 @@ __device__ __forceinline__ TileRef scalar_ref(const TileRef& r) {
   return {__builtin_amdgcn_readfirstlane(r.t), __builtin_amdgcn_readfirstlane(r.lo), __builtin_amdgcn_readfirstlane(r.hi), __builtin_amdgcn_readfirstlane(r.whole)};
 }
 
-// any of the four waves' verdicts
+// any of the four waves' verdicts (dK/dV)
 __device__ __forceinline__ bool any_odd(const char* p) {
   const int4 f = *(const int4*)p;
   return __builtin_amdgcn_readfirstlane(f.x | f.y | f.z | f.w) != 0;
@@ -537,8 +538,13 @@ __device__ __forceinline__ RowCtx row_ctx(const ModArgs& a, const MSeq& m, int i
 }
 
 // ------------------------------------------------------------------------------------------------ forward
+// 128 rows of a head per workgroup, 32 per wave; key tiles of 64 (K, V, positions, ids) go straight into one half of LDS while the other is worked on.
+// Three workgroups share a CU where 168 registers hold a wave's state; capped scores next to a bias or documents spill there (8 x 12 heads of 1370 rows
+// with both: 148 us with two, 169 with three).  Forward times, without / with that: 64 x 12 heads of 257 rows 41 / 49 us, 12 heads of 16384
+// causal rows 547 / 626 us (754 TFLOP/s of the visible half), 48 ragged sequences with a 2-D bias 140 / 172 us, capped 8 x 24 heads of
+// 1370 rows in fp16 215 / 241 us (429 TFLOP/s).
 template <bool CAP, int BIAS, bool DOCS>
-__global__ __launch_bounds__(256, CAP && DOCS ? 2 : 3) void attn_mod_fwd_kernel(ModArgs a) {
+__global__ __launch_bounds__(256, CAP && (DOCS || BIAS) ? 2 : 3) void attn_mod_fwd_kernel(ModArgs a) {
   __shared__ __attribute__((aligned(128))) char smem[2 * KT_BYTES], clean[8192];
   __shared__ TileRef list[DOCS ? LIST : 1];
   __shared__ int buf[16];
@@ -628,10 +634,10 @@ __global__ __launch_bounds__(256, CAP && DOCS ? 2 : 3) void attn_mod_fwd_kernel(
 
 // ------------------------------------------------------------------------------------------------ forward, few rows: keys split over waves and workgroups
 // The G * nq rows of the query heads that share a key head fill tiles of 16 columns (v_mfma_f32_16x16x32: a single token of 1 .. 16 heads is one
-// tile).  Every wave walks its own
-// 64-key tiles (every fourth of the workgroup's chunk) without a barrier: K straight into operand registers, V through the wave's own LDS for the
+// tile).  Every wave walks its own 64-key tiles (every fourth of the workgroup's chunk) without a barrier: K straight into operand registers, V through the wave's own LDS for the
 // transposed read, both a tile ahead.  The four waves' (maximum, sum, output) are joined in LDS, those of several workgroups by
-// attn_mod_join_kernel, both in a fixed order.
+// attn_mod_join_kernel, both in a fixed order.  Bound by the keys' way from memory: single tokens of 24 heads on 32 caches of up to 8192 keys with 8 heads
+// (188 MB) 48 us = 3.9 TB/s, the join 5 us.
 constexpr int RT_POS = 8192, RT_DOC = RT_POS + 512, RT_BYTES = RT_DOC + 256;      // LDS of a wave: V, positions [2][64], document ids
 constexpr int ROWS = 16;
 
@@ -866,7 +872,9 @@ __global__ __launch_bounds__(256) void attn_mod_join_kernel(ModArgs a) {
 
 // ------------------------------------------------------------------------------------------------ backward
 // P = exp2(z - L2) from the forward's lse, dS = P (dP - delta), with the cap times 1 - tanh^2 = 4 (r - r^2), r = 1 / (1 + e^(2 s / cap)).
-// With the cap `delta` is 4 delta, so that the factor 4 costs nothing.
+// With the cap `delta` is 4 delta, so that the factor 4 costs nothing (dQ of 8 x 24 heads of 1370 capped rows 308 -> 279 us).
+// Two kernels, each writing its gradient once: dQ by query rows, dK and dV by keys over the queries of all heads that share them.  The scores are computed
+// twice, but nothing is added across workgroups in an order that changes.
 template <bool CAP>
 __device__ __forceinline__ float dscore(float p, float dp, float delta, float r) {
   if constexpr (CAP) return p * fmaf(4.f, dp, -delta) * fmaf(-r, r, r);
@@ -902,6 +910,7 @@ __device__ __forceinline__ void dq_tile(f32x16 (&acc)[2], unsigned& poison, cons
   }
 }
 
+// dQ of 128 rows per workgroup, staged as in the forward; three workgroups per CU without the cap (64 x 12 heads of 257 rows 53 us, 62 with two).
 template <bool CAP, int BIAS, bool DOCS>
 __global__ __launch_bounds__(256, CAP ? 2 : 3) void attn_mod_dq_kernel(ModArgs a) {
   __shared__ __attribute__((aligned(128))) char smem[2 * KT_BYTES], clean[8192];
@@ -1005,6 +1014,8 @@ __global__ __launch_bounds__(256, CAP ? 2 : 3) void attn_mod_dq_kernel(ModArgs a
 }
 
 // dK, dV of 128 keys: every wave holds 32 keys (the key on the lane) and the workgroup walks the 64-row query tiles of all heads that share them.
+// Two workgroups per CU: K, V, dK and dV of a wave's keys take 96 registers, so tiles may come through registers as well (64 x 12 heads of 257 rows 73 us, 8 x 24
+// capped ones of 1370 382 us, 12 heads of 8192 rows in documents 96 us).
 // LDS of a query tile: Q, dO (8 KB each), then per row: lse (log2 units), delta, position x / y, lim, document, verdicts
 constexpr int QT_L = 16384, QT_D = QT_L + 256, QT_X = QT_D + 256, QT_Y = QT_X + 256, QT_LIM = QT_Y + 256, QT_DOC = QT_LIM + 256, QT_ODD = QT_DOC + 256, QT_BYTES = QT_ODD + 128;
 struct QuerySide { float L2, delta, x, y; int lim, doc; };

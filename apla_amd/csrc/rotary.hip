@@ -14,6 +14,10 @@
 // Norm backward, g = R^T dy, u = g w, x^ = (x - mean) rstd:  dx = rstd (u - mean(u) - x^ mean(u x^))  (RMS: without mean(u));
 // dw = sum g x^, db = sum g over tokens and heads.  The statistics are recomputed from x (it has to be read for x^ anyway).
 // All arithmetic is fp32; the only rounding is that of the stored result.
+//
+// Measured (a large copy reaches 4.95 TB/s): rotation forward and backward of 269 MB 55 us, 4.9 TB/s; norm and rotation of 25 216 tokens of 24 heads 31 us
+// forward, 46 us backward (310 MB in all, 82 us with the sums: 3.8 TB/s — the backward's statistics and sums over eight lanes fill the vector unit);
+// few tokens: the launch.
 #include "common.h"
 
 namespace {
@@ -107,7 +111,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotArgs a) {
       long p = a.pos ? (long)a.pos[t] : a.seq_len ? t % a.seq_len : t;
       const bool pv = p >= 0 && p < a.P;      // a position outside the table gives NaN, not a read outside it
       const float* row = a.table + (pv ? p : 0) * a.rot;
-if (a.vec) {      // the lane's eight angles are four (interleaved) or eight (half) neighbours in the table
+      if (a.vec) {    // the lane's eight angles are four (interleaved) or eight (half) neighbours in the table
         const bool in = e0 < 2 * r;
         const float* c = row + (!in ? 0 : a.interleaved ? e0 >> 1 : e0 < r ? e0 : e0 - r);
         const f32x4 c0 = *(const f32x4*)c, s0 = *(const f32x4*)(c + r);
