@@ -49,7 +49,7 @@ def test_attention_workspace_sizes():
     docs = attn_args(doc_q=1 << 20, doc_k=1 << 20, S=2, Tq=400, Tk=600, max_q=200, max_k=300)
     assert size(docs, 1) >= 2 * (5 + 4) * 8 and size(docs, 1) > size(docs, 0) > 0
     cache = attn_args(S=1, Tq=1, Tk=65536, max_q=1, max_k=65536, Hq=8, Hkv=1)       # one token against a long cache: split over the keys
-    assert size(cache, 0) > 0 and size(cache, 1) == 0
+    assert size(cache, 0) > 0 and size(cache, 1) == 8 * 8 * 256                     # backward: eight partial sums of dQ [1, 8, 64], fp32
 
 
 def test_rotary_entry_points_refuse():
@@ -118,3 +118,39 @@ def test_oracle_gradients_are_those_of_automatic_differentiation(cap):
     ref = torch.autograd.grad(p @ c, (a, b, c), do)
     assert all(float((x - y).abs().max()) < 1e-12 for x, y in zip(ref, (w["dq"], w["dk"], w["dv"])))
     assert bool((w["lse"][~see.any(1)] == -math.inf).all()) and bool((~see.any(1)).any())
+
+
+def test_overlap_of_row_strided_views():
+    b = torch.zeros(6, 64, dtype=torch.bfloat16)
+    row = lambda off, stride: torch.as_strided(b, (1, 8), (stride, 1), off)      # noqa: E731
+    assert ops._overlap(row(0, 0), row(0, 0)) and ops._overlap(row(0, 0), row(4, 7)) and not ops._overlap(row(0, 0), row(8, 0))
+    assert not ops._overlap(b[:, :32], b[:, 32:]) and ops._overlap(b[:, :40], b[:, 32:]) and not ops._overlap(b[:3], b[3:])
+    assert not ops._overlap(b[:, :32], row(64 + 32, 0)) and ops._overlap(b[:, :32], row(64 + 24, 0)) and not ops._overlap(row(64 + 32, 5), b[:, :32])
+    assert not ops._overlap(b[:0], b)
+
+
+def test_rows_set_where_one_side_is_empty_are_those_of_the_sequences():
+    t = lambda: torch.full((12, 2), 7.0)      # noqa: E731
+    rows = lambda x: [i for i in range(12) if float(x[i, 0]) == 0.0 and float(x[i, 1]) == 0.0]      # noqa: E731
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)      # noqa: E731
+    for args, want in (((None, 6, None), list(range(12))), ((None, 6, i32(2, 9)), [0, 1, 6, 7, 8, 9, 10, 11]), ((None, 6, i32(0, -1)), []),
+                       ((i32(1, 4, 4, 9), 5, None), [1, 2, 3, 4, 5, 6, 7, 8]), ((i32(1, 4, 4, 9), 2, None), [1, 2, 4, 5]), ((i32(1, 4, 4, 9), 5, i32(1, 3, 2)), [1, 4, 5]),
+                       ((i32(0, 0), 0, None), [])):
+        x = t()
+        ops._zero_rows(x, *args, 0.0, False)
+        assert rows(x) == want and float(x.sum()) == 14.0 * (12 - len(want)), args
+    x = t()
+    ops._zero_rows(x, i32(1, 4, 4, 9), 5, None, 0.0, True)
+    assert rows(x) == list(range(12))
+
+
+def test_plans_that_a_captured_graph_reads_are_kept(monkeypatch):
+    from apla_amd.attn_features import AttnFeatures
+    f, dev = AttnFeatures(dict(causal=True), 2), torch.device("cuda")
+    capturing = [True]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    first = f.plan([5], dev)
+    capturing[0] = False
+    for n in range(10, 60):
+        f.plan([n], dev)
+    assert f.plan([5], dev) is first and len(f._plans) <= 17
