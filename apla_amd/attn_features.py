@@ -50,16 +50,18 @@ class AttnFeatures:
         if self.prefix and not self.causal:
             raise ValueError("a prefix needs causal: true")
         self.num_heads = num_heads
-        self._plans = {}
+        self._plans, self._captured = {}, set()
 
     def plan(self, seqlens: Sequence[int], device, packed_mask=None) -> dict:
         """Keyword arguments of functional.attention_mod_qkv for these sequences (equal ones: [n] * batch)."""
         key = (tuple(seqlens), packed_mask is not None, str(device))
         p = self._plans.get(key)
         if p is None:
-            if len(self._plans) >= 16:      # layouts seen lately, not every one ever seen
-                self._plans.clear()
+            if len(self._plans) - len(self._captured) >= 16:      # layouts seen lately, not every one ever seen; a captured graph keeps reading its own
+                self._plans = {k: v for k, v in self._plans.items() if k in self._captured}
             p = self._plans[key] = self._build(list(seqlens), device, packed_mask)
+        if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+            self._captured.add(key)
         return p
 
     def _build(self, seqlens, device, packed_mask) -> dict:

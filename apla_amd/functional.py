@@ -532,9 +532,27 @@ def attention_module_forward(x, qkv_w, qkv_b, proj_w, proj_b, num_heads, scale, 
 
 # ------------------------------------------------------------------------------------------------ rotary positions, q / k norm, modified scores
 def _rows_h16(x):
-    """[..., C] as 16-bit rows [T, C]; a row-strided 16-bit view stays a view."""
+    """[..., C] as 16-bit rows [T, C]; a row-strided 16-bit view stays a view, one that the kernels cannot read (broadcast, unaligned) is copied."""
     x2 = x.reshape(-1, x.shape[-1])
-    return x2 if x2.dtype == _h() else x2.to(_h())
+    x2 = x2 if x2.dtype == _h() else x2.to(_h())
+    ld, inner = x2.stride()
+    readable = inner == 1 and (x2.shape[0] <= 1 or (ld >= x2.shape[1] and ld % 8 == 0)) and x2.data_ptr() % 16 == 0
+    return x2 if readable else x2.clone(memory_format=torch.contiguous_format)
+
+
+def _remember(ctx, *tensors):
+    """The versions of tensors that the backward pass reads again without having saved them."""
+    ctx.versions = [(t, t._version) for t in tensors if t is not None and not t.is_inference()]
+
+
+def _unchanged(ctx):
+    if any(t._version != v for t, v in ctx.versions):
+        raise RuntimeError("an argument that the backward pass reads was modified in place after the forward pass")
+
+
+def _mod_tensors(mod, seq):
+    m = () if mod is None else (mod.slopes, mod.pos_q, mod.pos_k, mod.doc_q, mod.doc_k, mod.prefix)
+    return (*m, *(t for t in seq.values() if isinstance(t, torch.Tensor)))
 
 
 class _RotaryFn(torch.autograd.Function):
@@ -542,10 +560,12 @@ class _RotaryFn(torch.autograd.Function):
     def forward(ctx, x, table, heads, layout, pos, seq_len):
         _require_cuda(x, "rotary")
         ctx.args, ctx.pos, ctx.table, ctx.dtype = (heads, layout, seq_len), pos, table, x.dtype
+        _remember(ctx, table, pos)
         return ops.rotary_fwd(_rows_h16(x), table, heads, layout=layout, pos=pos, seq_len=seq_len).reshape(x.shape)
 
     @staticmethod
     def backward(ctx, dy):
+        _unchanged(ctx)
         heads, layout, seq_len = ctx.args
         dx = ops.rotary_bwd(_as2d_bf16(dy), ctx.table, heads, layout=layout, pos=ctx.pos, seq_len=seq_len)
         return dx.reshape(dy.shape).to(ctx.dtype), None, None, None, None, None
@@ -564,11 +584,13 @@ class _QkNormRotaryFn(torch.autograd.Function):
         par = [b_f32(p) for p in (qw, kw, qb, kb)]
         args = dict(zip(("q_weight", "k_weight", "q_bias", "k_bias"), par), norm=norm, eps=eps, **rot)
         ctx.save_for_backward(x)
+        _remember(ctx, qw, kw, rot["table"], rot["pos"])
         ctx.args, ctx.heads, ctx.shape, ctx.dtype, ctx.pdt = args, (Hq, Hkv), qkv.shape, qkv.dtype, [None if p is None else p.dtype for p in (qw, kw, qb, kb)]
         return ops.qk_norm_rotary_fwd(x, Hq, Hkv, **args).reshape(qkv.shape[:-1] + ((Hq + Hkv) * 64,))
 
     @staticmethod
     def backward(ctx, dy):
+        _unchanged(ctx)
         (x,), (Hq, Hkv) = ctx.saved_tensors, ctx.heads
         n = (Hq + Hkv) * 64
         full = torch.zeros(x.shape, device=x.device, dtype=x.dtype) if x.shape[1] > n else torch.empty(x.shape, device=x.device, dtype=x.dtype)
@@ -592,11 +614,13 @@ class _AttnModFn(torch.autograd.Function):
         o, lse = ops.attn_mod_fwd(q2, k2, v2, Hq, Hkv, scale, mod, **seq)
         ctx.save_for_backward(q2, k2, v2, o, lse)
         ctx.args, ctx.like = (Hq, Hkv, scale, mod, seq), [(t.shape, t.dtype) for t in (q, k, v)]
+        _remember(ctx, *_mod_tensors(mod, seq))
         ctx.mark_non_differentiable(lse)
         return o.reshape(q.shape), lse
 
     @staticmethod
     def backward(ctx, do, _dlse):
+        _unchanged(ctx)
         q, k, v, o, lse = ctx.saved_tensors
         Hq, Hkv, scale, mod, seq = ctx.args
         g = ops.attn_mod_bwd(q, k, v, o, _as2d_bf16(do), lse, Hq, Hkv, scale, mod, **seq)
@@ -627,11 +651,13 @@ class _AttnModQkvFn(torch.autograd.Function):
             qk = x[:, :2 * n]
         o, lse = ops.attn_mod_fwd(qk[:, :n], qk[:, n:], x[:, 2 * n:], H, H, scale, mod, **seq)
         ctx.save_for_backward(x, qk, o, lse)
+        _remember(ctx, qw, kw, rot["table"], rot["pos"], *_mod_tensors(mod, seq))
         ctx.args, ctx.norm, ctx.like, ctx.pdt = (H, scale, rot, mod, seq), args, (qkv.shape, qkv.dtype), [None if p is None else p.dtype for p in (qw, kw, qb, kb)]
         return o.reshape(qkv.shape[:-1] + (n,))
 
     @staticmethod
     def backward(ctx, do):
+        _unchanged(ctx)
         x, qk, o, lse = ctx.saved_tensors
         H, scale, rot, mod, seq = ctx.args
         n = H * 64

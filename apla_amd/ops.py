@@ -712,6 +712,9 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     (ra, ca), (rb, cb), la, lb, w = a.shape, b.shape, a.stride(0), b.stride(0), a.element_size()
     if ra * ca == 0 or rb * cb == 0 or sa + ((ra - 1) * la + ca) * w <= sb or sb + ((rb - 1) * lb + cb) * w <= sa:
         return False
+    if ra == 1 and rb == 1:
+        return True
+    la, lb = lb if ra == 1 else la, la if rb == 1 else lb       # the stride of a single row says nothing
     if la == lb:
         d = (sb - sa) % (la * w)
         return d < ca * w or d + cb * w > la * w
@@ -972,20 +975,28 @@ def attn_mod_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, Hq: int, Hkv
                 raise ValueError("attn_mod_fwd: lse must lie on q's device")
         a.o, a.lse = o.data_ptr(), lse.data_ptr()
         if a.max_q == 0 or a.max_k == 0:       # no rows, or no keys at all: every row sees nothing
-            _zero_rows(o, cu_q, 0.0, a.fill & 1), _zero_rows(lse.t(), cu_q, float("-inf"), a.fill & 2)
+            _zero_rows(o, cu_q, a.max_q, None, 0.0, a.fill & 1), _zero_rows(lse.t(), cu_q, a.max_q, None, float("-inf"), a.fill & 2)
             return o, lse
         ws = _mod_workspace(a, False, q.device)     # noqa: F841  (alive until the launch)
         check(lib().apla_attn_mod_fwd(a, _raw_stream(q.device)), "apla_attn_mod_fwd")
     return o, lse
 
 
-def _zero_rows(t, cu, value, whole):
-    """The rows of the sequences (all rows where the buffer is ours) set to one value."""
-    if cu is None or whole:
+def _zero_rows(t, cu, longest, used, value, whole):
+    """The rows that sequences hold (all rows where the buffer is ours) set to one value: what the kernels do where one side has no rows at all."""
+    if whole:
         t.fill_(value)
-    else:
+    elif longest and t.shape[0]:
         rows = torch.arange(t.shape[0], device=t.device)
-        t.masked_fill_(((rows >= cu[0]) & (rows < cu[-1]))[:, None], value)
+        if cu is None:
+            seq = rows // longest
+            first, end = seq * longest, (seq + 1) * longest
+        else:
+            seq = (torch.searchsorted(cu, rows, right=True) - 1).clamp_(0, cu.numel() - 2)
+            first, end = cu[seq], torch.minimum(cu[seq + 1], cu[seq] + longest)
+        if used is not None:
+            end = torch.minimum(end, first + used[seq].clamp(min=0))
+        t.masked_fill_(((rows >= first) & (rows < end))[:, None], value)
 
 
 def attn_mod_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, do: torch.Tensor, lse: torch.Tensor, Hq: int, Hkv: int,
@@ -1020,7 +1031,8 @@ def attn_mod_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Ten
         else:
             a.lddv = _strided_rows(dv, "dv", nk, Tk)
         if a.max_q == 0 or a.max_k == 0:
-            _zero_rows(dq, cu_q, 0.0, a.fill & 4), _zero_rows(dk, cu_k, 0.0, a.fill & 8), _zero_rows(dv, cu_k, 0.0, a.fill & 16)
+            _zero_rows(dq, cu_q, a.max_q, None, 0.0, a.fill & 4)
+            _zero_rows(dk, cu_k, a.max_k, len_k, 0.0, a.fill & 8), _zero_rows(dv, cu_k, a.max_k, len_k, 0.0, a.fill & 16)
             return dq, dk, dv
         delta = torch.empty_like(lse)
         a.o, a.lse, a.d_o, a.delta = o.data_ptr(), lse.data_ptr(), do.data_ptr(), delta.data_ptr()

@@ -124,7 +124,7 @@ def test_plugin_keeps_the_norms_of_the_module_it_replaces(norm):
     o = torch.cat([O.attend(q[:, h], k[:, h], v[:, h], 0.125, O.visible(n, n))["o"] for h in range(H)], 1)
     want = o @ ref[2].t() + ref[3]
     plain = torch.cat([O.attend(*(t[:, h] for t in (X @ ref[0].t() + ref[1]).reshape(n, 3, H, 64).unbind(1)), 0.125, O.visible(n, n))["o"] for h in range(H)], 1) @ ref[2].t() + ref[3]
-    err = float((y[0].double().cpu() - want).norm() / want.norm())
+    err = float((y[0].detach().double().cpu() - want.detach()).norm() / want.detach().norm())
     # ten roundings of 2^-11 on the way, q and k twice with scores up to ~8: (10 + 2 * 2 * 8) 2^-11
     assert err <= 42 * 2.0 ** -11 and float((plain - want).norm() / want.norm()) > 0.1
 
@@ -212,3 +212,37 @@ def test_gradient_of_the_loss_through_a_model_against_differences():
     # noise: 2 * 34 * 128 output values with errors of ~8 roundings each, independent; curvature: h^2 (a step of 1/8 changes the gradient by O(1/64))
     noise = 8 * 2.0 ** -11 * float((2 * 17 * 128) ** 0.5) * 2 / (2 * h)
     assert abs(diff - an) <= noise + 0.05 * float(g.norm() * d.norm()) / 4, (diff, an, noise)
+
+
+def test_broadcast_and_unaligned_inputs():
+    """One key / value row for all tokens (stride 0) and rows at an odd address: copied, and the gradient of a broadcast input is summed."""
+    T, H = 40, 2
+    g = torch.Generator().manual_seed(3)
+    flat = torch.randn(T * 128 + 1, generator=g).bfloat16().cuda()
+    q = flat[1:].reshape(T, 128)
+    k1 = torch.randn(1, 128, generator=g).bfloat16().cuda().requires_grad_(True)
+    kc = k1.detach().expand(T, 128).contiguous().requires_grad_(True)
+    table = R.rotary_table(T, 64, device="cuda")
+    do = torch.randn(T, 128, generator=g).bfloat16().cuda()
+    o, _ = AF.attention_mod(q, AF.rotary(k1.expand(T, 128), table, H), k1.expand(T, 128), H, H, 0.125, ops.ScoreMod(causal=True), batch=1)
+    oc, _ = AF.attention_mod(q.clone(), AF.rotary(kc, table, H), kc, H, H, 0.125, ops.ScoreMod(causal=True), batch=1)
+    assert torch.equal(o, oc)
+    (a,), (b,) = torch.autograd.grad(o, k1, do), torch.autograd.grad(oc, kc, do)
+    # a: 16-bit sums over 40 rows of what b holds row by row; each of a sum's partial results may be rounded to 16 bits
+    want = b.double().sum(0)
+    assert ((a[0].double() - want).abs() <= 2 * T * 2.0 ** -8 * b.double().abs().sum(0)).all()
+
+
+def test_arguments_changed_between_forward_and_backward_are_refused():
+    T, H = 16, 1
+    z = lambda: torch.randn(T, 64, device="cuda").bfloat16().requires_grad_(True)      # noqa: E731
+    slopes, used, table = torch.ones(H, device="cuda"), torch.full((1,), T, dtype=torch.int32, device="cuda"), R.rotary_table(T, 64, device="cuda")
+    w = torch.ones(64, device="cuda")
+    for t, make in ((slopes, lambda: AF.attention_mod(z(), z(), z(), H, H, 0.125, ops.ScoreMod(slopes=slopes), batch=1)[0]),
+                    (used, lambda: AF.attention_mod(z(), z(), z(), H, H, 0.125, batch=1, len_k=used)[0]),
+                    (table, lambda: AF.rotary(z(), table, H)), (w, lambda: AF.qk_norm_rotary(z(), H, 0, q_weight=w))):
+        make().sum().backward()
+        o = make()
+        t.add_(0)
+        with pytest.raises(RuntimeError, match="in place"):
+            o.sum().backward()
