@@ -261,12 +261,13 @@ dim3 rot_plan(RotArgs& a, int T, int h1, int h2, bool par) {
   const int r = a.rot >> 1;
   a.vec = r > 0 && r % (a.interleaved ? 4 : 8) == 0 && apla_aligned16(a.table);
   const int groups = h2 ? 2 : 1;
+  const long cap = (par ? PARAM_WGS : ROT_WGS) / groups;      // (the workspace of the sums has PARAM_WGS rows)
   long sp = (4096 + waves * groups - 1) / (waves * groups);
-  a.splits = (int)(sp < most ? sp : most);
+  sp = sp < most ? sp : most;
+  a.splits = (int)(sp < cap ? sp : cap);
   a.T = T;
   long gx = (waves + 3) / 4;
-  const long cap = (par ? PARAM_WGS : ROT_WGS) / groups;
-  if (gx * a.splits > cap) gx = cap / a.splits > 0 ? cap / a.splits : 1;
+  if (gx * a.splits > cap) gx = cap / a.splits;
   return dim3((unsigned)gx, (unsigned)(groups * a.splits));
 }
 

@@ -124,6 +124,12 @@ def test_qk_norm_rotary_both_directions(T, Hq, Hkv, rot, layout, norm, dtype):
         assert bool(((dpar[2 + k].cpu().double() - gb[k]).abs() <= n * size[1]).all())
 
 
+@pytest.mark.parametrize("T,Hq,Hkv", [(2, 769, 1), (3, 401, 399), (1, 1, 1021)])
+def test_qk_norm_rotary_of_hundreds_of_odd_heads(T, Hq, Hkv):
+    """Few tokens of many heads that no block size divides: the blocks are spread over as many workgroups as the sums' workspace has rows, not more."""
+    test_qk_norm_rotary_both_directions(T, Hq, Hkv, 32, "half", "layer", "bf16")
+
+
 def test_qk_norm_rotary_constant_row_and_defaults():
     """A head of equal values: variance 0, LayerNorm gives the bias; no weights means 1 / 0, no table means no rotation."""
     x = torch.full((3, 192), 2.5, dtype=torch.bfloat16)
