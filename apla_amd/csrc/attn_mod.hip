@@ -34,6 +34,7 @@ struct ModArgs {
   const float *slopes, *pos_q, *pos_k;
   int S, Tq, Tk, max_q, max_k, Hq, G, causal;
   float scale, c, k1, kx, A;            // c = scale log2e; cap: 2 scale log2e / cap, scale / cap, cap log2e
+  int fine;                             // every tile counts as masked (see cap_fine)
   const int2 *rng_q, *rng_k;            // [S][tiles of 64]: smallest and largest document id
   int nt_q, nt_k, nblk, np;             // tiles per sequence in those; 128-row blocks per sequence; see where()
   const bf16* d_o;
@@ -171,7 +172,7 @@ __device__ __forceinline__ void apply_poison(f32x16 (&acc)[2], unsigned m) {
 // a condition that is the same for the whole wave, as a scalar: branches on it need no execution mask
 __device__ __forceinline__ bool uniform(bool c) { return __builtin_amdgcn_readfirstlane((int)c) != 0; }
 
-// ---- staging: 64 rows x 64 columns by 256 threads (two 16-byte pieces each) through registers; rows past nrows read row nrows - 1
+// ---- staging (byte offsets within a tile: at most 63 rows of 2^25 bytes, below 2^31): 64 rows x 64 columns by 256 threads (two 16-byte pieces each) through registers; rows past nrows read row nrows - 1
 struct Stage { bf16x8 v[2]; };
 __device__ __forceinline__ bool stage_odd(const Stage& t) { return __ballot((nonfinite_bits(t.v[0]) | nonfinite_bits(t.v[1])) != 0) != 0; }
 // byte offset of a thread's first piece from the tile's first row (its second lies 32 rows further)
@@ -247,7 +248,8 @@ struct RowCtx { int lim, doc; float pos[2], slope; };       // slope in log2 uni
 
 // cap tanh(s / cap) in log2 units: A (1 - 2 r), r = 1 / (1 + e^(2 s / cap)).  That is exact to 2^-23 A, which small scores feel relatively; cap_fine
 // takes the odd series below |s / cap| = 1/4 (its next term is 2^-27 there).  Masked tiles do so — every key of a short sequence is in one —,
-// full tiles hold 64 keys or more of a row, over which the difference averages out.
+// full tiles hold 64 keys or more of a row, over which the difference averages out, as long as A is small: they do so too with caps above 64 (2^-23 A is
+// 1.1e-5 there, and would be 0.15 at a cap of 9e5).
 __device__ __forceinline__ float cap_score(float s, const ModArgs& a, float& r, float sub = 0.f) {      // less `sub`
   r = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * a.k1));
   return fmaf(-2.f * a.A, r, a.A - sub);
@@ -304,7 +306,7 @@ __device__ __forceinline__ void hide_rows(f32x16& x, f32x16& y, int j, int doc, 
 
 // Scores s[16] of one row (on the lane) and 32 keys, or of one key and 32 rows, in log2 units and less sub(i); with neither cap nor bias they stay raw
 // and the caller multiplies by c.  `side`: LDS address of the positions of the other 32 (x, then y 256 bytes behind), r: cap_score's r of every
-// score.  masked (the same for the wave) only chooses the finer cap here.
+// score.  masked (the same for the wave) chooses the finer cap here, and nothing else.
 struct Nothing { __device__ __forceinline__ float operator()(int) const { return 0.f; } };
 template <bool CAP, int BIAS, class Sub = Nothing>
 __device__ __forceinline__ void modify(f32x16& s, f32x16& r, const ModArgs& a, const float (&pos)[2], float slope, const char* side, int h2, bool masked, Sub sub = {}) {
@@ -574,6 +576,7 @@ __global__ __launch_bounds__(256, CAP && (DOCS || BIAS) ? 2 : 3) void attn_mod_f
     wlim0 = row_lim(a, m, wq); wlim1 = row_lim(a, m, min(wq + 31, m.nq - 1));
     lim0 = row_lim(a, m, q0); lim = row_lim(a, m, min(q0 + 127, m.nq - 1));
   }
+  if (CAP && a.fine) lim0 = wlim0 = 0;
 
   f32x16 acc[2];
 #pragma unroll
@@ -705,7 +708,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_rows_kernel(ModArgs a) {
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) qf[ks] = *(const bf16x8*)(a.q + (m.q0 + qi) * a.ldq + h * 64 + 32 * ks + 8 * g);
   const RowCtx r = row_ctx<BIAS>(a, m, qi, h);
-  const int wlo = wave_min_i(r.doc), whi = wave_max_i(r.doc), wlim0 = wave_min_i(r.lim), wlim1 = wave_max_i(r.lim);
+  const int wlo = wave_min_i(r.doc), whi = wave_max_i(r.doc), wlim0 = CAP && a.fine ? 0 : wave_min_i(r.lim), wlim1 = wave_max_i(r.lim);
   f32x4 acc[4];
 #pragma unroll
   for (int d = 0; d < 4; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -958,6 +961,7 @@ __global__ __launch_bounds__(256, CAP ? 2 : 3) void attn_mod_dq_kernel(ModArgs a
     wlim0 = row_lim(a, m, wq); wlim1 = row_lim(a, m, min(wq + 31, m.nq - 1));
     lim0 = row_lim(a, m, q0); lim = row_lim(a, m, min(q0 + 127, m.nq - 1));
   }
+  if (CAP && a.fine) lim0 = wlim0 = 0;
   f32x16 acc[2];
 #pragma unroll
   for (int i = 0; i < 16; ++i) { acc[0][i] = 0.f; acc[1][i] = 0.f; }
@@ -1107,7 +1111,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
   const int ntiles = (m.nq + 63) / 64;
   // whole tiles: every row of theirs sees all 128 keys, all of them rows and keys of the sequence
   const int jlast = jb + 127;
-  const int w0 = jlast >= m.nk ? ntiles : (!a.causal || m.pre > jlast) ? 0 : (max(0, jlast - m.off) + 63) / 64, w1 = m.nq / 64;
+  const int w0 = jlast >= m.nk ? ntiles : (!a.causal || m.pre > jlast) ? 0 : (max(0, jlast - m.off) + 63) / 64, w1 = CAP && a.fine ? 0 : m.nq / 64;
   for (int t0 = first; t0 < ntiles; t0 = DOCS ? t0 + LIST : ntiles) {
     int n = ntiles - first;
     if constexpr (DOCS) n = build_list(list, buf, t0, ntiles, w0, w1, a.rng_q + (long)(w.unit / Hkv) * a.nt_q, dlo, dhi, tid);
@@ -1182,7 +1186,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
       }
       if (active && row_lim(a, m, last) > jw && (!docs || (cur.hi >= max(wlo, 0) && cur.lo <= whi))) {
         const float slope = BIAS ? a.slopes[hk * a.G + g] * LOG2E : 0.f;
-        const bool masked = !cur.whole && !(i0 + 64 <= m.nq && jw + 32 <= m.nk && row_lim(a, m, i0) >= jw + 32 &&
+        const bool masked = !cur.whole && !(!(CAP && a.fine) && i0 + 64 <= m.nq && jw + 32 <= m.nk && row_lim(a, m, i0) >= jw + 32 &&
                                                    (!docs || (cur.lo >= 0 && cur.lo == cur.hi && wlo == cur.lo && whi == cur.lo)));
         dkdv_tile<CAP, BIAS>(dk, dv, pk, pv, kf, vf, a, j, docj, pj, slope, tile, clean, lane, fr, masked, docs, masked && odd);
       }
@@ -1319,19 +1323,19 @@ int mod_check(const char* who, const apla_attn_mod_t* p, bool backward) {
   APLA_REQUIRE(p->Tq > 0 && p->Tk > 0 && p->max_q > 0 && p->max_k > 0 && p->max_q <= p->Tq && p->max_k <= p->Tk, "%s: need 0 < max_q <= Tq and 0 < max_k <= Tk (%d/%d, %d/%d)", who, p->max_q, p->Tq, p->max_k, p->Tk);
   APLA_REQUIRE((p->cu_q || (long)p->S * p->max_q == p->Tq) && (p->cu_k || (long)p->S * p->max_k == p->Tk), "%s: without offsets the rows must be S x max", who);
   APLA_REQUIRE(p->max_q <= (1 << 24) && p->max_k <= (1 << 24), "%s: sequences of at most 2^24 tokens", who);
-  APLA_REQUIRE(p->scale > 0.f && p->scale < 1e30f && p->softcap >= 0.f && p->softcap < 1e6f, "%s: need scale > 0 and 0 <= softcap < 1e6", who);
+  APLA_REQUIRE(p->scale > 0.f && p->scale < 1e30f && (p->softcap == 0.f || (p->softcap >= 1e-6f && p->softcap < 1e6f)), "%s: need scale > 0 and a softcap of 0 or 1e-6 .. 1e6", who);
   APLA_REQUIRE(p->q && p->k && p->v && p->o && p->lse, "%s: a pointer is missing", who);
   APLA_REQUIRE(apla_aligned16(p->q) && apla_aligned16(p->k) && apla_aligned16(p->v) && apla_aligned16(p->o), "%s: q, k, v, o must be 16-byte aligned", who);
   APLA_REQUIRE(p->ldq >= p->Hq * 64L && p->ldo >= p->Hq * 64L && p->ldk >= p->Hkv * 64L && p->ldv >= p->Hkv * 64L, "%s: a row stride is shorter than its heads", who);
-  APLA_REQUIRE(((p->ldq | p->ldk | p->ldv | p->ldo) & 7) == 0 && p->ldq < (1L << 23) && p->ldk < (1L << 23) && p->ldv < (1L << 23), "%s: row strides must be multiples of 8, below 2^23", who);
+  APLA_REQUIRE(((p->ldq | p->ldk | p->ldv | p->ldo) & 7) == 0 && p->ldq < (1L << 24) && p->ldk < (1L << 24) && p->ldv < (1L << 24), "%s: row strides must be multiples of 8, below 2^24", who);
   APLA_REQUIRE((!p->doc_q) == (!p->doc_k), "%s: document ids are needed for queries and keys", who);
   APLA_REQUIRE(p->pos_dim >= 0 && p->pos_dim <= 2 && (p->pos_dim == 0 ? !p->pos_q && !p->pos_k : p->pos_q && p->pos_k && p->slopes), "%s: positions need slopes, both sides and 1 or 2 coordinates", who);
   APLA_REQUIRE(!p->prefix || p->causal, "%s: a prefix needs the causal mask", who);
   if (backward) {
     APLA_REQUIRE(p->d_o && p->dq && p->dk && p->dv && p->delta, "%s: a pointer is missing", who);
     APLA_REQUIRE(apla_aligned16(p->d_o) && apla_aligned16(p->dq) && apla_aligned16(p->dk) && apla_aligned16(p->dv), "%s: d_o, dq, dk, dv must be 16-byte aligned", who);
-    APLA_REQUIRE(p->lddo >= p->Hq * 64L && p->lddq >= p->Hq * 64L && p->lddk >= p->Hkv * 64L && p->lddv >= p->Hkv * 64L && ((p->lddo | p->lddq | p->lddk | p->lddv) & 7) == 0 && p->lddo < (1L << 23),
-                 "%s: gradient row strides must cover their heads and be multiples of 8, below 2^23", who);
+    APLA_REQUIRE(p->lddo >= p->Hq * 64L && p->lddq >= p->Hq * 64L && p->lddk >= p->Hkv * 64L && p->lddv >= p->Hkv * 64L && ((p->lddo | p->lddq | p->lddk | p->lddv) & 7) == 0 && p->lddo < (1L << 24),
+                 "%s: gradient row strides must cover their heads and be multiples of 8, that of d_o below 2^24", who);
   }
   const Plan pl = plan_of(*p, backward);
   APLA_REQUIRE(pl.bytes == 0 || (p->workspace && apla_aligned16(p->workspace) && p->workspace_bytes >= pl.bytes), "%s: needs %ld bytes of 16-byte aligned workspace (got %ld)", who, pl.bytes, p->workspace_bytes);
@@ -1348,7 +1352,7 @@ ModArgs mod_args(const apla_attn_mod_t& p, const Plan& pl) {
   a.slopes = p.slopes; a.pos_q = p.pos_q; a.pos_k = p.pos_k;
   a.S = p.S; a.Tq = p.Tq; a.Tk = p.Tk; a.max_q = p.max_q; a.max_k = p.max_k; a.Hq = p.Hq; a.G = p.Hq / p.Hkv; a.causal = p.causal;
   a.scale = p.scale; a.c = p.scale * LOG2E;
-  if (p.softcap > 0.f) { a.k1 = 2.f * p.scale * LOG2E / p.softcap; a.kx = p.scale / p.softcap; a.A = p.softcap * LOG2E; }
+  if (p.softcap > 0.f) { a.k1 = 2.f * p.scale * LOG2E / p.softcap; a.kx = p.scale / p.softcap; a.A = p.softcap * LOG2E; a.fine = p.softcap > 64.f; }
   a.nt_q = (p.max_q + 63) / 64; a.nt_k = (p.max_k + 63) / 64;
   char* ws = (char*)p.workspace;
   if (p.doc_k) { a.rng_k = (const int2*)(ws + pl.rng_k); a.rng_q = (const int2*)(ws + pl.rng_q); }

@@ -860,8 +860,8 @@ class ScoreMod:
     __slots__ = ("softcap", "slopes", "pos_q", "pos_k", "doc_q", "doc_k", "causal", "prefix")
 
     def __init__(self, softcap: float = 0.0, slopes=None, pos_q=None, pos_k=None, doc_q=None, doc_k=None, causal: bool = False, prefix=None):
-        if not 0.0 <= float(softcap) < 1e6:
-            raise ValueError(f"softcap must be 0 (none) or positive, below 1e6; got {softcap}")
+        if float(softcap) != 0.0 and not 1e-6 <= float(softcap) < 1e6:
+            raise ValueError(f"softcap must be 0 (none) or 1e-6 .. 1e6; got {softcap}")
         if (pos_q is None) != (pos_k is None) or (doc_q is None) != (doc_k is None):
             raise ValueError("positions and document ids are given for queries and keys, or for neither")
         if pos_q is not None and slopes is None:

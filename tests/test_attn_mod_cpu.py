@@ -28,7 +28,7 @@ def attn_args(**kw):
 
 
 @pytest.mark.parametrize("bad", [dict(S=0), dict(S=70000), dict(Hq=3, Hkv=2), dict(Hkv=0), dict(Tq=0), dict(max_q=9), dict(max_k=0), dict(Tq=9), dict(scale=0.0),
-                                 dict(scale=-1.0), dict(scale=math.nan), dict(softcap=-1.0), dict(softcap=math.inf), dict(q=0), dict(lse=0), dict(k=(1 << 20) + 8), dict(ldq=64),
+                                 dict(scale=-1.0), dict(scale=math.nan), dict(softcap=-1.0), dict(softcap=math.inf), dict(softcap=1e-9), dict(q=0), dict(lse=0), dict(k=(1 << 20) + 8), dict(ldq=64),
                                  dict(ldk=68), dict(doc_q=1 << 20), dict(pos_dim=1), dict(pos_dim=3, pos_q=1 << 20, pos_k=1 << 20, slopes=1 << 20),
                                  dict(pos_dim=1, pos_q=1 << 20, pos_k=1 << 20), dict(prefix=1 << 20), dict(doc_q=1 << 20, doc_k=1 << 20),
                                  dict(Tq=1 << 25, Tk=1 << 25, S=1, max_q=1 << 25, max_k=4, cu_q=1 << 20, cu_k=1 << 20)], ids=str)
@@ -77,7 +77,7 @@ def test_no_cpu_path():
 
 def test_score_mod_refuses():
     t = torch.zeros(2)
-    for kw in (dict(softcap=-1.0), dict(softcap=math.nan), dict(pos_q=t, slopes=t), dict(pos_q=t, pos_k=t), dict(doc_k=t), dict(prefix=t)):
+    for kw in (dict(softcap=-1.0), dict(softcap=math.nan), dict(softcap=1e-9), dict(pos_q=t, slopes=t), dict(pos_q=t, pos_k=t), dict(doc_k=t), dict(prefix=t)):
         with pytest.raises(ValueError):
             ops.ScoreMod(**kw)
     with pytest.raises(NotImplementedError):

@@ -12,6 +12,7 @@ import pytest
 import torch
 
 from apla_amd import ops
+from apla_amd._lib import AplaHipError
 from oracle import mod_oracle as O
 
 pytestmark = pytest.mark.gpu
@@ -389,3 +390,38 @@ def test_refusals():
             f()
     with pytest.raises(NotImplementedError):
         M(slopes=f32(2).requires_grad_(True))
+
+
+@pytest.mark.parametrize("cap", [300.0, 9e5])
+def test_caps_far_above_the_scores_change_nothing(cap):
+    """cap tanh(s / cap) of scores |s| <= 12 is s to s^3 / (3 cap^2) = 6.4e-3 at 300 and 0 at 9e5; lse must keep to that plus fp32 rounding of the scores
+    (2^-20: eight roundings of values up to 2^5 in log2 units, half a step each) however large the cap is."""
+    T, H = 512, 2
+    q, k, v = (rnd((T, H * 64), torch.bfloat16, 40 + i).cuda() for i in range(3))
+    s = torch.stack([q[:, 64 * h:64 * h + 64].double() @ k[:, 64 * h:64 * h + 64].double().t() * 0.125 for h in range(H)])
+    assert float(s.abs().max()) <= 12
+    want = torch.logsumexp(cap * torch.tanh(s / cap), 2)
+    for mod in (ops.ScoreMod(softcap=cap), ops.ScoreMod(softcap=cap, slopes=torch.zeros(H, device="cuda"))):
+        for rows in (T, 3):      # whole tiles, and the few-row kernel
+            _, lse = ops.attn_mod_fwd(q[:rows], k, v, H, H, 0.125, mod, batch=1)
+            # per score: fp32 product and cap relative to the score (sum of 64 products: 2^-24 * 64 * 1 / 8 * |q||k| <= 2^-17), logarithm and its sum 2^-20
+            assert float((lse.double() - want[:, :rows]).abs().max()) <= 2.0 ** -16
+
+
+def test_row_strides_up_to_their_limit():
+    """Rows 2^24 - 8 elements apart (a column of very wide rows), tiles that end inside the sequence: offsets within a tile pass 2^30 bytes."""
+    T, ld = 70, (1 << 24) - 8
+    buf = torch.empty(T * ld, dtype=torch.bfloat16, device="cuda")
+    wide = torch.as_strided(buf, (T, 256), (ld, 1))
+    wide.copy_(rnd((T, 256), torch.bfloat16, 50))
+    flat, do = wide.contiguous(), rnd((T, 64), torch.bfloat16, 51).cuda()
+    for rows in (T, 2):
+        res = []
+        for x in (wide, flat):
+            q, k, v = x[:rows, :64], x[:, 64:128], x[:, 128:192]
+            mod = ops.ScoreMod(causal=True)
+            o, lse = ops.attn_mod_fwd(q, k, v, 1, 1, 0.125, mod, batch=1)
+            res.append((o, lse, *ops.attn_mod_bwd(q, k, v, o, do[:rows], lse, 1, 1, 0.125, mod, batch=1)))
+        assert all(torch.equal(a, b) for a, b in zip(*res))
+    with pytest.raises(AplaHipError, match="stride"):
+        ops.attn_mod_fwd(torch.as_strided(buf, (2, 64), (ld + 8, 1)), flat[:, :64], flat[:, :64], 1, 1, 0.125, batch=1)
