@@ -304,25 +304,23 @@ __device__ __forceinline__ void hide_rows(f32x16& x, f32x16& y, int j, int doc, 
   }
 }
 
-// Scores s[16] of one row (on the lane) and 32 keys, or of one key and 32 rows, in log2 units and less sub(i); with neither cap nor bias they stay raw
+// Scores s[16] of one row (on the lane) and 32 keys, or of one key and 32 rows, in log2 units; with neither cap nor bias they stay raw
 // and the caller multiplies by c.  `side`: LDS address of the positions of the other 32 (x, then y 256 bytes behind), r: cap_score's r of every
 // score.  masked (the same for the wave) chooses the finer cap here, and nothing else.
-struct Nothing { __device__ __forceinline__ float operator()(int) const { return 0.f; } };
-template <bool CAP, int BIAS, class Sub = Nothing>
-__device__ __forceinline__ void modify(f32x16& s, f32x16& r, const ModArgs& a, const float (&pos)[2], float slope, const char* side, int h2, bool masked, Sub sub = {}) {
-  constexpr bool SUB = !__is_same(Sub, Nothing);
+template <bool CAP, int BIAS>
+__device__ __forceinline__ void modify(f32x16& s, f32x16& r, const ModArgs& a, const float (&pos)[2], float slope, const char* side, int h2, bool masked) {
   if constexpr (CAP) {
     if (masked) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float t;
-        s[i] = cap_fine(s[i], a, t) - sub(i);
+        s[i] = cap_fine(s[i], a, t);
         r[i] = t;
         if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);      // (this path must not set the kernel's register count)
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) { float t; s[i] = cap_score(s[i], a, t, sub(i)); r[i] = t; }
+      for (int i = 0; i < 16; ++i) { float t; s[i] = cap_score(s[i], a, t); r[i] = t; }
     }
   }
   if constexpr (BIAS > 0) {
@@ -335,7 +333,7 @@ __device__ __forceinline__ void modify(f32x16& s, f32x16& r, const ModArgs& a, c
       for (int e = 0; e < 4; ++e) {
         const float d = dist<BIAS>(pos, px[e], BIAS > 1 ? py[e] : 0.f);
         const int i = 4 * g + e;
-        s[i] = CAP ? fmaf(-slope, d, s[i]) : fmaf(s[i], a.c, SUB ? fmaf(-slope, d, -sub(i)) : -slope * d);
+        s[i] = CAP ? fmaf(-slope, d, s[i]) : fmaf(s[i], a.c, -slope * d);
       }
     }
   }
@@ -874,8 +872,34 @@ __global__ __launch_bounds__(256) void attn_mod_join_kernel(ModArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward
+// Four scores s[4 g .. 4 g + 3] of a row to weights exp2(z - L2); the rest as modify().  Between matrix instructions: while the unit works on the next
+// product the wave works on these.
+template <bool CAP, int BIAS>
+__device__ __forceinline__ void weigh4(f32x16& s, f32x16& r, int g, float L2, const ModArgs& a, const float (&pos)[2], float slope, const char* side, int h2, bool masked) {
+  f32x4 px, py;
+  if constexpr (BIAS > 0) px = *(const f32x4*)(side + (8 * g + 4 * h2) * 4);
+  if constexpr (BIAS > 1) py = *(const f32x4*)(side + 256 + (8 * g + 4 * h2) * 4);
+  float z[4];
+  if constexpr (CAP) {
+    if (masked) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { float t; z[e] = cap_fine(s[4 * g + e], a, t) - L2; r[4 * g + e] = t; }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { float t; z[e] = cap_score(s[4 * g + e], a, t, L2); r[4 * g + e] = t; }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float d = 0.f;
+    if constexpr (BIAS > 0) d = dist<BIAS>(pos, px[e], BIAS > 1 ? py[e] : 0.f);
+    if constexpr (CAP) z[e] = BIAS ? fmaf(-slope, d, z[e]) : z[e];
+    else z[e] = fmaf(s[4 * g + e], a.c, BIAS ? fmaf(-slope, d, -L2) : -L2);
+    s[4 * g + e] = __builtin_amdgcn_exp2f(z[e]);
+  }
+}
 // P = exp2(z - L2) from the forward's lse, dS = P (dP - delta), with the cap times 1 - tanh^2 = 4 (r - r^2), r = 1 / (1 + e^(2 s / cap)).
-// With the cap `delta` is 4 delta, so that the factor 4 costs nothing (dQ of 8 x 24 heads of 1370 capped rows 308 -> 279 us).
+// With the cap `delta` is 4 delta, so that the factor 4 costs nothing (dQ of 8 x 24 heads of 1370 capped rows 308 -> 280 us).
 // Two kernels, each writing its gradient once: dQ by query rows, dK and dV by keys over the queries of all heads that share them.  The scores are computed
 // twice, but nothing is added across workgroups in an order that changes.
 template <bool CAP>
@@ -898,13 +922,17 @@ __device__ __forceinline__ void dq_tile(f32x16 (&acc)[2], unsigned& poison, cons
 #pragma unroll
     for (int i = 0; i < 16; ++i) { s[i] = 0.f; p[i] = 0.f; }
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) { s = MFMA_F32_32x32x16_H16(kf[ks], qf[ks], s); p = MFMA_F32_32x32x16_H16(vf[ks], df[ks], p); }
+    for (int ks = 0; ks < 4; ++ks) s = MFMA_F32_32x32x16_H16(kf[ks], qf[ks], s);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      p = MFMA_F32_32x32x16_H16(vf[g], df[g], p);
+      weigh4<CAP, BIAS>(s, rc, g, L2, a, r.pos, r.slope, tile + KT_POS + kt * 128, h2, masked);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     TrFrags tk;
     tr_load(tk, Kt + fr.tr, kt * 32);
-    __builtin_amdgcn_sched_barrier(0);
-    modify<CAP, BIAS>(s, rc, a, r.pos, r.slope, tile + KT_POS + kt * 128, h2, masked, [&](int) { return L2; });
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = dscore<CAP>(__builtin_amdgcn_exp2f((CAP || BIAS) ? s[i] : fmaf(s[i], a.c, -L2)), p[i], delta, rc[i]);
+    for (int i = 0; i < 16; ++i) s[i] = dscore<CAP>(s[i], p[i], delta, rc[i]);
     if (masked) {
       hide_keys(s, 0.f, r.lim, r.doc, j0 + kt * 32, tile + KT_DOC + kt * 128, h2, docs);
       if (__builtin_expect(odd, 0)) poison |= poison_bits(tile, kt * 32, s, lane);
@@ -913,9 +941,10 @@ __device__ __forceinline__ void dq_tile(f32x16 (&acc)[2], unsigned& poison, cons
   }
 }
 
-// dQ of 128 rows per workgroup, staged as in the forward; three workgroups per CU without the cap (64 x 12 heads of 257 rows 53 us, 62 with two).
+// dQ of 128 rows per workgroup, staged as in the forward; three workgroups per CU where 168 registers hold a wave's state, as there (64 x 12 heads of 257 rows
+// 53 us, 62 with two; 8 x 24 capped ones of 1370 255 us, 280 with two).
 template <bool CAP, int BIAS, bool DOCS>
-__global__ __launch_bounds__(256, CAP ? 2 : 3) void attn_mod_dq_kernel(ModArgs a) {
+__global__ __launch_bounds__(256, CAP && (DOCS || BIAS) ? 2 : 3) void attn_mod_dq_kernel(ModArgs a) {
   __shared__ __attribute__((aligned(128))) char smem[2 * KT_BYTES], clean[8192];
   __shared__ TileRef list[DOCS ? LIST : 1];
   __shared__ int buf[16];
