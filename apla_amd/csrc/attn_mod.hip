@@ -11,7 +11,8 @@
 // The products are those of attention.hip (S^T = K Q^T with the query row on the lane, P^T from the accumulator as the next operand).
 // In a masked tile a weight of zero times a non-finite value is zero (poison_bits): what stands in masked places never matters.
 // P and dS are rounded to 16 bits as MFMA operands (half a step of values <= 256 resp. of dS, relative); scores, softmax
-// statistics, sums and accumulators are fp32.
+// statistics, sums and accumulators are fp32.  A row's dS add up to 0, so over few keys their roundings weigh more than the result's own: sequences of up to
+// 64 tokens, a single tile, multiply what the rounding left of dS too (in all masked tiles that costs 5 to 13 % of the long cases' backward).
 //
 // What bounds the tile kernels is the vector unit: a score costs a multiply-add, an exponential, an addition and half a maximum in the forward (the cap
 // a further exponential and a reciprocal).  Counters of the forward over 16384 causal rows: vector unit 79 % busy, matrix unit 45 %, no LDS conflicts; capped fp16 forward 84 / 23 %, its dQ 71 / 27 %, dK/dV 61 / 26 %.
@@ -128,6 +129,15 @@ __device__ __forceinline__ void tr_product(f32x16 (&acc)[2], const TrFrags& t, c
     const bf16x8 wb = acc_to_operand(w, sk);
 #pragma unroll
     for (int dt = 0; dt < 2; ++dt) acc[dt] = MFMA_F32_32x32x16_H16(t.f[2 * dt + sk], wb, acc[dt]);
+  }
+}
+
+// what is left of w once it is rounded to 16 bits (none of what overflows there)
+__device__ __forceinline__ void rounding_rest(f32x16& w) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float hi = (float)(bf16)w[i];
+    w[i] = fabsf(hi) < INFINITY ? w[i] - hi : 0.f;
   }
 }
 
@@ -909,7 +919,7 @@ __device__ __forceinline__ float dscore(float p, float dp, float delta, float r)
 }
 template <bool CAP, int BIAS>
 __device__ __forceinline__ void dq_tile(f32x16 (&acc)[2], unsigned& poison, const bf16x8 (&qf)[4], const bf16x8 (&df)[4], float L2, float delta, const ModArgs& a,
-                                        const RowCtx& r, const char* tile, const char* clean, int j0, int lane, const Frag& fr, bool masked, bool docs, bool odd) {
+                                        const RowCtx& r, const char* tile, const char* clean, int j0, int lane, const Frag& fr, bool masked, bool docs, bool odd, bool few) {
   const int h2 = lane >> 5;
   const unsigned Ks = lds_of(tile), Vs = Ks + 8192, Kt = odd ? lds_of(clean) : Ks;
 #pragma unroll
@@ -938,6 +948,7 @@ __device__ __forceinline__ void dq_tile(f32x16 (&acc)[2], unsigned& poison, cons
       if (__builtin_expect(odd, 0)) poison |= poison_bits(tile, kt * 32, s, lane);
     }
     tr_product(acc, tk, s);
+    if (few) { rounding_rest(s); tr_product(acc, tk, s); }
   }
 }
 
@@ -1032,7 +1043,7 @@ __global__ __launch_bounds__(256, CAP && (DOCS || BIAS) ? 2 : 3) void attn_mod_d
       }
       if (active && j0 < wlim1 && (!docs || (cur.hi >= max(wlo, 0) && cur.lo <= whi))) {
         const bool masked = !cur.whole && !(j0 + 64 <= wlim0 && (!docs || (cur.lo == cur.hi && wlo == cur.lo && whi == cur.lo)));
-        dq_tile<CAP, BIAS>(acc, poison, qf, df, L2, delta, a, r, tile, clean, j0, lane, fr, masked, docs, masked && odd);
+        dq_tile<CAP, BIAS>(acc, poison, qf, df, L2, delta, a, r, tile, clean, j0, lane, fr, masked, docs, masked && odd, m.nk <= 64);
       }
       cur = next;
       next = known(ahead);
@@ -1055,7 +1066,7 @@ struct QuerySide { float L2, delta, x, y; int lim, doc; };
 
 template <bool CAP, int BIAS>
 __device__ __forceinline__ void dkdv_tile(f32x16 (&dk)[2], f32x16 (&dv)[2], unsigned& pk, unsigned& pv, const bf16x8 (&kf)[4], const bf16x8 (&vf)[4], const ModArgs& a, int j, int docj,
-                                          const float (&pj)[2], float slope, const char* tile, const char* clean, int lane, const Frag& fr, bool masked, bool docs, bool odd) {
+                                          const float (&pj)[2], float slope, const char* tile, const char* clean, int lane, const Frag& fr, bool masked, bool docs, bool odd, bool few) {
   const int h2 = lane >> 5;
   const unsigned Qs = lds_of(tile), Ds = Qs + 8192, Qt = odd ? lds_of(clean) : Qs;
 #pragma unroll
@@ -1098,6 +1109,7 @@ __device__ __forceinline__ void dkdv_tile(f32x16 (&dk)[2], f32x16 (&dv)[2], unsi
     tr_load(tq, Qt + fr.tr, qt * 32);
     tr_product(dv, td, p);
     tr_product(dk, tq, s);
+    if (few) { rounding_rest(s); tr_product(dk, tq, s); }
   }
 }
 
@@ -1217,7 +1229,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
         const float slope = BIAS ? a.slopes[hk * a.G + g] * LOG2E : 0.f;
         const bool masked = !cur.whole && !(!(CAP && a.fine) && i0 + 64 <= m.nq && jw + 32 <= m.nk && row_lim(a, m, i0) >= jw + 32 &&
                                                    (!docs || (cur.lo >= 0 && cur.lo == cur.hi && wlo == cur.lo && whi == cur.lo)));
-        dkdv_tile<CAP, BIAS>(dk, dv, pk, pv, kf, vf, a, j, docj, pj, slope, tile, clean, lane, fr, masked, docs, masked && odd);
+        dkdv_tile<CAP, BIAS>(dk, dv, pk, pv, kf, vf, a, j, docj, pj, slope, tile, clean, lane, fr, masked, docs, masked && odd, m.nq <= 64);
       }
       if (x + 1 < total) put(smem + ((x + 1) & 1) * QT_BYTES, next.whole);
       if (x + 2 < total) fetch(t2, gn);

@@ -425,3 +425,23 @@ def test_row_strides_up_to_their_limit():
         assert all(torch.equal(a, b) for a, b in zip(*res))
     with pytest.raises(AplaHipError, match="stride"):
         ops.attn_mod_fwd(torch.as_strided(buf, (2, 64), (ld + 8, 1)), flat[:, :64], flat[:, :64], 1, 1, 0.125, batch=1)
+
+
+def test_gradients_of_short_sequences_are_rounded_once():
+    """Two keys of equal scores (q = 0, or k = 0): P = 1/2, o = (v1 + v2) / 2 and dS = +-(dO.v1 - dO.v2) / 4 in whole sixteenths, up to 13 bits.  With operands of
+    small integers dq and dk are then off by the rounding of the result (2^-8, bf16) and 2^-16 of what is added, though dS itself has more bits than bf16."""
+    S, g = 96, torch.Generator().manual_seed(60)
+    ints = lambda rows, lo, hi, step=1: (torch.randint(lo, hi + 1, (rows, 64), generator=g) * step).double()      # noqa: E731
+    a, v, do = ints(2 * S, -8, 8), ints(2 * S, -4, 4, 2), ints(2 * S, -8, 8)
+    zero = torch.zeros_like(a)
+    vs, ds_ = v.reshape(S, 2, 64), do.reshape(S, 2, 64)
+    o = vs.mean(1, keepdim=True)
+    dS = 0.5 * ((ds_ @ vs.transpose(1, 2)) - (ds_ * o).sum(-1, keepdim=True))          # [S, query, key]
+    h = lambda t: t.bfloat16().cuda()      # noqa: E731
+    for q, k in ((zero, a), (a, zero)):
+        og, lse = ops.attn_mod_fwd(h(q), h(k), h(v), 1, 1, 0.125, batch=S)
+        assert torch.equal(og.double().cpu().reshape(S, 2, 64), o.expand(S, 2, 64))
+        dq, dk, _ = ops.attn_mod_bwd(h(q), h(k), h(v), og, h(do), lse, 1, 1, 0.125, batch=S)
+        for got, x, w in ((dq, k, dS), (dk, q, dS.transpose(1, 2))):
+            want, mag = 0.125 * (w @ x.reshape(S, 2, 64)), 0.125 * (w.abs() @ x.reshape(S, 2, 64).abs())
+            assert ((got.double().cpu().reshape(S, 2, 64) - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -16 * mag).all()
