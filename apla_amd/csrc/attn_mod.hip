@@ -15,7 +15,7 @@
 // 64 tokens, a single tile, multiply what the rounding left of dS too (in all masked tiles that costs 5 to 13 % of the long cases' backward).
 //
 // What bounds the tile kernels is the vector unit: a score costs a multiply-add, an exponential, an addition and half a maximum in the forward (the cap
-// a further exponential and a reciprocal).  Counters of the forward over 16384 causal rows: vector unit 79 % busy, matrix unit 45 %, no LDS conflicts; capped fp16 forward 84 / 23 %, its dQ 71 / 27 %, dK/dV 61 / 26 %.
+// a further exponential and a reciprocal).  Counters of the forward over 16384 causal rows: vector unit 79 % busy, matrix unit 45 %, no LDS conflicts; capped fp16 forward 84 / 23 %, its dQ 80 / 30 %, dK/dV 61 / 26 %.
 #include "attn_tiles.h"
 #include "common.h"
 
@@ -551,8 +551,8 @@ __device__ __forceinline__ RowCtx row_ctx(const ModArgs& a, const MSeq& m, int i
 // 128 rows of a head per workgroup, 32 per wave; key tiles of 64 (K, V, positions, ids) go straight into one half of LDS while the other is worked on.
 // Three workgroups share a CU where 168 registers hold a wave's state; capped scores next to a bias or documents spill there (8 x 12 heads of 1370 rows
 // with both: 148 us with two, 169 with three).  Forward times, without / with that: 64 x 12 heads of 257 rows 41 / 49 us, 12 heads of 16384
-// causal rows 547 / 626 us (754 TFLOP/s of the visible half), 48 ragged sequences with a 2-D bias 140 / 172 us, capped 8 x 24 heads of
-// 1370 rows in fp16 215 / 241 us (429 TFLOP/s).
+// causal rows 538 / 626 us (766 TFLOP/s of the visible half), 48 ragged sequences with a 2-D bias 140 / 172 us, capped 8 x 24 heads of
+// 1370 rows in fp16 218 / 241 us (423 TFLOP/s).
 template <bool CAP, int BIAS, bool DOCS>
 __global__ __launch_bounds__(256, CAP && (DOCS || BIAS) ? 2 : 3) void attn_mod_fwd_kernel(ModArgs a) {
   __shared__ __attribute__((aligned(128))) char smem[2 * KT_BYTES], clean[8192];
