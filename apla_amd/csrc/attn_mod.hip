@@ -1254,22 +1254,25 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
   }
 }
 
-// out rows = mul * the sum of n fp32 partial sums, in their order; rows that no sequence holds are left.  blockIdx: (32-row group of a sequence, head, sequence)
-__global__ __launch_bounds__(256) void attn_mod_sum_kernel(ModArgs a, const float* part, int n, int queries, bf16* out, long ldo, float mul) {
-  const int row = blockIdx.x * 32 + (threadIdx.x >> 3), h = blockIdx.y, heads = gridDim.y, c = (threadIdx.x & 7) * 8;
+// Rows = mul * the sum of n fp32 partial sums [n][T][heads * 64], in their order; rows that no sequence holds are left.  One output, or two of them with
+// their partial sums one behind the other.  blockIdx: (32-row group of a sequence, output and head, sequence)
+struct SumOut { bf16* out; long ld; float mul; };
+__global__ __launch_bounds__(256) void attn_mod_sum_kernel(ModArgs a, const float* part, int n, int queries, int heads, SumOut o0, SumOut o1) {
+  const int row = blockIdx.x * 32 + (threadIdx.x >> 3), second = blockIdx.y >= heads, h = blockIdx.y - (second ? heads : 0), c = (threadIdx.x & 7) * 8;
   const MSeq m = mseq(a, blockIdx.z);
   if (row >= (queries ? m.nq : m.nk)) return;
+  const SumOut o = second ? o1 : o0;
   const long r = (queries ? m.q0 : m.k0) + row, T = queries ? a.Tq : a.Tk;
   f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
-  for (int i = 0; i < n; ++i) {
+  for (int i = second ? n : 0, end = i + n; i < end; ++i) {
     const float* p = part + ((i * T + r) * heads + h) * 64 + c;
     x += *(const f32x4*)p;
     y += *(const f32x4*)(p + 4);
   }
   bf16x8 v;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) { v[e] = (bf16)(x[e] * mul); v[4 + e] = (bf16)(y[e] * mul); }
-  *(bf16x8*)(out + r * ldo + h * 64 + c) = v;
+  for (int e = 0; e < 4; ++e) { v[e] = (bf16)(x[e] * o.mul); v[4 + e] = (bf16)(y[e] * o.mul); }
+  *(bf16x8*)(o.out + r * o.ld + h * 64 + c) = v;
 }
 
 // The rows that no sequence holds (before the first, behind the last, past a sequence's used or cut length) of the outputs named in `fill`: 0, -inf in lse.
@@ -1483,17 +1486,16 @@ extern "C" int apla_attn_mod_bwd(const apla_attn_mod_t* p, hipStream_t stream) {
     const dim3 grid((unsigned)unit_grid(units, a.np, (long)a.G * a.nblk * a.sq));
     APLA_MOD_LAUNCH_DOCS(attn_mod_dq_kernel, grid);
     if (a.sq > 1)
-      hipLaunchKernelGGL(attn_mod_sum_kernel, dim3((unsigned)((p->max_q + 31) / 32), (unsigned)p->Hq, (unsigned)p->S), dim3(256), 0, stream, a, (const float*)a.part_q, a.sq, 1, a.dq, a.lddq, a.scale);
+      hipLaunchKernelGGL(attn_mod_sum_kernel, dim3((unsigned)((p->max_q + 31) / 32), (unsigned)p->Hq, (unsigned)p->S), dim3(256), 0, stream, a, (const float*)a.part_q, a.sq, 1, p->Hq,
+                         (SumOut{a.dq, a.lddq, a.scale}), (SumOut{}));
   }
   a.nblk = (p->max_k + 127) / 128;
   {
     const dim3 grid((unsigned)unit_grid(units, a.np, (long)a.nblk * a.sk));
     APLA_MOD_LAUNCH_DOCS(attn_mod_dkdv_kernel, grid);
-    if (a.sk > 1) {
-      const dim3 sum((unsigned)((p->max_k + 31) / 32), (unsigned)p->Hkv, (unsigned)p->S);
-      hipLaunchKernelGGL(attn_mod_sum_kernel, sum, dim3(256), 0, stream, a, (const float*)a.part_k, a.sk, 0, a.dk, a.lddk, a.scale);
-      hipLaunchKernelGGL(attn_mod_sum_kernel, sum, dim3(256), 0, stream, a, (const float*)(a.part_k + (long)a.sk * a.Tk * p->Hkv * 64), a.sk, 0, a.dv, a.lddv, 1.f);
-    }
+    if (a.sk > 1)
+      hipLaunchKernelGGL(attn_mod_sum_kernel, dim3((unsigned)((p->max_k + 31) / 32), 2u * (unsigned)p->Hkv, (unsigned)p->S), dim3(256), 0, stream, a, (const float*)a.part_k, a.sk, 0, p->Hkv,
+                         (SumOut{a.dk, a.lddk, a.scale}), (SumOut{a.dv, a.lddv, 1.f}));
   }
   APLA_CHECK_LAUNCH("apla_attn_mod_bwd");
   return APLA_OK;
