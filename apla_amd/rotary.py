@@ -14,7 +14,8 @@ def rotary_frequencies(rot: int, base: float = 10000.0, *, scaling: Optional[str
     "linear"  every angle divided by factor (positions squeezed into the trained range);
     "ntk"     the base raised by factor^(rot / (rot - 2)): the slowest pair is squeezed by factor, the fastest not at all;
     "yarn"    per pair: those that turn more than beta_fast times over the ``trained`` range stay, those below beta_slow turns are divided by
-              factor, a linear ramp over the pair index between."""
+              factor, a linear ramp over the pair index between.  The ramp's ends are rounded outwards to whole indices and cut to
+              0 .. rot - 1, as published: its upper end may lie past the last pair, rot / 2 - 1, which then is divided in part."""
     if rot % 2 or not 2 <= rot <= 64:
         raise ValueError(f"rot must be even, 2..64, got {rot}")
     if base <= 1.0 or factor < 1.0:
@@ -30,8 +31,9 @@ def rotary_frequencies(rot: int, base: float = 10000.0, *, scaling: Optional[str
         if trained <= 0 or not beta_fast > beta_slow > 0:
             raise ValueError("yarn scaling needs the trained range and beta_fast > beta_slow > 0")
         pair = lambda turns: rot / 2 * math.log(trained / (2 * math.pi * turns)) / math.log(base)      # noqa: E731  (index of the pair with that many turns)
-        lo, hi = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), rot // 2 - 1)
-        ramp = ((torch.arange(rot // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        lo, hi = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), rot - 1)
+        i = torch.arange(rot // 2, dtype=torch.float64)
+        ramp = torch.where(i >= hi, 1.0, ((i - lo) / max(hi - lo, 1e-3)).clamp(0, 1))      # (hi <= lo: no pair turns even beta_slow times)
         return f * (1 - ramp) + f / factor * ramp
     if scaling not in (None, "ntk"):
         raise ValueError(f"unknown scaling {scaling!r}")
