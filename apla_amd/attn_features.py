@@ -54,17 +54,21 @@ class AttnFeatures:
 
     def plan(self, seqlens: Sequence[int], device, packed_mask=None) -> dict:
         """Keyword arguments of functional.attention_mod_qkv for these sequences (equal ones: [n] * batch)."""
-        key = (tuple(seqlens), packed_mask is not None, str(device))
+        key, cuda = (tuple(seqlens), packed_mask is not None, str(device)), torch.device(device).type == "cuda"
+        capturing = cuda and torch.cuda.is_current_stream_capturing()
         p = self._plans.get(key)
         if p is None:
+            p = self._build(list(seqlens), device, packed_mask, capturing)
+            if capturing and self.prefix:      # a node of this graph fills the prefix at every replay: a plan for this graph alone
+                return p
             if len(self._plans) - len(self._captured) >= 16:      # layouts seen lately, not every one ever seen; a captured graph keeps reading its own
                 self._plans = {k: v for k, v in self._plans.items() if k in self._captured}
-            p = self._plans[key] = self._build(list(seqlens), device, packed_mask)
-        if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+            self._plans[key] = p
+        if capturing:
             self._captured.add(key)
         return p
 
-    def _build(self, seqlens, device, packed_mask) -> dict:
+    def _build(self, seqlens, device, packed_mask, capturing: bool) -> dict:
         out = {}
         kinds = sorted(set(seqlens))
         if self.rope is not None:
@@ -82,7 +86,7 @@ class AttnFeatures:
             places = {n: _places(grid_side(n)) for n in kinds}
             pos = torch.cat([places[n] for n in seqlens]).contiguous().to(device)
         if self.prefix:
-            prefix = torch.full((len(seqlens),), self.prefix, dtype=torch.int32, device=device)
+            prefix = torch.full((len(seqlens),), self.prefix, dtype=torch.int32, device=device if capturing else None).to(device)
         out["mod"] = ops.ScoreMod(softcap=self.softcap, slopes=slopes, pos_q=pos, pos_k=pos, causal=self.causal, prefix=prefix)
         if packed_mask is None:
             out["batch"] = len(seqlens)
