@@ -56,16 +56,23 @@ class AttnFeatures:
         """Keyword arguments of functional.attention_mod_qkv for these sequences (equal ones: [n] * batch)."""
         key, cuda = (tuple(seqlens), packed_mask is not None, str(device)), torch.device(device).type == "cuda"
         capturing = cuda and torch.cuda.is_current_stream_capturing()
-        p = self._plans.get(key)
+        p, home = self._plans.get(key, (None, None))
         if p is None:
             p = self._build(list(seqlens), device, packed_mask, capturing)
             if capturing and self.prefix:      # a node of this graph fills the prefix at every replay: a plan for this graph alone
                 return p
             if len(self._plans) - len(self._captured) >= 16:      # layouts seen lately, not every one ever seen; a captured graph keeps reading its own
                 self._plans = {k: v for k, v in self._plans.items() if k in self._captured}
-            self._plans[key] = p
+            home = torch.cuda.current_stream(device) if cuda and torch.cuda.is_available() else None
+            self._plans[key] = (p, home)
         if capturing:
             self._captured.add(key)
+        elif home is not None and torch.cuda.current_stream(device) != home:
+            # what a plan holds was copied from the host and is complete on every stream; given up, its memory waits for this one too
+            mod = p["mod"]
+            for t in (mod.slopes, mod.pos_q, mod.prefix, *(p.get(n) for n in ("table", "pos", "cu_q"))):
+                if t is not None:
+                    t.record_stream(torch.cuda.current_stream(device))
         return p
 
     def _build(self, seqlens, device, packed_mask, capturing: bool) -> dict:

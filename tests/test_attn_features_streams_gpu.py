@@ -62,3 +62,19 @@ def test_a_plan_built_on_one_stream_is_complete_on_another():
     torch.cuda.synchronize()
     assert torch.equal(got, want)
 
+
+@torch.no_grad()
+def test_memory_of_a_plan_given_up_waits_for_the_streams_that_read_it():
+    attn, qkv, want = setup()
+    side = torch.cuda.Stream()
+    attn.features.plan([N] * 2, qkv.device)
+    torch.cuda.synchronize()
+    keep_busy(side)
+    with torch.cuda.stream(side):
+        got = AF.attention_features(attn, qkv)
+    attn.features.prefix = 1        # what later plans write into memory that comes free
+    for n in range(100, 120):
+        attn.features.plan([n] * 2, qkv.device)
+    held = small_blocks(0)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and len(held) == 64
