@@ -63,11 +63,11 @@ class AttnFeatures:
                 return p
             if len(self._plans) - len(self._captured) >= 16:      # layouts seen lately, not every one ever seen; a captured graph keeps reading its own
                 self._plans = {k: v for k, v in self._plans.items() if k in self._captured}
-            home = torch.cuda.current_stream(device) if cuda and torch.cuda.is_available() else None
+            home = torch.cuda.current_stream(device).cuda_stream if cuda and torch.cuda.is_available() else None      # (a number: modules are copied and stored)
             self._plans[key] = (p, home)
         if capturing:
             self._captured.add(key)
-        elif home is not None and torch.cuda.current_stream(device) != home:
+        elif home is not None and torch.cuda.current_stream(device).cuda_stream != home:
             # what a plan holds was copied from the host and is complete on every stream; given up, its memory waits for this one too
             mod = p["mod"]
             for t in (mod.slopes, mod.pos_q, mod.prefix, *(p.get(n) for n in ("table", "pos", "cu_q"))):

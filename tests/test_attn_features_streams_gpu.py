@@ -1,4 +1,7 @@
 """Plans of attention features (attn_features.py) that several streams and captured graphs share."""
+import copy
+import io
+
 import pytest
 import torch
 
@@ -78,3 +81,11 @@ def test_memory_of_a_plan_given_up_waits_for_the_streams_that_read_it():
     held = small_blocks(0)
     torch.cuda.synchronize()
     assert torch.equal(got, want) and len(held) == 64
+
+
+@torch.no_grad()
+def test_modules_with_plans_are_copied_and_stored():
+    attn, qkv, want = setup()
+    AF.attention_features(attn, qkv)
+    assert torch.equal(AF.attention_features(copy.deepcopy(attn), qkv), want)
+    torch.save(attn, io.BytesIO())
