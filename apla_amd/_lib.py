@@ -91,6 +91,7 @@ SIGNATURES = {
     "apla_qk_norm_rotary_bwd": (c_int, [c_void_p, c_long, c_void_p, c_long, c_void_p, c_long, c_int, c_int, c_int, c_int, c_float, c_void_p,
                                         c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_long, c_void_p]),
     "apla_attn_mod_workspace_bytes": (c_long, [ctypes.POINTER(AttnMod), c_int]),
+    "apla_attn_mod_few_rows": (c_int, [ctypes.POINTER(AttnMod)]),
     "apla_attn_mod_fwd": (c_int, [ctypes.POINTER(AttnMod), c_void_p]),
     "apla_attn_mod_bwd": (c_int, [ctypes.POINTER(AttnMod), c_void_p]),
     "apla_attn_probs_dropout": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_float, c_ulonglong, c_uint, c_void_p]),

@@ -1447,6 +1447,11 @@ extern "C" long apla_attn_mod_workspace_bytes(const apla_attn_mod_t* p, int back
   return plan_of(*p, backward != 0).bytes;
 }
 
+extern "C" int apla_attn_mod_few_rows(const apla_attn_mod_t* p) {
+  if (apla_attn_mod_workspace_bytes(p, 0) < 0) return -1;
+  return plan_of(*p, false).rows ? 1 : 0;
+}
+
 extern "C" int apla_attn_mod_fwd(const apla_attn_mod_t* p, hipStream_t stream) {
   const int rc = mod_check("apla_attn_mod_fwd", p, false);
   if (rc != APLA_OK) return rc;

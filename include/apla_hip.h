@@ -345,6 +345,9 @@ typedef struct {
   float scale, softcap;
 } apla_attn_mod_t;
 long apla_attn_mod_workspace_bytes(const apla_attn_mod_t* p, int backward);
+/* Host query: 1 where the forward takes the form for few rows (16 rows of a key head's group, keys split over workgroups), 0 where it takes 128-row
+ * blocks, -1 for arguments without sizes. */
+int apla_attn_mod_few_rows(const apla_attn_mod_t* p);
 int apla_attn_mod_fwd(const apla_attn_mod_t* p, hipStream_t stream);
 int apla_attn_mod_bwd(const apla_attn_mod_t* p, hipStream_t stream);
 
