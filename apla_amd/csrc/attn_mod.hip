@@ -10,7 +10,7 @@
 //
 // The products are those of attention.hip (S^T = K Q^T with the query row on the lane, P^T from the accumulator as the next operand).
 // In a masked tile a weight of zero times a non-finite value is zero (poison_bits): what stands in masked places never matters.
-// P and dS are rounded to 16 bits as MFMA operands (half a step of values <= 256 resp. of dS, relative); scores, softmax
+// P and dS are rounded to 16 bits as MFMA operands (half a step of values <= 256 resp. of dS, relative; fp16 over many keys: see LIFT); scores, softmax
 // statistics, sums and accumulators are fp32.  A row's dS add up to 0, so over few keys their roundings weigh more than the result's own: sequences of up to
 // 64 tokens, a single tile, multiply what the rounding left of dS too (in all masked tiles that costs 5 to 13 % of the long cases' backward).
 //
@@ -48,6 +48,17 @@ struct ModArgs {
   int sq, sk;                           // workgroups that share a block's tiles
   int nsplit, chunk, nrt;
 };
+
+// fp16: P of n keys is about 1 / n, below its normal range (2^-14) from some thousand keys on, where operands would lose bits (errors of 1.4e-3 at 50 000 equal
+// weights, 1e-2 at 2^20).  The backward lifts P, and dS with it, by 2^lift through the exponent's subtrahend and takes it out of the stored results: weights down to
+// 1 / (4 n) keep the type's precision.  What is then too large for a dS in fp16 shows as a result that is not finite, and the workgroup starts again without.
+#if defined(APLA_FP16)
+constexpr bool LIFT = true;
+#else
+constexpr bool LIFT = false;
+#endif
+constexpr int LIFT_FROM = 4096;         // up to here 1 / (4 n) is a normal number
+__device__ __forceinline__ int lift_of(int nk) { return LIFT && nk > LIFT_FROM ? 20 - __builtin_clz((unsigned)nk - 1u) : 0; }     // ceil(log2(nk / 4096))
 
 struct MSeq { long q0, k0; int nq, nk, off, pre; };
 // Offsets that do not fit the tensors are cut to them, so no access leaves the tensors whatever the device-side arrays hold.
@@ -528,11 +539,29 @@ static inline int unit_parts(long units) { return units % 8 == 0 ? 1 : units % 4
 static inline long unit_grid(long units, int np, long per) { return units * np * ((per + np - 1) / np); }
 
 // a transposed accumulator pair (store_acc_T's layout) as fp32 partial sums of one split
-__device__ __forceinline__ void store_part(const f32x16 (&acc)[2], float* rowptr, int h) {
+template <bool MUL>
+__device__ __forceinline__ void store_part(const f32x16 (&acc)[2], float* rowptr, int h, float mul) {
 #pragma unroll
   for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) *(f32x4*)(rowptr + 32 * dt + 8 * g + 4 * h) = f32x4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+    for (int g = 0; g < 4; ++g) {
+      f32x4 v = {acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+      if constexpr (MUL) v *= mul;
+      *(f32x4*)(rowptr + 32 * dt + 8 * g + 4 * h) = v;
+    }
+}
+// does any wave of the workgroup hold infinities or NaN?  (all threads call it; buf: 4 ints that nobody else uses meanwhile)
+__device__ __forceinline__ bool overflowed(const f32x16 (&a)[2], const f32x16 (&b)[2], int* buf, int wave, int lane) {
+  unsigned r = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    r |= (unsigned)!(fabsf(a[i >> 4][i & 15]) < INFINITY) | (unsigned)!(fabsf(b[i >> 4][i & 15]) < INFINITY);
+  const bool any = __ballot(r != 0) != 0;
+  if (lane == 0) buf[wave] = any;
+  __syncthreads();
+  const int all = buf[0] | buf[1] | buf[2] | buf[3];
+  __syncthreads();
+  return uniform(all != 0);
 }
 
 // what a lane knows of its query row
@@ -985,7 +1014,7 @@ __global__ __launch_bounds__(256, CAP && (DOCS || BIAS) ? 2 : 3) void attn_mod_d
     delta += __shfl_xor(delta, 32, 64);
   }
   const float ls = a.lse[stat];
-  const float L2 = ls == -INFINITY ? -NEG_BIG : ls * LOG2E;
+  float L2 = ls == -INFINITY ? -NEG_BIG : ls * LOG2E;
   if constexpr (CAP) delta *= 4.f;         // (as dscore takes it; the dK/dV kernel reads it so)
   if (sp == 0 && qr < m.nq && h2 == 0) a.delta[stat] = delta;
   const RowCtx r = row_ctx<BIAS>(a, m, qi, h);
@@ -1003,57 +1032,64 @@ __global__ __launch_bounds__(256, CAP && (DOCS || BIAS) ? 2 : 3) void attn_mod_d
   }
   if (CAP && a.fine) lim0 = wlim0 = 0;
   f32x16 acc[2];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) { acc[0][i] = 0.f; acc[1][i] = 0.f; }
-  unsigned poison = 0;
+  unsigned poison;
   const bf16 *kb = a.k + m.k0 * a.ldk + (hk) * 64, *vb = a.v + m.k0 * a.ldv + (hk) * 64;
   const unsigned offk = dma_off(a.ldk, tid), offv = dma_off(a.ldv, tid);
   const int ntiles = (lim + 63) / 64;
-  for (int t0 = 0; t0 < ntiles; t0 = DOCS ? t0 + LIST : ntiles) {
-    int n = __builtin_amdgcn_readfirstlane(ntiles);
-    if constexpr (DOCS) n = build_list(list, buf, t0, ntiles, 0, lim0 / 64, a.rng_k + (long)(w.unit / Hkv) * a.nt_k, dlo, dhi, tid);
-    // entry e of the tiles to visit (past the last: the last): from the list, or simply tile e
-    auto entry = [&](int e) -> TileRef {
-      e = min(e, n - 1);
-      if constexpr (DOCS) return list[e];
-      else return TileRef{e, 0, 0, e < lim0 / 64};
-    };
-    auto known = [&](const TileRef& x) -> TileRef { return DOCS ? scalar_ref(x) : x; };
-    auto fetch = [&](char* tile, int t) {
-      dma_tile(tile, kb, a.ldk, offk, t * 64, m.nk, tid, wave);
-      dma_tile(tile + 8192, vb, a.ldv, offv, t * 64, m.nk, tid, wave);
-      dma_side<BIAS, DOCS>(tile, a, m, t * 64, lane, wave);
-    };
-    const int each = (n + a.sq - 1) / a.sq, e0 = min(n, sp * each), e1 = min(n, e0 + each);      // this split's part of the list
-    TileRef cur, next;
-    if (e0 < e1) {
-      cur = known(entry(e0)); next = known(entry(e0 + 1));
-      fetch(smem, cur.t);
-    }
-    tile_ready();
-    for (int e = e0; e < e1; ++e) {      // tile e is in LDS, e + 1 on its way to the other half
-      char *tile = smem + ((e - e0) & 1) * KT_BYTES, *other = smem + ((e + 1 - e0) & 1) * KT_BYTES;
-      const TileRef ahead = entry(e + 2);
-      if (e + 1 < e1) fetch(other, next.t);
-      const int j0 = cur.t * 64;
-      const bool odd = !cur.whole && tile_odd(tile + 0, lane);
-      if (__builtin_expect(odd, 0)) {
-        clean_tile(tile + 0, clean, tid);
-        __syncthreads();
+  int lift = lift_of(m.nk);
+  L2 -= lift;
+  for (;; L2 += lift, lift = 0) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) { acc[0][i] = 0.f; acc[1][i] = 0.f; }
+    poison = 0;
+    for (int t0 = 0; t0 < ntiles; t0 = DOCS ? t0 + LIST : ntiles) {
+      int n = __builtin_amdgcn_readfirstlane(ntiles);
+      if constexpr (DOCS) n = build_list(list, buf, t0, ntiles, 0, lim0 / 64, a.rng_k + (long)(w.unit / Hkv) * a.nt_k, dlo, dhi, tid);
+      // entry e of the tiles to visit (past the last: the last): from the list, or simply tile e
+      auto entry = [&](int e) -> TileRef {
+        e = min(e, n - 1);
+        if constexpr (DOCS) return list[e];
+        else return TileRef{e, 0, 0, e < lim0 / 64};
+      };
+      auto known = [&](const TileRef& x) -> TileRef { return DOCS ? scalar_ref(x) : x; };
+      auto fetch = [&](char* tile, int t) {
+        dma_tile(tile, kb, a.ldk, offk, t * 64, m.nk, tid, wave);
+        dma_tile(tile + 8192, vb, a.ldv, offv, t * 64, m.nk, tid, wave);
+        dma_side<BIAS, DOCS>(tile, a, m, t * 64, lane, wave);
+      };
+      const int each = (n + a.sq - 1) / a.sq, e0 = min(n, sp * each), e1 = min(n, e0 + each);      // this split's part of the list
+      TileRef cur, next;
+      if (e0 < e1) {
+        cur = known(entry(e0)); next = known(entry(e0 + 1));
+        fetch(smem, cur.t);
       }
-      if (active && j0 < wlim1 && (!docs || (cur.hi >= max(wlo, 0) && cur.lo <= whi))) {
-        const bool masked = !cur.whole && !(j0 + 64 <= wlim0 && (!docs || (cur.lo == cur.hi && wlo == cur.lo && whi == cur.lo)));
-        dq_tile<CAP, BIAS>(acc, poison, qf, df, L2, delta, a, r, tile, clean, j0, lane, fr, masked, docs, masked && odd, m.nk <= 64);
-      }
-      cur = next;
-      next = known(ahead);
       tile_ready();
+      for (int e = e0; e < e1; ++e) {      // tile e is in LDS, e + 1 on its way to the other half
+        char *tile = smem + ((e - e0) & 1) * KT_BYTES, *other = smem + ((e + 1 - e0) & 1) * KT_BYTES;
+        const TileRef ahead = entry(e + 2);
+        if (e + 1 < e1) fetch(other, next.t);
+        const int j0 = cur.t * 64;
+        const bool odd = !cur.whole && tile_odd(tile + 0, lane);
+        if (__builtin_expect(odd, 0)) {
+          clean_tile(tile + 0, clean, tid);
+          __syncthreads();
+        }
+        if (active && j0 < wlim1 && (!docs || (cur.hi >= max(wlo, 0) && cur.lo <= whi))) {
+          const bool masked = !cur.whole && !(j0 + 64 <= wlim0 && (!docs || (cur.lo == cur.hi && wlo == cur.lo && whi == cur.lo)));
+          dq_tile<CAP, BIAS>(acc, poison, qf, df, L2, delta, a, r, tile, clean, j0, lane, fr, masked, docs, masked && odd, m.nk <= 64);
+        }
+        cur = next;
+        next = known(ahead);
+        tile_ready();
+      }
     }
+    if (!LIFT || lift == 0 || !overflowed(acc, acc, buf, wave, lane)) break;
   }
+  const float unlift = LIFT ? __builtin_ldexpf(1.f, -lift) : 1.f;
   apply_poison(acc, poison);
   if (qr < m.nq) {
-    if (a.sq == 1) store_acc_T(acc, a.dq + (m.q0 + qr) * a.lddq + h * 64, h2, a.scale);
-    else store_part(acc, a.part_q + (((long)sp * a.Tq + m.q0 + qr) * a.Hq + h) * 64, h2);
+    if (a.sq == 1) store_acc_T(acc, a.dq + (m.q0 + qr) * a.lddq + h * 64, h2, a.scale * unlift);
+    else store_part<LIFT>(acc, a.part_q + (((long)sp * a.Tq + m.q0 + qr) * a.Hq + h) * 64, h2, unlift);
   }
 }
 
@@ -1113,13 +1149,14 @@ __device__ __forceinline__ void dkdv_tile(f32x16 (&dk)[2], f32x16 (&dv)[2], unsi
   }
 }
 
-template <bool CAP, int BIAS, bool DOCS>
+// LONG (fp16 only): sequences whose weights are lifted.  Its second pass costs registers and the order of the products: 12 heads of 8192 causal rows 304 us against 290
+// without, so shorter sequences run without it.
+template <bool CAP, int BIAS, bool DOCS, bool LONG = false>
 __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
   __shared__ __attribute__((aligned(128))) char smem[2 * QT_BYTES], clean[16384];
   __shared__ TileRef list[DOCS ? LIST : 1];
   __shared__ int buf[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5;
-  const Frag fr = frag_consts(lane);
   const Where w = where(a, a.nblk * a.sk);
   if (w.j >= a.nblk * a.sk) return;
   const int Hkv = a.Hq / a.G, hk = w.unit % Hkv, sp = w.j % a.sk;
@@ -1142,114 +1179,124 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
     dlo = wlo; dhi = whi;
     group_range(dlo, dhi, none0, none1, buf, wave, lane);
   }
-  unsigned pk = 0, pv = 0;
-  const unsigned offq = stage_off(a.ldq, tid), offd = stage_off(a.lddo, tid);
+  unsigned pk, pv;
   f32x16 dk[2], dv[2];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) { dk[0][i] = dk[1][i] = 0.f; dv[0][i] = dv[1][i] = 0.f; }
   // query tiles that can see key jb: rows i with lim_i > jb, a suffix of the rows (all of them if the prefix reaches jb)
   const int first = m.nq == 0 ? 0 : (!a.causal || m.pre > jb) ? 0 : max(0, jb - m.off) / 64;
   const int ntiles = (m.nq + 63) / 64;
   // whole tiles: every row of theirs sees all 128 keys, all of them rows and keys of the sequence
   const int jlast = jb + 127;
   const int w0 = jlast >= m.nk ? ntiles : (!a.causal || m.pre > jlast) ? 0 : (max(0, jlast - m.off) + 63) / 64, w1 = CAP && a.fine ? 0 : m.nq / 64;
-  for (int t0 = first; t0 < ntiles; t0 = DOCS ? t0 + LIST : ntiles) {
-    int n = ntiles - first;
-    if constexpr (DOCS) n = build_list(list, buf, t0, ntiles, w0, w1, a.rng_q + (long)(w.unit / Hkv) * a.nt_q, dlo, dhi, tid);
-    auto entry = [&](int e) -> TileRef {       // e < n
-      if constexpr (DOCS) return list[e];
-      else return TileRef{first + e, 0, 0, first + e >= w0 && first + e < w1};
-    };
-    auto known = [&](const TileRef& x) -> TileRef { return DOCS ? scalar_ref(x) : x; };
-    const int each = (n * a.G + a.sk - 1) / a.sk, x0 = min(n * a.G, sp * each), total = min(n * a.G, x0 + each) - x0;      // this split's part
-    Stage qs, os;
-    QuerySide sd;
-    auto fetch = [&](int t, int g) {      // a query tile of head g of the group
-      const int h = hk * a.G + g, i0 = t * 64;
-      stage_load(qs, a.q + m.q0 * a.ldq + h * 64, a.ldq, offq, i0, m.nq, tid);
-      stage_load(os, a.d_o + m.q0 * a.lddo + h * 64, a.lddo, offd, i0, m.nq, tid);
-      if (tid < 64) {
-        const int i = min(i0 + tid, m.nq - 1);
-        const long stat = (long)h * a.Tq + m.q0 + i;
-        const float ls = a.lse[stat];
-        sd.L2 = ls == -INFINITY ? -NEG_BIG : ls * LOG2E;
-        sd.delta = a.delta[stat];
-        float p[2] = {0.f, 0.f};
-        row_pos<BIAS>(p, a.pos_q, m.q0 + i, i + m.off);
-        sd.x = p[0]; sd.y = p[1];
-        sd.doc = a.doc_q ? a.doc_q[m.q0 + i] : 0;
-        sd.lim = i0 + tid < m.nq && sd.doc >= 0 ? row_lim(a, m, i) : 0;
+  int lift = LONG ? lift_of(m.nk) : 0;
+  int tid_ = tid;
+  for (;; lift = 0) {
+    if constexpr (LONG) asm volatile("" : "+v"(tid_));       // (what follows from the lane is formed again: hipcc would keep it in registers over both passes)
+    const int tid = tid_, lane = tid & 63;
+    const Frag fr = frag_consts(lane);
+    const unsigned offq = stage_off(a.ldq, tid), offd = stage_off(a.lddo, tid);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) { dk[0][i] = dk[1][i] = 0.f; dv[0][i] = dv[1][i] = 0.f; }
+    pk = pv = 0;
+    for (int t0 = first; t0 < ntiles; t0 = DOCS ? t0 + LIST : ntiles) {
+      int n = ntiles - first;
+      if constexpr (DOCS) n = build_list(list, buf, t0, ntiles, w0, w1, a.rng_q + (long)(w.unit / Hkv) * a.nt_q, dlo, dhi, tid);
+      auto entry = [&](int e) -> TileRef {       // e < n
+        if constexpr (DOCS) return list[e];
+        else return TileRef{first + e, 0, 0, first + e >= w0 && first + e < w1};
+      };
+      auto known = [&](const TileRef& x) -> TileRef { return DOCS ? scalar_ref(x) : x; };
+      const int each = (n * a.G + a.sk - 1) / a.sk, x0 = min(n * a.G, sp * each), total = min(n * a.G, x0 + each) - x0;      // this split's part
+      Stage qs, os;
+      QuerySide sd;
+      auto fetch = [&](int t, int g) {      // a query tile of head g of the group
+        const int h = hk * a.G + g, i0 = t * 64;
+        stage_load(qs, a.q + m.q0 * a.ldq + h * 64, a.ldq, offq, i0, m.nq, tid);
+        stage_load(os, a.d_o + m.q0 * a.lddo + h * 64, a.lddo, offd, i0, m.nq, tid);
+        if (tid < 64) {
+          const int i = min(i0 + tid, m.nq - 1);
+          const long stat = (long)h * a.Tq + m.q0 + i;
+          const float ls = a.lse[stat];
+          sd.L2 = ls == -INFINITY ? -NEG_BIG : LONG ? ls * LOG2E - lift : ls * LOG2E;
+          sd.delta = a.delta[stat];
+          float p[2] = {0.f, 0.f};
+          row_pos<BIAS>(p, a.pos_q, m.q0 + i, i + m.off);
+          sd.x = p[0]; sd.y = p[1];
+          sd.doc = a.doc_q ? a.doc_q[m.q0 + i] : 0;
+          sd.lim = i0 + tid < m.nq && sd.doc >= 0 ? row_lim(a, m, i) : 0;
+        }
+      };
+      auto put = [&](char* tile, bool whole) {
+        stage_store(qs, tile, tid);
+        stage_store(os, tile + 8192, tid);
+        if (tid < 64) {
+          *(float*)(tile + QT_L + tid * 4) = sd.L2;
+          *(float*)(tile + QT_D + tid * 4) = sd.delta;
+          if constexpr (BIAS > 0) *(float*)(tile + QT_X + tid * 4) = sd.x;
+          if constexpr (BIAS > 1) *(float*)(tile + QT_Y + tid * 4) = sd.y;
+          *(int*)(tile + QT_LIM + tid * 4) = sd.lim;
+          *(int*)(tile + QT_DOC + tid * 4) = sd.doc;
+        }
+        if (!whole) {
+          const bool odd = stage_odd(qs) || stage_odd(os);
+          if (lane == 0) *(int*)(tile + QT_ODD + wave * 4) = odd;
+        }
+      };
+      // entry e of head g is in LDS, the next in registers; the one behind that, e2 of head g2, is requested when those are free
+      TileRef cur, next;
+      int e = n ? x0 % n : 0, g = n ? x0 / n : 0, e2 = e, g2 = g, t2 = 0;
+      auto step = [&](int& e_, int& g_) { if (++e_ == n) { e_ = 0; ++g_; } };
+      if (total > 0) {
+        cur = known(entry(e2));
+        step(e2, g2);
+        next = known(entry(e2));
+        fetch(cur.t, g);
+        put(smem, cur.whole);
+        if (total > 1) fetch(next.t, g2);
+        step(e2, g2);
+        t2 = known(entry(e2)).t;
       }
-    };
-    auto put = [&](char* tile, bool whole) {
-      stage_store(qs, tile, tid);
-      stage_store(os, tile + 8192, tid);
-      if (tid < 64) {
-        *(float*)(tile + QT_L + tid * 4) = sd.L2;
-        *(float*)(tile + QT_D + tid * 4) = sd.delta;
-        if constexpr (BIAS > 0) *(float*)(tile + QT_X + tid * 4) = sd.x;
-        if constexpr (BIAS > 1) *(float*)(tile + QT_Y + tid * 4) = sd.y;
-        *(int*)(tile + QT_LIM + tid * 4) = sd.lim;
-        *(int*)(tile + QT_DOC + tid * 4) = sd.doc;
-      }
-      if (!whole) {
-        const bool odd = stage_odd(qs) || stage_odd(os);
-        if (lane == 0) *(int*)(tile + QT_ODD + wave * 4) = odd;
-      }
-    };
-    // entry e of head g is in LDS, the next in registers; the one behind that, e2 of head g2, is requested when those are free
-    TileRef cur, next;
-    int e = n ? x0 % n : 0, g = n ? x0 / n : 0, e2 = e, g2 = g, t2 = 0;
-    auto step = [&](int& e_, int& g_) { if (++e_ == n) { e_ = 0; ++g_; } };
-    if (total > 0) {
-      cur = known(entry(e2));
-      step(e2, g2);
-      next = known(entry(e2));
-      fetch(cur.t, g);
-      put(smem, cur.whole);
-      if (total > 1) fetch(next.t, g2);
-      step(e2, g2);
-      t2 = known(entry(e2)).t;
-    }
-    __syncthreads();
-    for (int x = 0; x < total; ++x) {
-      char* tile = smem + (x & 1) * QT_BYTES;
-      const TileRef ahead = entry(e2);
-      const int gn = g2;
-      step(e2, g2);
-      const int t3 = entry(e2).t;
-      const int i0 = cur.t * 64, jw = jb + wave * 32, last = min(i0 + 63, m.nq - 1);
-      const bool odd = !cur.whole && any_odd(tile + QT_ODD);
-      if (__builtin_expect(odd, 0)) {
-        clean_tile(tile, clean, tid);
-        clean_tile(tile + 8192, clean + 8192, tid);
+      __syncthreads();
+      for (int x = 0; x < total; ++x) {
+        char* tile = smem + (x & 1) * QT_BYTES;
+        const TileRef ahead = entry(e2);
+        const int gn = g2;
+        step(e2, g2);
+        const int t3 = entry(e2).t;
+        const int i0 = cur.t * 64, jw = jb + wave * 32, last = min(i0 + 63, m.nq - 1);
+        const bool odd = !cur.whole && any_odd(tile + QT_ODD);
+        if (__builtin_expect(odd, 0)) {
+          clean_tile(tile, clean, tid);
+          clean_tile(tile + 8192, clean + 8192, tid);
+          __syncthreads();
+        }
+        if (active && row_lim(a, m, last) > jw && (!docs || (cur.hi >= max(wlo, 0) && cur.lo <= whi))) {
+          const float slope = BIAS ? a.slopes[hk * a.G + g] * LOG2E : 0.f;
+          const bool masked = !cur.whole && !(!(CAP && a.fine) && i0 + 64 <= m.nq && jw + 32 <= m.nk && row_lim(a, m, i0) >= jw + 32 &&
+                                                     (!docs || (cur.lo >= 0 && cur.lo == cur.hi && wlo == cur.lo && whi == cur.lo)));
+          dkdv_tile<CAP, BIAS>(dk, dv, pk, pv, kf, vf, a, j, docj, pj, slope, tile, clean, lane, fr, masked, docs, masked && odd, m.nq <= 64);
+        }
+        if (x + 1 < total) put(smem + ((x + 1) & 1) * QT_BYTES, next.whole);
+        if (x + 2 < total) fetch(t2, gn);
+        step(e, g);
+        cur = next;
+        next = known(ahead);
+        t2 = DOCS ? __builtin_amdgcn_readfirstlane(t3) : t3;
         __syncthreads();
       }
-      if (active && row_lim(a, m, last) > jw && (!docs || (cur.hi >= max(wlo, 0) && cur.lo <= whi))) {
-        const float slope = BIAS ? a.slopes[hk * a.G + g] * LOG2E : 0.f;
-        const bool masked = !cur.whole && !(!(CAP && a.fine) && i0 + 64 <= m.nq && jw + 32 <= m.nk && row_lim(a, m, i0) >= jw + 32 &&
-                                                   (!docs || (cur.lo >= 0 && cur.lo == cur.hi && wlo == cur.lo && whi == cur.lo)));
-        dkdv_tile<CAP, BIAS>(dk, dv, pk, pv, kf, vf, a, j, docj, pj, slope, tile, clean, lane, fr, masked, docs, masked && odd, m.nq <= 64);
-      }
-      if (x + 1 < total) put(smem + ((x + 1) & 1) * QT_BYTES, next.whole);
-      if (x + 2 < total) fetch(t2, gn);
-      step(e, g);
-      cur = next;
-      next = known(ahead);
-      t2 = DOCS ? __builtin_amdgcn_readfirstlane(t3) : t3;
-      __syncthreads();
     }
+    if (!LONG || lift == 0 || !overflowed(dk, dv, buf, wave, lane)) break;
   }
+  const float unlift = LONG ? __builtin_ldexpf(1.f, -lift) : 1.f;
   apply_poison(dk, pk);
   apply_poison(dv, pv);
   if (jr < m.nk) {
     if (a.sk == 1) {
-      store_acc_T(dk, a.dk + (m.k0 + jr) * a.lddk + hk * 64, h2, a.scale);
-      store_acc_T(dv, a.dv + (m.k0 + jr) * a.lddv + hk * 64, h2, 1.f);
+      store_acc_T(dk, a.dk + (m.k0 + jr) * a.lddk + hk * 64, h2, a.scale * unlift);
+      store_acc_T(dv, a.dv + (m.k0 + jr) * a.lddv + hk * 64, h2, unlift);
     } else {
       float* p = a.part_k + (((long)sp * a.Tk + m.k0 + jr) * Hkv + hk) * 64;
-      store_part(dk, p, h2);
-      store_part(dv, p + (long)a.sk * a.Tk * Hkv * 64, h2);
+      store_part<LONG>(dk, p, h2, unlift);
+      store_part<LONG>(dv, p + (long)a.sk * a.Tk * Hkv * 64, h2, unlift);
     }
   }
 }
@@ -1434,10 +1481,10 @@ void launch_ranges(const ModArgs& a, bool queries, hipStream_t stream) {
       else hipLaunchKernelGGL((KERNEL<false, 2 __VA_ARGS__>), grid, dim3(256), 0, stream, a);                     \
     }                                                                                                             \
   } while (0)
-#define APLA_MOD_LAUNCH_DOCS(KERNEL, grid)                                                                        \
+#define APLA_MOD_LAUNCH_DOCS(KERNEL, grid, ...)                                                                   \
   do {                                                                                                            \
-    if (a.doc_k) APLA_MOD_LAUNCH(KERNEL, grid, , true);                                                           \
-    else APLA_MOD_LAUNCH(KERNEL, grid, , false);                                                                  \
+    if (a.doc_k) APLA_MOD_LAUNCH(KERNEL, grid, , true __VA_ARGS__);                                               \
+    else APLA_MOD_LAUNCH(KERNEL, grid, , false __VA_ARGS__);                                                      \
   } while (0)
 
 }  // namespace
@@ -1467,7 +1514,7 @@ extern "C" int apla_attn_mod_fwd(const apla_attn_mod_t* p, hipStream_t stream) {
   } else {
     a.nblk = (p->max_q + 127) / 128;
     const dim3 grid((unsigned)unit_grid(units, a.np, (long)a.G * a.nblk));
-    APLA_MOD_LAUNCH_DOCS(attn_mod_fwd_kernel, grid);
+    APLA_MOD_LAUNCH_DOCS(attn_mod_fwd_kernel, grid, );
   }
   APLA_CHECK_LAUNCH("apla_attn_mod_fwd");
   return APLA_OK;
@@ -1489,7 +1536,7 @@ extern "C" int apla_attn_mod_bwd(const apla_attn_mod_t* p, hipStream_t stream) {
   a.nblk = (p->max_q + 127) / 128;
   {
     const dim3 grid((unsigned)unit_grid(units, a.np, (long)a.G * a.nblk * a.sq));
-    APLA_MOD_LAUNCH_DOCS(attn_mod_dq_kernel, grid);
+    APLA_MOD_LAUNCH_DOCS(attn_mod_dq_kernel, grid, );
     if (a.sq > 1)
       hipLaunchKernelGGL(attn_mod_sum_kernel, dim3((unsigned)((p->max_q + 31) / 32), (unsigned)p->Hq, (unsigned)p->S), dim3(256), 0, stream, a, (const float*)a.part_q, a.sq, 1, p->Hq,
                          (SumOut{a.dq, a.lddq, a.scale}), (SumOut{}));
@@ -1497,7 +1544,11 @@ extern "C" int apla_attn_mod_bwd(const apla_attn_mod_t* p, hipStream_t stream) {
   a.nblk = (p->max_k + 127) / 128;
   {
     const dim3 grid((unsigned)unit_grid(units, a.np, (long)a.nblk * a.sk));
-    APLA_MOD_LAUNCH_DOCS(attn_mod_dkdv_kernel, grid);
+#if defined(APLA_FP16)
+    if (p->max_k > LIFT_FROM) APLA_MOD_LAUNCH_DOCS(attn_mod_dkdv_kernel, grid, , true);
+    else
+#endif
+      APLA_MOD_LAUNCH_DOCS(attn_mod_dkdv_kernel, grid, );
     if (a.sk > 1)
       hipLaunchKernelGGL(attn_mod_sum_kernel, dim3((unsigned)((p->max_k + 31) / 32), 2u * (unsigned)p->Hkv, (unsigned)p->S), dim3(256), 0, stream, a, (const float*)a.part_k, a.sk, 0, p->Hkv,
                          (SumOut{a.dk, a.lddk, a.scale}), (SumOut{a.dv, a.lddv, 1.f}));
