@@ -22,7 +22,14 @@
 namespace {
 
 constexpr float NEG_BIG = -1e30f;       // running maximum before the first visible key: finite, so that masked scores give exp2(-inf) = 0
-constexpr float LAZY = 8.f;             // the running maximum follows only when a score exceeds it by 2^8: weights stay <= 256
+constexpr float LAZY = 8.f;             // the running maximum follows only when a score exceeds it by 2^8: weights stay <= 256 (times 2^FWD_LIFT)
+// fp16: weights of the forward are 2^FWD_LIFT times larger (at most 2^15), so that many small ones next to a large one, of 2^-14 .. 2^-21 of it, are normal numbers
+// too: 2^18 keys of weight 2^-20.6 beside one of weight 1 gave an output off by 5 %.  Statistics count in the same unit.
+#if defined(APLA_FP16)
+constexpr float FWD_LIFT = 7.f;
+#else
+constexpr float FWD_LIFT = 0.f;
+#endif
 constexpr int LIST = 256;               // tiles listed per pass (one per thread)
 
 struct ModArgs {
@@ -264,7 +271,16 @@ __device__ __forceinline__ float dist(const float (&p)[2], float x, float y) {
 // LDS of a key tile: K, V (8 KB each), positions [2][64], document ids [64]
 constexpr int KT_POS = 16384, KT_DOC = KT_POS + 512, KT_BYTES = KT_DOC + 256;
 
-struct RowState { float m, l; };
+struct RowState { float m, l; };       // m: the maximum that weights refer to, less FWD_LIFT
+// log of the sum l of weights that refer to m (log2 units); the lift is taken out before the logarithm, whose rounding would grow with it
+__device__ __forceinline__ float log_sum(float m, float l) {
+  if constexpr (FWD_LIFT > 0.f) return (m + FWD_LIFT + __builtin_amdgcn_logf(l * (1.f / 128.f))) * LN2;
+  return (m + __builtin_amdgcn_logf(l)) * LN2;
+}
+__device__ __forceinline__ float reference(float mx, float zm) {       // of scores up to mx, zm: their unit in log2 units
+  if constexpr (FWD_LIFT > 0.f) return mx - FWD_LIFT / zm;
+  return mx;
+}
 struct RowCtx { int lim, doc; float pos[2], slope; };       // slope in log2 units
 
 // cap tanh(s / cap) in log2 units: A (1 - 2 r), r = 1 / (1 + e^(2 s / cap)).  That is exact to 2^-23 A, which small scores feel relatively; cap_fine
@@ -383,8 +399,8 @@ __device__ __forceinline__ void fwd_tile(f32x16 (&acc)[2], RowState& st, unsigne
 #pragma unroll
     for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[kt][i]);
     mx = half_max(mx);
-    if (__ballot((mx - st.m) * zm > LAZY)) {
-      const float m_new = fmaxf(st.m, mx), alpha = __builtin_amdgcn_exp2f((st.m - m_new) * zm);
+    if (__ballot((mx - st.m) * zm > LAZY + FWD_LIFT)) {
+      const float m_new = fmaxf(st.m, reference(mx, zm)), alpha = __builtin_amdgcn_exp2f((st.m - m_new) * zm);
       st.m = m_new;
       st.l *= alpha;
 #pragma unroll
@@ -668,7 +684,7 @@ __global__ __launch_bounds__(256, CAP && (DOCS || BIAS) ? 2 : 3) void attn_mod_f
   if (qr < m.nq) {
     store_acc_T(acc, a.o + (m.q0 + qr) * a.ldo + h * 64, h2, l != 0.f ? 1.f / l : 0.f);
     if (h2 == 0)
-      a.lse[(long)h * a.Tq + m.q0 + qr] = l != 0.f ? (st.m * ((CAP || BIAS) ? 1.f : a.c) + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+      a.lse[(long)h * a.Tq + m.q0 + qr] = l != 0.f ? log_sum(st.m * ((CAP || BIAS) ? 1.f : a.c), l) : -INFINITY;
   }
 }
 
@@ -801,8 +817,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_rows_kernel(ModArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[b][e]);
       mx = quad_max(mx);
-      if (__ballot((mx - st.m) * zm > LAZY)) {
-        const float m_new = fmaxf(st.m, mx), alpha = __builtin_amdgcn_exp2f((st.m - m_new) * zm);
+      if (__ballot((mx - st.m) * zm > LAZY + FWD_LIFT)) {
+        const float m_new = fmaxf(st.m, reference(mx, zm)), alpha = __builtin_amdgcn_exp2f((st.m - m_new) * zm);
         st.m = m_new;
         st.l *= alpha;
 #pragma unroll
@@ -879,7 +895,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_rows_kernel(ModArgs a) {
   if (a.nsplit == 1) {
     const float inv = L != 0.f ? 1.f / L : 0.f;
     *(bf16x4*)(a.o + qo * a.ldo + ho * 64 + ch * 4) = pack4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-    if (ch == 0) a.lse[(long)ho * a.Tq + qo] = L != 0.f ? (M + __builtin_amdgcn_logf(L)) * LN2 : -INFINITY;
+    if (ch == 0) a.lse[(long)ho * a.Tq + qo] = L != 0.f ? log_sum(M, L) : -INFINITY;
   } else {
     const long p = ((((long)s * Hkv + hk) * a.nrt + rt) * a.nsplit + sp) * ROWS + row;
     *(f32x4*)(a.part_o + p * 64 + ch * 4) = x;
@@ -907,7 +923,7 @@ __global__ __launch_bounds__(256) void attn_mod_join_kernel(ModArgs a) {
   const long qo = m.q0 + ro / a.G;
   const float inv = L != 0.f ? 1.f / L : 0.f;
   *(bf16x4*)(a.o + qo * a.ldo + ho * 64 + ch * 4) = pack4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-  if (ch == 0) a.lse[(long)ho * a.Tq + qo] = L != 0.f ? (M + __builtin_amdgcn_logf(L)) * LN2 : -INFINITY;
+  if (ch == 0) a.lse[(long)ho * a.Tq + qo] = L != 0.f ? log_sum(M, L) : -INFINITY;
 }
 
 // ------------------------------------------------------------------------------------------------ backward

@@ -1,11 +1,11 @@
-"""fp16 over many keys: weights far below fp16's normal range (2^-14) keep its relative precision.
+"""fp16 over many keys: weights far below fp16's normal range (2^-14) keep its relative precision, forward and backward.
 
 u = 2^-11: half a step.  A weight or score gradient is rounded once (u), the result once more (u, 2^-25 absolute where it is below the normal range).  fp32 sums go by
 16 products at a time: n / 16 additions of half a step 2^-24 relative to their partial sums, statistics and exponentials 2^-18."""
 import pytest
 import torch
 
-from apla_amd import ops
+from apla_amd import _lib, ops
 from test_attn_mod_gpu import SCALE, rnd, within
 
 pytestmark = pytest.mark.gpu
@@ -84,3 +84,20 @@ def test_gradients_of_random_rows(nq, n, H):
     within(dk, wk, bk + U * wk.abs() + 2.0 ** -25, "dk")
     within(dv, wv, bv + U * wv.abs() + 2.0 ** -25, "dv")
 
+
+@pytest.mark.parametrize("H,nq", [(1, 1), (66, 1), (66, 3)])
+def test_forward_of_many_small_weights_next_to_a_large_one(H, nq):
+    """One key of weight 1 (value 0) and n of weight w = 2^-20.6 (value 1): o = n w / (1 + n w) though w is ten and a half of fp16's smallest steps."""
+    n = 1 << 18
+    q, k, v = torch.zeros(nq, H * 64), torch.zeros(n + 1, 64), torch.ones(n + 1, 64)
+    q[:, ::64], k[0, 0], v[0] = 16, 7.140625, 0
+    w = torch.exp(torch.tensor(-16 * 7.140625 * SCALE, dtype=torch.float64))
+    a = _lib.AttnMod()
+    a.S, a.Hq, a.Hkv, a.max_q, a.max_k = 1, H, 1, nq, n + 1
+    with ops.use_half(HALF):
+        assert _lib.lib().apla_attn_mod_few_rows(a) == (H == 1)
+        o, lse = ops.attn_mod_fwd(*(t.to(HALF).cuda() for t in (q, k, v)), H, 1, SCALE, batch=1)
+    want = float(n * w / (1 + n * w))
+    # a lane adds n / 2 weights one by one: half a step 2^-24 each, relative to the sum so far
+    assert float((o.double() - want).abs().max()) <= (2 * U + n / 2 * 2.0 ** -25 + f_of(n)) * want
+    assert float((lse.double() - float(torch.log1p(n * w)) - 16 * 7.140625 * SCALE).abs().max()) <= 2.0 ** -19 * 16 + n / 2 * 2.0 ** -25
