@@ -825,7 +825,8 @@ def qk_norm_rotary_bwd(dqk: torch.Tensor, qkv: torch.Tensor, Hq: int, Hkv: int, 
                        k_bias=None, eps: float = 1e-6, table: Optional[torch.Tensor] = None, layout: str = "half",
                        pos: Optional[torch.Tensor] = None, seq_len: int = 0, out: Optional[torch.Tensor] = None, want_params: bool = True):
     """Gradients of qk_norm_rotary_fwd: (d of the query / key columns [T, (Hq+Hkv)*64], fp32 [4, 64] = d q_weight, d k_weight, d q_bias,
-    d k_bias, or None without ``want_params``).  ``qkv``: the forward's input; ``out`` may be columns of a fused gradient buffer."""
+    d k_bias, or None without ``want_params``).  ``qkv``: the forward's input; ``out`` may be columns of a fused gradient buffer.  A head
+    whose gradient is all zero passes none on, whatever ``qkv`` holds there (masked places may hold infinities and NaN)."""
     x, ldx = _qk_rows(qkv, "qkv", Hq, Hkv)
     T, n = x.shape
     ldd = _strided_rows(dqk, "dqk", n, T)

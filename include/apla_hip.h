@@ -307,7 +307,7 @@ int apla_rotary(const void* x, long ldx, void* y, long ldy, int T, int heads, co
 /* Norm of every query and key head (LayerNorm or RMS norm over its 64 values, fp32 statistics; qw / qb for the first Hq heads of a row, kw /
  * kb for the Hkv behind them; NULL: 1 / 0), then the rotation above (rot 0: none), in one pass: the q_norm / k_norm modules of timm-style
  * attention (the host-model contract of apla_vit.py:17-37).  x: [T, >= (Hq + Hkv) * 64] rows, y: [T, (Hq + Hkv) * 64] rows.
- * Backward: dy, x -> dx (same columns); dparams [4][64] = d qw, d kw, d qb, d kb (fp32, overwritten; NULL: not wanted) through a
+ * Backward: dy, x -> dx (same columns; a head of zeros in dy gives zeros, whatever x holds there); dparams [4][64] = d qw, d kw, d qb, d kb (fp32, overwritten; NULL: not wanted) through a
  * workspace of apla_qk_norm_rotary_workspace_bytes().  Deterministic. */
 enum { APLA_NORM_LAYER = 1, APLA_NORM_RMS = 2 };
 long apla_qk_norm_rotary_workspace_bytes(void);
