@@ -770,7 +770,7 @@ def rotary_fwd(x: torch.Tensor, table: torch.Tensor, heads: int, *, layout: str 
 
 def rotary_bwd(dy: torch.Tensor, table: torch.Tensor, heads: int, *, layout: str = "half", pos: Optional[torch.Tensor] = None, seq_len: int = 0,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """The gradient of rotary_fwd with respect to x: dy turned back."""
+    """The gradient of rotary_fwd with respect to x: dy turned back (a head of zeros stays one, also where ``pos`` lies outside the table)."""
     return _rotary(dy, table, heads, layout, pos, seq_len, out, True, "rotary_bwd")
 
 

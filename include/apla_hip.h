@@ -299,7 +299,8 @@ int apla_attn_probs_dropout(const void* qkv, const float* lse, float* attn, int 
  * with row strides ldx / ldy (the query and key columns of a fused qkv activation are such a view; y may be x itself).  The first `rot` values
  * of every head are turned, pair i by the angle of table row `position`: table [P, rot] fp32 = cos of the rot / 2 angles, then their sin.
  * APLA_ROT_HALF pairs (i, i + rot / 2), APLA_ROT_INTERLEAVED (2i, 2i + 1); rot even, 0..64.  Position of row t: pos[t] if given, else
- * t % seq_len (seq_len 0: t).  A pos outside [0, P) makes the turned values of its row NaN.  inverse != 0 turns back: the backward pass. */
+ * t % seq_len (seq_len 0: t).  A pos outside [0, P) makes the turned values of its row NaN.  inverse != 0 turns back: the
+ * backward pass, in which a head of zeros stays one (padding behind a mask may stand anywhere). */
 enum { APLA_ROT_HALF = 0, APLA_ROT_INTERLEAVED = 1 };
 int apla_rotary(const void* x, long ldx, void* y, long ldy, int T, int heads, const float* table, int P, int rot, int layout,
                 const int32_t* pos, int seq_len, int inverse, hipStream_t stream);

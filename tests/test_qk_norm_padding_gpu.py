@@ -54,3 +54,29 @@ def test_padding_of_the_fused_node_may_hold_anything():
         o = AF.attention_mod_qkv(a, H, 0.125, mod=mod, q_norm=norms[0], k_norm=norms[1], table=R.rotary_table(T, 64, device="cuda"), batch=1)
         res.append((o, *torch.autograd.grad(o, [a] + par, do)))
     assert all(torch.equal(u, v) for u, v in zip(*res)) and bool((res[0][1][doc < 0] == 0).all())
+
+
+@pytest.mark.parametrize("norm", [False, True])
+def test_padding_may_stand_outside_the_table(norm):
+    """Padding tokens of position -1: NaN in their q and k, which the mask hides, and a gradient of 0."""
+    T, H = 90, 2
+    g = torch.Generator().manual_seed(3)
+    x, do = torch.randn(T, 3 * H * 64, generator=g).bfloat16().cuda(), torch.randn(T, H * 64, generator=g).bfloat16().cuda()
+    doc = torch.arange(T, dtype=torch.int32) // 31
+    doc[60:70] = doc[85:] = -1
+    doc, pos = doc.cuda(), torch.arange(T, dtype=torch.int32).cuda()
+    norms = [nn.RMSNorm(64).cuda() for _ in range(2)] if norm else [None, None]
+    par = [p for n in norms if norm for p in n.parameters()]
+    res = []
+    for p in (pos, torch.where(doc < 0, -1, pos).int()):
+        a = x.clone().requires_grad_(True)
+        o = AF.attention_mod_qkv(a, H, 0.125, mod=ops.ScoreMod(doc_q=doc, doc_k=doc), q_norm=norms[0], k_norm=norms[1], table=R.rotary_table(T, 64, device="cuda"), pos=p, batch=1)
+        res.append((o, *torch.autograd.grad(o, [a] + par, do)))
+    assert all(torch.equal(u, v) for u, v in zip(*res)) and bool((res[0][1][doc < 0] == 0).all())
+
+
+def test_a_position_outside_the_table_is_nan_in_gradients_that_arrive():
+    dy, pos = torch.randn(4, 128).bfloat16().cuda(), torch.tensor([0, 9, -1, 3], dtype=torch.int32, device="cuda")
+    dy[2, 64:] = 0
+    dx = ops.rotary_bwd(dy, R.rotary_table(8, 32, device="cuda"), 2, pos=pos).view(4, 2, 64)
+    assert bool(torch.isnan(dx[1, :, :32]).all()) and bool(torch.isnan(dx[2, 0, :32]).all()) and bool((dx[2, 1] == 0).all()) and bool(torch.isfinite(dx[[0, 3]]).all())
