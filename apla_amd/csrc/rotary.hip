@@ -115,10 +115,12 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotArgs a) {
     const bool tv = tb + tsub < a.T;
     const long t = tv ? tb + tsub : a.T - 1;
     float cs[8], sn[8];
+    bool outside = false;      // of the wave's tokens any
     if (r > 0) {
       long p = a.pos ? (long)a.pos[t] : a.seq_len ? t % a.seq_len : t;
       const bool pv = p >= 0 && p < a.P;      // a position outside the table gives NaN, not a read outside it
       const float* row = a.table + (pv ? p : 0) * a.rot;
+      if (!BWD && NORM == 0) outside = a.sign < 0.f && __ballot(!pv) != 0;
       if (a.vec) {    // the lane's eight angles are four (interleaved) or eight (half) neighbours in the table
         const bool in = e0 < 2 * r;
         const float* c = row + (!in ? 0 : a.interleaved ? e0 >> 1 : e0 < r ? e0 : e0 - r);
@@ -159,11 +161,11 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotArgs a) {
         float v[8], d[8];
         bool none = false;       // no gradient arrives at this head: it passes none on, whatever x holds (masked places may hold infinities and NaN)
         unpack8(nx[i], v);
-        if (BWD || a.sign < 0.f) {       // (a gradient: turned back)
-          const unsigned long long some = __ballot(any_value(BWD ? nd[i] : nx[i]));
+        if constexpr (BWD) {
+          unpack8(nd[i], d);
+          const unsigned long long some = __ballot(any_value(nd[i]));
           none = ((some >> (lane & 56)) & 255) == 0;
         }
-        if constexpr (BWD) unpack8(nd[i], d);
         float rs = 1.f;
         if constexpr (NORM != 0) {
           if constexpr (NORM == 1) {
@@ -187,9 +189,12 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotArgs a) {
             for (int e = 0; e < 8; ++e) v[e] = v[e] * w[e] + bi[e];
           }
           if (r > 0) rotate8(v, cs, sn, a.interleaved, r, e0, xch);
-          if (NORM == 0 && none) {
+          if (NORM == 0 && outside) {      // a gradient turned back at positions outside the table
+            const unsigned long long some = __ballot(any_value(nx[i]));
+            if (((some >> (lane & 56)) & 255) == 0) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = 0.f;
+              for (int e = 0; e < 8; ++e) v[e] = 0.f;
+            }
           }
         } else {
           if (r > 0) rotate8(d, cs, sn, a.interleaved, r, e0, xch);
