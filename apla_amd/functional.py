@@ -14,6 +14,7 @@ import weakref
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 from ._lib import AplaHipError
@@ -564,6 +565,7 @@ class _RotaryFn(torch.autograd.Function):
         return ops.rotary_fwd(_rows_h16(x), table, heads, layout=layout, pos=pos, seq_len=seq_len).reshape(x.shape)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         _unchanged(ctx)
         heads, layout, seq_len = ctx.args
@@ -589,6 +591,7 @@ class _QkNormRotaryFn(torch.autograd.Function):
         return ops.qk_norm_rotary_fwd(x, Hq, Hkv, **args).reshape(qkv.shape[:-1] + ((Hq + Hkv) * 64,))
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         _unchanged(ctx)
         (x,), (Hq, Hkv) = ctx.saved_tensors, ctx.heads
@@ -619,6 +622,7 @@ class _AttnModFn(torch.autograd.Function):
         return o.reshape(q.shape), lse
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do, _dlse):
         _unchanged(ctx)
         q, k, v, o, lse = ctx.saved_tensors
@@ -656,6 +660,7 @@ class _AttnModQkvFn(torch.autograd.Function):
         return o.reshape(qkv.shape[:-1] + (n,))
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do):
         _unchanged(ctx)
         x, qk, o, lse = ctx.saved_tensors

@@ -1,0 +1,46 @@
+"""Rotary positions, q / k norm and attention with modified scores as autograd nodes: what they save, and what they refuse."""
+import pytest
+import torch
+from torch import nn
+
+from apla_amd import functional as AF
+from apla_amd import ops
+from apla_amd import rotary as R
+
+pytestmark = pytest.mark.gpu
+T, H = 48, 2
+
+
+def rows(seed, cols=H * 64):
+    return torch.randn(T, cols, generator=torch.Generator().manual_seed(seed)).bfloat16().cuda().requires_grad_(True)
+
+
+def nodes():
+    """name -> (function of its differentiable inputs, those inputs, the other tensors that its backward reads)"""
+    table, pos = R.rotary_table(T, 64, device="cuda"), torch.arange(T, dtype=torch.int32).flip(0).cuda()
+    slopes, doc, prefix = torch.full((H,), 0.25, device="cuda"), (torch.arange(T, dtype=torch.int32) // 20).cuda(), torch.tensor([5], dtype=torch.int32).cuda()
+    mod = ops.ScoreMod(softcap=9.0, slopes=slopes, doc_q=doc, doc_k=doc, causal=True, prefix=prefix)
+    used = torch.tensor([T - 3], dtype=torch.int32).cuda()
+    w = [(torch.rand(64, generator=torch.Generator().manual_seed(9 + i)) + 0.5).cuda().requires_grad_(True) for i in range(2)]
+    w16 = [p.detach().bfloat16().requires_grad_(True) for p in w]
+    norms = [nn.LayerNorm(64).cuda() for _ in range(2)]
+    return {
+        "rotary": (lambda x: AF.rotary(x, table, H, pos=pos), [rows(1)], [table, pos]),
+        "norm": (lambda x, a, b: AF.qk_norm_rotary(x, 1, 1, q_weight=a, k_weight=b, table=table, pos=pos), [rows(2), *w], [table, pos]),
+        "norm16": (lambda x, a, b: AF.qk_norm_rotary(x, 1, 1, norm="rms", q_weight=a, k_weight=b, table=table, pos=pos), [rows(2), *w16], [table, pos]),
+        "attention": (lambda q, k, v: AF.attention_mod(q, k, v, H, H, 0.125, mod, batch=1, len_k=used)[0], [rows(3), rows(4), rows(5)], [slopes, doc, prefix, used]),
+        "qkv": (lambda x, *_: AF.attention_mod_qkv(x, H, 0.125, mod=mod, q_norm=norms[0], k_norm=norms[1], table=table, pos=pos, batch=1),
+                [rows(6, 3 * H * 64), norms[0].weight, norms[1].weight], [table, pos, slopes, doc, prefix]),
+    }
+
+
+NAMES = ["rotary", "norm", "norm16", "attention", "qkv"]
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_second_derivatives_are_refused(name):
+    f, inputs, _ = nodes()[name]
+    o = f(*inputs)
+    (g, *_) = torch.autograd.grad(o.float().square().sum(), inputs, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):      # (not the part of it that other nodes know)
+        (g.float().square().sum() + o.float().sum()).backward()
