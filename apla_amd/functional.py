@@ -541,35 +541,53 @@ def _rows_h16(x):
     return x2 if readable else x2.clone(memory_format=torch.contiguous_format)
 
 
-def _remember(ctx, *tensors):
-    """The versions of tensors that the backward pass reads again without having saved them."""
-    ctx.versions = [(t, t._version) for t in tensors if t is not None and not t.is_inference()]
+def _save(ctx, *tensors):
+    """Tensors (or None) that the backward pass reads, saved: with their versions, and for saved-tensor hooks.  Inference tensors can be neither changed nor
+    saved; they stay on ctx."""
+    ctx.kept = [t if t is not None and t.is_inference() else None for t in tensors]
+    ctx.save_for_backward(*(None if k is not None else t for t, k in zip(tensors, ctx.kept)))
 
 
-def _unchanged(ctx):
-    if any(t._version != v for t, v in ctx.versions):
-        raise RuntimeError("an argument that the backward pass reads was modified in place after the forward pass")
+def _saved(ctx):
+    try:
+        tensors = ctx.saved_tensors
+    except RuntimeError as e:
+        if "inplace" not in str(e):
+            raise
+        raise RuntimeError("an argument that the backward pass reads was modified in place after the forward pass") from e
+    return [t if k is None else k for t, k in zip(tensors, ctx.kept)]
 
 
-def _mod_tensors(mod, seq):
-    m = () if mod is None else (mod.slopes, mod.pos_q, mod.pos_k, mod.doc_q, mod.doc_k, mod.prefix)
-    return (*m, *(t for t in seq.values() if isinstance(t, torch.Tensor)))
+_MOD = ("slopes", "pos_q", "pos_k", "doc_q", "doc_k", "prefix")
+_SEQ = ("cu_q", "cu_k", "len_k")
+
+
+def _unpack_mod(mod, seq):
+    """(rest, tensors) of a ScoreMod and sequence arguments, as they are now: the tensors are saved, the rest holds what else the backward pass needs."""
+    m = ops.ScoreMod() if mod is None else mod
+    return (m.softcap, m.causal, {n: v for n, v in seq.items() if n not in _SEQ}), [getattr(m, n) for n in _MOD] + [seq.get(n) for n in _SEQ]
+
+
+def _pack_mod(rest, tensors):
+    softcap, causal, seq = rest
+    mod = ops.ScoreMod(softcap=softcap, causal=causal, **dict(zip(_MOD, tensors)))
+    return mod, dict(seq, **{n: t for n, t in zip(_SEQ, tensors[len(_MOD):]) if t is not None})
 
 
 class _RotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, table, heads, layout, pos, seq_len):
         _require_cuda(x, "rotary")
-        ctx.args, ctx.pos, ctx.table, ctx.dtype = (heads, layout, seq_len), pos, table, x.dtype
-        _remember(ctx, table, pos)
+        ctx.args, ctx.dtype = (heads, layout, seq_len), x.dtype
+        _save(ctx, table, pos)
         return ops.rotary_fwd(_rows_h16(x), table, heads, layout=layout, pos=pos, seq_len=seq_len).reshape(x.shape)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        _unchanged(ctx)
+        table, pos = _saved(ctx)
         heads, layout, seq_len = ctx.args
-        dx = ops.rotary_bwd(_as2d_bf16(dy), ctx.table, heads, layout=layout, pos=ctx.pos, seq_len=seq_len)
+        dx = ops.rotary_bwd(_as2d_bf16(dy), table, heads, layout=layout, pos=pos, seq_len=seq_len)
         return dx.reshape(dy.shape).to(ctx.dtype), None, None, None, None, None
 
 
@@ -578,26 +596,30 @@ def rotary(x, table, heads: int, *, layout: str = "half", pos=None, seq_len: int
     return _RotaryFn.apply(x, table, heads, layout, pos, seq_len)
 
 
+def _norm_args(norm, eps, par, rot):
+    """Keyword arguments of ops.qk_norm_rotary_*; par: fp32 weights of q and k, then biases."""
+    return dict(zip(("q_weight", "k_weight", "q_bias", "k_bias"), par), norm=norm, eps=eps, **rot)
+
+
 class _QkNormRotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, qw, kw, qb, kb, Hq, Hkv, norm, eps, rot):
         _require_cuda(qkv, "qk_norm_rotary")
-        x = _rows_h16(qkv)
-        par = [b_f32(p) for p in (qw, kw, qb, kb)]
-        args = dict(zip(("q_weight", "k_weight", "q_bias", "k_bias"), par), norm=norm, eps=eps, **rot)
-        ctx.save_for_backward(x)
-        _remember(ctx, qw, kw, rot["table"], rot["pos"])
-        ctx.args, ctx.heads, ctx.shape, ctx.dtype, ctx.pdt = args, (Hq, Hkv), qkv.shape, qkv.dtype, [None if p is None else p.dtype for p in (qw, kw, qb, kb)]
-        return ops.qk_norm_rotary_fwd(x, Hq, Hkv, **args).reshape(qkv.shape[:-1] + ((Hq + Hkv) * 64,))
+        x, par = _rows_h16(qkv), [b_f32(p) for p in (qw, kw, qb, kb)]
+        _save(ctx, x, *par[:2], rot["table"], rot["pos"], qw, kw)      # (the parameters themselves for their versions: par may be copies)
+        ctx.norm, ctx.rot, ctx.heads, ctx.shape, ctx.dtype = (norm, eps), (rot["layout"], rot["seq_len"]), (Hq, Hkv), qkv.shape, qkv.dtype
+        ctx.pdt = [None if p is None else p.dtype for p in (qw, kw, qb, kb)]
+        return ops.qk_norm_rotary_fwd(x, Hq, Hkv, **_norm_args(norm, eps, par, rot)).reshape(qkv.shape[:-1] + ((Hq + Hkv) * 64,))
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        _unchanged(ctx)
-        (x,), (Hq, Hkv) = ctx.saved_tensors, ctx.heads
+        x, qw, kw, table, pos, *_ = _saved(ctx)
+        (Hq, Hkv), (layout, seq_len) = ctx.heads, ctx.rot
         n = (Hq + Hkv) * 64
         full = torch.zeros(x.shape, device=x.device, dtype=x.dtype) if x.shape[1] > n else torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        _, dpar = ops.qk_norm_rotary_bwd(_as2d_bf16(dy), x, Hq, Hkv, out=full[:, :n], want_params=any(ctx.needs_input_grad[1:5]), **ctx.args)
+        args = _norm_args(*ctx.norm, (qw, kw, None, None), dict(table=table, pos=pos, layout=layout, seq_len=seq_len))
+        _, dpar = ops.qk_norm_rotary_bwd(_as2d_bf16(dy), x, Hq, Hkv, out=full[:, :n], want_params=any(ctx.needs_input_grad[1:5]), **args)
         g = [None if not ctx.needs_input_grad[1 + i] else dpar[i].to(ctx.pdt[i]) for i in range(4)]
         return full.reshape(ctx.shape).to(ctx.dtype), *g, None, None, None, None, None
 
@@ -615,19 +637,18 @@ class _AttnModFn(torch.autograd.Function):
         _require_cuda(q, "attention_mod")
         q2, k2, v2 = _rows_h16(q), _rows_h16(k), _rows_h16(v)
         o, lse = ops.attn_mod_fwd(q2, k2, v2, Hq, Hkv, scale, mod, **seq)
-        ctx.save_for_backward(q2, k2, v2, o, lse)
-        ctx.args, ctx.like = (Hq, Hkv, scale, mod, seq), [(t.shape, t.dtype) for t in (q, k, v)]
-        _remember(ctx, *_mod_tensors(mod, seq))
+        ctx.rest, tensors = _unpack_mod(mod, seq)
+        _save(ctx, q2, k2, v2, o, lse, *tensors)
+        ctx.args, ctx.like = (Hq, Hkv, scale), [(t.shape, t.dtype) for t in (q, k, v)]
         ctx.mark_non_differentiable(lse)
         return o.reshape(q.shape), lse
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do, _dlse):
-        _unchanged(ctx)
-        q, k, v, o, lse = ctx.saved_tensors
-        Hq, Hkv, scale, mod, seq = ctx.args
-        g = ops.attn_mod_bwd(q, k, v, o, _as2d_bf16(do), lse, Hq, Hkv, scale, mod, **seq)
+        q, k, v, o, lse, *tensors = _saved(ctx)
+        mod, seq = _pack_mod(ctx.rest, tensors)
+        g = ops.attn_mod_bwd(q, k, v, o, _as2d_bf16(do), lse, *ctx.args, mod, **seq)
         return (*(t.reshape(s).to(dt) for t, (s, dt) in zip(g, ctx.like)), None, None, None, None, None)
 
 
@@ -645,36 +666,34 @@ class _AttnModQkvFn(torch.autograd.Function):
     def forward(ctx, qkv, qw, kw, qb, kb, H, scale, norm, eps, rot, mod, seq):
         _require_cuda(qkv, "attention_mod_qkv")
         x, n = _rows_h16(qkv), H * 64
-        args = None
+        par = [b_f32(p) for p in (qw, kw, qb, kb)]
         if norm is not None:
-            args = dict(zip(("q_weight", "k_weight", "q_bias", "k_bias"), [b_f32(p) for p in (qw, kw, qb, kb)]), norm=norm, eps=eps, **rot)
-            qk = ops.qk_norm_rotary_fwd(x, H, H, **args)
+            qk = ops.qk_norm_rotary_fwd(x, H, H, **_norm_args(norm, eps, par, rot))
         elif rot["table"] is not None:
             qk = ops.rotary_fwd(x[:, :2 * n], rot["table"], 2 * H, **{a: b for a, b in rot.items() if a != "table"})
         else:
             qk = x[:, :2 * n]
         o, lse = ops.attn_mod_fwd(qk[:, :n], qk[:, n:], x[:, 2 * n:], H, H, scale, mod, **seq)
-        ctx.save_for_backward(x, qk, o, lse)
-        _remember(ctx, qw, kw, rot["table"], rot["pos"], *_mod_tensors(mod, seq))
-        ctx.args, ctx.norm, ctx.like, ctx.pdt = (H, scale, rot, mod, seq), args, (qkv.shape, qkv.dtype), [None if p is None else p.dtype for p in (qw, kw, qb, kb)]
+        ctx.rest, tensors = _unpack_mod(mod, seq)
+        _save(ctx, x, qk, o, lse, qw, kw, *par[:2], rot["table"], rot["pos"], *tensors)
+        ctx.args, ctx.norm, ctx.rot, ctx.like, ctx.pdt = (H, scale), (norm, eps), (rot["layout"], rot["seq_len"]), (qkv.shape, qkv.dtype), [None if p is None else p.dtype for p in (qw, kw, qb, kb)]
         return o.reshape(qkv.shape[:-1] + (n,))
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        _unchanged(ctx)
-        x, qk, o, lse = ctx.saved_tensors
-        H, scale, rot, mod, seq = ctx.args
-        n = H * 64
+        x, qk, o, lse, _, _, qw, kw, table, pos, *tensors = _saved(ctx)
+        (H, scale), (layout, seq_len), (mod, seq) = ctx.args, ctx.rot, _pack_mod(ctx.rest, tensors)
+        n, rot = H * 64, dict(layout=layout, pos=pos, seq_len=seq_len)
         dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
         ops.attn_mod_bwd(qk[:, :n], qk[:, n:], x[:, 2 * n:], o, _as2d_bf16(do), lse, H, H, scale, mod, dq=dx[:, :n], dk=dx[:, n:2 * n], dv=dx[:, 2 * n:], zero_rest=True, **seq)
         g = [None] * 4
-        if ctx.norm is not None:        # in place: every lane reads its row's gradient before it writes it
+        if ctx.norm[0] is not None:     # in place: every lane reads its row's gradient before it writes it
             want = any(ctx.needs_input_grad[1:5])
-            _, dpar = ops.qk_norm_rotary_bwd(dx[:, :2 * n], x, H, H, out=dx[:, :2 * n], want_params=want, **ctx.norm)
+            _, dpar = ops.qk_norm_rotary_bwd(dx[:, :2 * n], x, H, H, out=dx[:, :2 * n], want_params=want, **_norm_args(*ctx.norm, (qw, kw, None, None), dict(rot, table=table)))
             g = [dpar[i].to(ctx.pdt[i]) if ctx.needs_input_grad[1 + i] else None for i in range(4)]
-        elif rot["table"] is not None:
-            ops.rotary_bwd(dx[:, :2 * n], rot["table"], 2 * H, out=dx[:, :2 * n], **{a: b for a, b in rot.items() if a != "table"})
+        elif table is not None:
+            ops.rotary_bwd(dx[:, :2 * n], table, 2 * H, out=dx[:, :2 * n], **rot)
         return dx.reshape(ctx.like[0]).to(ctx.like[1]), *g, None, None, None, None, None, None, None
 
 

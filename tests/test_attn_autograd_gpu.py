@@ -37,6 +37,27 @@ def nodes():
 NAMES = ["rotary", "norm", "norm16", "attention", "qkv"]
 
 
+def gradients(f, inputs):
+    o = f(*inputs)
+    return torch.autograd.grad(o, inputs, torch.ones_like(o))
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_what_the_backward_reads_passes_saved_tensor_hooks(name):
+    """Kept on the host between the passes: every tensor that the backward reads is handed out, and the gradients are the same bits."""
+    f, inputs, side = nodes()[name]
+    seen = []
+
+    def out(t):
+        seen.append(t.data_ptr())
+        return t.cpu()
+    want = gradients(f, inputs)
+    with torch.autograd.graph.saved_tensors_hooks(out, lambda t: t.cuda()):
+        got = gradients(f, inputs)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    assert {t.data_ptr() for t in side} <= set(seen)
+
+
 @pytest.mark.parametrize("name", NAMES)
 def test_second_derivatives_are_refused(name):
     f, inputs, _ = nodes()[name]
@@ -44,3 +65,34 @@ def test_second_derivatives_are_refused(name):
     (g, *_) = torch.autograd.grad(o.float().square().sum(), inputs, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):      # (not the part of it that other nodes know)
         (g.float().square().sum() + o.float().sum()).backward()
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_arguments_changed_in_place_are_refused(name):
+    f, inputs, side = nodes()[name]
+    for t in side + inputs[1:]:
+        o = f(*inputs)
+        with torch.no_grad():
+            t.add_(0)
+        with pytest.raises(RuntimeError, match="in place"):
+            torch.autograd.grad(o, inputs, torch.ones_like(o))
+
+
+def test_a_score_modification_changed_after_the_forward_does_not_matter():
+    q, k, v = rows(1), rows(2), rows(3)
+    mod = ops.ScoreMod(softcap=5.0, slopes=torch.full((H,), 0.5, device="cuda"), causal=True)
+    o, _ = AF.attention_mod(q, k, v, H, H, 0.125, mod, batch=1)
+    want = torch.autograd.grad(o, (q, k, v), torch.ones_like(o), retain_graph=True)
+    mod.softcap, mod.slopes, mod.causal = 0.0, None, False
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(o, (q, k, v), torch.ones_like(o))))
+
+
+def test_tensors_made_in_inference_mode_may_be_arguments():
+    """A plan or table that an evaluation built first is used in training."""
+    with torch.inference_mode():
+        table, slopes = R.rotary_table(T, 64, device="cuda"), torch.full((H,), 0.5, device="cuda")
+    q, k, v = rows(1), rows(2), rows(3)
+    f = lambda a, b, c: AF.attention_mod(AF.rotary(a, table, H), b, c, H, H, 0.125, ops.ScoreMod(slopes=slopes), batch=1)[0]      # noqa: E731
+    got = gradients(f, [q, k, v])
+    table, slopes = table.clone(), slopes.clone()
+    assert all(torch.equal(a, b) for a, b in zip(got, gradients(f, [q, k, v])))
