@@ -574,6 +574,11 @@ def _pack_mod(rest, tensors):
     return mod, dict(seq, **{n: t for n, t in zip(_SEQ, tensors[len(_MOD):]) if t is not None})
 
 
+def _fixed_table(table):
+    if table is not None and table.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError("table: no gradient is computed for it")
+
+
 class _RotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, table, heads, layout, pos, seq_len):
@@ -593,6 +598,7 @@ class _RotaryFn(torch.autograd.Function):
 
 def rotary(x, table, heads: int, *, layout: str = "half", pos=None, seq_len: int = 0):
     """Rotary positions on [..., heads * 64] (16-bit result); ``table`` from apla_amd.rotary, see ops.rotary_fwd for the positions."""
+    _fixed_table(table)
     return _RotaryFn.apply(x, table, heads, layout, pos, seq_len)
 
 
@@ -628,6 +634,7 @@ def qk_norm_rotary(qkv, Hq: int, Hkv: int, *, norm: str = "layer", q_weight=None
                    table=None, layout: str = "half", pos=None, seq_len: int = 0):
     """Norm of every query / key head and rotation: [..., >= (Hq + Hkv) * 64] -> [..., (Hq + Hkv) * 64] (16 bits), with the gradients of the
     weights and biases that ask for one."""
+    _fixed_table(table)
     return _QkNormRotaryFn.apply(qkv, q_weight, k_weight, q_bias, k_bias, Hq, Hkv, norm, eps, dict(table=table, layout=layout, pos=pos, seq_len=seq_len))
 
 
@@ -702,6 +709,7 @@ def attention_mod_qkv(qkv, H: int, scale: float, *, mod=None, q_norm=None, k_nor
     the rotation of ``table`` (None: none) and the score modification ``mod``; ``seq`` as in attention_mod.  Returns o [..., H * 64]."""
     if qkv.shape[-1] != 3 * H * 64:
         raise NotImplementedError(f"the HIP attention kernel needs head_dim 64 (got {qkv.shape[-1] // (3 * H)})")
+    _fixed_table(table)
     norm, eps, w = None, 0.0, [None] * 4
     if q_norm is not None or k_norm is not None:
         norm, eps = qk_norm_kind(q_norm, k_norm)

@@ -96,3 +96,12 @@ def test_tensors_made_in_inference_mode_may_be_arguments():
     got = gradients(f, [q, k, v])
     table, slopes = table.clone(), slopes.clone()
     assert all(torch.equal(a, b) for a, b in zip(got, gradients(f, [q, k, v])))
+
+
+def test_a_learned_table_is_refused():
+    table, x = R.rotary_table(T, 64, device="cuda").requires_grad_(True), rows(1, 3 * H * 64)
+    for f in (lambda: AF.rotary(x, table, 3 * H), lambda: AF.qk_norm_rotary(x, H, H, table=table), lambda: AF.attention_mod_qkv(x, H, 0.125, table=table, batch=1)):
+        with pytest.raises(NotImplementedError, match="table"):
+            f()
+        with torch.no_grad():
+            assert torch.isfinite(f().float()).all()
