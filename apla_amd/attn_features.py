@@ -38,7 +38,8 @@ class AttnFeatures:
         self.qk_norm = conf.get("qk_norm") or None
         if self.qk_norm not in (None, "layer", "rms"):
             raise ValueError(f"qk_norm must be layer or rms, got {self.qk_norm!r}")
-        rope = conf.get("rope") or None
+        rope = conf.get("rope")
+        rope = None if rope is False else rope      # ({}: all defaults)
         if rope is not None:
             rope = {} if rope is True else dict(rope)
             if set(rope) - _ROPE_KEYS:
