@@ -1424,6 +1424,18 @@ Plan plan_of(const apla_attn_mod_t& p, bool backward) {
   return pl;
 }
 
+// workgroups of the largest launch of a call
+long most_blocks(const apla_attn_mod_t& p, const Plan& pl, bool backward) {
+  const long units = (long)p.S * p.Hkv, G = p.Hq / p.Hkv, nq = (p.max_q + 127L) / 128, nk = (p.max_k + 127L) / 128;
+  const int np = unit_parts(units);
+  long n = (p.S + 1L) * 64;                                                        // fill
+  auto also = [&](long m) { n = m > n ? m : n; };
+  if (p.doc_k) also((p.S * (((p.max_q > p.max_k ? p.max_q : p.max_k) + 63L) / 64) + 3) / 4);        // ranges
+  if (!backward) also(pl.rows ? units * pl.nrt * pl.nsplit : unit_grid(units, np, G * nq));
+  else also(unit_grid(units, np, G * nq * pl.sq)), also(unit_grid(units, np, nk * pl.sk));
+  return n;
+}
+
 int mod_check(const char* who, const apla_attn_mod_t* p, bool backward) {
   APLA_REQUIRE(p, "%s: no arguments", who);
   APLA_REQUIRE(p->S > 0 && p->S <= 65535 && p->Hq > 0 && p->Hq <= 65535 && p->Hkv > 0 && p->Hq % p->Hkv == 0, "%s: need 1..65535 sequences and Hq a multiple of Hkv (S=%d Hq=%d Hkv=%d)", who, p->S, p->Hq, p->Hkv);
@@ -1446,8 +1458,8 @@ int mod_check(const char* who, const apla_attn_mod_t* p, bool backward) {
   }
   const Plan pl = plan_of(*p, backward);
   APLA_REQUIRE(pl.bytes == 0 || (p->workspace && apla_aligned16(p->workspace) && p->workspace_bytes >= pl.bytes), "%s: needs %ld bytes of 16-byte aligned workspace (got %ld)", who, pl.bytes, p->workspace_bytes);
-  const long nb = (long)p->S * p->Hkv * 8 * 8 * ((long)(p->Hq / p->Hkv) * (((long)(p->max_q > p->max_k ? p->max_q : p->max_k) + 127) / 128) + 1);
-  APLA_REQUIRE(nb < (1L << 31) && (long)p->S * p->Hkv * pl.nrt * pl.nsplit < (1L << 31), "%s: too many blocks", who);
+  const long blocks = most_blocks(*p, pl, backward);
+  APLA_REQUIRE(blocks < (1L << 24), "%s: %ld workgroups in one launch (below 2^24 are possible: 2^32 work items)", who, blocks);
   return APLA_OK;
 }
 

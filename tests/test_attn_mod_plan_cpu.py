@@ -18,3 +18,17 @@ def test_few_rows_or_few_blocks_take_the_form_for_few_rows(kw, want):
 
 def test_no_arguments():
     assert _lib.lib().apla_attn_mod_few_rows(None) == -1
+
+
+@pytest.mark.parametrize("kw", [dict(S=65535, Tq=65535, Tk=65535, max_q=1, max_k=1, Hq=300, Hkv=300), dict(S=60000, Tq=1 << 20, Tk=1 << 20, max_q=4096, max_k=4096, Hq=12, Hkv=12, cu_q=1 << 20, cu_k=1 << 20)], ids=str)
+def test_more_workgroups_than_a_launch_takes_are_refused(kw):
+    a = _lib.AttnMod()
+    for n in ("q", "k", "v", "o", "lse", "d_o", "dq", "dk", "dv", "delta", "workspace"):
+        setattr(a, n, 1 << 20)
+    a.scale, a.workspace_bytes = 0.125, 1 << 60
+    for n, v in kw.items():
+        setattr(a, n, v)
+    a.ldq = a.ldo = a.lddo = a.lddq = a.Hq * 64
+    a.ldk = a.ldv = a.lddk = a.lddv = a.Hkv * 64
+    for f in (_lib.lib().apla_attn_mod_fwd, _lib.lib().apla_attn_mod_bwd):
+        assert f(a, None) == -22 and b"workgroups" in _lib.lib().apla_last_error()
