@@ -191,6 +191,11 @@ __device__ __forceinline__ unsigned poison_bits(const char* raw, int rbase, cons
   }
   return m;
 }
+// a single key has weight 1 and its score no gradient: what dP - delta leaves of it is rounding (infinities and NaN stay NaN)
+__device__ __forceinline__ void no_gradient(f32x16 (&acc)[2]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) acc[i >> 4][i & 15] *= 0.f;
+}
 __device__ __forceinline__ void apply_poison(f32x16 (&acc)[2], unsigned m) {
   if (__ballot(m != 0) == 0) return;
 #pragma unroll
@@ -1103,6 +1108,7 @@ __global__ __launch_bounds__(256, CAP && (DOCS || BIAS) ? 2 : 3) void attn_mod_d
   }
   const float unlift = LIFT ? __builtin_ldexpf(1.f, -lift) : 1.f;
   apply_poison(acc, poison);
+  if (m.nk == 1) no_gradient(acc);
   if (qr < m.nq) {
     if (a.sq == 1) store_acc_T(acc, a.dq + (m.q0 + qr) * a.lddq + h * 64, h2, a.scale * unlift);
     else store_part<LIFT>(acc, a.part_q + (((long)sp * a.Tq + m.q0 + qr) * a.Hq + h) * 64, h2, unlift);
@@ -1304,6 +1310,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dkdv_kernel(ModArgs a) {
   }
   const float unlift = LONG ? __builtin_ldexpf(1.f, -lift) : 1.f;
   apply_poison(dk, pk);
+  if (m.nk == 1) no_gradient(dk);
   apply_poison(dv, pv);
   if (jr < m.nk) {
     if (a.sk == 1) {
