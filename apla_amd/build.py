@@ -18,6 +18,7 @@ SOURCE_FLAGS = {s: ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # Sources whose kernels count their own s_waitcnt (LDS-DMA rings, ds_read_tr pipelines, asm operand loads): a register spill puts scratch
 # loads and stores into the same in-order vmcnt queue and silently breaks those counts (round 4: the fused attention backward at
 # three waves per SIMD spilled 74 registers and returned wrong gradients).  Their objects are only accepted spill-free.
+# (attn_mod.hip is not among them: its LDS-DMA is waited for with vmcnt(0) only, which scratch accesses in the queue cannot mislead.)
 NO_SPILL = ("gemm_nt.hip", "gemm_pp2.hip", "gemm_w4.hip", "gemm_tp.hip", "gemm_lw.hip", "attention.hip", "apla_dw.hip", "layernorm.hip")
 
 

@@ -599,10 +599,11 @@ __device__ __forceinline__ RowCtx row_ctx(const ModArgs& a, const MSeq& m, int i
 
 // ------------------------------------------------------------------------------------------------ forward
 // 128 rows of a head per workgroup, 32 per wave; key tiles of 64 (K, V, positions, ids) go straight into one half of LDS while the other is worked on.
-// Three workgroups share a CU where 168 registers hold a wave's state; capped scores next to a bias or documents spill there (8 x 12 heads of 1370 rows
-// with both: 148 us with two, 169 with three).  Forward times, without / with that: 64 x 12 heads of 257 rows 41 / 49 us, 12 heads of 16384
-// causal rows 538 / 626 us (766 TFLOP/s of the visible half), 48 ragged sequences with a 2-D bias 140 / 172 us, capped 8 x 24 heads of
-// 1370 rows in fp16 218 / 241 us (423 TFLOP/s).
+// Three workgroups share a CU where 168 registers hold a wave's state, or nearly (the capped forward without a bias keeps 7 registers in scratch, bf16 documents
+// with a 2-D bias one); capped scores next to a bias or documents would keep many (8 x 12 heads of 1370 rows with both: 148 us with two, 169
+// with three).  Three take 10 % (cap) to 19 % (ragged, 2-D bias) less time than two.  Forward on a warm card: 64 x 12 heads of 257 rows 38 us, 12 heads
+// of 16384 causal rows 487 us (847 TFLOP/s of the visible half), 48 ragged sequences with a 2-D bias 125 us, capped 8 x 24 heads of 1370
+// rows in fp16 191 us (484 TFLOP/s).
 template <bool CAP, int BIAS, bool DOCS>
 __global__ __launch_bounds__(256, CAP && (DOCS || BIAS) ? 2 : 3) void attn_mod_fwd_kernel(ModArgs a) {
   __shared__ __attribute__((aligned(128))) char smem[2 * KT_BYTES], clean[8192];
@@ -697,8 +698,9 @@ __global__ __launch_bounds__(256, CAP && (DOCS || BIAS) ? 2 : 3) void attn_mod_f
 // The G * nq rows of the query heads that share a key head fill tiles of 16 columns (v_mfma_f32_16x16x32: a single token of 1 .. 16 heads is one
 // tile).  Every wave walks its own 64-key tiles (every fourth of the workgroup's chunk) without a barrier: K straight into operand registers, V through the wave's own LDS for the
 // transposed read, both a tile ahead.  The four waves' (maximum, sum, output) are joined in LDS, those of several workgroups by
-// attn_mod_join_kernel, both in a fixed order.  Bound by the keys' way from memory: single tokens of 24 heads on 32 caches of up to 8192 keys with 8 heads
-// (188 MB) 48 us = 3.9 TB/s, the join 5 us.
+// attn_mod_join_kernel, both in a fixed order.  Bound by the keys' way from memory and by uneven chunks: single tokens of 24 heads on 32 ragged caches of up to 8192
+// keys with 8 heads (188 MB) 54 us = 3.5 TB/s (39 us where they lie in the last-level cache), the join 5 us; about 500 workgroups start at
+// once on 512 places, and the busiest CU has 1.4 times the mean number of keys.
 constexpr int RT_POS = 8192, RT_DOC = RT_POS + 512, RT_BYTES = RT_DOC + 256;      // LDS of a wave: V, positions [2][64], document ids
 constexpr int ROWS = 16;
 
@@ -1002,8 +1004,8 @@ __device__ __forceinline__ void dq_tile(f32x16 (&acc)[2], unsigned& poison, cons
   }
 }
 
-// dQ of 128 rows per workgroup, staged as in the forward; three workgroups per CU where 168 registers hold a wave's state, as there (64 x 12 heads of 257 rows
-// 53 us, 62 with two; 8 x 24 capped ones of 1370 255 us, 280 with two).
+// dQ of 128 rows per workgroup, staged as in the forward; three workgroups per CU where 168 registers hold a wave's state, as there: 15 % less time than two at
+// 64 x 12 heads of 257 rows (51 us), 9 % at 8 x 24 capped ones of 1370 (230 us).  (fp16 documents with a 1-D bias keep 4 registers in scratch.)
 template <bool CAP, int BIAS, bool DOCS>
 __global__ __launch_bounds__(256, CAP && (DOCS || BIAS) ? 2 : 3) void attn_mod_dq_kernel(ModArgs a) {
   __shared__ __attribute__((aligned(128))) char smem[2 * KT_BYTES], clean[8192];
@@ -1116,8 +1118,8 @@ __global__ __launch_bounds__(256, CAP && (DOCS || BIAS) ? 2 : 3) void attn_mod_d
 }
 
 // dK, dV of 128 keys: every wave holds 32 keys (the key on the lane) and the workgroup walks the 64-row query tiles of all heads that share them.
-// Two workgroups per CU: K, V, dK and dV of a wave's keys take 96 registers, so tiles may come through registers as well (64 x 12 heads of 257 rows 73 us, 8 x 24
-// capped ones of 1370 382 us, 12 heads of 8192 rows in documents 96 us).
+// Two workgroups per CU: K, V, dK and dV of a wave's keys take 96 registers, so tiles may come through registers as well (64 x 12 heads of 257 rows 67 us, 8 x 24
+// capped ones of 1370 335 us, 12 heads of 8192 rows in documents 91 us).  Caps next to documents keep 1 to 8 registers in scratch, 15 to 20 with LONG.
 // LDS of a query tile: Q, dO (8 KB each), then per row: lse (log2 units), delta, position x / y, lim, document, verdicts
 constexpr int QT_L = 16384, QT_D = QT_L + 256, QT_X = QT_D + 256, QT_Y = QT_X + 256, QT_LIM = QT_Y + 256, QT_DOC = QT_LIM + 256, QT_ODD = QT_DOC + 256, QT_BYTES = QT_ODD + 128;
 struct QuerySide { float L2, delta, x, y; int lim, doc; };

@@ -17,8 +17,8 @@
 // the raw bits and a ballot.
 // All arithmetic is fp32; the only rounding is that of the stored result.
 //
-// Measured (a large copy reaches 4.95 TB/s): rotation forward and backward of 269 MB 55 us, 4.9 TB/s; norm and rotation of 25 216 tokens of 24 heads 31 us
-// forward, 46 us backward (310 MB in all, 82 us with the sums: 3.8 TB/s — the backward's statistics and sums over eight lanes fill the vector unit);
+// Measured (a large copy reaches 4.95 TB/s): rotation forward and backward of 269 MB 56 us, 4.8 TB/s; norm and rotation of 25 216 tokens of 24 heads forward
+// (155 MB) 34 us, backward (dy and x read, dx written: 232 MB) 45 us = 5.2 TB/s, the copy's rate, with the vector unit 72 % busy, its sums 5 us;
 // few tokens: the launch.
 #include "common.h"
 

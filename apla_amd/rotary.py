@@ -1,7 +1,8 @@
 """Tables of rotary positions for ops.rotary_* / ops.qk_norm_rotary_* (cosines, then sines, of rot / 2 angles per position).
 
 The angles are formed in 64 bits and rounded once: fp32 arithmetic on position * frequency would lose 2^-24 * position of the angle, half a
-turn at position 10^7 and 2^-7 at 131072.  A table is built once per model (1370 positions x 64: 350 KB) and shared by all blocks."""
+turn at position 10^7 and 2^-7 at 131072.  A caller builds a table once and passes it to every call; modules with attention features build one
+each per geometry (1370 positions x 64: 350 KB)."""
 import math
 from typing import Optional, Sequence
 
