@@ -544,11 +544,25 @@ def _rows_h16(x):
 def _save(ctx, *tensors):
     """Tensors (or None) that the backward pass reads, saved: with their versions, and for saved-tensor hooks.  Inference tensors can be neither changed nor
     saved; they stay on ctx."""
+    _note_leaves(ctx, tensors[0].device)
     ctx.kept = [t if t is not None and t.is_inference() else None for t in tensors]
     ctx.save_for_backward(*(None if k is not None else t for t, k in zip(tensors, ctx.kept)))
 
 
+def _note_leaves(ctx, device):
+    """A leaf's gradient is added on the stream of the oldest living graph that holds the leaf.  A backward pass captured meanwhile would send the engine to that
+    stream in the middle of the capture, which ends the process.  So the node that adds remembers an eager stream, and _saved refuses."""
+    if not torch.cuda.is_current_stream_capturing():
+        for node, _ in ctx.next_functions:
+            if node is not None and node.name().endswith("AccumulateGrad"):
+                node.metadata.setdefault("apla_stream", ops._raw_stream(device))
+
+
 def _saved(ctx):
+    if torch.cuda.is_current_stream_capturing():
+        here = torch.cuda.current_stream().cuda_stream
+        if any(node is not None and node.metadata.get("apla_stream", here) != here for node, _ in ctx.next_functions):
+            raise RuntimeError("a backward pass is captured while an eager graph of the same leaves lives, whose stream adds their gradients: delete the outputs of the eager passes first")
     try:
         tensors = ctx.saved_tensors
     except RuntimeError as e:

@@ -105,3 +105,23 @@ def test_a_learned_table_is_refused():
             f()
         with torch.no_grad():
             assert torch.isfinite(f().float()).all()
+
+
+def test_a_captured_backward_refuses_leaves_of_a_living_eager_graph():
+    """The gradient of such a leaf is added on the eager graph's stream, which a capture must not touch.  Without the eager graph the backward is captured."""
+    w, x = torch.rand(64, device="cuda").add_(0.5).requires_grad_(True), rows(1)
+    step = lambda: torch.autograd.grad(AF.qk_norm_rotary(x, H, 0, q_weight=w), [x, w], torch.ones_like(x))      # noqa: E731
+    eager = AF.qk_norm_rotary(x, H, 0, q_weight=w)
+    refused, g = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(refused):
+            step()
+    del eager
+    with torch.cuda.graph(g):
+        got = step()
+    for i in range(3):
+        with torch.no_grad():
+            x.copy_(rows(20 + i))
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
